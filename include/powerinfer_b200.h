@@ -36,6 +36,7 @@ extern "C" {
 #define PI_ERR_TIMEOUT      5   /* a bounded device-side wait ran out (multi-GPU exchange) */
 
 /* weight storage types (ggml.h GGML_TYPE_F16 / GGML_TYPE_Q4_0) */
+#define PI_TYPE_F32   0         /* rows of activations only */
 #define PI_TYPE_F16   1         /* IEEE half, row of n halves */
 #define PI_TYPE_Q4_0  2         /* ggml block_q4_0 {fp16 d; uint8 qs[16]} (ggml-quants.h:11-15), 18 bytes per 32 weights.
                                  * Device copies are held in the PLANAR form made by pi_q4_0_repack. */
@@ -170,6 +171,73 @@ void pi_rope_table_host(float * host_cs, int n_pos, int head_dim, float freq_bas
 int pi_attention_decode(const float * q, const float * k, const float * v, void * k_cache, void * v_cache,
                         const int32_t * seq, const int32_t * pos, int T, int n_head, int n_head_kv, int head_dim,
                         int n_ctx, float * out, void * stream);
+
+/* ---- a long context: scaled rotary positions, a KV cache in 8 bits, its attention and eviction -------------------- */
+
+/* Frequencies of ggml_rope_custom's scaled forms (llama.cpp:4383-4418 with rope_freq_scale, ggml.c:11142-11200): n_rot / 2 angles per position, in
+ * 64 bits, and the factor of the rotated values.  f_i = freq_base^(-2i / n_rot), over host_freq_factors[i] where given.  ext_factor 0: times
+ * freq_scale (linear; 1: unscaled).  ext_factor > 0 (YaRN): the pairs that make more than beta_fast turns within n_orig_ctx positions keep
+ * f_i, those with fewer than beta_slow take freq_scale * f_i, between them a ramp; mscale = attn_factor * (1 + 0.1 ln(1 / freq_scale)). */
+int pi_rope_freqs_host(double * host_freqs, float * host_mscale, int n_rot, float freq_base, float freq_scale, float ext_factor, float attn_factor,
+                       float beta_fast, float beta_slow, int n_orig_ctx, const float * host_freq_factors);
+
+/* Rotation of the first n_rot dimensions of every head of q [T, n_head * head_dim] and, where k is not NULL, k [T, n_head_kv * head_dim]: pairs
+ * (2i, 2i + 1), or (i, i + n_rot / 2) with neox; the other dimensions pass.  xtype PI_TYPE_F32 or PI_TYPE_F16 (of inputs and results; angles
+ * are made in 64 bits, products in 32).  Strides are values between rows; addresses and rows are 16-byte aligned.  Results may take the place of the
+ * inputs (same address and stride).  head_dim % 8 == 0, up to 256.  pos int32 [T]; freqs F64 [n_rot / 2] from pi_rope_freqs_host. */
+int pi_rope_ext(int xtype, const void * q, int64_t q_stride, int n_head, void * q_out, int64_t q_out_stride,
+                const void * k, int64_t k_stride, int n_head_kv, void * k_out, int64_t k_out_stride,
+                int T, int head_dim, int n_rot, int neox, const int32_t * pos, const double * freqs, float mscale, void * stream);
+
+/* A KV cache in 8 bits: codes int8 [n_seq, n_head_kv, n_ctx, head_dim], 16-byte aligned, and for every block of `block` slots of a sequence and KV
+ * head a scale, F32 [n_seq, n_head_kv, n_ctx / block]; a value is code * scale.  head_dim 64, 96, 128, 192 or 256; block 16, 32, 64 or 128;
+ * n_ctx a multiple of block.  A slot is a place in the cache; it equals the token's position until slots are evicted. */
+typedef struct {
+    void * k, * v; float * k_scale, * v_scale;
+    int n_seq, n_head_kv, n_ctx, head_dim, block;
+} pi_kv_q8;
+
+/* Consecutive tokens of n sequences, of different numbers: entry i is rows q_start[i] .. q_start[i + 1] - 1 of the row arrays (T rows), in slots
+ * pos0[i] and on of sequence seq[i] (seq NULL: i).  q_start int32 [n + 1], seq and pos0 int32 [n], on the device.  max_new: an upper bound of the tokens
+ * of an entry (tokens beyond it are not handled).  An entry whose sequence or first slot the cache lacks is not stored, attends to
+ * nothing and reads zeros; so do tokens whose slots lie behind n_ctx.  Rows of no entry are left as they were. */
+typedef struct {
+    const int32_t * q_start, * seq, * pos0;
+    int n, T, max_new;
+} pi_kv_batch;
+
+/* llm_build_kv_store (llama.cpp:4383-4418) into 8 bits: k, v [T, n_head_kv * head_dim] (F32 or F16).  With a the largest finite magnitude that
+ * the call brings into a block and s_old the block's scale where earlier tokens are in it (else 0), in FP32: s = max(a * (1 / 127), s_old), codes
+ * rne(x * (1 / s)) within +-127 (infinities +-127, NaN 0), earlier codes rne(code * (s_old / s)) where s grew; s below FLT_MIN: zeros.  Slots behind
+ * the new ones keep their codes, but belong to no token any more.  Of entries that name one sequence the last one with tokens is stored. */
+int pi_kv_store_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, const void * k, int64_t k_stride, const void * v, int64_t v_stride, void * stream);
+
+/* The same slots read back as values (F32 or F16). */
+int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, void * k, int64_t k_stride, void * v, int64_t v_stride, void * stream);
+
+/* llm_build_kqv (llama.cpp:4764-4850) over the 8-bit cache, the new tokens' keys and values in it already: token t of entry i sees slots
+ * 0 .. pos0[i] + t; out = softmax(scale * q . k) v for every query head, heads h of group h / (n_head / n_head_kv).  q, out [T, n_head * head_dim]
+ * (F32 or F16); products are made with 22 bits of queries and probabilities and summed in FP32, whatever the type.  max_kv: the slots that the longest
+ * sequence is expected to see (it sets how the work is cut; more slots are read too, more slowly).  A token that sees nothing has zeros.
+ * weights_out F32 [n_seq, n_head_kv, n_ctx] (NULL: none): for every slot that an entry's tokens see the sum of its probabilities over
+ * those tokens and the heads of the group, plus weights_in (same shape, may be the same array; NULL: 0) for slots before pos0; the sums' order is
+ * fixed.  Other elements are left as they were.  Of entries that name one sequence the last one with tokens counts.
+ * workspace: pi_attention_q8_workspace_bytes with the same arguments (`weights`: whether weights_out is given), 256-byte aligned; 0 bytes may be NULL. */
+size_t pi_attention_q8_workspace_bytes(const pi_kv_q8 * cache, const pi_kv_batch * batch, int n_head, int max_kv, int weights);
+int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, const void * q, int64_t q_stride, int n_head, int max_kv, float scale,
+                    void * out, int64_t out_stride, const float * weights_in, float * weights_out,
+                    void * workspace, size_t workspace_bytes, void * stream);
+
+/* Eviction by accumulated weight (it has no counterpart in the reference, whose cache only shifts: llama.cpp:1573-1693): sequence seq[i] (NULL: i) with
+ * len[i] slots in use is cut to `keep` (a multiple of block) where it has more.  Every KV head keeps its own slots: the first n_sink, the last
+ * n_recent, and of the others those with the largest weights (F32 [n_seq, n_head_kv, n_ctx]; the lowest slots among equals; NaN is
+ * the largest).  Kept slots below `keep` stay; the others, ascending, take the places of the evicted ones below `keep`, ascending.  A block that takes rows in
+ * gets the largest scale of its rows, codes of other scales rne(code * (scale / that)).  kept int32 [n, n_head_kv, keep]: the slot that each slot's
+ * row came from, -1 behind the end.  weights_out (NULL: none; may be `weights`): the weights in the new order.  The sequence then has
+ * min(len, keep) slots.  With len - keep >= n_recent the last n_recent slots are the newest tokens, also after earlier evictions.
+ * Of entries that name one sequence the last one counts, the others' kept are -1.  n_ctx up to 262144. */
+int pi_kv_evict_q8(const pi_kv_q8 * cache, const int32_t * len, const int32_t * seq, int n, int keep, int n_sink, int n_recent,
+                   const float * weights, float * weights_out, int32_t * kept, void * stream);
 
 /* ---- the decode token loop ------------------------------------------------------------------------------ */
 

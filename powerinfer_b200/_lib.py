@@ -11,11 +11,19 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpowerinfer_b200.so")
 
-PI_TYPE_F16, PI_TYPE_Q4_0 = 1, 2
+PI_TYPE_F32, PI_TYPE_F16, PI_TYPE_Q4_0 = 0, 1, 2
 
 
 class PiError(RuntimeError):
     pass
+
+
+class KvQ8(C.Structure):                  # pi_kv_q8
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [(n, C.c_int) for n in ("n_seq", "n_head_kv", "n_ctx", "head_dim", "block")]
+
+
+class KvBatch(C.Structure):               # pi_kv_batch
+    _fields_ = [(n, C.c_void_p) for n in ("q_start", "seq", "pos0")] + [(n, C.c_int) for n in ("n", "T", "max_new")]
 
 
 def _load():
@@ -44,6 +52,13 @@ def _load():
         "pi_norm": (i32, [vp, i32, i64, i32, f32, vp, vp, vp, vp]),
         "pi_rope": (i32, [vp, i32, i32, i32, vp, vp, i32, vp]),
         "pi_rope_table_host": (None, [vp, i32, i32, f32]),
+        "pi_rope_freqs_host": (i32, [vp, vp, i32, f32, f32, f32, f32, f32, f32, i32, vp]),
+        "pi_rope_ext": (i32, [i32, vp, i64, i32, vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, f32, vp]),
+        "pi_kv_store_q8": (i32, [vp, vp, i32, vp, i64, vp, i64, vp]),
+        "pi_kv_load_q8": (i32, [vp, vp, i32, vp, i64, vp, i64, vp]),
+        "pi_attention_q8_workspace_bytes": (sz, [vp, vp, i32, i32, i32]),
+        "pi_attention_q8": (i32, [vp, vp, i32, vp, i64, i32, i32, f32, vp, i64, vp, vp, vp, sz, vp]),
+        "pi_kv_evict_q8": (i32, [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]),
         "pi_attention_decode": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     }
     for name, (res, args) in sig.items():
@@ -56,7 +71,8 @@ lib = _load()
 EXPORTS = ["pi_last_error", "pi_version", "pi_row_bytes", "pi_workspace_bytes", "pi_quantize_q4_0", "pi_q4_0_repack",
            "pi_dequantize_q4_0", "pi_quantize_q8_0", "pi_mul_mat_idx", "pi_axpy", "pi_sparse_ffn", "pi_axpy_static_max_bytes", "pi_axpy_static", "pi_op_status",
            "pi_mul_mat", "pi_predictor",
-           "pi_active_list", "pi_norm", "pi_rope", "pi_rope_table_host", "pi_attention_decode"]
+           "pi_active_list", "pi_norm", "pi_rope", "pi_rope_table_host", "pi_attention_decode",
+           "pi_rope_freqs_host", "pi_rope_ext", "pi_kv_store_q8", "pi_kv_load_q8", "pi_attention_q8_workspace_bytes", "pi_attention_q8", "pi_kv_evict_q8"]
 
 
 def check(rc: int) -> None:

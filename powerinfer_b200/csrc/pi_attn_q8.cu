@@ -1,0 +1,509 @@
+// Attention over the KV cache in 8 bits, for a ragged batch: query t of sequence i (slot pos0[i] + t) sees slots 0 .. pos0[i] + t.
+//
+//     s_j = scale * ks[j / B] * (q . k_j)     p_j = exp(s_j - max s)     out = sum_j p_j vs[j / B] v_j / sum_j p_j
+//
+// Bound by the bytes of the codes.  A CTA takes 8 or 16 query rows that read one KV head (the query heads of a group, of one or more
+// tokens) and a range of slots; its four warps take 16 slots each in turn, copied ahead into a ring of their own (cp.async; no barrier
+// between warps), keep a maximum, a sum and all sums of values of their own, and join them at the end.  Long ranges are
+// split over CTAs, whose sums k_attn_q8_join joins.
+//
+// Precision.  A code is exact as a half.  A query row is scaled by a power of two and held as the sum of two halves, rows 0 .. 7 of the
+// tensor cores' tile the upper, rows 8 .. 15 the lower parts, so the tile that a group of up to 8 heads would leave half empty makes the products
+// with 22 bits; the sum of both is in one lane.  Probabilities go the same way, times vs over the largest vs so far (at most 1): out = sums *
+// that scale.  Maxima, sums and the exponents' arguments are FP32.
+//
+// Layouts.  mma.m16n8k16 sums over 16 columns (scores) or slots (values) in any order that both operands share: a lane's piece of a key row is
+// 16 contiguous codes, of a value row hd / 8 of them, and every 4 codes are operands of one product.  The probabilities of the score tile's layout
+// are the value product's operand as they stand.  Where the maximum rises by less than 2^8, sums are not scaled anew.
+#include "pi_kv_q8.cuh"
+
+namespace pi {
+
+static constexpr int AQ_WARPS = 4, AQ_THREADS = AQ_WARPS * 32, AQ_STEP = AQ_WARPS * 16;
+static constexpr float AQ_RISE = 8.f, AQ_P = 128.f;                   // bits a maximum may lag; probabilities are held times this (2^8 * 128 < 65504)
+
+struct AttnQ8P {
+    KvQ8 c; RaggedB b;
+    int xtype; const void * q; int64_t q_stride; int n_head, group;
+    float scale_log2; void * out; int64_t out_stride;
+    int split, n_splits, row_tiles;                                   // slots of a split (a multiple of AQ_STEP), splits, tiles of rows of a sequence and KV head
+    float * part; float2 * part_ml; float * lse;                      // [item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
+};
+
+// rows of the tile, as (token, head): row r of the group's tokens is token r / group, head r % group
+struct TileB { int n_rows, first, seen; };                            // rows there are, first row's number, slots that the last row sees (0: none)
+
+__device__ __forceinline__ int aq_sees(const SeqB & s, int n_ctx, int tok) {          // slots that token tok sees
+    const int slot = s.pos + tok;
+    return s.sq < 0 || slot >= n_ctx ? 0 : slot + 1;
+}
+__device__ __forceinline__ TileB aq_tile(const SeqB & s, int n_ctx, int group, int rt, int R) {
+    TileB t;
+    t.first = rt * R;
+    t.n_rows = min(R, s.n_new * group - t.first);
+    t.seen = 0;
+    if (t.n_rows > 0 && s.sq >= 0) {                                  // the last of its rows whose slot there is
+        const int last = min((t.first + t.n_rows - 1) / group, n_ctx - 1 - s.pos);
+        if (last >= t.first / group) t.seen = s.pos + last + 1;
+    }
+    return t;
+}
+__device__ __forceinline__ void aq_put(int xtype, void * out, size_t at, float v) {
+    if (xtype == PI_TYPE_F16) ((__half *)out)[at] = __float2half_rn(v); else ((float *)out)[at] = v;
+}
+// four values of a query row from column d
+__device__ __forceinline__ float4 aq_query(int xtype, const void * q, size_t at) {
+    if (xtype == PI_TYPE_F16) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>((const __half *)q + at));
+        const float2 a = h2f(u.x), b = h2f(u.y);
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    return __ldg(reinterpret_cast<const float4 *>((const float *)q + at));
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+// x, y as the sum of two pairs of halves
+__device__ __forceinline__ void aq_split(float x, float y, uint32_t & hi, uint32_t & lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = h2u(h);
+    lo = h2u(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+template <int HD> struct AqShape {
+    static constexpr int KW = HD % 64 == 0 ? 16 : 8, KG = HD / (4 * KW);                   // codes a lane takes of a key row at once, and how often
+    static constexpr int VW = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : 4, VG = HD / (8 * VW);
+    static constexpr int KS = HD / 16, NT = HD / 8;
+    // 16-byte pieces of a slot's row, permuted so that the lanes that load together meet all banks
+    static __device__ __forceinline__ int k_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ ((row & 1) << 6) : byte); }
+    static __device__ __forceinline__ int v_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ (((row >> 1) & 3) << 5) : byte); }
+    static constexpr int STAGES = HD <= 128 ? 4 : 3, STAGE = 2 * 16 * HD;
+    static constexpr size_t ring() { return (size_t)AQ_WARPS * STAGES * STAGE; }
+    static constexpr size_t smem(int mt) {
+        const size_t sums = (size_t)AQ_WARPS * 8 * mt * (HD + 4) * 4;
+        return ring() > sums ? ring() : sums;
+    }
+};
+
+template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], const unsigned char * p) {
+    if constexpr (W == 16)     { const uint4 u = *reinterpret_cast<const uint4 *>(p); r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w; }
+    else if constexpr (W == 8) { const uint2 u = *reinterpret_cast<const uint2 *>(p); r[0] = u.x; r[1] = u.y; }
+    else                       r[0] = *reinterpret_cast<const uint32_t *>(p);
+}
+
+// The query rows of a tile as A operands, scaled; e: by which power of two the scores have to be multiplied.  Lane (g, q) holds row g (upper
+// parts) and row g + 8 (lower parts) of every 4 of its 16 columns.
+template <int HD>
+__device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[HD / 16][4]) {
+    using S = AqShape<HD>;
+    float4 x[S::KS];
+    float m = 0.f;
+    const size_t at = there ? (size_t)(s.first + row / p.group) * p.q_stride + (size_t)(hk * p.group + row % p.group) * HD : 0;
+#pragma unroll
+    for (int c = 0; c < S::KG; c++)
+#pragma unroll
+        for (int w = 0; w < S::KW / 4; w++) {
+            float4 & v = x[c * (S::KW / 4) + w];
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there) v = aq_query(p.xtype, p.q, at + c * 4 * S::KW + q * S::KW + w * 4);
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25 (what is not finite stays that: the row's scores are)
+    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;
+    const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < S::KS; i++) {
+        aq_split(x[i].x * up, x[i].y * up, a[i][0], a[i][1]);
+        aq_split(x[i].z * up, x[i].w * up, a[i][2], a[i][3]);
+    }
+    return down;
+}
+
+template <int HD, int MT>
+__global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
+    using S = AqShape<HD>;
+    constexpr int R = 8 * MT, ST = S::STAGES;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int split = blockIdx.x % p.n_splits, item = blockIdx.x / p.n_splits, rt = item % p.row_tiles, hk = item / p.row_tiles;
+    pdl_launch();
+    pdl_wait();
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
+    if (t.n_rows <= 0) return;
+    const int k0 = split * p.split, k1 = split == p.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
+    if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
+
+    const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
+    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
+    const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
+    unsigned char * ring = smem + (size_t)warp * ST * S::STAGE;
+    const int first = k0 + warp * 16, steps = first < k1 ? (k1 - first + AQ_STEP - 1) / AQ_STEP : 0;
+    auto issue = [&](int it) {
+        if (it < steps) {
+            const size_t from = (size_t)(first + it * AQ_STEP) * HD;  // (16 slots from a multiple of 16: inside the cache)
+            const uint32_t to = smem_u32(ring + (it % ST) * S::STAGE);
+#pragma unroll
+            for (int u = 0; u < HD / 32; u++) {
+                const int b = (u * 32 + lane) * 16, row = b / HD, byte = b % HD;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + S::k_at(row, byte)), "l"(kc + from + b) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + 16 * HD + S::v_at(row, byte)), "l"(vc + from + b) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int it = 0; it < ST - 1; it++) issue(it);
+
+    uint32_t a[MT][S::KS][4];
+    float f[MT], m[MT], l[MT]; int sees[MT], least = 0x7fffffff;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const int row = mt * 8 + g;
+        const bool there = row < t.n_rows;
+        f[mt] = aq_load_query<HD>(p, s, t.first + row, there, hk, q, a[mt]) * p.scale_log2;
+        sees[mt] = there ? aq_sees(s, p.c.n_ctx, (t.first + row) / p.group) : 0;
+        if (there) least = min(least, sees[mt]);
+        m[mt] = -INFINITY; l[mt] = 0.f;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    float o[MT][S::NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int n = 0; n < S::NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[mt][n][j] = 0.f;
+    float v_ref = 0.f, v_inv = 0.f;                                   // scale of the value sums, and AQ_P over it
+
+    for (int it = 0; it < steps; it++) {
+        asm volatile("cp.async.wait_group %0;" :: "n"(ST - 2) : "memory");
+        __syncwarp();                                                 // the stage is there for all lanes, and all have read the last one
+        issue(it + ST - 1);                                           // (into which this goes)
+        const unsigned char * kt = ring + (it % ST) * S::STAGE, * vt = kt + 16 * HD;
+        const int j0 = first + it * AQ_STEP;
+        const float sk = __ldg(ks + (j0 >> p.c.shift)), sv = __ldg(vs + (j0 >> p.c.shift));
+
+        // ---- scores of 16 slots
+        float x[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[mt][n][j] = 0.f;
+#pragma unroll
+        for (int c = 0; c < S::KG; c++) {
+            uint32_t w[2][S::KW / 4];
+#pragma unroll
+            for (int n = 0; n < 2; n++) aq_lds<S::KW>(w[n], kt + S::k_at(n * 8 + g, c * 4 * S::KW + q * S::KW));
+#pragma unroll
+            for (int i = 0; i < S::KW / 4; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const uint32_t u = w[n][i] ^ 0x80808080u, b0 = q8_lo(u), b1 = q8_hi(u);
+                    const int k = c * (S::KW / 4) + i;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) mma16816(x[mt][n], a[mt][k][0], a[mt][k][1], a[mt][k][2], a[mt][k][3], b0, b1);
+                }
+        }
+        // ---- probabilities, as A operands of the value products
+        float ratio = 1.f;
+        if (sv > v_ref) { ratio = v_ref / sv; v_ref = sv; v_inv = AQ_P / sv; }
+        const float pv = sv == 0.f ? 0.f : sv * v_inv;
+        uint32_t pa[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            float y[2][2];
+            const float fk = f[mt] * sk;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) y[n][j] = (x[mt][n][j] + x[mt][n][j + 2]) * fk;
+            if (j0 + 16 > least) {
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j >= sees[mt]) y[n][j] = -INFINITY;
+            }
+            float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
+            float down = ratio;
+            if (__any_sync(0xffffffffu, top > m[mt] + AQ_RISE)) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float now = fmaxf(m[mt], top), alpha = now == m[mt] ? 1.f : exp2_approx(m[mt] - now);
+                m[mt] = now;
+                l[mt] *= alpha;
+                down *= alpha;
+            }
+            if (__any_sync(0xffffffffu, down != 1.f)) {
+#pragma unroll
+                for (int n = 0; n < S::NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[mt][n][j] *= down;
+            }
+            const float ref = m[mt] == -INFINITY ? 0.f : m[mt];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float p0 = exp2_approx(y[n][0] - ref), p1 = exp2_approx(y[n][1] - ref);
+                l[mt] += p0 + p1;
+                // (a masked slot counts nothing whatever its block's scale is)
+                aq_split(p0 == 0.f ? 0.f : p0 * pv, p1 == 0.f ? 0.f : p1 * pv, pa[mt][2 * n], pa[mt][2 * n + 1]);
+            }
+        }
+        // ---- values: the lane's slots are 2q, 2q + 1, 8 + 2q, 9 + 2q
+#pragma unroll
+        for (int c = 0; c < S::VG; c++) {
+            uint32_t w[4][S::VW / 4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) aq_lds<S::VW>(w[r], vt + S::v_at((r >> 1) * 8 + 2 * q + (r & 1), c * 8 * S::VW + g * S::VW));
+#pragma unroll
+            for (int i = 0; i < S::VW / 4; i++) {
+                const uint32_t lo0 = __byte_perm(w[0][i], w[1][i], 0x5140) ^ 0x80808080u, hi0 = __byte_perm(w[0][i], w[1][i], 0x7362) ^ 0x80808080u;
+                const uint32_t lo1 = __byte_perm(w[2][i], w[3][i], 0x5140) ^ 0x80808080u, hi1 = __byte_perm(w[2][i], w[3][i], 0x7362) ^ 0x80808080u;
+                const uint32_t b[4][2] = {{q8_lo(lo0), q8_lo(lo1)}, {q8_hi(lo0), q8_hi(lo1)}, {q8_lo(hi0), q8_lo(hi1)}, {q8_hi(hi0), q8_hi(hi1)}};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) mma16816(o[mt][c * S::VW + i * 4 + j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b[j][0], b[j][1]);
+            }
+        }
+    }
+
+    // ---- the four warps' sums together
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    constexpr int PITCH = HD + 4;
+    float * so = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        float sum = l[mt];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; }
+        float * row = so + (size_t)(warp * R + mt * 8 + g) * PITCH;
+        const float back = v_ref * (1.f / AQ_P);
+#pragma unroll
+        for (int c = 0; c < S::VG; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)                               // columns 2q and 2q + 1 of the tiles: VW contiguous dimensions each
+#pragma unroll
+                for (int j = 0; j < S::VW; j += 4) {
+                    float4 v;
+                    v.x = (o[mt][c * S::VW + j][h] + o[mt][c * S::VW + j][h + 2]) * back;
+                    v.y = (o[mt][c * S::VW + j + 1][h] + o[mt][c * S::VW + j + 1][h + 2]) * back;
+                    v.z = (o[mt][c * S::VW + j + 2][h] + o[mt][c * S::VW + j + 2][h + 2]) * back;
+                    v.w = (o[mt][c * S::VW + j + 3][h] + o[mt][c * S::VW + j + 3][h + 2]) * back;
+                    *reinterpret_cast<float4 *>(row + c * 8 * S::VW + (2 * q + h) * S::VW + j) = v;
+                }
+    }
+    __syncthreads();
+    const size_t part0 = (((size_t)blockIdx.y * p.c.H * p.row_tiles + item) * p.n_splits + split) * R;
+    for (int e = threadIdx.x; e < t.n_rows * (HD / 4); e += AQ_THREADS) {
+        const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+        float top = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < AQ_WARPS; w++) top = fmaxf(top, s_m[w][r]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < AQ_WARPS; w++) {
+            const float k = exp2_approx(s_m[w][r] - ref);
+            const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * R + r) * PITCH + d);
+            sum = fmaf(k, s_l[w][r], sum);
+            v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);
+        }
+        if (p.n_splits > 1) {
+            *reinterpret_cast<float4 *>(p.part + (part0 + r) * HD + d) = v;
+            if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
+        } else {
+            const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const size_t at = (size_t)tok * p.out_stride + (size_t)h * HD + d;
+            aq_put(p.xtype, p.out, at, v.x * inv); aq_put(p.xtype, p.out, at + 1, v.y * inv);
+            aq_put(p.xtype, p.out, at + 2, v.z * inv); aq_put(p.xtype, p.out, at + 3, v.w * inv);
+            if (d == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
+        }
+    }
+}
+
+// The splits of a tile joined, in their order
+__global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
+    const int hd = p.c.hd, rt = blockIdx.x % p.row_tiles, hk = blockIdx.x / p.row_tiles;
+    pdl_launch();
+    pdl_wait();
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
+    if (t.n_rows <= 0) return;
+    const int used = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));
+    const size_t part0 = ((size_t)blockIdx.y * p.c.H * p.row_tiles + blockIdx.x) * p.n_splits * R;
+    for (int e = threadIdx.x; e < t.n_rows * (hd / 4); e += 256) {
+        const int r = e / (hd / 4), d = (e - r * (hd / 4)) * 4;
+        float top = -INFINITY;
+        for (int k = 0; k < used; k++) top = fmaxf(top, __ldcg(&p.part_ml[part0 + (size_t)k * R + r]).x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < used; k++) {
+            const size_t at = part0 + (size_t)k * R + r;
+            const float2 ml = __ldcg(&p.part_ml[at]);
+            const float4 u = __ldcg(reinterpret_cast<const float4 *>(p.part + at * hd + d));
+            const float w = exp2_approx(ml.x - ref);
+            sum = fmaf(w, ml.y, sum);
+            v.x = fmaf(w, u.x, v.x); v.y = fmaf(w, u.y, v.y); v.z = fmaf(w, u.z, v.z); v.w = fmaf(w, u.w, v.w);
+        }
+        const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const size_t at = (size_t)tok * p.out_stride + (size_t)h * hd + d;
+        aq_put(p.xtype, p.out, at, v.x * inv); aq_put(p.xtype, p.out, at + 1, v.y * inv);
+        aq_put(p.xtype, p.out, at + 2, v.z * inv); aq_put(p.xtype, p.out, at + 3, v.w * inv);
+        if (d == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
+    }
+}
+
+// weights_out[j] = (j < pos0 ? weights_in[j] : 0) + sum over the sequence's new tokens and the heads of the group of p_j.  A warp keeps 16 slots as
+// B operands, goes over the rows and makes their scores again (the keys a second time, instead of every score written and read).
+// One warp owns a slot: the sum's order is fixed.
+template <int HD>
+__global__ void __launch_bounds__(AQ_THREADS) k_attn_q8_weights(const AttnQ8P p, const float * w_in, float * w_out) {
+    using S = AqShape<HD>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, hk = blockIdx.y, i = blockIdx.z;
+    pdl_launch();
+    pdl_wait();
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, i);
+    if (s.sq < 0 || s.n_new == 0) return;
+    if (p.b.seq) {                                                    // of entries that name one sequence the last one counts
+        bool later = false;
+        for (int j = i + 1 + lane; j < p.b.n; j += 32) {
+            const SeqB o = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, j);
+            later |= o.sq == s.sq && o.n_new > 0;
+        }
+        if (__any_sync(0xffffffffu, later)) return;
+    }
+    const size_t head = (size_t)s.sq * p.c.H + hk;
+    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD;
+    const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift);
+    const int end = min(s.pos + s.n_new, p.c.n_ctx), n_rows = s.n_new * p.group;
+    for (int j0 = (blockIdx.x * AQ_WARPS + warp) * 16; j0 < end; j0 += gridDim.x * AQ_STEP) {
+        uint32_t b[2][S::KS][2];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int c = 0; c < S::KG; c++)
+#pragma unroll
+                for (int w = 0; w < S::KW / 4; w++) {
+                    const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(kc + (size_t)(j0 + n * 8 + g) * HD + c * 4 * S::KW + q * S::KW + w * 4)) ^ 0x80808080u;
+                    b[n][c * (S::KW / 4) + w][0] = q8_lo(u);
+                    b[n][c * (S::KW / 4) + w][1] = q8_hi(u);
+                }
+        const float sk = __ldg(ks + (j0 >> p.c.shift));
+        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        const int tok0 = max(0, j0 - s.pos);                          // the first token that sees one of these slots
+        for (int r0 = tok0 * p.group / 8 * 8; r0 < n_rows; r0 += 8) {
+            const int row = r0 + g;
+            const bool there = row < n_rows;
+            uint32_t a[S::KS][4];
+            const float f = aq_load_query<HD>(p, s, row, there, hk, q, a) * p.scale_log2 * sk;
+            const int tok = row / p.group, sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
+            const float lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row % p.group) : 0.f;
+            float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int k = 0; k < S::KS; k++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) mma16816(x[n], a[k][0], a[k][1], a[k][2], a[k][3], b[n][k][0], b[n][k][1]);
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx((x[n][j] + x[n][j + 2]) * f - lse);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], o);
+                const int slot = j0 + n * 8 + 2 * q + j;
+                const size_t at = head * p.c.n_ctx + slot;
+                if (g == 0 && slot < end) w_out[at] = (w_in && slot < s.pos ? w_in[at] : 0.f) + sum[n][j];
+            }
+    }
+}
+
+// ---- how the work is cut
+struct AqPlan { int mt, row_tiles, split, n_splits; size_t lse, ml, part; };           // bytes of each piece of scratch
+
+static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
+    AqPlan r;
+    const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
+    r.mt = rows <= 8 || c.hd > 128 ? 1 : 2;
+    const int R = 8 * r.mt;
+    r.row_tiles = (int)((rows + R - 1) / R);
+    const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
+    const int64_t slots = (int64_t)sm_count() * 2, most = (keys + 255) / 256;
+    int64_t n = (slots + items - 1) / items;
+    if (items >= slots) n = 1;
+    if (n > most) n = most;
+    if (n > 128) n = 128;
+    const int64_t per = ((keys + n - 1) / n + AQ_STEP - 1) / AQ_STEP * AQ_STEP;
+    r.split = (int)per; r.n_splits = (int)((keys + per - 1) / per);
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    r.lse = weights ? up((size_t)b.T * n_head * 4) : 0;
+    r.ml = r.n_splits > 1 ? up((size_t)items * r.n_splits * R * 8) : 0;
+    r.part = r.n_splits > 1 ? up((size_t)items * r.n_splits * R * c.hd * 4) : 0;
+    return r;
+}
+
+size_t attn_q8_scratch(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
+    const AqPlan r = aq_plan(c, b, n_head, max_kv, weights);
+    return r.lse + r.ml + r.part;
+}
+
+template <int HD, int MT>
+static int aq_go(const AttnQ8P & p, cudaStream_t st) {
+    static bool done[16] = {false};
+    int dev = 0;
+    PI_CUDA(cudaGetDevice(&dev));
+    constexpr size_t smem = AqShape<HD>::smem(MT);
+    if (dev < 0 || dev >= 16 || !done[dev]) {
+        PI_CUDA(cudaFuncSetAttribute(k_attn_q8<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 16) done[dev] = true;
+    }
+    PI_CUDA(launch_k(k_attn_q8<HD, MT>, dim3((unsigned)((int64_t)p.c.H * p.row_tiles * p.n_splits), p.b.n), dim3(AQ_THREADS), smem, st, true, p));
+    return PI_OK;
+}
+
+template <int HD>
+static int aq_run(const AttnQ8P & p, int mt, const float * w_in, float * w_out, int max_kv, cudaStream_t st) {
+    int rc;
+    if constexpr (HD <= 128) rc = mt == 1 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
+    else                     rc = aq_go<HD, 1>(p, st);
+    if (rc) return rc;
+    if (p.n_splits > 1) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.c.H * p.row_tiles, p.b.n), dim3(256), 0, st, true, p, 8 * mt));
+    if (w_out) {
+        const int keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv;
+        PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((keys + AQ_STEP - 1) / AQ_STEP, p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));
+    }
+    return PI_OK;
+}
+
+int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
+    const AqPlan r = aq_plan(a.c, a.b, a.n_head, a.max_kv, a.w_out != nullptr);
+    AttnQ8P p;
+    p.c = a.c; p.b = a.b; p.xtype = a.xtype; p.q = a.q; p.q_stride = a.q_stride; p.n_head = a.n_head; p.group = a.n_head / a.c.H;
+    p.scale_log2 = a.scale * 1.44269504088896340736f; p.out = a.out; p.out_stride = a.out_stride;
+    p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles;
+    char * s = (char *)a.scratch;
+    p.lse = a.w_out ? (float *)s : nullptr;
+    p.part_ml = (float2 *)(s + r.lse); p.part = (float *)(s + r.lse + r.ml);
+    switch (a.c.hd) {
+        case 64:  return aq_run<64>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+        case 96:  return aq_run<96>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+        case 128: return aq_run<128>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+        case 192: return aq_run<192>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+        default:  return aq_run<256>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+    }
+}
+
+}  // namespace pi

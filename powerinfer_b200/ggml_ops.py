@@ -11,13 +11,15 @@ ggml_cuda_transform_tensor): F16 rows, or Q4_0 blocks re-laid out for aligned 12
 """
 from __future__ import annotations
 
+import ctypes as C
 import dataclasses
+import math
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import PI_TYPE_F16, PI_TYPE_Q4_0, check, lib
+from ._lib import PI_TYPE_F16, PI_TYPE_F32, PI_TYPE_Q4_0, check, lib
 
 sparse_pred_threshold = 0.0        # ggml.h:2219 `extern float sparse_pred_threshold`
 
@@ -251,3 +253,180 @@ def attention_decode(q, k, v, k_cache, v_cache, pos, n_head, n_head_kv, seq=None
     check(lib.pi_attention_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                   _p(seq), pos.data_ptr(), T, n_head, n_head_kv, hd, k_cache.shape[1], out.data_ptr(), _stream()))
     return out
+
+
+# ---- a long context: scaled rotary positions, a KV cache in 8 bits, its attention and eviction.
+# Rows are float32 or float16 and may be columns of a wider matrix (q, k and v as one projection leaves them); results are new tensors.
+# Scratch and results come from torch's allocator at every call, so calls on several streams and captured graphs share none.
+
+_ROW_TYPES = {torch.float32: PI_TYPE_F32, torch.float16: PI_TYPE_F16}
+
+
+def _here(*tensors):
+    device = torch.cuda.current_device() if _raw_device is None else _raw_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{device}")
+
+
+def _row_matrix(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
+    """t [T, width] (or [T, heads, head_dim]) as rows that the kernels take: 16-byte aligned, values of a row side by side"""
+    if t.dim() == 3:
+        t = t.flatten(1)
+    if t.dim() != 2 or t.shape[1] != width:
+        raise ValueError(f"{what} is {list(t.shape)}: rows of {width} values are needed")
+    if t.dtype not in _ROW_TYPES:
+        raise ValueError(f"{what} is {t.dtype}: float32 or float16 is needed")
+    step, side = t.stride()
+    if side != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (step < width or step * t.element_size() % 16)):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _row_step(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _ints(t: torch.Tensor | None, n: int, what: str):
+    if t is not None and (t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n}")
+    return _p(t)
+
+
+@dataclasses.dataclass(frozen=True)
+class RopeFreqs:
+    freqs: torch.Tensor            # float64 [n_rot / 2] on the device: angle per position of each pair
+    mscale: float = 1.0            # factor of the rotated values
+
+
+def rope_freqs(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0, n_orig_ctx: int = 0, freq_factors=None) -> RopeFreqs:
+    """The parameters of ggml_rope_custom (ggml.h:1266-1283) as frequencies: made once, like rope_table."""
+    host, mscale = np.empty(max(0, n_rot) // 2, np.float64), C.c_float(1.0)
+    factors = None if freq_factors is None else np.ascontiguousarray(freq_factors, np.float32)
+    if factors is not None and factors.shape != host.shape:
+        raise ValueError(f"freq_factors must be {host.shape[0]} values")
+    check(lib.pi_rope_freqs_host(host.ctypes.data, C.addressof(mscale), n_rot, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow,
+                                 n_orig_ctx, None if factors is None else factors.ctypes.data))
+    return RopeFreqs(torch.from_numpy(host).cuda(), mscale.value)
+
+
+def rope_ext(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, freqs: RopeFreqs, head_dim: int, mode: int = 0, inplace: bool = False):
+    """Queries [T, n_head * head_dim] and keys [T, n_head_kv * head_dim] rotated to pos int32 [T]; mode 0 (pairs (2i, 2i+1)) or 2 (neox).  The first
+    2 * len(freqs) dimensions of each head turn.  Returns (q, k), new tensors, or the same ones with inplace."""
+    T = q.shape[0]
+    x = [t if t is None else _row_matrix(t, t.shape[1] if t.dim() == 2 else t.shape[1] * t.shape[2], "q / k") for t in (q, k)]
+    for t in x:
+        if t is not None and (t.shape[0] != T or t.shape[1] % head_dim or t.dtype is not x[0].dtype):
+            raise ValueError(f"q and k must be of one type, {T} rows of heads of {head_dim}")
+    if freqs.freqs.dtype is not torch.float64 or not freqs.freqs.is_contiguous():
+        raise ValueError("frequencies must be contiguous float64")
+    if inplace and any(t is not None and t.data_ptr() != o.data_ptr() for t, o in zip(x, (q, k))):
+        raise ValueError("in place needs rows that are 16-byte aligned")
+    y = x if inplace else [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in x]
+    _here(x[0], x[1], pos, freqs.freqs)
+    keys = (None, 0, 0, None, 0) if k is None else (x[1].data_ptr(), _row_step(x[1]), x[1].shape[1] // head_dim, y[1].data_ptr(), _row_step(y[1]))
+    check(lib.pi_rope_ext(_ROW_TYPES[x[0].dtype], x[0].data_ptr(), _row_step(x[0]), x[0].shape[1] // head_dim, y[0].data_ptr(), _row_step(y[0]), *keys,
+                          T, head_dim, 2 * freqs.freqs.numel(), 1 if mode & 2 else 0, _ints(pos, T, "pos"), freqs.freqs.data_ptr(), freqs.mscale, _stream()))
+    return (q, k) if inplace else (y[0], y[1])
+
+
+class KvCacheQ8:
+    """A KV cache in 8 bits: codes int8 [n_seq, n_head_kv, n_ctx, head_dim], scales float32 [n_seq, n_head_kv, n_ctx / block]."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "c", "at")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        n_seq, n_head_kv, n_ctx, head_dim = k.shape
+        blocks = k_scale.shape[2]
+        if k.dtype is not torch.int8 or v.dtype is not torch.int8 or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
+            raise ValueError("codes are int8, scales float32")
+        if v.shape != k.shape or k_scale.shape != v_scale.shape or k_scale.shape[:2] != k.shape[:2] or blocks == 0 or n_ctx % blocks:
+            raise ValueError("codes [n_seq, n_head_kv, n_ctx, head_dim] and scales [n_seq, n_head_kv, n_ctx / block] do not fit each other")
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise ValueError("the caches must be contiguous")
+        _here(k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = _lib.KvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_seq, n_head_kv, n_ctx, head_dim, n_ctx // blocks)
+        self.at = C.addressof(self.c)
+
+    @classmethod
+    def empty(cls, n_seq: int, n_ctx: int, n_head_kv: int, head_dim: int, block: int = 64) -> "KvCacheQ8":
+        codes = [torch.zeros(n_seq, n_head_kv, n_ctx, head_dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+        return cls(*codes, *(torch.zeros(n_seq, n_head_kv, n_ctx // block, device="cuda") for _ in range(2)))
+
+
+def _batch(q_start, pos0, seq, T, max_new):
+    n = pos0.numel()
+    return _lib.KvBatch(_ints(q_start, n + 1, "q_start"), _ints(seq, n, "seq"), _ints(pos0, n, "pos0"), n, T, T if max_new is None else max_new)
+
+
+def kv_store_q8(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None,
+                max_new: int | None = None) -> None:
+    """k, v [T, n_head_kv * head_dim] into the cache: rows q_start[i] .. q_start[i + 1] to the slots pos0[i] and on of sequence seq[i] (None: i); at
+    most max_new rows of an entry (None: T)."""
+    c, T = cache.c, k.shape[0]
+    k, v = _row_matrix(k, c.n_head_kv * c.head_dim, "k"), _row_matrix(v, c.n_head_kv * c.head_dim, "v")
+    if v.shape[0] != T or k.dtype is not v.dtype:
+        raise ValueError("k and v must have the same rows and type")
+    _here(cache.k, k, v, q_start, pos0, seq)
+    b = _batch(q_start, pos0, seq, T, max_new)
+    check(lib.pi_kv_store_q8(cache.at, C.addressof(b), _ROW_TYPES[k.dtype], k.data_ptr(), _row_step(k), v.data_ptr(), _row_step(v), _stream()))
+
+
+def kv_load_q8(cache: KvCacheQ8, q_start: torch.Tensor, pos0: torch.Tensor, T: int, seq: torch.Tensor | None = None, max_new: int | None = None,
+               dtype: torch.dtype = torch.float32):
+    """The values of the slots that kv_store_q8 with the same batch writes: k, v [T, n_head_kv * head_dim] (rows of no entry hold anything)."""
+    c = cache.c
+    if dtype not in _ROW_TYPES:
+        raise ValueError("values are read as float32 or float16")
+    k, v = (torch.empty(T, c.n_head_kv * c.head_dim, dtype=dtype, device=cache.k.device) for _ in range(2))
+    _here(cache.k, q_start, pos0, seq)
+    b = _batch(q_start, pos0, seq, T, max_new)
+    check(lib.pi_kv_load_q8(cache.at, C.addressof(b), _ROW_TYPES[dtype], k.data_ptr(), _row_step(k), v.data_ptr(), _row_step(v), _stream()))
+    return k, v
+
+
+def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None, max_new: int | None = None,
+                 max_kv: int | None = None, scale: float | None = None, weights_in: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """The KQV block over the 8-bit cache, the batch's own keys and values stored before: q [T, n_head * head_dim] -> the same shape and type.  Token t
+    of entry i sees the slots up to pos0[i] + t.  max_kv: slots that the longest sequence sees (None: all).  weights_out float32 [n_seq,
+    n_head_kv, n_ctx] takes each seen slot's probabilities, plus weights_in for slots before pos0.  Rows of no entry are left as `out` has them."""
+    c = cache.c
+    if q.shape[-1] % c.head_dim:
+        raise ValueError(f"q is {list(q.shape)}: heads of {c.head_dim} are needed")
+    q = _row_matrix(q, q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2], "q")
+    T, n_head = q.shape[0], q.shape[1] // c.head_dim
+    if out is None:
+        out = torch.empty(T, q.shape[1], dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and type")
+    for w in (weights_in, weights_out):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != cache.k.shape[:3] or not w.is_contiguous()):
+            raise ValueError("weights are contiguous float32 [n_seq, n_head_kv, n_ctx]")
+    _here(cache.k, q, out, q_start, pos0, seq, weights_in, weights_out)
+    b = _batch(q_start, pos0, seq, T, max_new)
+    most = c.n_ctx if max_kv is None else max_kv
+    need = lib.pi_attention_q8_workspace_bytes(cache.at, C.addressof(b), n_head, most, 0 if weights_out is None else 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(lib.pi_attention_q8(cache.at, C.addressof(b), _ROW_TYPES[q.dtype], q.data_ptr(), _row_step(q), n_head, most,
+                              1.0 / math.sqrt(c.head_dim) if scale is None else scale, out.data_ptr(), _row_step(out), _p(weights_in), _p(weights_out),
+                              _p(ws), need, _stream()))
+    return out
+
+
+def kv_evict_q8(cache: KvCacheQ8, weights: torch.Tensor, lens: torch.Tensor, keep: int, n_sink: int = 4, n_recent: int = 0, seq: torch.Tensor | None = None,
+                weights_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sequences of lens[i] slots cut to `keep` by their accumulated weights (float32 [n_seq, n_head_kv, n_ctx], as attention_q8 leaves them): the first
+    n_sink slots, the last n_recent and the heaviest others stay, for every KV head its own.  Returns the slot that each kept row came from,
+    int32 [n, n_head_kv, keep] (-1: none); weights_out (may be `weights`) takes the weights in the new order."""
+    n, c = lens.numel(), cache.c
+    for w in (weights, weights_out):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != cache.k.shape[:3] or not w.is_contiguous()):
+            raise ValueError("weights are contiguous float32 [n_seq, n_head_kv, n_ctx]")
+    _here(cache.k, weights, weights_out, lens, seq)
+    kept = torch.empty(n, c.n_head_kv, max(0, keep), dtype=torch.int32, device=lens.device)
+    check(lib.pi_kv_evict_q8(cache.at, _ints(lens, n, "lens"), _ints(seq, n, "seq"), n, keep, n_sink, n_recent, weights.data_ptr(), _p(weights_out),
+                             kept.data_ptr(), _stream()))
+    return kept
