@@ -15,59 +15,12 @@
 // Layouts.  mma.m16n8k16 sums over 16 columns (scores) or slots (values) in any order that both operands share: a lane's piece of a key row is
 // 16 contiguous codes, of a value row hd / 8 of them, and every 4 codes are operands of one product.  The probabilities of the score tile's layout
 // are the value product's operand as they stand.  Where the maximum rises by less than 2^8, sums are not scaled anew.
-#include "pi_kv_q8.cuh"
+#include "pi_attn_q8.cuh"
 
 namespace pi {
 
 static constexpr int AQ_WARPS = 4, AQ_THREADS = AQ_WARPS * 32, AQ_STEP = AQ_WARPS * 16;
 static constexpr float AQ_RISE = 8.f, AQ_P = 128.f;                   // bits a maximum may lag; probabilities are held times this (2^8 * 128 < 65504)
-
-struct AttnQ8P {
-    KvQ8 c; RaggedB b;
-    int xtype; const void * q; int64_t q_stride; int n_head, group;
-    float scale_log2; void * out; int64_t out_stride;
-    int split, n_splits, row_tiles;                                   // slots of a split (a multiple of AQ_STEP), splits, tiles of rows of a sequence and KV head
-    float * part; float2 * part_ml; float * lse;                      // [item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
-};
-
-// rows of the tile, as (token, head): row r of the group's tokens is token r / group, head r % group
-struct TileB { int n_rows, first, seen; };                            // rows there are, first row's number, slots that the last row sees (0: none)
-
-__device__ __forceinline__ int aq_sees(const SeqB & s, int n_ctx, int tok) {          // slots that token tok sees
-    const int slot = s.pos + tok;
-    return s.sq < 0 || slot >= n_ctx ? 0 : slot + 1;
-}
-__device__ __forceinline__ TileB aq_tile(const SeqB & s, int n_ctx, int group, int rt, int R) {
-    TileB t;
-    t.first = rt * R;
-    t.n_rows = min(R, s.n_new * group - t.first);
-    t.seen = 0;
-    if (t.n_rows > 0 && s.sq >= 0) {                                  // the last of its rows whose slot there is
-        const int last = min((t.first + t.n_rows - 1) / group, n_ctx - 1 - s.pos);
-        if (last >= t.first / group) t.seen = s.pos + last + 1;
-    }
-    return t;
-}
-__device__ __forceinline__ void aq_put(int xtype, void * out, size_t at, float v) {
-    if (xtype == PI_TYPE_F16) ((__half *)out)[at] = __float2half_rn(v); else ((float *)out)[at] = v;
-}
-// four values of a query row from column d
-__device__ __forceinline__ float4 aq_query(int xtype, const void * q, size_t at) {
-    if (xtype == PI_TYPE_F16) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2 *>((const __half *)q + at));
-        const float2 a = h2f(u.x), b = h2f(u.y);
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    return __ldg(reinterpret_cast<const float4 *>((const float *)q + at));
-}
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-// x, y as the sum of two pairs of halves
-__device__ __forceinline__ void aq_split(float x, float y, uint32_t & hi, uint32_t & lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2u(h);
-    lo = h2u(__floats2half2_rn(x - f.x, y - f.y));
-}
 
 template <int HD> struct AqShape {
     static constexpr int KW = HD % 64 == 0 ? 16 : 8, KG = HD / (4 * KW);                   // codes a lane takes of a key row at once, and how often
@@ -432,32 +385,34 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8_weights(const AttnQ8P p,
 }
 
 // ---- how the work is cut
-struct AqPlan { int mt, row_tiles, split, n_splits; size_t lse, ml, part; };           // bytes of each piece of scratch
+struct AqPlan { bool tc; int R, row_tiles, split, n_splits; size_t words, lse, ml, part; };     // rows of a tile; bytes of each piece of scratch
 
 static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     AqPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
-    r.mt = rows <= 8 || c.hd > 128 ? 1 : 2;
-    const int R = 8 * r.mt;
-    r.row_tiles = (int)((rows + R - 1) / R);
+    r.tc = attn_q8_tc_takes(c.hd, rows);
+    r.R = r.tc ? AT_ROWS : rows <= 8 || c.hd > 128 ? 8 : 16;
+    r.row_tiles = (int)((rows + r.R - 1) / r.R);
+    const int step = r.tc ? AT_KEYS : AQ_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    const int64_t slots = (int64_t)sm_count() * 2, most = (keys + 255) / 256;
+    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : 2), most = (keys + 255) / 256;
     int64_t n = (slots + items - 1) / items;
     if (items >= slots) n = 1;
     if (n > most) n = most;
     if (n > 128) n = 128;
-    const int64_t per = ((keys + n - 1) / n + AQ_STEP - 1) / AQ_STEP * AQ_STEP;
+    const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;
     r.split = (int)per; r.n_splits = (int)((keys + per - 1) / per);
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    r.words = r.tc ? 256 : 0;                                         // (the status word where pi_op_status looks for it)
     r.lse = weights ? up((size_t)b.T * n_head * 4) : 0;
-    r.ml = r.n_splits > 1 ? up((size_t)items * r.n_splits * R * 8) : 0;
-    r.part = r.n_splits > 1 ? up((size_t)items * r.n_splits * R * c.hd * 4) : 0;
+    r.ml = r.n_splits > 1 ? up((size_t)items * r.n_splits * r.R * 8) : 0;
+    r.part = r.n_splits > 1 ? up((size_t)items * r.n_splits * r.R * c.hd * 4) : 0;
     return r;
 }
 
 size_t attn_q8_scratch(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     const AqPlan r = aq_plan(c, b, n_head, max_kv, weights);
-    return r.lse + r.ml + r.part;
+    return r.words + r.lse + r.ml + r.part;
 }
 
 template <int HD, int MT>
@@ -475,12 +430,13 @@ static int aq_go(const AttnQ8P & p, cudaStream_t st) {
 }
 
 template <int HD>
-static int aq_run(const AttnQ8P & p, int mt, const float * w_in, float * w_out, int max_kv, cudaStream_t st) {
+static int aq_run(const AttnQ8P & p, const AqPlan & r, const float * w_in, float * w_out, int max_kv, cudaStream_t st) {
     int rc;
-    if constexpr (HD <= 128) rc = mt == 1 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
-    else                     rc = aq_go<HD, 1>(p, st);
+    if (r.tc)                     rc = launch_attn_q8_tc(p, st);
+    else if constexpr (HD <= 128) rc = r.R == 8 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
+    else                          rc = aq_go<HD, 1>(p, st);
     if (rc) return rc;
-    if (p.n_splits > 1) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.c.H * p.row_tiles, p.b.n), dim3(256), 0, st, true, p, 8 * mt));
+    if (p.n_splits > 1) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.c.H * p.row_tiles, p.b.n), dim3(256), 0, st, true, p, r.R));
     if (w_out) {
         const int keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv;
         PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((keys + AQ_STEP - 1) / AQ_STEP, p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));
@@ -495,14 +451,16 @@ int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
     p.scale_log2 = a.scale * 1.44269504088896340736f; p.out = a.out; p.out_stride = a.out_stride;
     p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles;
     char * s = (char *)a.scratch;
+    p.status = (unsigned int *)(s + 8);
+    s += r.words;
     p.lse = a.w_out ? (float *)s : nullptr;
     p.part_ml = (float2 *)(s + r.lse); p.part = (float *)(s + r.lse + r.ml);
     switch (a.c.hd) {
-        case 64:  return aq_run<64>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
-        case 96:  return aq_run<96>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
-        case 128: return aq_run<128>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
-        case 192: return aq_run<192>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
-        default:  return aq_run<256>(p, r.mt, a.w_in, a.w_out, a.max_kv, st);
+        case 64:  return aq_run<64>(p, r, a.w_in, a.w_out, a.max_kv, st);
+        case 96:  return aq_run<96>(p, r, a.w_in, a.w_out, a.max_kv, st);
+        case 128: return aq_run<128>(p, r, a.w_in, a.w_out, a.max_kv, st);
+        case 192: return aq_run<192>(p, r, a.w_in, a.w_out, a.max_kv, st);
+        default:  return aq_run<256>(p, r, a.w_in, a.w_out, a.max_kv, st);
     }
 }
 

@@ -1,0 +1,373 @@
+// Attention over the KV cache in 8 bits for many query rows of a KV head (prompts and chunks) on tcgen05; formulas and layouts of rows as in
+// pi_attn_q8.cu.
+//
+// A CTA takes 128 query rows (the lanes) of one KV head and walks over its slots in tiles of 128.  Queries lie in tensor memory for the whole walk.
+// A tile's codes go from global memory through registers into shared memory as halves (exact), keys and values in the same
+// layout: 128-byte rows of 64 halves, K-major for the scores, MN-major for the values.  Scores S = Q K^T are made into one of two buffers in tensor
+// memory; the probabilities take their place, 32 slots a piece; sums of values O = P V of ONE tile go to a third buffer, which is
+// drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer than a tile.
+// So every tile has its own maximum (no exchange between tiles; the two score buffers are two groups of warps' own): the drain joins tiles.
+//
+// Precision.  FP32 rows: queries and probabilities as the sum of two halves each, i.e. two products in the place of one, 22 bits.  FP16 rows:
+// queries as they are, probabilities rounded to a half (2^-11 of each, beside the result's own rounding).  Values' scales ride on the probabilities, over the
+// tile's largest one; probabilities are held times 2^14.
+//
+// Warps: 0 issues the products; 4..7 and 8..11 have the even and the odd tiles' probabilities, a row a thread; 12..19 bring the tiles in and drain the sums,
+// a row and half of the columns a thread.
+#include "pi_attn_q8.cuh"
+#include "pi_tc.cuh"
+
+#include <cfloat>
+
+namespace pi {
+
+#ifndef AT_F16_P
+#define AT_F16_P true
+#endif
+static constexpr int AT_THREADS = 640;
+static constexpr int AT_REGS_M = 32, AT_REGS_S = 104, AT_REGS_D = 120; // 32 + 2 x 104 + 2 x 120 of the 5 x 96 of the launch
+static constexpr float AT_P = 16384.f;
+static constexpr uint32_t AT_SUB = AT_KEYS * 128;                     // bytes of 64 columns of a tile
+
+__device__ __forceinline__ void at_ld32(float (&v)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                   "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]) : "r"(addr));
+}
+
+// TWO_Q, TWO_P: two halves for each query, for each probability
+template <int HD, bool TWO_Q, bool TWO_P>
+__global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
+    constexpr int KS = HD / 16, SUBS = HD / 64, U = HD / 32;          // steps of 16 columns; pieces of 64 columns; chunks of 16 codes of a tile a thread
+    constexpr uint32_t TILE = SUBS * AT_SUB;
+    constexpr uint32_t T_Q = 0, T_S = HD, T_O = HD + 2 * AT_KEYS;     // tensor memory: queries (upper, lower), two buffers of scores, sums
+    static_assert(T_O + HD <= 512 && AT_REGS_M + 2 * AT_REGS_S + 2 * AT_REGS_D <= 5 * 96, "");
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ uint64_t s_kfull[2], s_vfull[2], s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_dead;
+    __shared__ float s_f[AT_ROWS];                                    // factor of a row's scores
+    __shared__ float2 s_stat[2][AT_ROWS];                             // (maximum, sum of the probabilities) of a tile
+    __shared__ float s_ref[2];                                        // largest scale of its values
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE;
+    const int split = blockIdx.x % p.n_splits, item = blockIdx.x / p.n_splits, rt = p.row_tiles - 1 - item % p.row_tiles, hk = item / p.row_tiles;
+    pdl_launch();
+    pdl_wait();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.status = 0u;
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, AT_ROWS);
+    if (t.n_rows <= 0) return;
+    const int k0 = split * p.split, k1 = split == p.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
+    if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
+    const int n_tiles = k0 < k1 ? (k1 - k0 + AT_KEYS - 1) / AT_KEYS : 0;
+    const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
+
+    if (tid < 2) {
+        mbar_init(s_kfull + tid, 8); mbar_init(s_vfull + tid, 8); mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1);
+        mbar_init(s_pfull + tid, 4); mbar_init(s_free + tid, 8);
+    }
+    if (tid == 0) { mbar_init(&s_fin, 1); s_dead = 0; }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (warp == 0) tc_alloc(&s_tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    auto wait = [&](uint64_t * bar, unsigned parity) -> bool {        // warp-uniform; false: the wait ran out, here or elsewhere
+        bool ok = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+        if (__builtin_expect(ok, 1)) return true;
+        for (int spins = 0; spins < (1 << 20) && !ok && !s_dead; spins++) ok = mbar_try_wait(bar, parity);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok && lane == 0) { s_dead = 1; atomicOr(p.status, 16u); }
+        return ok;
+    };
+
+    // ---- a tile's codes: a warp takes 8 rows x 64 columns, so that what it stores together meets all banks
+    const int ct = tid - 384, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a bringing thread
+    auto bring = [&](const int8_t * from, int tile, uint4 (&c)[U]) {
+        const int j0 = k0 + tile * AT_KEYS;
+#pragma unroll
+        for (int u = 0; u < U; u++) {                                 // (rows behind the cache: its last one; no row sees them)
+            const int r = (u & 1) * 64 + cr, sub = u >> 1;
+            c[u] = __ldg(reinterpret_cast<const uint4 *>(from + (size_t)min(j0 + r, p.c.n_ctx - 1) * HD + sub * 64 + cc * 16));
+        }
+    };
+    auto put = [&](uint32_t to, const uint4 (&c)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int r = (u & 1) * 64 + cr;
+            const uint32_t at = to + (uint32_t)(u >> 1) * AT_SUB + (uint32_t)r * 128u;
+            const uint32_t w[4] = {c[u].x ^ 0x80808080u, c[u].y ^ 0x80808080u, c[u].z ^ 0x80808080u, c[u].w ^ 0x80808080u};
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at + (uint32_t)(((2 * cc + h) ^ (r & 7)) * 16)), "r"(q8_lo(w[2 * h])), "r"(q8_hi(w[2 * h])), "r"(q8_lo(w[2 * h + 1])), "r"(q8_hi(w[2 * h + 1])) : "memory");
+        }
+    };
+    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
+    uint4 ck[U], cv[U];
+    if (warp >= 12 && n_tiles) { bring(kc, 0, ck); bring(vc, 0, cv); }
+
+    // ---- queries into tensor memory, a row a thread
+    if (warp >= 4 && warp < 8) {
+        const int r = tid - 128, row = t.first + r;
+        const bool there = r < t.n_rows;
+        const size_t at = there ? (size_t)(s.first + row / p.group) * p.q_stride + (size_t)(hk * p.group + row % p.group) * HD : 0;
+        float m = 0.f;
+        if (there)
+            for (int d = 0; d < HD; d += 4) {
+                const float4 v = aq_query(p.xtype, p.q, at + d);
+                m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            }
+        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11, as there
+        const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
+        s_f[r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
+        const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q;
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float4 v = there ? aq_query(p.xtype, p.q, at + d + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                aq_split(v.x * up, v.y * up, hi[2 * j], lo[2 * j]);
+                aq_split(v.z * up, v.w * up, hi[2 * j + 1], lo[2 * j + 1]);
+            }
+            tc_st16(to + d / 2, hi);
+            if (TWO_Q) tc_st16(to + HD / 2 + d / 2, lo);
+        }
+        tc_wait_st();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    float top = -INFINITY, sum = 0.f;                                 // of a draining thread's row
+    float acc[HD / 2];
+#pragma unroll
+    for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(AT_REGS_M));
+        if (warp == 0) {
+            // ============================================================= products
+            constexpr uint32_t idesc_v = tc_idesc(HD, true);
+            bool ok = true;
+            auto scores = [&](int i) {
+                const int b = i & 1, n = min(AT_KEYS, (k1 - k0 - i * AT_KEYS + 15) / 16 * 16);
+                ok = wait(s_kfull + b, i >> 1 & 1) && ok;
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t idesc = tc_idesc(n, false), d = tmem + T_S + (uint32_t)(b * AT_KEYS);
+                const uint64_t k = tc_desc_k(kbuf + (uint32_t)b * TILE);
+                if (TWO_Q) {
+#pragma unroll
+                    for (int j = 0; j < KS; j++) tc_mma_f16_ta(d, tmem + T_Q + HD / 2 + 8 * j, k + (j >> 2) * (AT_SUB >> 4) + 2 * (j & 3), idesc, j > 0);
+                }
+#pragma unroll
+                for (int j = 0; j < KS; j++) tc_mma_f16_ta(d, tmem + T_Q + 8 * j, k + (j >> 2) * (AT_SUB >> 4) + 2 * (j & 3), idesc, TWO_Q || j > 0);
+                tc_commit(s_qk + b);
+            };
+            if (n_tiles > 0) scores(0);
+            if (n_tiles > 1) scores(1);
+            for (int i = 0; i < n_tiles && ok; i++) {
+                const int b = i & 1, steps = min(AT_KEYS / 16, (k1 - k0 - i * AT_KEYS + 15) / 16);
+                ok = wait(s_pfull + b, i >> 1 & 1) && ok;
+                ok = wait(s_vfull + b, i >> 1 & 1) && ok;
+                if (i > 0) ok = wait(s_free + (b ^ 1), (i - 1) >> 1 & 1) && ok;
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t a = tmem + T_S + (uint32_t)(b * AT_KEYS), d = tmem + T_O;
+                const uint64_t v = tc_desc_mn(vbuf + (uint32_t)b * TILE, AT_SUB);
+                if (TWO_P)
+                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)((j >> 1) * 32 + 16 + (j & 1) * 8), v + 128 * j, idesc_v, j > 0);
+                for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)((j >> 1) * 32 + (j & 1) * 8), v + 128 * j, idesc_v, TWO_P || j > 0);
+                tc_commit(s_pv + b);
+                if (i + 2 < n_tiles) scores(i + 2);
+            }
+            tc_commit(&s_fin);                                        // nothing is in flight when tensor memory is given back
+            for (int spins = 0; spins < (1 << 20) && !mbar_try_wait(&s_fin, 0u); spins++) {}
+            __syncwarp();
+        }
+    } else if (warp < 12) {
+        // ================================================================= probabilities
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(AT_REGS_S));
+        const int b = (warp >> 2) - 1, r = (warp & 3) * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * AT_KEYS);
+        const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
+        const bool there = r < t.n_rows;
+        const int sees = there ? aq_sees(s, p.c.n_ctx, (t.first + r) / p.group) : 0;
+        const int least = __reduce_min_sync(0xffffffffu, there ? sees : 0x7fffffff);
+        const float f = s_f[r];
+        auto scales = [&](int i, float & k, float & v) {              // lane j: those of the 16 slots j of the tile (0 behind the range)
+            const int j = k0 + i * AT_KEYS + (lane & 7) * 16;
+            k = v = 0.f;
+            if (j < k1) { k = __ldg(ks + (j >> p.c.shift)); v = __ldg(vs + (j >> p.c.shift)); }
+        };
+        float sk, sv;
+        if (b < n_tiles) scales(b, sk, sv);
+        bool ok = true;
+        for (int i = b; i < n_tiles && ok; i += 2) {
+            const int j0 = k0 + i * AT_KEYS;
+            float largest = fabsf(sv) <= FLT_MAX ? sv : 0.f;          // (of the finite ones)
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            const float back = largest > 0.f ? AT_P / largest : 0.f, wv = sv == 0.f ? 0.f : sv * back, wk = sk;
+            if (i + 2 < n_tiles) scales(i + 2, sk, sv);
+            const bool masked = j0 + AT_KEYS > least;                 // (of this warp's rows)
+            ok = wait(s_qk + b, i >> 1 & 1);
+            tc_fence_after();
+            float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < AT_KEYS / 32; c++) {
+                float x[32];
+                at_ld32(x, mine + 32 * c);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float fk = f * __shfl_sync(0xffffffffu, wk, 2 * c + h);
+                    if (masked) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) if (j0 + c * 32 + h * 16 + j < sees) m = fmaxf(m, x[h * 16 + j] * fk);
+                    } else {
+                        float a = x[h * 16], e = x[h * 16 + 1];
+#pragma unroll
+                        for (int j = 2; j < 16; j += 2) { a = fmaxf(a, x[h * 16 + j]); e = fmaxf(e, x[h * 16 + j + 1]); }
+                        m = fmaxf(m, fmaxf(a, e) * fk);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int c = 0; c < AT_KEYS / 32; c++) {
+                float x[32];
+                at_ld32(x, mine + 32 * c);
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float fk = f * __shfl_sync(0xffffffffu, wk, 2 * c + h), pv = __shfl_sync(0xffffffffu, wv, 2 * c + h);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        float p0 = exp2_approx(fmaf(x[h * 16 + j], fk, -ref)), p1 = exp2_approx(fmaf(x[h * 16 + j + 1], fk, -ref));
+                        float q0, q1;
+                        if (masked) {                                 // (a masked slot counts nothing whatever its scores and its block's scales are)
+                            const int at = j0 + c * 32 + h * 16 + j;
+                            const bool s0 = at < sees, s1 = at + 1 < sees;
+                            p0 = s0 ? p0 : 0.f; p1 = s1 ? p1 : 0.f;
+                            q0 = s0 ? p0 * pv : 0.f; q1 = s1 ? p1 * pv : 0.f;
+                        } else { q0 = p0 * pv; q1 = p1 * pv; }
+                        l[j & 2] += p0; l[(j & 2) + 1] += p1;
+                        if (TWO_P) aq_split(q0, q1, hi[h * 8 + j / 2], lo[h * 8 + j / 2]);
+                        else     hi[h * 8 + j / 2] = h2u(__floats2half2_rn(q0, q1));
+                    }
+                }
+                tc_st16(mine + 32 * c, hi);
+                if (TWO_P) tc_st16(mine + 32 * c + 16, lo);
+            }
+            if (i >= 2) ok = wait(s_free + b, (i - 2) >> 1 & 1) && ok;       // the tile before has been drained: its statistics are no more needed
+            s_stat[b][r] = make_float2(m, (l[0] + l[1]) + (l[2] + l[3]));
+            if (r == 0) s_ref[b] = largest * (1.f / AT_P);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_pfull + b);
+        }
+    } else {
+        // ================================================================= tiles in, sums out
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(AT_REGS_D));
+        const int r = (warp & 3) * 32 + lane, d0 = warp >= 16 ? HD / 2 : 0;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_O + (uint32_t)d0;
+        bool ok = true;
+        auto drain = [&](int i) {
+            const int b = i & 1;
+            ok = wait(s_pfull + b, i >> 1 & 1) && ok;
+            const float2 st = s_stat[b][r];
+            const float ref = s_ref[b], now = fmaxf(top, st.x);
+            const float was = top == now ? 1.f : exp2_approx(top - now), is = st.x == -INFINITY ? 0.f : exp2_approx(st.x - now);
+            top = now;
+            sum = fmaf(sum, was, st.y * is);
+            const float k = is * ref;
+            ok = wait(s_pv + b, i >> 1 & 1) && ok;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 16) {
+                float v[16];
+                tc_ld16(v, mine + c);
+                if (c + 16 == HD / 2) {                               // the buffer goes back
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free + b);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) acc[c + j] = fmaf(v[j], k, acc[c + j] * was);
+            }
+        };
+        for (int i = 0; i < n_tiles && ok; i++) {
+            const int b = i & 1;
+            if (i >= 2) ok = wait(s_qk + b, (i - 2) >> 1 & 1) && ok;
+            put(kbuf + (uint32_t)b * TILE, ck);
+            tc_fence_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_kfull + b);
+            if (i + 1 < n_tiles) bring(kc, i + 1, ck);
+            if (i >= 2) drain(i - 2);                                 // (which waits for the value products of tile i - 2: their buffer is free)
+            put(vbuf + (uint32_t)b * TILE, cv);
+            tc_fence_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_vfull + b);
+            if (i + 1 < n_tiles) bring(vc, i + 1, cv);
+        }
+        for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);
+
+        if (r < t.n_rows) {
+            const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
+            if (!ok) sum = __int_as_float(0x7fc00000);                // a wait ran out: no numbers instead of wrong ones
+            if (p.n_splits > 1) {
+                const size_t at = (((size_t)blockIdx.y * p.c.H * p.row_tiles + (size_t)hk * p.row_tiles + rt) * p.n_splits + split) * AT_ROWS + r;
+#pragma unroll
+                for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>(p.part + at * HD + d0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const size_t at = (size_t)tok * p.out_stride + (size_t)h * HD + d0;
+                if (p.xtype == PI_TYPE_F16) {
+#pragma unroll
+                    for (int j = 0; j < HD / 2; j += 8) {
+                        uint4 u;
+                        u.x = h2u(__floats2half2_rn(acc[j] * inv, acc[j + 1] * inv)); u.y = h2u(__floats2half2_rn(acc[j + 2] * inv, acc[j + 3] * inv));
+                        u.z = h2u(__floats2half2_rn(acc[j + 4] * inv, acc[j + 5] * inv)); u.w = h2u(__floats2half2_rn(acc[j + 6] * inv, acc[j + 7] * inv));
+                        *reinterpret_cast<uint4 *>((__half *)p.out + at + j) = u;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>((float *)p.out + at + j) = make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
+                }
+                if (d0 == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tc_dealloc(tmem, 512);
+}
+
+bool attn_q8_tc_takes(int hd, int64_t rows) { return (hd == 64 || hd == 128) && rows >= 64; }
+
+template <int HD, bool TWO_Q, bool TWO_P>
+static int at_go(const AttnQ8P & p, cudaStream_t st) {
+    constexpr size_t smem = (size_t)4 * (HD / 64) * AT_SUB + 1024;
+    static bool done[16] = {false};
+    int dev = 0;
+    PI_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 16 || !done[dev]) {
+        PI_CUDA(cudaFuncSetAttribute(k_attn_q8_tc<HD, TWO_Q, TWO_P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 16) done[dev] = true;
+    }
+    PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q, TWO_P>, dim3((unsigned)((int64_t)p.c.H * p.row_tiles * p.n_splits), p.b.n), dim3(AT_THREADS), smem, st, true, p));
+    return PI_OK;
+}
+
+int launch_attn_q8_tc(const AttnQ8P & p, cudaStream_t st) {
+    if (p.c.hd == 64) return p.xtype == PI_TYPE_F16 ? at_go<64, false, AT_F16_P>(p, st) : at_go<64, true, true>(p, st);
+    return p.xtype == PI_TYPE_F16 ? at_go<128, false, AT_F16_P>(p, st) : at_go<128, true, true>(p, st);
+}
+
+}  // namespace pi
