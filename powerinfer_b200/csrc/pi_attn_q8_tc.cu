@@ -12,20 +12,21 @@
 // queries as they are, probabilities rounded to a half (2^-11 of each, beside the result's own rounding).  Values' scales ride on the probabilities, over the
 // tile's largest one; probabilities are held times 2^14.
 //
-// Warps: 0 issues the products; 4..7 and 8..11 have the even and the odd tiles' probabilities, a row a thread; 12..19 bring the tiles in and drain the sums,
-// a row and half of the columns a thread.
+// Warps: 0 issues the products; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
+// their maxima); 20..27 bring the tiles in and drain the sums, a row and half of the columns a thread.
 #include "pi_attn_q8.cuh"
 #include "pi_tc.cuh"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace pi {
 
 #ifndef AT_F16_P
 #define AT_F16_P true
 #endif
-static constexpr int AT_THREADS = 640;
-static constexpr int AT_REGS_M = 32, AT_REGS_S = 104, AT_REGS_D = 120; // 32 + 2 x 104 + 2 x 120 of the 5 x 96 of the launch
+static constexpr int AT_THREADS = 896;
+static constexpr int AT_REGS_M = 24, AT_REGS_S = 64, AT_REGS_D = 104;  // 24 + 4 x 64 + 2 x 104 of the 7 x 72 of the launch
 static constexpr float AT_P = 16384.f;
 static constexpr uint32_t AT_SUB = AT_KEYS * 128;                     // bytes of 64 columns of a tile
 
@@ -35,19 +36,50 @@ __device__ __forceinline__ void at_ld32(float (&v)[32], uint32_t addr) {
                    "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]) : "r"(addr));
 }
 
+__device__ __forceinline__ void at_st8(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// two FP32 operations in one instruction
+__device__ __forceinline__ float2 f2_fma(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 f2_mul(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 f2_add(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 f2(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+// a pair as the sum of two pairs of halves
+__device__ __forceinline__ void f2_split(float2 x, uint32_t & hi, uint32_t & lo) {
+    const __half2 h = __floats2half2_rn(x.x, x.y);
+    const float2 f = __half22float2(h), r = f2_fma(f, f2(-1.f), x);
+    hi = h2u(h);
+    lo = h2u(__floats2half2_rn(r.x, r.y));
+}
+
 // TWO_Q, TWO_P: two halves for each query, for each probability
 template <int HD, bool TWO_Q, bool TWO_P>
 __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     constexpr int KS = HD / 16, SUBS = HD / 64, U = HD / 32;          // steps of 16 columns; pieces of 64 columns; chunks of 16 codes of a tile a thread
     constexpr uint32_t TILE = SUBS * AT_SUB;
     constexpr uint32_t T_Q = 0, T_S = HD, T_O = HD + 2 * AT_KEYS;     // tensor memory: queries (upper, lower), two buffers of scores, sums
-    static_assert(T_O + HD <= 512 && AT_REGS_M + 2 * AT_REGS_S + 2 * AT_REGS_D <= 5 * 96, "");
+    static_assert(T_O + HD <= 512 && AT_REGS_M + 4 * AT_REGS_S + 2 * AT_REGS_D <= 7 * 72, "");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ uint64_t s_kfull[2], s_vfull[2], s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
+    __shared__ uint64_t s_kfull[2], s_vfull, s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_dead;
     __shared__ float s_f[AT_ROWS];                                    // factor of a row's scores
-    __shared__ float2 s_stat[2][AT_ROWS];                             // (maximum, sum of the probabilities) of a tile
+    __shared__ float s_max[2][2][AT_ROWS], s_sum[2][2][AT_ROWS];       // of a tile's halves: maximum, sum of the probabilities
+    __shared__ float s_top[2][AT_ROWS];                               // maximum of a tile
     __shared__ float s_ref[2];                                        // largest scale of its values
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE;
@@ -64,10 +96,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
 
     if (tid < 2) {
-        mbar_init(s_kfull + tid, 8); mbar_init(s_vfull + tid, 8); mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1);
-        mbar_init(s_pfull + tid, 4); mbar_init(s_free + tid, 8);
+        mbar_init(s_kfull + tid, 8); mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1);
+        mbar_init(s_pfull + tid, 8); mbar_init(s_free + tid, 8);
     }
-    if (tid == 0) { mbar_init(&s_fin, 1); s_dead = 0; }
+    if (tid == 0) { mbar_init(&s_fin, 1); mbar_init(&s_vfull, 8); s_dead = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
     tc_fence_before();
@@ -84,7 +116,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     };
 
     // ---- a tile's codes: a warp takes 8 rows x 64 columns, so that what it stores together meets all banks
-    const int ct = tid - 384, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a bringing thread
+    const int ct = tid - 640, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a bringing thread
     auto bring = [&](const int8_t * from, int tile, uint4 (&c)[U]) {
         const int j0 = k0 + tile * AT_KEYS;
 #pragma unroll
@@ -105,8 +137,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         }
     };
     const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
-    uint4 ck[U], cv[U];
-    if (warp >= 12 && n_tiles) { bring(kc, 0, ck); bring(vc, 0, cv); }
+    uint4 code[U];
+    if (warp >= 20 && n_tiles) bring(kc, 0, code);
 
     // ---- queries into tensor memory, a row a thread
     if (warp >= 4 && warp < 8) {
@@ -150,9 +182,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         if (warp == 0) {
             // ============================================================= products
             constexpr uint32_t idesc_v = tc_idesc(HD, true);
+            const int tiles = __shfl_sync(0xffffffffu, n_tiles, 0), span = __shfl_sync(0xffffffffu, k1 - k0, 0);      // (uniform for the compiler)
             bool ok = true;
             auto scores = [&](int i) {
-                const int b = i & 1, n = min(AT_KEYS, (k1 - k0 - i * AT_KEYS + 15) / 16 * 16);
+                const int b = i & 1, n = min(AT_KEYS, (span - i * AT_KEYS + 15) / 16 * 16);
                 ok = wait(s_kfull + b, i >> 1 & 1) && ok;
                 if (!ok) return;
                 tc_fence_after();
@@ -166,32 +199,33 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 for (int j = 0; j < KS; j++) tc_mma_f16_ta(d, tmem + T_Q + 8 * j, k + (j >> 2) * (AT_SUB >> 4) + 2 * (j & 3), idesc, TWO_Q || j > 0);
                 tc_commit(s_qk + b);
             };
-            if (n_tiles > 0) scores(0);
-            if (n_tiles > 1) scores(1);
-            for (int i = 0; i < n_tiles && ok; i++) {
-                const int b = i & 1, steps = min(AT_KEYS / 16, (k1 - k0 - i * AT_KEYS + 15) / 16);
+            if (tiles > 0) scores(0);
+            if (tiles > 1) scores(1);
+            for (int i = 0; i < tiles && ok; i++) {
+                const int b = i & 1, steps = min(AT_KEYS / 16, (span - i * AT_KEYS + 15) / 16);
                 ok = wait(s_pfull + b, i >> 1 & 1) && ok;
-                ok = wait(s_vfull + b, i >> 1 & 1) && ok;
-                if (i > 0) ok = wait(s_free + (b ^ 1), (i - 1) >> 1 & 1) && ok;
+                // (whoever has drained tile i - 1 has put the values of tile i there before: a wait that is over costs 150 clocks)
+                if (i == 0) ok = wait(&s_vfull, 0u) && ok;
+                else        ok = wait(s_free + (b ^ 1), (i - 1) >> 1 & 1) && ok;
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t a = tmem + T_S + (uint32_t)(b * AT_KEYS), d = tmem + T_O;
                 const uint64_t v = tc_desc_mn(vbuf + (uint32_t)b * TILE, AT_SUB);
                 if (TWO_P)
-                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)((j >> 1) * 32 + 16 + (j & 1) * 8), v + 128 * j, idesc_v, j > 0);
-                for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)((j >> 1) * 32 + (j & 1) * 8), v + 128 * j, idesc_v, TWO_P || j > 0);
+                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
+                for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
                 tc_commit(s_pv + b);
-                if (i + 2 < n_tiles) scores(i + 2);
+                if (i + 2 < tiles) scores(i + 2);
             }
             tc_commit(&s_fin);                                        // nothing is in flight when tensor memory is given back
             for (int spins = 0; spins < (1 << 20) && !mbar_try_wait(&s_fin, 0u); spins++) {}
             __syncwarp();
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ================================================================= probabilities
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(AT_REGS_S));
-        const int b = (warp >> 2) - 1, r = (warp & 3) * 32 + lane;
-        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * AT_KEYS);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(AT_REGS_S));
+        const int b = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, r = (warp & 3) * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * AT_KEYS + half * 64);
         const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
         const bool there = r < t.n_rows;
         const int sees = there ? aq_sees(s, p.c.n_ctx, (t.first + r) / p.group) : 0;
@@ -204,66 +238,69 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         };
         float sk, sv;
         if (b < n_tiles) scales(b, sk, sv);
-        bool ok = true;
-        for (int i = b; i < n_tiles && ok; i += 2) {
-            const int j0 = k0 + i * AT_KEYS;
+        for (int i = b; i < n_tiles; i += 2) {                        // (to the end whatever waits ran out: the halves meet at a barrier)
+            const int left = sees - (k0 + i * AT_KEYS + half * 64);   // slots of this half that the row sees
             float largest = fabsf(sv) <= FLT_MAX ? sv : 0.f;          // (of the finite ones)
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             const float back = largest > 0.f ? AT_P / largest : 0.f, wv = sv == 0.f ? 0.f : sv * back, wk = sk;
             if (i + 2 < n_tiles) scales(i + 2, sk, sv);
-            const bool masked = j0 + AT_KEYS > least;                 // (of this warp's rows)
-            ok = wait(s_qk + b, i >> 1 & 1);
+            const bool masked = k0 + i * AT_KEYS + half * 64 + 64 > least;       // (of this warp's rows)
+            wait(s_qk + b, i >> 1 & 1);
             tc_fence_after();
-            float m = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < AT_KEYS / 32; c++) {
+            float m = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 2; c++) {
                 float x[32];
                 at_ld32(x, mine + 32 * c);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float fk = f * __shfl_sync(0xffffffffu, wk, 2 * c + h);
+                    const float fk = f * __shfl_sync(0xffffffffu, wk, half * 4 + 2 * c + h);
+                    float * y = x + h * 16;
                     if (masked) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) if (j0 + c * 32 + h * 16 + j < sees) m = fmaxf(m, x[h * 16 + j] * fk);
-                    } else {
-                        float a = x[h * 16], e = x[h * 16 + 1];
-#pragma unroll
-                        for (int j = 2; j < 16; j += 2) { a = fmaxf(a, x[h * 16 + j]); e = fmaxf(e, x[h * 16 + j + 1]); }
-                        m = fmaxf(m, fmaxf(a, e) * fk);
+                        for (int j = 0; j < 16; j++) if (c * 32 + h * 16 + j >= left) y[j] = -INFINITY;
                     }
+                    float a = max3(y[0], y[1], y[2]), e = max3(y[3], y[4], y[5]);
+#pragma unroll
+                    for (int j = 6; j < 14; j += 4) { a = max3(a, y[j], y[j + 1]); e = max3(e, y[j + 2], y[j + 3]); }
+                    a = fmaxf(max3(a, y[14], y[15]), e);
+                    if (a > -INFINITY) m = fmaxf(m, a * fk);          // (-infinity times a factor of 0 is no number)
                 }
             }
-            const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int c = 0; c < AT_KEYS / 32; c++) {
-                float x[32];
-                at_ld32(x, mine + 32 * c);
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float fk = f * __shfl_sync(0xffffffffu, wk, 2 * c + h), pv = __shfl_sync(0xffffffffu, wv, 2 * c + h);
+            s_max[b][half][r] = m;
+            asm volatile("bar.sync %0, 256;" :: "r"(1 + b) : "memory");
+            m = fmaxf(m, s_max[b][half ^ 1][r]);
+            const float2 ref = f2(m == -INFINITY ? 0.f : -m);
+            float2 l[2] = {f2(0.f), f2(0.f)};
+            auto exps = [&](auto with_mask) {
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float x[16];
+                    tc_ld16(x, mine + 16 * c);
+                    uint32_t hl[16];                                  // upper parts of 16 slots, then lower parts
+                    const float2 fk = f2(f * __shfl_sync(0xffffffffu, wk, half * 4 + c)), pv = f2(__shfl_sync(0xffffffffu, wv, half * 4 + c));
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        float p0 = exp2_approx(fmaf(x[h * 16 + j], fk, -ref)), p1 = exp2_approx(fmaf(x[h * 16 + j + 1], fk, -ref));
-                        float q0, q1;
-                        if (masked) {                                 // (a masked slot counts nothing whatever its scores and its block's scales are)
-                            const int at = j0 + c * 32 + h * 16 + j;
-                            const bool s0 = at < sees, s1 = at + 1 < sees;
-                            p0 = s0 ? p0 : 0.f; p1 = s1 ? p1 : 0.f;
-                            q0 = s0 ? p0 * pv : 0.f; q1 = s1 ? p1 * pv : 0.f;
-                        } else { q0 = p0 * pv; q1 = p1 * pv; }
-                        l[j & 2] += p0; l[(j & 2) + 1] += p1;
-                        if (TWO_P) aq_split(q0, q1, hi[h * 8 + j / 2], lo[h * 8 + j / 2]);
-                        else     hi[h * 8 + j / 2] = h2u(__floats2half2_rn(q0, q1));
+                        const float2 y = f2_fma(make_float2(x[j], x[j + 1]), fk, ref);
+                        float2 pr = make_float2(exp2_approx(y.x), exp2_approx(y.y)), w = f2_mul(pr, pv);
+                        if (decltype(with_mask)::value) {             // (a masked slot counts nothing whatever its scores and its block's scales are)
+                            if (c * 16 + j >= left) pr.x = w.x = 0.f;
+                            if (c * 16 + j + 1 >= left) pr.y = w.y = 0.f;
+                        }
+                        l[j >> 1 & 1] = f2_add(l[j >> 1 & 1], pr);
+                        if (TWO_P) f2_split(w, hl[j / 2], hl[8 + j / 2]);
+                        else       hl[j / 2] = h2u(__floats2half2_rn(w.x, w.y));
                     }
+                    if (TWO_P) tc_st16(mine + 16 * c, hl);
+                    else       at_st8(mine + 16 * c, hl);
                 }
-                tc_st16(mine + 32 * c, hi);
-                if (TWO_P) tc_st16(mine + 32 * c + 16, lo);
-            }
-            if (i >= 2) ok = wait(s_free + b, (i - 2) >> 1 & 1) && ok;       // the tile before has been drained: its statistics are no more needed
-            s_stat[b][r] = make_float2(m, (l[0] + l[1]) + (l[2] + l[3]));
-            if (r == 0) s_ref[b] = largest * (1.f / AT_P);
+            };
+            if (masked) exps(std::true_type()); else exps(std::false_type());
+            if (i >= 2) wait(s_free + b, (i - 2) >> 1 & 1);           // the tile before has been drained: its sums are no more needed
+            s_sum[b][half][r] = (l[0].x + l[0].y) + (l[1].x + l[1].y);
+            if (half == 0) s_top[b][r] = m;
+            if (r == 0 && half == 0) s_ref[b] = largest * (1.f / AT_P);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -272,17 +309,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     } else {
         // ================================================================= tiles in, sums out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(AT_REGS_D));
-        const int r = (warp & 3) * 32 + lane, d0 = warp >= 16 ? HD / 2 : 0;
+        const int r = (warp & 3) * 32 + lane, d0 = warp >= 24 ? HD / 2 : 0;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_O + (uint32_t)d0;
         bool ok = true;
         auto drain = [&](int i) {
             const int b = i & 1;
             ok = wait(s_pfull + b, i >> 1 & 1) && ok;
-            const float2 st = s_stat[b][r];
-            const float ref = s_ref[b], now = fmaxf(top, st.x);
-            const float was = top == now ? 1.f : exp2_approx(top - now), is = st.x == -INFINITY ? 0.f : exp2_approx(st.x - now);
+            const float m = s_top[b][r], now = fmaxf(top, m);
+            const float was = top == now ? 1.f : exp2_approx(top - now), is = m == -INFINITY ? 0.f : exp2_approx(m - now);
             top = now;
-            sum = fmaf(sum, was, st.y * is);
+            sum = fmaf(sum, was, (s_sum[b][0][r] + s_sum[b][1][r]) * is);
+            const float ref = s_ref[b];
             const float k = is * ref;
             ok = wait(s_pv + b, i >> 1 & 1) && ok;
             tc_fence_after();
@@ -296,23 +333,26 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                     if (lane == 0) mbar_arrive(s_free + b);
                 }
 #pragma unroll
-                for (int j = 0; j < 16; j++) acc[c + j] = fmaf(v[j], k, acc[c + j] * was);
+                for (int j = 0; j < 16; j += 2) {
+                    const float2 o = f2_fma(make_float2(v[j], v[j + 1]), f2(k), f2_mul(make_float2(acc[c + j], acc[c + j + 1]), f2(was)));
+                    acc[c + j] = o.x; acc[c + j + 1] = o.y;
+                }
             }
         };
         for (int i = 0; i < n_tiles && ok; i++) {
             const int b = i & 1;
             if (i >= 2) ok = wait(s_qk + b, (i - 2) >> 1 & 1) && ok;
-            put(kbuf + (uint32_t)b * TILE, ck);
+            put(kbuf + (uint32_t)b * TILE, code);
             tc_fence_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(s_kfull + b);
-            if (i + 1 < n_tiles) bring(kc, i + 1, ck);
+            bring(vc, i, code);
             if (i >= 2) drain(i - 2);                                 // (which waits for the value products of tile i - 2: their buffer is free)
-            put(vbuf + (uint32_t)b * TILE, cv);
+            put(vbuf + (uint32_t)b * TILE, code);
             tc_fence_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(s_vfull + b);
-            if (i + 1 < n_tiles) bring(vc, i + 1, cv);
+            if (i == 0 && lane == 0) mbar_arrive(&s_vfull);
+            if (i + 1 < n_tiles) bring(kc, i + 1, code);
         }
         for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);
 
