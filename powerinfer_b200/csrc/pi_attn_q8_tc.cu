@@ -2,8 +2,8 @@
 // pi_attn_q8.cu.
 //
 // A CTA takes 128 query rows (the lanes) of one KV head and walks over its slots in tiles of 128.  Queries lie in tensor memory for the whole walk.
-// A tile's codes go from global memory through registers into shared memory as halves (exact), keys and values in the same
-// layout: 128-byte rows of 64 halves, K-major for the scores, MN-major for the values.  Scores S = Q K^T are made into one of two buffers in tensor
+// A tile's codes, contiguous in the cache, come as one bulk copy each of keys and values, and go through registers into shared memory as halves (exact), both in
+// the same layout: 128-byte rows of 64 halves, K-major for the scores, MN-major for the values.  Scores S = Q K^T are made into one of two buffers in tensor
 // memory; the probabilities take their place, 32 slots a piece; sums of values O = P V of ONE tile go to a third buffer, which is
 // drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer than a tile.
 // So every tile has its own maximum (no exchange between tiles; the two score buffers are two groups of warps' own): the drain joins tiles.
@@ -12,8 +12,8 @@
 // queries as they are, probabilities rounded to a half (2^-11 of each, beside the result's own rounding).  Values' scales ride on the probabilities, over the
 // tile's largest one; probabilities are held times 2^14.
 //
-// Warps: 0 issues the products; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
-// their maxima); 20..27 bring the tiles in and drain the sums, a row and half of the columns a thread.
+// Warps: 0 issues the products; 1 asks for the codes; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
+// their maxima); 20..27 make the halves and drain the sums, a row and half of the columns a thread.
 #include "pi_attn_q8.cuh"
 #include "pi_tc.cuh"
 
@@ -29,6 +29,7 @@ static constexpr int AT_THREADS = 896;
 static constexpr int AT_REGS_M = 24, AT_REGS_S = 64, AT_REGS_D = 104;  // 24 + 4 x 64 + 2 x 104 of the 7 x 72 of the launch
 static constexpr float AT_P = 16384.f;
 static constexpr uint32_t AT_SUB = AT_KEYS * 128;                     // bytes of 64 columns of a tile
+static constexpr int AT_RAW = 4;                                      // tiles of codes on their way: keys and values in turn
 
 __device__ __forceinline__ void at_ld32(float (&v)[32], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
@@ -74,6 +75,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     constexpr uint32_t T_Q = 0, T_S = HD, T_O = HD + 2 * AT_KEYS;     // tensor memory: queries (upper, lower), two buffers of scores, sums
     static_assert(T_O + HD <= 512 && AT_REGS_M + 4 * AT_REGS_S + 2 * AT_REGS_D <= 7 * 72, "");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ uint64_t s_rfull[AT_RAW], s_rempty[AT_RAW];
     __shared__ uint64_t s_kfull[2], s_vfull, s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_dead;
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     __shared__ float s_top[2][AT_ROWS];                               // maximum of a tile
     __shared__ float s_ref[2];                                        // largest scale of its values
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE;
+    const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE, raw = vbuf + 2 * TILE;
     const int split = blockIdx.x % p.n_splits, item = blockIdx.x / p.n_splits, rt = p.row_tiles - 1 - item % p.row_tiles, hk = item / p.row_tiles;
     pdl_launch();
     pdl_wait();
@@ -99,6 +101,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         mbar_init(s_kfull + tid, 8); mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1);
         mbar_init(s_pfull + tid, 8); mbar_init(s_free + tid, 8);
     }
+    if (tid < AT_RAW) { mbar_init(s_rfull + tid, 1); mbar_init(s_rempty + tid, 8); }
     if (tid == 0) { mbar_init(&s_fin, 1); mbar_init(&s_vfull, 8); s_dead = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
@@ -115,30 +118,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         return ok;
     };
 
-    // ---- a tile's codes: a warp takes 8 rows x 64 columns, so that what it stores together meets all banks
-    const int ct = tid - 640, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a bringing thread
-    auto bring = [&](const int8_t * from, int tile, uint4 (&c)[U]) {
-        const int j0 = k0 + tile * AT_KEYS;
+    // ---- the halves of a tile: a warp takes 8 rows x 64 columns, so that what it stores together meets all banks
+    const int ct = tid - 640, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a thread
+    const uint32_t from0 = (uint32_t)(cr * HD + cc * 16), to0 = (uint32_t)cr * 128u + (uint32_t)(((2 * cc) ^ (cr & 7)) * 16);
+    auto put = [&](uint32_t from, uint32_t to) {
+        uint4 c[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {                                 // (rows behind the cache: its last one; no row sees them)
-            const int r = (u & 1) * 64 + cr, sub = u >> 1;
-            c[u] = __ldg(reinterpret_cast<const uint4 *>(from + (size_t)min(j0 + r, p.c.n_ctx - 1) * HD + sub * 64 + cc * 16));
-        }
-    };
-    auto put = [&](uint32_t to, const uint4 (&c)[U]) {
+        for (int u = 0; u < U; u++)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[u].x), "=r"(c[u].y), "=r"(c[u].z), "=r"(c[u].w) : "r"(from + from0 + (uint32_t)((u & 1) * 64 * HD + (u >> 1) * 64)) : "memory");
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int r = (u & 1) * 64 + cr;
-            const uint32_t at = to + (uint32_t)(u >> 1) * AT_SUB + (uint32_t)r * 128u;
+            const uint32_t at = to + to0 + (uint32_t)(u >> 1) * AT_SUB + (uint32_t)(u & 1) * 8192u;
             const uint32_t w[4] = {c[u].x ^ 0x80808080u, c[u].y ^ 0x80808080u, c[u].z ^ 0x80808080u, c[u].w ^ 0x80808080u};
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at + (uint32_t)(((2 * cc + h) ^ (r & 7)) * 16)), "r"(q8_lo(w[2 * h])), "r"(q8_hi(w[2 * h])), "r"(q8_lo(w[2 * h + 1])), "r"(q8_hi(w[2 * h + 1])) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(q8_lo(w[0])), "r"(q8_hi(w[0])), "r"(q8_lo(w[1])), "r"(q8_hi(w[1])) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at ^ 16u), "r"(q8_lo(w[2])), "r"(q8_hi(w[2])), "r"(q8_lo(w[3])), "r"(q8_hi(w[3])) : "memory");
         }
     };
-    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
-    uint4 code[U];
-    if (warp >= 20 && n_tiles) bring(kc, 0, code);
 
     // ---- queries into tensor memory, a row a thread
     if (warp >= 4 && warp < 8) {
@@ -211,14 +206,39 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 tc_fence_after();
                 const uint32_t a = tmem + T_S + (uint32_t)(b * AT_KEYS), d = tmem + T_O;
                 const uint64_t v = tc_desc_mn(vbuf + (uint32_t)b * TILE, AT_SUB);
-                if (TWO_P)
-                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
-                for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
+                if (steps == AT_KEYS / 16) {
+                    if (TWO_P) {
+#pragma unroll
+                        for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
+                } else {
+                    if (TWO_P)
+                        for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
+                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
+                }
                 tc_commit(s_pv + b);
                 if (i + 2 < tiles) scores(i + 2);
             }
             tc_commit(&s_fin);                                        // nothing is in flight when tensor memory is given back
             for (int spins = 0; spins < (1 << 20) && !mbar_try_wait(&s_fin, 0u); spins++) {}
+            __syncwarp();
+        } else if (warp == 1) {
+            // ============================================================= codes
+            const int8_t * kc = p.c.k + (head * p.c.n_ctx + k0) * HD, * vc = p.c.v + (head * p.c.n_ctx + k0) * HD;
+            int i = 0;
+            for (; i < 2 * n_tiles; i++) {                            // (slots behind the cache are not read: their halves are of anything, and count nothing)
+                const int slot = i % AT_RAW;
+                if (!wait(s_rempty + slot, i / AT_RAW & 1 ^ 1)) break;
+                if (lane == 0) {
+                    const unsigned bytes = (unsigned)min(AT_KEYS, p.c.n_ctx - k0 - (i >> 1) * AT_KEYS) * HD;
+                    mbar_expect_tx(s_rfull + slot, bytes);
+                    bulk_g2s(smem_raw + (raw - smem_u32(smem_raw)) + (size_t)slot * AT_KEYS * HD, (i & 1 ? vc : kc) + (size_t)(i >> 1) * AT_KEYS * HD, bytes, s_rfull + slot);
+                }
+                __syncwarp();
+            }
+            if (lane == 0) ring_land(s_rfull, i, AT_RAW);
             __syncwarp();
         }
     } else if (warp < 20) {
@@ -339,20 +359,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 }
             }
         };
+        auto take = [&](int n, uint32_t to) {                         // the n-th tile of codes
+            const int slot = n % AT_RAW;
+            ok = wait(s_rfull + slot, n / AT_RAW & 1) && ok;
+            put(raw + (uint32_t)(slot * AT_KEYS * HD), to);
+            tc_fence_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_rempty + slot);
+        };
         for (int i = 0; i < n_tiles && ok; i++) {
             const int b = i & 1;
             if (i >= 2) ok = wait(s_qk + b, (i - 2) >> 1 & 1) && ok;
-            put(kbuf + (uint32_t)b * TILE, code);
-            tc_fence_smem();
-            __syncwarp();
+            take(2 * i, kbuf + (uint32_t)b * TILE);
             if (lane == 0) mbar_arrive(s_kfull + b);
-            bring(vc, i, code);
             if (i >= 2) drain(i - 2);                                 // (which waits for the value products of tile i - 2: their buffer is free)
-            put(vbuf + (uint32_t)b * TILE, code);
-            tc_fence_smem();
-            __syncwarp();
+            take(2 * i + 1, vbuf + (uint32_t)b * TILE);
             if (i == 0 && lane == 0) mbar_arrive(&s_vfull);
-            if (i + 1 < n_tiles) bring(kc, i + 1, code);
         }
         for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);
 
@@ -393,7 +415,7 @@ bool attn_q8_tc_takes(int hd, int64_t rows) { return (hd == 64 || hd == 128) && 
 
 template <int HD, bool TWO_Q, bool TWO_P>
 static int at_go(const AttnQ8P & p, cudaStream_t st) {
-    constexpr size_t smem = (size_t)4 * (HD / 64) * AT_SUB + 1024;
+    constexpr size_t smem = (size_t)4 * (HD / 64) * AT_SUB + AT_RAW * AT_KEYS * HD + 1024;
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
