@@ -80,13 +80,14 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const int split = blockIdx.x % p.n_splits, item = blockIdx.x / p.n_splits, rt = item % p.row_tiles, hk = item / p.row_tiles;
+    const AqItem wk = aq_item(p, blockIdx.x);
+    const int split = wk.split, rt = wk.rt, hk = wk.hk;
     pdl_launch();
     pdl_wait();
-    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
     const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
     if (t.n_rows <= 0) return;
-    const int k0 = split * p.split, k1 = split == p.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
+    const int k0 = split * p.split, k1 = split == wk.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
     if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
 
     const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
                 }
     }
     __syncthreads();
-    const size_t part0 = (((size_t)blockIdx.y * p.c.H * p.row_tiles + item) * p.n_splits + split) * R;
+    const size_t part0 = ((size_t)(wk.item - p.whole) * p.n_splits + split) * R;
     for (int e = threadIdx.x; e < t.n_rows * (HD / 4); e += AQ_THREADS) {
         const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
         float top = s_m[0][r];
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
             sum = fmaf(k, s_l[w][r], sum);
             v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);
         }
-        if (p.n_splits > 1) {
+        if (wk.n_splits > 1) {
             *reinterpret_cast<float4 *>(p.part + (part0 + r) * HD + d) = v;
             if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
         } else {
@@ -284,14 +285,15 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
 
 // The splits of a tile joined, in their order
 __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
-    const int hd = p.c.hd, rt = blockIdx.x % p.row_tiles, hk = blockIdx.x / p.row_tiles;
+    const AqItem wk = aq_item(p, p.whole + blockIdx.x * p.n_splits);
+    const int hd = p.c.hd, rt = R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, hk = wk.hk;
     pdl_launch();
     pdl_wait();
-    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
     const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
     if (t.n_rows <= 0) return;
     const int used = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));
-    const size_t part0 = ((size_t)blockIdx.y * p.c.H * p.row_tiles + blockIdx.x) * p.n_splits * R;
+    const size_t part0 = (size_t)blockIdx.x * p.n_splits * R;
     for (int e = threadIdx.x; e < t.n_rows * (hd / 4); e += 256) {
         const int r = e / (hd / 4), d = (e - r * (hd / 4)) * 4;
         float top = -INFINITY;
@@ -385,8 +387,11 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8_weights(const AttnQ8P p,
 }
 
 // ---- how the work is cut
-struct AqPlan { bool tc; int R, row_tiles, split, n_splits; size_t words, lse, ml, part; };     // rows of a tile; bytes of each piece of scratch
+struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, lse, ml, part; };     // rows of a tile; bytes of each piece of scratch
 
+// CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split so
+// that they fill it, into ranges of at least AQ_LEAST slots.
+static constexpr int AQ_LEAST = 256;
 static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     AqPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
@@ -395,18 +400,19 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? AT_KEYS : AQ_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : 2), most = (keys + 255) / 256;
-    int64_t n = (slots + items - 1) / items;
-    if (items >= slots) n = 1;
+    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : 2), most = (keys + AQ_LEAST - 1) / AQ_LEAST, rest = items % slots;
+    int64_t n = rest ? slots / rest : 1;
     if (n > most) n = most;
     if (n > 128) n = 128;
     const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;
     r.split = (int)per; r.n_splits = (int)((keys + per - 1) / per);
+    r.items = (int)items;
+    r.whole = (int)(r.n_splits == 1 ? items : items - rest);
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
     r.words = r.tc ? 256 : 0;                                         // (the status word where pi_op_status looks for it)
     r.lse = weights ? up((size_t)b.T * n_head * 4) : 0;
-    r.ml = r.n_splits > 1 ? up((size_t)items * r.n_splits * r.R * 8) : 0;
-    r.part = r.n_splits > 1 ? up((size_t)items * r.n_splits * r.R * c.hd * 4) : 0;
+    r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
+    r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
     return r;
 }
 
@@ -425,7 +431,7 @@ static int aq_go(const AttnQ8P & p, cudaStream_t st) {
         PI_CUDA(cudaFuncSetAttribute(k_attn_q8<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_attn_q8<HD, MT>, dim3((unsigned)((int64_t)p.c.H * p.row_tiles * p.n_splits), p.b.n), dim3(AQ_THREADS), smem, st, true, p));
+    PI_CUDA(launch_k(k_attn_q8<HD, MT>, dim3(aq_grid(p)), dim3(AQ_THREADS), smem, st, true, p));
     return PI_OK;
 }
 
@@ -436,7 +442,7 @@ static int aq_run(const AttnQ8P & p, const AqPlan & r, const float * w_in, float
     else if constexpr (HD <= 128) rc = r.R == 8 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
     else                          rc = aq_go<HD, 1>(p, st);
     if (rc) return rc;
-    if (p.n_splits > 1) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.c.H * p.row_tiles, p.b.n), dim3(256), 0, st, true, p, r.R));
+    if (p.items > p.whole) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.items - p.whole), dim3(256), 0, st, true, p, r.R));
     if (w_out) {
         const int keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv;
         PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((keys + AQ_STEP - 1) / AQ_STEP, p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));
@@ -449,7 +455,7 @@ int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
     AttnQ8P p;
     p.c = a.c; p.b = a.b; p.xtype = a.xtype; p.q = a.q; p.q_stride = a.q_stride; p.n_head = a.n_head; p.group = a.n_head / a.c.H;
     p.scale_log2 = a.scale * 1.44269504088896340736f; p.out = a.out; p.out_stride = a.out_stride;
-    p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles;
+    p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles; p.items = r.items; p.whole = r.whole;
     char * s = (char *)a.scratch;
     p.status = (unsigned int *)(s + 8);
     s += r.words;

@@ -8,10 +8,26 @@ struct AttnQ8P {
     KvQ8 c; RaggedB b;
     int xtype; const void * q; int64_t q_stride; int n_head, group;
     float scale_log2; void * out; int64_t out_stride;
-    int split, n_splits, row_tiles;                                   // slots of a split (a multiple of AQ_STEP), splits, tiles of rows of a sequence and KV head
-    float * part; float2 * part_ml; float * lse;                      // [item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
+    // An item is a tile of rows of a KV head of an entry.  The first `whole` items are a CTA each, the others n_splits: ranges of `split` slots.
+    int split, n_splits, row_tiles, items, whole;
+    float * part; float2 * part_ml; float * lse;                      // [split item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
     unsigned int * status;                                            // tcgen05 alone: bit 4, a wait ran out
 };
+
+struct AqItem { int item, entry, hk, rt, split, n_splits; };
+__device__ __forceinline__ AqItem aq_item(const AttnQ8P & p, int cta) {
+    AqItem w;
+    const int k = cta - p.whole;
+    w.n_splits = k < 0 ? 1 : p.n_splits;
+    w.item = k < 0 ? cta : p.whole + k / p.n_splits;
+    w.split = k < 0 ? 0 : k % p.n_splits;
+    const int of_head = w.item / p.row_tiles;
+    w.rt = w.item - of_head * p.row_tiles;
+    w.entry = of_head / p.c.H;
+    w.hk = of_head - w.entry * p.c.H;
+    return w;
+}
+static inline unsigned aq_grid(const AttnQ8P & p) { return (unsigned)(p.whole + (int64_t)(p.items - p.whole) * p.n_splits); }
 
 // rows of the tile, as (token, head): row r of the group's tokens is token r / group, head r % group
 struct TileB { int n_rows, first, seen; };                            // rows there are, first row's number, slots that the last row sees (0: none)

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     static_assert(T_O + HD <= 512 && AT_REGS_M + 4 * AT_REGS_S + 2 * AT_REGS_D <= 7 * 72, "");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint64_t s_rfull[AT_RAW], s_rempty[AT_RAW];
-    __shared__ uint64_t s_kfull[2], s_vfull, s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
+    __shared__ uint64_t s_kfull[2], s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_dead;
     __shared__ float s_f[AT_ROWS];                                    // factor of a row's scores
@@ -85,24 +85,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     __shared__ float s_ref[2];                                        // largest scale of its values
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE, raw = vbuf + 2 * TILE;
-    const int split = blockIdx.x % p.n_splits, item = blockIdx.x / p.n_splits, rt = p.row_tiles - 1 - item % p.row_tiles, hk = item / p.row_tiles;
+    const AqItem w = aq_item(p, blockIdx.x);
+    const int split = w.split, hk = w.hk, rt = p.row_tiles - 1 - w.rt;      // (the longest rows first)
     pdl_launch();
     pdl_wait();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.status = 0u;
-    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, blockIdx.y);
+    if (blockIdx.x == 0 && tid == 0) *p.status = 0u;
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, w.entry);
     const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, AT_ROWS);
     if (t.n_rows <= 0) return;
-    const int k0 = split * p.split, k1 = split == p.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
+    const int k0 = split * p.split, k1 = split == w.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
     if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
     const int n_tiles = k0 < k1 ? (k1 - k0 + AT_KEYS - 1) / AT_KEYS : 0;
     const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
 
     if (tid < 2) {
         mbar_init(s_kfull + tid, 8); mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1);
-        mbar_init(s_pfull + tid, 8); mbar_init(s_free + tid, 8);
+        mbar_init(s_pfull + tid, 16); mbar_init(s_free + tid, 8);
     }
     if (tid < AT_RAW) { mbar_init(s_rfull + tid, 1); mbar_init(s_rempty + tid, 8); }
-    if (tid == 0) { mbar_init(&s_fin, 1); mbar_init(&s_vfull, 8); s_dead = 0; }
+    if (tid == 0) { mbar_init(&s_fin, 1); s_dead = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
     tc_fence_before();
@@ -135,34 +136,52 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         }
     };
 
-    // ---- queries into tensor memory, a row a thread
-    if (warp >= 4 && warp < 8) {
-        const int r = tid - 128, row = t.first + r;
-        const bool there = r < t.n_rows;
-        const size_t at = there ? (size_t)(s.first + row / p.group) * p.q_stride + (size_t)(hk * p.group + row % p.group) * HD : 0;
-        float m = 0.f;
-        if (there)
-            for (int d = 0; d < HD; d += 4) {
-                const float4 v = aq_query(p.xtype, p.q, at + d);
-                m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-            }
-        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11, as there
-        const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
-        s_f[r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
-        const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q;
+    // ---- queries into tensor memory: rows to shared memory (the halves' place) as they lie, then a row and a quarter of its columns a thread
+    {
+        constexpr int NQ = HD / 4, PITCH = HD + 4, LPR = HD / 4;      // lanes that read a row
+        const bool mine = warp >= 4 && warp < 20;
+        const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+        float * rows = reinterpret_cast<float *>(smem_raw + (kbuf - smem_u32(smem_raw)));
+        constexpr int RPW = 32 / LPR * 4;                             // rows of a warp's turn: four loads on their way
 #pragma unroll 1
-        for (int d = 0; d < HD; d += 32) {
+        for (int r0 = warp * RPW; r0 < AT_ROWS; r0 += AT_THREADS / 32 * RPW) {
+            float4 u[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int q = r0 + k * (32 / LPR) + lane / LPR, row = t.first + q, tok = row / p.group;
+                u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q < t.n_rows) u[k] = aq_query(p.xtype, p.q, (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD + lane % LPR * 4);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) *reinterpret_cast<float4 *>(rows + (r0 + k * (32 / LPR) + lane / LPR) * PITCH + lane % LPR * 4) = u[k];
+        }
+        __syncthreads();
+        float4 v[NQ / 4];
+        if (mine) {
+            float m = 0.f;
+#pragma unroll
+            for (int j = 0; j < NQ / 4; j++) v[j] = *reinterpret_cast<const float4 *>(rows + r * PITCH + part * NQ + j * 4);
+#pragma unroll
+            for (int j = 0; j < NQ / 4; j++) m = fmaxf(fmaxf(m, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
+            s_max[part >> 1][part & 1][r] = m;
+        }
+        __syncthreads();
+        if (mine) {
+            const float m = fmaxf(fmaxf(s_max[0][0][r], s_max[0][1][r]), fmaxf(s_max[1][0][r], s_max[1][1][r]));
+            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11, as there
+            const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
+            if (part == 0) s_f[r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
+            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q + (uint32_t)(part * NQ / 2);
             uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float4 v = there ? aq_query(p.xtype, p.q, at + d + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                aq_split(v.x * up, v.y * up, hi[2 * j], lo[2 * j]);
-                aq_split(v.z * up, v.w * up, hi[2 * j + 1], lo[2 * j + 1]);
+            for (int j = 0; j < NQ / 4; j++) {
+                aq_split(v[j].x * up, v[j].y * up, hi[2 * j], lo[2 * j]);
+                aq_split(v[j].z * up, v[j].w * up, hi[2 * j + 1], lo[2 * j + 1]);
             }
-            tc_st16(to + d / 2, hi);
-            if (TWO_Q) tc_st16(to + HD / 2 + d / 2, lo);
+            if (NQ == 32) { tc_st16(to, hi); if (TWO_Q) tc_st16(to + HD / 2, lo); }
+            else          { at_st8(to, hi);  if (TWO_Q) at_st8(to + HD / 2, lo); }
+            tc_wait_st();
         }
-        tc_wait_st();
     }
     tc_fence_before();
     __syncthreads();
@@ -198,10 +217,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             if (tiles > 1) scores(1);
             for (int i = 0; i < tiles && ok; i++) {
                 const int b = i & 1, steps = min(AT_KEYS / 16, (span - i * AT_KEYS + 15) / 16);
-                ok = wait(s_pfull + b, i >> 1 & 1) && ok;
-                // (whoever has drained tile i - 1 has put the values of tile i there before: a wait that is over costs 150 clocks)
-                if (i == 0) ok = wait(&s_vfull, 0u) && ok;
-                else        ok = wait(s_free + (b ^ 1), (i - 1) >> 1 & 1) && ok;
+                ok = wait(s_pfull + b, i >> 1 & 1) && ok;             // the sums before are drained too, and the values of this tile there (a wait that is over costs 150 clocks)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t a = tmem + T_S + (uint32_t)(b * AT_KEYS), d = tmem + T_O;
@@ -350,7 +366,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 if (c + 16 == HD / 2) {                               // the buffer goes back
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(s_free + b);
+                    if (lane == 0) { mbar_arrive(s_free + b); mbar_arrive(s_pfull + (b ^ 1)); }
                 }
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
@@ -374,15 +390,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             if (lane == 0) mbar_arrive(s_kfull + b);
             if (i >= 2) drain(i - 2);                                 // (which waits for the value products of tile i - 2: their buffer is free)
             take(2 * i + 1, vbuf + (uint32_t)b * TILE);
-            if (i == 0 && lane == 0) mbar_arrive(&s_vfull);
+            if (i == 0 && lane == 0) mbar_arrive(s_pfull);            // (whoever drains tile i - 1 later has put the values of tile i there before)
         }
         for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);
 
         if (r < t.n_rows) {
             const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
             if (!ok) sum = __int_as_float(0x7fc00000);                // a wait ran out: no numbers instead of wrong ones
-            if (p.n_splits > 1) {
-                const size_t at = (((size_t)blockIdx.y * p.c.H * p.row_tiles + (size_t)hk * p.row_tiles + rt) * p.n_splits + split) * AT_ROWS + r;
+            if (w.n_splits > 1) {
+                const size_t at = ((size_t)(w.item - p.whole) * p.n_splits + split) * AT_ROWS + r;
 #pragma unroll
                 for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>(p.part + at * HD + d0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
                 if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
@@ -423,7 +439,7 @@ static int at_go(const AttnQ8P & p, cudaStream_t st) {
         PI_CUDA(cudaFuncSetAttribute(k_attn_q8_tc<HD, TWO_Q, TWO_P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q, TWO_P>, dim3((unsigned)((int64_t)p.c.H * p.row_tiles * p.n_splits), p.b.n), dim3(AT_THREADS), smem, st, true, p));
+    PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q, TWO_P>, dim3(aq_grid(p)), dim3(AT_THREADS), smem, st, true, p));
     return PI_OK;
 }
 

@@ -124,7 +124,8 @@ static int check_attention(const pi_kv_q8 * cache, const pi_kv_batch * batch, in
     int rc;
     if ((rc = check_cache(cache, c, "attention_q8")) || (rc = check_batch(batch, b, "attention_q8"))) return rc;
     PI_REQUIRE(n_head > 0 && n_head % c.H == 0 && n_head <= KV_BIG / c.hd, "attention_q8: n_head=%d must be a multiple of n_head_kv=%d", n_head, c.H);
-    PI_REQUIRE((int64_t)b.max_new * n_head < (int64_t(1) << 27), "attention_q8: %d tokens of %d heads are too many for one sequence of a call", b.max_new, n_head);
+    PI_REQUIRE((int64_t)b.max_new * n_head < (int64_t(1) << 27) && (int64_t)b.n * ((int64_t)b.max_new * (n_head / c.H) / 8 + 1) * c.H < (int64_t(1) << 28),
+               "attention_q8: %d sequences of %d tokens of %d heads are too many for a call", b.n, b.max_new, n_head);
     return PI_OK;
 }
 
