@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
-import math
+import struct
 
 import numpy as np
 import torch
@@ -258,8 +258,12 @@ def attention_decode(q, k, v, k_cache, v_cache, pos, n_head, n_head_kv, seq=None
 # ---- a long context: scaled rotary positions, a KV cache in 8 bits, its attention and eviction.
 # Rows are float32 or float16 and may be columns of a wider matrix (q, k and v as one projection leaves them); results are new tensors.
 # Scratch and results come from torch's allocator at every call, so calls on several streams and captured graphs share none.
+# (Every attribute of a tensor costs 0.1 to 0.3 us: it is asked for once.  The two C structures are packed bytes: 0.5 us each, ctypes' own 1.5.)
 
 _ROW_TYPES = {torch.float32: PI_TYPE_F32, torch.float16: PI_TYPE_F16}
+_KV_Q8 = struct.Struct("@4P5i4x")          # pi_kv_q8
+_KV_BATCH = struct.Struct("@3P3i4x")       # pi_kv_batch
+assert _KV_Q8.size == C.sizeof(_lib.KvQ8) and _KV_BATCH.size == C.sizeof(_lib.KvBatch)
 
 
 def _here(*tensors):
@@ -269,34 +273,44 @@ def _here(*tensors):
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{device}")
 
 
-def _row_matrix(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
-    """t [T, width] (or [T, heads, head_dim]) as rows that the kernels take: 16-byte aligned, values of a row side by side"""
+def _row_matrix(t: torch.Tensor, what: str, width: int = 0):
+    """t [T, n] (or [T, heads, head_dim]) as rows that the kernels take, 16-byte aligned and a row's values side by side (a copy where it is not):
+    (tensor, address, rows, values of a row, values between rows, type)"""
     if t.dim() == 3:
         t = t.flatten(1)
-    if t.dim() != 2 or t.shape[1] != width:
-        raise ValueError(f"{what} is {list(t.shape)}: rows of {width} values are needed")
-    if t.dtype not in _ROW_TYPES:
+    if t.dim() != 2:
+        raise ValueError(f"{what} must have 2 or 3 dimensions: rows of heads")
+    T, n = t.shape
+    xtype = _ROW_TYPES.get(t.dtype)
+    if xtype is None:
         raise ValueError(f"{what} is {t.dtype}: float32 or float16 is needed")
+    if width and n != width:
+        raise ValueError(f"{what} is [{T}, {n}]: rows of {width} values are needed")
     step, side = t.stride()
-    if side != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (step < width or step * t.element_size() % 16)):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    at = t.data_ptr()
+    if T <= 1:
+        step = n
+    if side != 1 or at % 16 or step < n or step * (2 if xtype == PI_TYPE_F16 else 4) % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        step, at = n, t.data_ptr()
+    return t, at, T, n, step, xtype
 
 
-def _row_step(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _ints(t: torch.Tensor | None, n: int, what: str):
-    if t is not None and (t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous()):
+def _ints(t: torch.Tensor, n: int, what: str) -> int:
+    if t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n}")
-    return _p(t)
+    return t.data_ptr()
 
 
-@dataclasses.dataclass(frozen=True)
 class RopeFreqs:
-    freqs: torch.Tensor            # float64 [n_rot / 2] on the device: angle per position of each pair
-    mscale: float = 1.0            # factor of the rotated values
+    """freqs: float64 [n_rot / 2] on the device, the angle per position of each pair; mscale: factor of the rotated values"""
+
+    __slots__ = ("freqs", "mscale")
+
+    def __init__(self, freqs: torch.Tensor, mscale: float = 1.0):
+        if freqs.dtype is not torch.float64 or not freqs.is_contiguous():
+            raise ValueError("frequencies must be contiguous float64")
+        self.freqs, self.mscale = freqs, mscale
 
 
 def rope_freqs(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0,
@@ -314,41 +328,56 @@ def rope_freqs(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, 
 def rope_ext(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, freqs: RopeFreqs, head_dim: int, mode: int = 0, inplace: bool = False):
     """Queries [T, n_head * head_dim] and keys [T, n_head_kv * head_dim] rotated to pos int32 [T]; mode 0 (pairs (2i, 2i+1)) or 2 (neox).  The first
     2 * len(freqs) dimensions of each head turn.  Returns (q, k), new tensors, or the same ones with inplace."""
-    T = q.shape[0]
-    x = [t if t is None else _row_matrix(t, t.shape[1] if t.dim() == 2 else t.shape[1] * t.shape[2], "q / k") for t in (q, k)]
-    for t in x:
-        if t is not None and (t.shape[0] != T or t.shape[1] % head_dim or t.dtype is not x[0].dtype):
-            raise ValueError(f"q and k must be of one type, {T} rows of heads of {head_dim}")
-    if freqs.freqs.dtype is not torch.float64 or not freqs.freqs.is_contiguous():
-        raise ValueError("frequencies must be contiguous float64")
-    if inplace and any(t is not None and t.data_ptr() != o.data_ptr() for t, o in zip(x, (q, k))):
-        raise ValueError("in place needs rows that are 16-byte aligned")
-    y = x if inplace else [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in x]
-    _here(x[0], x[1], pos, freqs.freqs)
-    keys = (None, 0, 0, None, 0) if k is None else (x[1].data_ptr(), _row_step(x[1]), x[1].shape[1] // head_dim, y[1].data_ptr(), _row_step(y[1]))
-    check(lib.pi_rope_ext(_ROW_TYPES[x[0].dtype], x[0].data_ptr(), _row_step(x[0]), x[0].shape[1] // head_dim, y[0].data_ptr(), _row_step(y[0]), *keys,
-                          T, head_dim, 2 * freqs.freqs.numel(), 1 if mode & 2 else 0, _ints(pos, T, "pos"), freqs.freqs.data_ptr(), freqs.mscale, _stream()))
-    return (q, k) if inplace else (y[0], y[1])
+    xq, q_at, T, nq, q_step, xtype = _row_matrix(q, "q")
+    f = freqs.freqs
+    if nq % head_dim:
+        raise ValueError(f"q has rows of {nq} values: heads of {head_dim} are needed")
+    if inplace:
+        yq, yq_at, yq_step = q, q_at, q_step
+        if q_at != q.data_ptr():
+            raise ValueError("in place needs rows that are 16-byte aligned")
+    else:
+        yq, yq_step = xq.new_empty((T, nq)), nq
+        yq_at = yq.data_ptr()
+    if k is None:
+        _here(xq, pos, f)
+        check(lib.pi_rope_ext(xtype, q_at, q_step, nq // head_dim, yq_at, yq_step, None, 0, 0, None, 0, T, head_dim, 2 * f.numel(), 1 if mode & 2 else 0,
+                              _ints(pos, T, "pos"), f.data_ptr(), freqs.mscale, _stream()))
+        return yq, None
+    xk, k_at, Tk, nk, k_step, ktype = _row_matrix(k, "k")
+    if Tk != T or ktype != xtype or nk % head_dim:
+        raise ValueError(f"q and k must be of one type, {T} rows of heads of {head_dim}")
+    if inplace:
+        yk, yk_at, yk_step = k, k_at, k_step
+        if k_at != k.data_ptr():
+            raise ValueError("in place needs rows that are 16-byte aligned")
+    else:
+        yk, yk_step = xk.new_empty((T, nk)), nk
+        yk_at = yk.data_ptr()
+    _here(xq, xk, pos, f)
+    check(lib.pi_rope_ext(xtype, q_at, q_step, nq // head_dim, yq_at, yq_step, k_at, k_step, nk // head_dim, yk_at, yk_step, T, head_dim, 2 * f.numel(),
+                          1 if mode & 2 else 0, _ints(pos, T, "pos"), f.data_ptr(), freqs.mscale, _stream()))
+    return yq, yk
 
 
 class KvCacheQ8:
     """A KV cache in 8 bits: codes int8 [n_seq, n_head_kv, n_ctx, head_dim], scales float32 [n_seq, n_head_kv, n_ctx / block]."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "c", "at")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_seq", "n_head_kv", "n_ctx", "head_dim", "block", "c")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        n_seq, n_head_kv, n_ctx, head_dim = k.shape
-        blocks = k_scale.shape[2]
+        shape, blocks = k.shape, k_scale.shape
         if k.dtype is not torch.int8 or v.dtype is not torch.int8 or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
             raise ValueError("codes are int8, scales float32")
-        if v.shape != k.shape or k_scale.shape != v_scale.shape or k_scale.shape[:2] != k.shape[:2] or blocks == 0 or n_ctx % blocks:
+        if len(shape) != 4 or len(blocks) != 3 or v.shape != shape or v_scale.shape != blocks or blocks[:2] != shape[:2] or not blocks[2] or shape[2] % blocks[2]:
             raise ValueError("codes [n_seq, n_head_kv, n_ctx, head_dim] and scales [n_seq, n_head_kv, n_ctx / block] do not fit each other")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("the caches must be contiguous")
         _here(k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.c = _lib.KvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_seq, n_head_kv, n_ctx, head_dim, n_ctx // blocks)
-        self.at = C.addressof(self.c)
+        n_seq, n_head_kv, n_ctx, head_dim = shape
+        self.n_seq, self.n_head_kv, self.n_ctx, self.head_dim, self.block = n_seq, n_head_kv, n_ctx, head_dim, n_ctx // blocks[2]
+        self.c = _KV_Q8.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_seq, n_head_kv, n_ctx, head_dim, self.block)
 
     @classmethod
     def empty(cls, n_seq: int, n_ctx: int, n_head_kv: int, head_dim: int, block: int = 64) -> "KvCacheQ8":
@@ -356,35 +385,44 @@ class KvCacheQ8:
         return cls(*codes, *(torch.zeros(n_seq, n_head_kv, n_ctx // block, device="cuda") for _ in range(2)))
 
 
-def _batch(q_start, pos0, seq, T, max_new):
+def _batch(q_start, pos0, seq, T, max_new) -> bytes:
     n = pos0.numel()
-    return _lib.KvBatch(_ints(q_start, n + 1, "q_start"), _ints(seq, n, "seq"), _ints(pos0, n, "pos0"), n, T, T if max_new is None else max_new)
+    return _KV_BATCH.pack(_ints(q_start, n + 1, "q_start"), 0 if seq is None else _ints(seq, n, "seq"), _ints(pos0, n, "pos0"), n, T,
+                          T if max_new is None else max_new)
 
 
 def kv_store_q8(cache: KvCacheQ8, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None,
                 max_new: int | None = None) -> None:
     """k, v [T, n_head_kv * head_dim] into the cache: rows q_start[i] .. q_start[i + 1] to the slots pos0[i] and on of sequence seq[i] (None: i); at
     most max_new rows of an entry (None: T)."""
-    c, T = cache.c, k.shape[0]
-    k, v = _row_matrix(k, c.n_head_kv * c.head_dim, "k"), _row_matrix(v, c.n_head_kv * c.head_dim, "v")
-    if v.shape[0] != T or k.dtype is not v.dtype:
+    width = cache.n_head_kv * cache.head_dim
+    k, k_at, T, _, k_step, xtype = _row_matrix(k, "k", width)
+    v, v_at, Tv, _, v_step, vtype = _row_matrix(v, "v", width)
+    if Tv != T or vtype != xtype:
         raise ValueError("k and v must have the same rows and type")
     _here(cache.k, k, v, q_start, pos0, seq)
-    b = _batch(q_start, pos0, seq, T, max_new)
-    check(lib.pi_kv_store_q8(cache.at, C.addressof(b), _ROW_TYPES[k.dtype], k.data_ptr(), _row_step(k), v.data_ptr(), _row_step(v), _stream()))
+    check(lib.pi_kv_store_q8(cache.c, _batch(q_start, pos0, seq, T, max_new), xtype, k_at, k_step, v_at, v_step, _stream()))
 
 
 def kv_load_q8(cache: KvCacheQ8, q_start: torch.Tensor, pos0: torch.Tensor, T: int, seq: torch.Tensor | None = None, max_new: int | None = None,
                dtype: torch.dtype = torch.float32):
     """The values of the slots that kv_store_q8 with the same batch writes: k, v [T, n_head_kv * head_dim] (rows of no entry hold anything)."""
-    c = cache.c
-    if dtype not in _ROW_TYPES:
+    width, xtype = cache.n_head_kv * cache.head_dim, _ROW_TYPES.get(dtype)
+    if xtype is None:
         raise ValueError("values are read as float32 or float16")
-    k, v = (torch.empty(T, c.n_head_kv * c.head_dim, dtype=dtype, device=cache.k.device) for _ in range(2))
+    k = cache.k.new_empty((T, width), dtype=dtype)
+    v = cache.k.new_empty((T, width), dtype=dtype)
     _here(cache.k, q_start, pos0, seq)
-    b = _batch(q_start, pos0, seq, T, max_new)
-    check(lib.pi_kv_load_q8(cache.at, C.addressof(b), _ROW_TYPES[dtype], k.data_ptr(), _row_step(k), v.data_ptr(), _row_step(v), _stream()))
+    check(lib.pi_kv_load_q8(cache.c, _batch(q_start, pos0, seq, T, max_new), xtype, k.data_ptr(), width, v.data_ptr(), width, _stream()))
     return k, v
+
+
+def _slot_weights(w: torch.Tensor | None, cache: KvCacheQ8):
+    if w is None:
+        return None
+    if w.dtype is not torch.float32 or w.shape != (cache.n_seq, cache.n_head_kv, cache.n_ctx) or not w.is_contiguous():
+        raise ValueError("weights are contiguous float32 [n_seq, n_head_kv, n_ctx]")
+    return w.data_ptr()
 
 
 def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None, max_new: int | None = None,
@@ -393,26 +431,21 @@ def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0:
     """The KQV block over the 8-bit cache, the batch's own keys and values stored before: q [T, n_head * head_dim] -> the same shape and type.  Token t
     of entry i sees the slots up to pos0[i] + t.  max_kv: slots that the longest sequence sees (None: all).  weights_out float32 [n_seq,
     n_head_kv, n_ctx] takes each seen slot's probabilities, plus weights_in for slots before pos0.  Rows of no entry are left as `out` has them."""
-    c = cache.c
-    if q.shape[-1] % c.head_dim:
-        raise ValueError(f"q is {list(q.shape)}: heads of {c.head_dim} are needed")
-    q = _row_matrix(q, q.shape[1] if q.dim() == 2 else q.shape[1] * q.shape[2], "q")
-    T, n_head = q.shape[0], q.shape[1] // c.head_dim
+    hd = cache.head_dim
+    q, q_at, T, n, q_step, xtype = _row_matrix(q, "q")
+    if n % hd:
+        raise ValueError(f"q has rows of {n} values: heads of {hd} are needed")
     if out is None:
-        out = torch.empty(T, q.shape[1], dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
+        out = q.new_empty((T, n))
+    elif out.shape != (T, n) or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and type")
-    for w in (weights_in, weights_out):
-        if w is not None and (w.dtype is not torch.float32 or w.shape != cache.k.shape[:3] or not w.is_contiguous()):
-            raise ValueError("weights are contiguous float32 [n_seq, n_head_kv, n_ctx]")
+    w_in, w_out = _slot_weights(weights_in, cache), _slot_weights(weights_out, cache)
     _here(cache.k, q, out, q_start, pos0, seq, weights_in, weights_out)
-    b = _batch(q_start, pos0, seq, T, max_new)
-    most = c.n_ctx if max_kv is None else max_kv
-    need = lib.pi_attention_q8_workspace_bytes(cache.at, C.addressof(b), n_head, most, 0 if weights_out is None else 1)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib.pi_attention_q8(cache.at, C.addressof(b), _ROW_TYPES[q.dtype], q.data_ptr(), _row_step(q), n_head, most,
-                              1.0 / math.sqrt(c.head_dim) if scale is None else scale, out.data_ptr(), _row_step(out), _p(weights_in), _p(weights_out),
-                              _p(ws), need, _stream()))
+    b, most = _batch(q_start, pos0, seq, T, max_new), cache.n_ctx if max_kv is None else max_kv
+    need = lib.pi_attention_q8_workspace_bytes(cache.c, b, n // hd, most, 0 if w_out is None else 1)
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    check(lib.pi_attention_q8(cache.c, b, xtype, q_at, q_step, n // hd, most, hd ** -0.5 if scale is None else scale, out.data_ptr(), n, w_in, w_out,
+                              None if ws is None else ws.data_ptr(), need, _stream()))
     return out
 
 
@@ -421,12 +454,10 @@ def kv_evict_q8(cache: KvCacheQ8, weights: torch.Tensor, lens: torch.Tensor, kee
     """Sequences of lens[i] slots cut to `keep` by their accumulated weights (float32 [n_seq, n_head_kv, n_ctx], as attention_q8 leaves them): the first
     n_sink slots, the last n_recent and the heaviest others stay, for every KV head its own.  Returns the slot that each kept row came from,
     int32 [n, n_head_kv, keep] (-1: none); weights_out (may be `weights`) takes the weights in the new order."""
-    n, c = lens.numel(), cache.c
-    for w in (weights, weights_out):
-        if w is not None and (w.dtype is not torch.float32 or w.shape != cache.k.shape[:3] or not w.is_contiguous()):
-            raise ValueError("weights are contiguous float32 [n_seq, n_head_kv, n_ctx]")
+    n = lens.numel()
+    w, w_out = _slot_weights(weights, cache), _slot_weights(weights_out, cache)
     _here(cache.k, weights, weights_out, lens, seq)
-    kept = torch.empty(n, c.n_head_kv, max(0, keep), dtype=torch.int32, device=lens.device)
-    check(lib.pi_kv_evict_q8(cache.at, _ints(lens, n, "lens"), _ints(seq, n, "seq"), n, keep, n_sink, n_recent, weights.data_ptr(), _p(weights_out),
+    kept = lens.new_empty((n, cache.n_head_kv, max(0, keep)))
+    check(lib.pi_kv_evict_q8(cache.c, _ints(lens, n, "lens"), None if seq is None else _ints(seq, n, "seq"), n, keep, n_sink, n_recent, w, w_out,
                              kept.data_ptr(), _stream()))
     return kept
