@@ -283,39 +283,61 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
     }
 }
 
-// The splits of a tile joined, in their order
+// The splits of a tile joined, in their order.  WPR warps have a row (its splits dealt to them): one where splits are few, eight where one row's
+// many partial sums are all there is to wait for (64 rows of 37 splits: a CTA for each tile of rows took 25 us).
+static constexpr int AQ_JOIN_FEW = 8;
+
+template <int WPR>
 __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
-    const AqItem wk = aq_item(p, p.whole + blockIdx.x * p.n_splits);
-    const int hd = p.c.hd, rt = R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, hk = wk.hk;
+    __shared__ float s_sum[8][257];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR, hd = p.c.hd, nd = hd / 32;
+    const int at_row = blockIdx.x * (8 / WPR) + warp / WPR, k_item = at_row / R, r = at_row - k_item * R;
     pdl_launch();
     pdl_wait();
+    if (k_item >= p.items - p.whole) return;                          // (with WPR = 8: the whole CTA)
+    const AqItem wk = aq_item(p, p.whole + k_item * p.n_splits);
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
-    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
-    if (t.n_rows <= 0) return;
+    const TileB t = aq_tile(s, p.c.n_ctx, p.group, R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, R);
+    if (r >= t.n_rows) return;
     const int used = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));
-    const size_t part0 = (size_t)blockIdx.x * p.n_splits * R;
-    for (int e = threadIdx.x; e < t.n_rows * (hd / 4); e += 256) {
-        const int r = e / (hd / 4), d = (e - r * (hd / 4)) * 4;
-        float top = -INFINITY;
-        for (int k = 0; k < used; k++) top = fmaxf(top, __ldcg(&p.part_ml[part0 + (size_t)k * R + r]).x);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int k = 0; k < used; k++) {
-            const size_t at = part0 + (size_t)k * R + r;
-            const float2 ml = __ldcg(&p.part_ml[at]);
-            const float4 u = __ldcg(reinterpret_cast<const float4 *>(p.part + at * hd + d));
-            const float w = exp2_approx(ml.x - ref);
-            sum = fmaf(w, ml.y, sum);
-            v.x = fmaf(w, u.x, v.x); v.y = fmaf(w, u.y, v.y); v.z = fmaf(w, u.z, v.z); v.w = fmaf(w, u.w, v.w);
-        }
-        const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const size_t at = (size_t)tok * p.out_stride + (size_t)h * hd + d;
-        aq_put(p.xtype, p.out, at, v.x * inv); aq_put(p.xtype, p.out, at + 1, v.y * inv);
-        aq_put(p.xtype, p.out, at + 2, v.z * inv); aq_put(p.xtype, p.out, at + 3, v.w * inv);
-        if (d == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
+    const size_t part0 = (size_t)k_item * p.n_splits * R + r;
+    float top = -INFINITY;
+    for (int k = lane; k < used; k += 32) top = fmaxf(top, __ldcg(&p.part_ml[part0 + (size_t)k * R]).x);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = sub; k < used; k += WPR) {
+        const size_t at = part0 + (size_t)k * R;
+        const float2 ml = __ldcg(&p.part_ml[at]);
+        const float w = exp2_approx(ml.x - ref);
+        sum = fmaf(w, ml.y, sum);
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (j < nd) v[j] = fmaf(w, __ldcg(p.part + at * hd + lane + 32 * j), v[j]);
     }
+    if (WPR > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (j < nd) s_sum[warp][lane + 32 * j] = v[j];
+        if (lane == 0) s_sum[warp][256] = sum;
+        __syncthreads();
+        if (warp > 0) return;
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; w++) sum += s_sum[w][256];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < nd) {
+                v[j] = 0.f;
+#pragma unroll
+                for (int w = 0; w < WPR; w++) v[j] += s_sum[w][lane + 32 * j];
+            }
+    }
+    const int row = t.first + r, tok = s.first + row / p.group, h = wk.hk * p.group + row % p.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t at = (size_t)tok * p.out_stride + (size_t)h * hd + lane;
+#pragma unroll
+    for (int j = 0; j < 8; j++) if (j < nd) aq_put(p.xtype, p.out, at + 32 * j, v[j] * inv);
+    if (lane == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
 // weights_out[j] = (j < pos0 ? weights_in[j] : 0) + sum over the sequence's new tokens and the heads of the group of p_j.  A warp keeps 16 slots as
@@ -442,7 +464,11 @@ static int aq_run(const AttnQ8P & p, const AqPlan & r, const float * w_in, float
     else if constexpr (HD <= 128) rc = r.R == 8 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
     else                          rc = aq_go<HD, 1>(p, st);
     if (rc) return rc;
-    if (p.items > p.whole) PI_CUDA(launch_k(k_attn_q8_join, dim3(p.items - p.whole), dim3(256), 0, st, true, p, r.R));
+    if (p.items > p.whole) {
+        const int64_t rows = (int64_t)(p.items - p.whole) * r.R;
+        if (p.n_splits <= AQ_JOIN_FEW) PI_CUDA(launch_k(k_attn_q8_join<1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, true, p, r.R));
+        else                           PI_CUDA(launch_k(k_attn_q8_join<8>, dim3((unsigned)rows), dim3(256), 0, st, true, p, r.R));
+    }
     if (w_out) {
         const int keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv;
         PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((keys + AQ_STEP - 1) / AQ_STEP, p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));

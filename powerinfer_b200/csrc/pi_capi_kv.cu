@@ -116,6 +116,7 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
     if ((rc = check_cache(cache, c, "kv_load_q8")) || (rc = check_batch(batch, b, "kv_load_q8")) || (rc = check_type(xtype, "kv_load_q8"))) return rc;
     if (b.n == 0 || b.T == 0 || b.max_new == 0) return PI_OK;
     const int64_t width = (int64_t)c.H * c.hd;
+    PI_REQUIRE((int64_t)(b.max_new / 16 + 1) * c.H < (int64_t(1) << 30), "kv_load_q8: too many slots for one call");
     if ((rc = check_rows(k, k_stride, width, xtype, "kv_load_q8", "k")) || (rc = check_rows(v, v_stride, width, xtype, "kv_load_q8", "v"))) return rc;
     return launch_kv_load_q8(c, b, xtype, k, k_stride, v, v_stride, (cudaStream_t)stream);
 }

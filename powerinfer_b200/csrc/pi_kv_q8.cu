@@ -45,10 +45,11 @@ __device__ __forceinline__ uint32_t q8_rescale(uint32_t w, float ratio) {
     return r;
 }
 
-// NT threads per unit
-template <typename T, int NT>
-__global__ void __launch_bounds__(KV_THREADS) k_kv_store(const StoreP p) {
-    constexpr int HOLD = NT == 32 ? 4 : 8, UNITS = KV_THREADS / NT;
+// NT threads per unit, HOLD vectors of four values in registers (others are read again): a block of 32 x 128 or less needs 4, and leaves room for
+// more CTAs, which is what hides the way from one's loads to its stores
+template <typename T, int NT, int HOLD>
+__global__ void __launch_bounds__(KV_THREADS, HOLD <= 4 ? 5 : 3) k_kv_store(const StoreP p) {
+    constexpr int UNITS = KV_THREADS / NT;
     __shared__ float s_max[KV_THREADS / 32];
     const int lane = threadIdx.x & 31, tid = NT == 32 ? lane : (int)threadIdx.x;
     const int64_t unit = (int64_t)blockIdx.x * UNITS + (NT == 32 ? threadIdx.x >> 5 : 0);      // (block, keys or values, head), blocks of a head side by side
@@ -134,8 +135,9 @@ static constexpr int STORE_FEW = 4;
 template <typename T>
 static int store_go(const StoreP & p, cudaStream_t st) {
     const int64_t units = (int64_t)p.n_blocks * 2 * p.c.H;
-    if (p.b.max_new <= STORE_FEW) PI_CUDA(launch_k(k_kv_store<T, 32>, dim3((unsigned)((units + 7) / 8), p.b.n), dim3(KV_THREADS), 0, st, true, p));
-    else                          PI_CUDA(launch_k(k_kv_store<T, KV_THREADS>, dim3((unsigned)units, p.b.n), dim3(KV_THREADS), 0, st, true, p));
+    if (p.b.max_new <= STORE_FEW)       PI_CUDA(launch_k(k_kv_store<T, 32, 4>, dim3((unsigned)((units + 7) / 8), p.b.n), dim3(KV_THREADS), 0, st, true, p));
+    else if (p.c.block * p.c.hd <= 4096) PI_CUDA(launch_k(k_kv_store<T, KV_THREADS, 4>, dim3((unsigned)units, p.b.n), dim3(KV_THREADS), 0, st, true, p));
+    else                                PI_CUDA(launch_k(k_kv_store<T, KV_THREADS, 8>, dim3((unsigned)units, p.b.n), dim3(KV_THREADS), 0, st, true, p));
     return PI_OK;
 }
 
@@ -149,58 +151,72 @@ int launch_kv_store_q8(const KvQ8 & c, const RaggedB & b, int xtype, const void 
 }
 
 // ------------------------------------------------------------------------------------------------
-struct LoadP { KvQ8 c; RaggedB b; void * y[2]; int64_t stride[2]; };
+struct LoadP { KvQ8 c; RaggedB b; void * y[2]; int64_t stride[2]; int groups; };
 
-// x = code * scale: four codes a thread, LOAD_U of them in flight
-static constexpr int LOAD_U = 4;
+// x = code * scale.  A warp takes LOAD_ROWS slots of a head, contiguous in the cache: all of its loads, four codes each, are on their way at once.
+// Bound by the bytes of the values.
+static constexpr int LOAD_ROWS = 16;
 
-template <typename T>
+template <typename T, int HD>
 __global__ void __launch_bounds__(KV_THREADS) k_kv_load(const LoadP p) {
-    const int i = blockIdx.y, which = blockIdx.z;
+    constexpr int V4 = HD / 4, N = LOAD_ROWS * V4 / 32;
+    const int i = blockIdx.y, which = blockIdx.z, lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * (KV_THREADS / 32) + (threadIdx.x >> 5), h = unit / p.groups, t0 = (unit - h * p.groups) * LOAD_ROWS;
     pdl_launch();
     pdl_wait();
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, i);
-    const int64_t row4 = (int64_t)p.c.H * p.c.hd / 4, total = (int64_t)s.n_new * row4;
-    const int64_t e0 = (int64_t)blockIdx.x * KV_THREADS * LOAD_U + threadIdx.x;
-    if ((int64_t)blockIdx.x * KV_THREADS * LOAD_U >= total) return;
-    uint32_t w[LOAD_U]; float sc[LOAD_U];
+    if (h >= p.c.H || t0 >= s.n_new) return;
+    const size_t head = (size_t)max(s.sq, 0) * p.c.H + h;
+    const int8_t * codes = (which ? p.c.v : p.c.k) + (head * p.c.n_ctx + s.pos + t0) * HD;
+    const float * scale = (which ? p.c.vs : p.c.ks) + head * (p.c.n_ctx >> p.c.shift);
+    const int there = s.sq < 0 ? 0 : p.c.n_ctx - s.pos - t0, rows = min(LOAD_ROWS, s.n_new - t0);     // (slots that the cache lacks: zeros)
+    uint32_t w[N]; float sc[N];
 #pragma unroll
-    for (int u = 0; u < LOAD_U; u++) {
-        const int64_t e = e0 + u * KV_THREADS;
+    for (int u = 0; u < N; u++) {
+        const int e = u * 32 + lane, t = e / V4;
         w[u] = 0u; sc[u] = 0.f;
-        if (e >= total || s.sq < 0) continue;
-        const int t = (int)(e / row4), c = (int)(e - t * row4) * 4, h = c / p.c.hd, d = c - h * p.c.hd, slot = s.pos + t;
-        if (slot >= p.c.n_ctx) continue;                              // (no such slot: zeros)
-        const size_t head = (size_t)s.sq * p.c.H + h;
-        w[u] = __ldg(reinterpret_cast<const uint32_t *>((which ? p.c.v : p.c.k) + (head * p.c.n_ctx + slot) * p.c.hd + d));
-        sc[u] = __ldg((which ? p.c.vs : p.c.ks) + head * (p.c.n_ctx >> p.c.shift) + (slot >> p.c.shift));
+        if (t < rows && t < there) {
+            w[u] = __ldg(reinterpret_cast<const uint32_t *>(codes + (size_t)e * 4));
+            sc[u] = __ldg(scale + ((s.pos + t0 + t) >> p.c.shift));
+        }
     }
+    const int64_t stride = which ? p.stride[1] : p.stride[0];
+    T * y = (T *)(which ? p.y[1] : p.y[0]) + (int64_t)(s.first + t0) * stride + h * HD;
 #pragma unroll
-    for (int u = 0; u < LOAD_U; u++) {
-        const int64_t e = e0 + u * KV_THREADS;
-        if (e >= total) continue;
-        const int64_t t = e / row4;
-        T * y = (T *)(which ? p.y[1] : p.y[0]) + (s.first + t) * (which ? p.stride[1] : p.stride[0]) + (e - t * row4) * 4;
+    for (int u = 0; u < N; u++) {
+        const int e = u * 32 + lane, t = e / V4;
+        if (t >= rows) continue;
+        T * at = y + t * stride + (e - t * V4) * 4;
         float f[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) f[j] = (float)(int8_t)(w[u] >> (8 * j)) * sc[u];
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(y) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4 *>(at) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
-            __half2 h[2] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3])};
-            *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<uint2 *>(h);
+            __half2 hh[2] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3])};
+            *reinterpret_cast<uint2 *>(at) = *reinterpret_cast<uint2 *>(hh);
         }
     }
+}
+
+template <typename T>
+static int load_go(const LoadP & p, dim3 grid, cudaStream_t st) {
+    switch (p.c.hd) {
+        case 64:  PI_CUDA(launch_k(k_kv_load<T, 64>, grid, dim3(KV_THREADS), 0, st, true, p)); break;
+        case 96:  PI_CUDA(launch_k(k_kv_load<T, 96>, grid, dim3(KV_THREADS), 0, st, true, p)); break;
+        case 128: PI_CUDA(launch_k(k_kv_load<T, 128>, grid, dim3(KV_THREADS), 0, st, true, p)); break;
+        case 192: PI_CUDA(launch_k(k_kv_load<T, 192>, grid, dim3(KV_THREADS), 0, st, true, p)); break;
+        default:  PI_CUDA(launch_k(k_kv_load<T, 256>, grid, dim3(KV_THREADS), 0, st, true, p));
+    }
+    return PI_OK;
 }
 
 int launch_kv_load_q8(const KvQ8 & c, const RaggedB & b, int xtype, void * k, int64_t k_stride, void * v, int64_t v_stride, cudaStream_t st) {
     LoadP p;
     p.c = c; p.b = b; p.y[0] = k; p.y[1] = v; p.stride[0] = k_stride; p.stride[1] = v_stride;
-    const int64_t total = (int64_t)b.max_new * c.H * c.hd / 4, of_cta = (int64_t)KV_THREADS * LOAD_U;
-    const dim3 grid((unsigned)((total + of_cta - 1) / of_cta), b.n, 2);
-    if (xtype == PI_TYPE_F16) PI_CUDA(launch_k(k_kv_load<__half>, grid, dim3(KV_THREADS), 0, st, true, p));
-    else                      PI_CUDA(launch_k(k_kv_load<float>, grid, dim3(KV_THREADS), 0, st, true, p));
-    return PI_OK;
+    p.groups = (b.max_new + LOAD_ROWS - 1) / LOAD_ROWS;
+    const dim3 grid((unsigned)(((int64_t)p.groups * c.H + KV_THREADS / 32 - 1) / (KV_THREADS / 32)), b.n, 2);
+    return xtype == PI_TYPE_F16 ? load_go<__half>(p, grid, st) : load_go<float>(p, grid, st);
 }
 
 }  // namespace pi
