@@ -30,6 +30,7 @@ template <int HD> struct AqShape {
     static __device__ __forceinline__ int k_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ ((row & 1) << 6) : byte); }
     static __device__ __forceinline__ int v_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ (((row >> 1) & 3) << 5) : byte); }
     static constexpr int STAGES = HD <= 128 ? 4 : 3, STAGE = 2 * 16 * HD;
+    static constexpr int ctas(int mt) { return HD <= 128 && mt == 1 ? 3 : 2; }           // that an SM holds
     static constexpr size_t ring() { return (size_t)AQ_WARPS * STAGES * STAGE; }
     static constexpr size_t smem(int mt) {
         const size_t sums = (size_t)AQ_WARPS * 8 * mt * (HD + 4) * 4;
@@ -74,7 +75,7 @@ __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s
 }
 
 template <int HD, int MT>
-__global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
+__global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(const AttnQ8P p) {
     using S = AqShape<HD>;
     constexpr int R = 8 * MT, ST = S::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -93,33 +94,38 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
     const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
     const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
     const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
-    unsigned char * ring = smem + (size_t)warp * ST * S::STAGE;
+    const unsigned char * ring = smem + (size_t)warp * ST * S::STAGE;
     const int first = k0 + warp * 16, steps = first < k1 ? (k1 - first + AQ_STEP - 1) / AQ_STEP : 0;
-    auto issue = [&](int it) {
-        if (it < steps) {
-            const size_t from = (size_t)(first + it * AQ_STEP) * HD;  // (16 slots from a multiple of 16: inside the cache)
-            const uint32_t to = smem_u32(ring + (it % ST) * S::STAGE);
+    const int8_t * k_next = kc + (size_t)first * HD + lane * 16, * v_next = vc + (size_t)first * HD + lane * 16;     // (16 slots from a multiple of 16: inside the cache)
+    const uint32_t ring_at = smem_u32(ring);
+    int left = steps; uint32_t fill = ring_at;                        // steps to be asked for, and where the next one goes
+    auto issue = [&]() {
+        if (left > 0) {
 #pragma unroll
             for (int u = 0; u < HD / 32; u++) {
                 const int b = (u * 32 + lane) * 16, row = b / HD, byte = b % HD;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + S::k_at(row, byte)), "l"(kc + from + b) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + 16 * HD + S::v_at(row, byte)), "l"(vc + from + b) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(fill + S::k_at(row, byte)), "l"(k_next + u * 512) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(fill + 16 * HD + S::v_at(row, byte)), "l"(v_next + u * 512) : "memory");
             }
+            k_next += AQ_STEP * HD; v_next += AQ_STEP * HD;
+            left--;
+            fill = fill == ring_at + (ST - 1) * S::STAGE ? ring_at : fill + S::STAGE;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int it = 0; it < ST - 1; it++) issue(it);
+    for (int it = 0; it < ST - 1; it++) issue();
 
     uint32_t a[MT][S::KS][4];
-    float f[MT], m[MT], l[MT]; int sees[MT], least = 0x7fffffff;
+    float f[MT], m[MT], l[MT]; int sees[MT], score_row[MT], least = 0x7fffffff; bool there[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const int row = mt * 8 + g;
-        const bool there = row < t.n_rows;
-        f[mt] = aq_load_query<HD>(p, s, t.first + row, there, hk, q, a[mt]) * p.scale_log2;
-        sees[mt] = there ? aq_sees(s, p.c.n_ctx, (t.first + row) / p.group) : 0;
-        if (there) least = min(least, sees[mt]);
+        there[mt] = row < t.n_rows;
+        f[mt] = aq_load_query<HD>(p, s, t.first + row, there[mt], hk, q, a[mt]) * p.scale_log2;
+        sees[mt] = there[mt] ? aq_sees(s, p.c.n_ctx, (t.first + row) / p.group) : 0;
+        if (there[mt]) least = min(least, sees[mt]);
+        score_row[mt] = (s.first + (t.first + row) / p.group) * p.n_head + hk * p.group + (t.first + row) % p.group;
         m[mt] = -INFINITY; l[mt] = 0.f;
     }
     least = __reduce_min_sync(0xffffffffu, least);
@@ -132,11 +138,13 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
             for (int j = 0; j < 4; j++) o[mt][n][j] = 0.f;
     float v_ref = 0.f, v_inv = 0.f;                                   // scale of the value sums, and AQ_P over it
 
+    const unsigned char * kt = ring + (ST - 1) * S::STAGE;
     for (int it = 0; it < steps; it++) {
         asm volatile("cp.async.wait_group %0;" :: "n"(ST - 2) : "memory");
         __syncwarp();                                                 // the stage is there for all lanes, and all have read the last one
-        issue(it + ST - 1);                                           // (into which this goes)
-        const unsigned char * kt = ring + (it % ST) * S::STAGE, * vt = kt + 16 * HD;
+        issue();                                                      // (into which this goes)
+        kt = kt == ring + (ST - 1) * S::STAGE ? ring : kt + S::STAGE;
+        const unsigned char * vt = kt + 16 * HD;
         const int j0 = first + it * AQ_STEP;
         const float sk = __ldg(ks + (j0 >> p.c.shift)), sv = __ldg(vs + (j0 >> p.c.shift));
 
@@ -176,11 +184,17 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) y[n][j] = (x[mt][n][j] + x[mt][n][j + 2]) * fk;
-            if (j0 + 16 > least) {
+            const bool masked = j0 + 16 > least;
+            if (masked) {
 #pragma unroll
                 for (int n = 0; n < 2; n++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j >= sees[mt]) y[n][j] = -INFINITY;
+            }
+            if (p.scores && there[mt]) {
+                float * to = p.scores + (size_t)score_row[mt] * p.score_pitch + j0 + 2 * q;
+                *reinterpret_cast<float2 *>(to) = make_float2(y[0][0], y[0][1]);
+                *reinterpret_cast<float2 *>(to + 8) = make_float2(y[1][0], y[1][1]);
             }
             float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
             float down = ratio;
@@ -203,8 +217,9 @@ __global__ void __launch_bounds__(AQ_THREADS) k_attn_q8(const AttnQ8P p) {
             for (int n = 0; n < 2; n++) {
                 const float p0 = exp2_approx(y[n][0] - ref), p1 = exp2_approx(y[n][1] - ref);
                 l[mt] += p0 + p1;
-                // (a masked slot counts nothing whatever its block's scale is)
-                aq_split(p0 == 0.f ? 0.f : p0 * pv, p1 == 0.f ? 0.f : p1 * pv, pa[mt][2 * n], pa[mt][2 * n + 1]);
+                float w0 = p0 * pv, w1 = p1 * pv;
+                if (masked) { if (p0 == 0.f) w0 = 0.f; if (p1 == 0.f) w1 = 0.f; }       // (a masked slot counts nothing whatever its block's scale is)
+                aq_split(w0, w1, pa[mt][2 * n], pa[mt][2 * n + 1]);
             }
         }
         // ---- values: the lane's slots are 2q, 2q + 1, 8 + 2q, 9 + 2q
@@ -295,25 +310,44 @@ __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
     pdl_launch();
     pdl_wait();
     if (k_item >= p.items - p.whole) return;                          // (with WPR = 8: the whole CTA)
+    // (the sums are asked for before it is known which splits there are: the others' are dropped.  One way to memory instead of three.)
+    const size_t part0 = (size_t)k_item * p.n_splits * R + r;
+    float top = -INFINITY, mk[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) mk[u] = lane + 32 * u < p.n_splits ? __ldcg(&p.part_ml[part0 + (size_t)(lane + 32 * u) * R]).x : -INFINITY;      // (128 splits at most)
+    constexpr int U = 8;
+    float2 ml[U]; float pv[U][8];
+    auto ask = [&](int k0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = min(k0 + u * WPR, p.n_splits - 1);
+            const size_t at = part0 + (size_t)k * R;
+            ml[u] = __ldcg(&p.part_ml[at]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) if (j < nd) pv[u][j] = __ldcg(p.part + at * hd + lane + 32 * j);
+        }
+    };
+    ask(sub);
     const AqItem wk = aq_item(p, p.whole + k_item * p.n_splits);
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
     const TileB t = aq_tile(s, p.c.n_ctx, p.group, R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, R);
     if (r >= t.n_rows) return;
     const int used = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));
-    const size_t part0 = (size_t)k_item * p.n_splits * R + r;
-    float top = -INFINITY;
-    for (int k = lane; k < used; k += 32) top = fmaxf(top, __ldcg(&p.part_ml[part0 + (size_t)k * R]).x);
+#pragma unroll
+    for (int u = 0; u < 4; u++) if (lane + 32 * u < used) top = fmaxf(top, mk[u]);
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = sub; k < used; k += WPR) {
-        const size_t at = part0 + (size_t)k * R;
-        const float2 ml = __ldcg(&p.part_ml[at]);
-        const float w = exp2_approx(ml.x - ref);
-        sum = fmaf(w, ml.y, sum);
+    for (int k0 = sub; k0 < used; k0 += U * WPR) {
+        if (k0 != sub) ask(k0);
 #pragma unroll
-        for (int j = 0; j < 8; j++) if (j < nd) v[j] = fmaf(w, __ldcg(p.part + at * hd + lane + 32 * j), v[j]);
+        for (int u = 0; u < U; u++) {
+            if (k0 + u * WPR >= used) break;
+            const float w = exp2_approx(ml[u].x - ref);
+            sum = fmaf(w, ml[u].y, sum);
+#pragma unroll
+            for (int j = 0; j < 8; j++) if (j < nd) v[j] = fmaf(w, pv[u][j], v[j]);
+        }
     }
     if (WPR > 1) {
 #pragma unroll
@@ -340,80 +374,156 @@ __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
     if (lane == 0 && p.lse) p.lse[(size_t)tok * p.n_head + h] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
-// weights_out[j] = (j < pos0 ? weights_in[j] : 0) + sum over the sequence's new tokens and the heads of the group of p_j.  A warp keeps 16 slots as
-// B operands, goes over the rows and makes their scores again (the keys a second time, instead of every score written and read).
-// One warp owns a slot: the sum's order is fixed.
+// The accumulated weights where the scores were kept (AqPlan::scores): four slots a thread.  With w_j = sum over the sequence's new tokens and the heads of the
+// group of p_j, weights_out[j] = (j < pos0 ? weights_in[j] : 0) + w_j, rows in their order.
+__global__ void __launch_bounds__(128) k_attn_q8_weights_kept(const AttnQ8P p, const float * w_in, float * w_out) {
+    const int hk = blockIdx.y, i = blockIdx.z, lane = threadIdx.x & 31, j0 = (blockIdx.x * 128 + threadIdx.x) * 4;
+    pdl_launch();
+    pdl_wait();
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, i);
+    const int end = min(s.pos + s.n_new, p.c.n_ctx);
+    if (s.sq < 0 || s.n_new == 0 || blockIdx.x * 512 >= end) return;
+    bool later = false;                                               // of entries that name one sequence the last one counts
+    if (p.b.seq)
+        for (int j = i + 1 + lane; j < p.b.n; j += 32) {
+            const SeqB o = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, j);
+            later |= o.sq == s.sq && o.n_new > 0;
+        }
+    if (__any_sync(0xffffffffu, later) || j0 >= end) return;
+    const size_t at = ((size_t)s.sq * p.c.H + hk) * p.c.n_ctx + j0;  // (n_ctx is a multiple of 16)
+    const bool before = w_in && j0 < s.pos;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 had = before ? make_float4(w_in[at], w_in[at + 1], w_in[at + 2], w_in[at + 3]) : sum;
+    const int rows = s.n_new * p.group;
+#pragma unroll 8
+    for (int r = 0; r < rows; r++) {
+        const int tok = r / p.group, row = (s.first + tok) * p.n_head + hk * p.group + r - tok * p.group;
+        const float lse = __ldcg(p.lse + row);
+        const int sees = aq_sees(s, p.c.n_ctx, tok) - j0;             // (scores of what a row does not see were not all made)
+        const float4 y = __ldcg(reinterpret_cast<const float4 *>(p.scores + (size_t)row * p.score_pitch + j0));
+        if (sees > 0) sum.x += exp2_approx(y.x - lse);
+        if (sees > 1) sum.y += exp2_approx(y.y - lse);
+        if (sees > 2) sum.z += exp2_approx(y.z - lse);
+        if (sees > 3) sum.w += exp2_approx(y.w - lse);
+    }
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w}, h[4] = {had.x, had.y, had.z, had.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (j0 + j < end) w_out[at + j] = (j0 + j < s.pos ? h[j] : 0.f) + v[j];
+}
+
+// weights_out[j] = (j < pos0 ? weights_in[j] : 0) + sum over the sequence's new tokens and the heads of the group of p_j.  The keys are read a second time
+// and the scores made again, instead of every score written and read: a warp has the codes of AQ_WT x 16 slots in registers and goes over the rows, 8 at a
+// time.  One warp owns a slot: the sum's order is fixed.  Bound by the way from one load to the next: a CTA takes several tiles of slots, and where there are no more
+// than 8 rows their queries are made once (8 sequences of 64 heads, 8000 slots: a tile a CTA 47 us, and its loads one after the other).
+static constexpr int AQ_WT = 2, AQ_WSTEP = AQ_WARPS * AQ_WT * 16;
+
 template <int HD>
-__global__ void __launch_bounds__(AQ_THREADS) k_attn_q8_weights(const AttnQ8P p, const float * w_in, float * w_out) {
+__global__ void __launch_bounds__(AQ_THREADS, HD <= 128 ? 4 : 2) k_attn_q8_weights(const AttnQ8P p, const float * w_in, float * w_out) {
     using S = AqShape<HD>;
+    constexpr int NK = 2 * AQ_WT;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, hk = blockIdx.y, i = blockIdx.z;
     pdl_launch();
     pdl_wait();
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, i);
     if (s.sq < 0 || s.n_new == 0) return;
-    if (p.b.seq) {                                                    // of entries that name one sequence the last one counts
-        bool later = false;
+    const int end = min(s.pos + s.n_new, p.c.n_ctx), n_rows = s.n_new * p.group;
+    int j0 = blockIdx.x * AQ_WSTEP + warp * AQ_WT * 16;
+    if (j0 >= end) return;
+    const size_t head = (size_t)s.sq * p.c.H + hk;
+    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD;
+    const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift);
+    uint32_t w[NK][S::KG][S::KW / 4];
+    float sk[AQ_WT], had[NK][2];
+    auto load = [&]() {
+#pragma unroll
+        for (int n = 0; n < NK; n++) {
+            const int8_t * row = kc + (size_t)min(j0 + n * 8 + g, p.c.n_ctx - 1) * HD + q * S::KW;       // (slots behind the cache: its last one; no row sees them)
+#pragma unroll
+            for (int c = 0; c < S::KG; c++) {
+                if constexpr (S::KW == 16) {
+                    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(row + c * 64));
+                    w[n][c][0] = u.x; w[n][c][1] = u.y; w[n][c][2] = u.z; w[n][c][3] = u.w;
+                } else {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(row + c * 32));
+                    w[n][c][0] = u.x; w[n][c][1] = u.y;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int slot = j0 + n * 8 + 2 * q + j;
+                had[n][j] = w_in && g == 0 && slot < min(s.pos, end) ? w_in[head * p.c.n_ctx + slot] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < AQ_WT; n++) sk[n] = __ldg(ks + (min(j0 + n * 16, p.c.n_ctx - 1) >> p.c.shift));
+    };
+    load();
+    bool later = false;                                               // of entries that name one sequence the last one counts
+    if (p.b.seq) {
         for (int j = i + 1 + lane; j < p.b.n; j += 32) {
             const SeqB o = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, j);
             later |= o.sq == s.sq && o.n_new > 0;
         }
-        if (__any_sync(0xffffffffu, later)) return;
+        later = __any_sync(0xffffffffu, later);
     }
-    const size_t head = (size_t)s.sq * p.c.H + hk;
-    const int8_t * kc = p.c.k + head * p.c.n_ctx * HD;
-    const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift);
-    const int end = min(s.pos + s.n_new, p.c.n_ctx), n_rows = s.n_new * p.group;
-    for (int j0 = (blockIdx.x * AQ_WARPS + warp) * 16; j0 < end; j0 += gridDim.x * AQ_STEP) {
-        uint32_t b[2][S::KS][2];
+    uint32_t a[S::KS][4];
+    float f = 0.f, lse = 0.f;
+    int a_row = -1, sees = 0;
+    if (later) return;
+    while (true) {
+        float sum[NK][2];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int c = 0; c < S::KG; c++)
-#pragma unroll
-                for (int w = 0; w < S::KW / 4; w++) {
-                    const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(kc + (size_t)(j0 + n * 8 + g) * HD + c * 4 * S::KW + q * S::KW + w * 4)) ^ 0x80808080u;
-                    b[n][c * (S::KW / 4) + w][0] = q8_lo(u);
-                    b[n][c * (S::KW / 4) + w][1] = q8_hi(u);
-                }
-        const float sk = __ldg(ks + (j0 >> p.c.shift));
-        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        for (int n = 0; n < NK; n++) sum[n][0] = sum[n][1] = 0.f;
         const int tok0 = max(0, j0 - s.pos);                          // the first token that sees one of these slots
         for (int r0 = tok0 * p.group / 8 * 8; r0 < n_rows; r0 += 8) {
-            const int row = r0 + g;
-            const bool there = row < n_rows;
-            uint32_t a[S::KS][4];
-            const float f = aq_load_query<HD>(p, s, row, there, hk, q, a) * p.scale_log2 * sk;
-            const int tok = row / p.group, sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
-            const float lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row % p.group) : 0.f;
-            float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            if (r0 != a_row) {
+                const int row = r0 + g, tok = row / p.group;
+                const bool there = row < n_rows;
+                lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row % p.group) : 0.f;
+                f = aq_load_query<HD>(p, s, row, there, hk, q, a) * p.scale_log2;
+                sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
+                a_row = r0;
+            }
 #pragma unroll
-            for (int k = 0; k < S::KS; k++)
+            for (int n = 0; n < NK; n++) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < 2; n++) mma16816(x[n], a[k][0], a[k][1], a[k][2], a[k][3], b[n][k][0], b[n][k][1]);
+                for (int k = 0; k < S::KS; k++) {
+                    const uint32_t u = w[n][k / (S::KW / 4)][k % (S::KW / 4)] ^ 0x80808080u;
+                    mma16816(x, a[k][0], a[k][1], a[k][2], a[k][3], q8_lo(u), q8_hi(u));
+                }
 #pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx((x[n][j] + x[n][j + 2]) * f - lse);
+                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx((x[j] + x[j + 2]) * (f * sk[n >> 1]) - lse);
+            }
         }
+        const int at = j0;
+        float before[NK][2];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NK; n++) { before[n][0] = had[n][0]; before[n][1] = had[n][1]; }
+        j0 += gridDim.x * AQ_WSTEP;
+        const bool more = j0 < end;
+        if (more) load();                                             // (on its way while these are added up)
+#pragma unroll
+        for (int n = 0; n < NK; n++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], o);
-                const int slot = j0 + n * 8 + 2 * q + j;
-                const size_t at = head * p.c.n_ctx + slot;
-                if (g == 0 && slot < end) w_out[at] = (w_in && slot < s.pos ? w_in[at] : 0.f) + sum[n][j];
+                const int slot = at + n * 8 + 2 * q + j;
+                if (g == 0 && slot < end) w_out[head * p.c.n_ctx + slot] = before[n][j] + sum[n][j];
             }
+        if (!more) return;
     }
 }
 
 // ---- how the work is cut
-struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, lse, ml, part; };     // rows of a tile; bytes of each piece of scratch
+struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole, pitch; size_t words, lse, ml, part, scores; };     // rows of a tile; bytes of each piece of scratch
 
 // CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split so
 // that they fill it, into ranges of at least AQ_LEAST slots.
 static constexpr int AQ_LEAST = 256;
+// Weights: scores of few rows are kept, if they take no more than this (8 sequences of 64 heads and 8000 slots, 16 MB: 28 us for reading the keys again, 6 so)
+static constexpr int64_t AQ_SCORES = int64_t(256) << 20;
 static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     AqPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
@@ -422,7 +532,7 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? AT_KEYS : AQ_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : 2), most = (keys + AQ_LEAST - 1) / AQ_LEAST, rest = items % slots;
+    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd <= 128 && r.R == 8 ? 3 : 2), most = (keys + AQ_LEAST - 1) / AQ_LEAST, rest = items % slots;
     int64_t n = rest ? slots / rest : 1;
     if (n > most) n = most;
     if (n > 128) n = 128;
@@ -435,12 +545,17 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     r.lse = weights ? up((size_t)b.T * n_head * 4) : 0;
     r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
     r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
+    // (a sequence may see more slots than expected: their scores need room too)
+    const int64_t bytes = (int64_t)b.T * n_head * c.n_ctx * 4;
+    const bool kept = weights && !r.tc && bytes <= AQ_SCORES;
+    r.pitch = kept ? c.n_ctx : 0;
+    r.scores = kept ? up((size_t)bytes) : 0;
     return r;
 }
 
 size_t attn_q8_scratch(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     const AqPlan r = aq_plan(c, b, n_head, max_kv, weights);
-    return r.words + r.lse + r.ml + r.part;
+    return r.words + r.lse + r.ml + r.part + r.scores;
 }
 
 template <int HD, int MT>
@@ -469,9 +584,12 @@ static int aq_run(const AttnQ8P & p, const AqPlan & r, const float * w_in, float
         if (p.n_splits <= AQ_JOIN_FEW) PI_CUDA(launch_k(k_attn_q8_join<1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, true, p, r.R));
         else                           PI_CUDA(launch_k(k_attn_q8_join<8>, dim3((unsigned)rows), dim3(256), 0, st, true, p, r.R));
     }
-    if (w_out) {
-        const int keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv;
-        PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((keys + AQ_STEP - 1) / AQ_STEP, p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));
+    if (w_out && p.scores) {
+        PI_CUDA(launch_k(k_attn_q8_weights_kept, dim3((unsigned)((p.c.n_ctx + 511) / 512), p.c.H, p.b.n), dim3(128), 0, st, true, p, w_in, w_out));
+    } else if (w_out) {
+        const int64_t keys = max_kv < 1 ? 1 : max_kv > p.c.n_ctx ? p.c.n_ctx : max_kv, tiles = (keys + AQ_WSTEP - 1) / AQ_WSTEP, of_sms = (int64_t)sm_count() * 8;
+        const int64_t most = (of_sms + (int64_t)p.c.H * p.b.n - 1) / ((int64_t)p.c.H * p.b.n);     // CTAs of a head: two rounds of four an SM
+        PI_CUDA(launch_k(k_attn_q8_weights<HD>, dim3((unsigned)(tiles < most ? tiles : most), p.c.H, p.b.n), dim3(AQ_THREADS), 0, st, true, p, w_in, w_out));
     }
     return PI_OK;
 }
@@ -487,6 +605,7 @@ int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
     s += r.words;
     p.lse = a.w_out ? (float *)s : nullptr;
     p.part_ml = (float2 *)(s + r.lse); p.part = (float *)(s + r.lse + r.ml);
+    p.scores = r.scores ? (float *)(s + r.lse + r.ml + r.part) : nullptr; p.score_pitch = r.pitch;
     switch (a.c.hd) {
         case 64:  return aq_run<64>(p, r, a.w_in, a.w_out, a.max_kv, st);
         case 96:  return aq_run<96>(p, r, a.w_in, a.w_out, a.max_kv, st);

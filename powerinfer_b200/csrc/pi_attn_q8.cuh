@@ -11,6 +11,7 @@ struct AttnQ8P {
     // An item is a tile of rows of a KV head of an entry.  The first `whole` items are a CTA each, the others n_splits: ranges of `split` slots.
     int split, n_splits, row_tiles, items, whole;
     float * part; float2 * part_ml; float * lse;                      // [split item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
+    float * scores; int score_pitch;                                  // (null: not kept) the rows' scores in bits, [T * n_head][pitch]
     unsigned int * status;                                            // tcgen05 alone: bit 4, a wait ran out
 };
 
