@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(128) k_attn_q8_weights_kept(const AttnQ8P p, c
 static constexpr int AQ_WT = 2, AQ_WSTEP = AQ_WARPS * AQ_WT * 16;
 
 template <int HD>
-__global__ void __launch_bounds__(AQ_THREADS, HD <= 128 ? 4 : 2) k_attn_q8_weights(const AttnQ8P p, const float * w_in, float * w_out) {
+__global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) k_attn_q8_weights(const AttnQ8P p, const float * w_in, float * w_out) {
     using S = AqShape<HD>;
     constexpr int NK = 2 * AQ_WT;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3, hk = blockIdx.y, i = blockIdx.z;

@@ -166,26 +166,50 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
             else if (from == 0 && m >> lane & 1u) kept[j] = j;
         }
         __syncthreads();
-        for (int x = p.keep / 32 + warp; x < words; x += warps) {
-            const uint32_t m = below(x), e = above[x] & ~m;
-            const int rank = (m ? 0 : (int)equal[x]) + __popc(e & ((1u << lane) - 1u)) - from;
-            if ((e >> lane & 1u) && rank >= 0 && rank < cached) {
-                const int to = keys[rank];
-                kept[to] = x * 32 + lane;
-                if (w_out) w_out[to] = w[x * 32 + lane];
+        for (int xb = p.keep / 32 + warp; xb < words; xb += 8 * warps) {
+            int to[8]; float v[8];                                    // (eight words' weights on their way; nothing behind the budget is written)
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int x = xb + u * warps;
+                to[u] = -1;
+                if (x >= words) continue;
+                const uint32_t m = below(x), e = above[x] & ~m;
+                const int rank = (m ? 0 : (int)equal[x]) + __popc(e & ((1u << lane) - 1u)) - from;
+                if ((e >> lane & 1u) && rank >= 0 && rank < cached) {
+                    to[u] = keys[rank];
+                    if (w_out) v[u] = __ldcg(w + x * 32 + lane);
+                }
             }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (to[u] >= 0) {
+                    kept[to[u]] = (xb + u * warps) * 32 + lane;
+                    if (w_out) w_out[to[u]] = v[u];
+                }
         }
         __syncthreads();
     }
     if (w_out && w_out != w)
-        for (int x = warp; x < keep_words; x += warps) if (above[x] & below(x) & 1u << lane) w_out[x * 32 + lane] = w[x * 32 + lane];
+        for (int xb = warp; xb < keep_words; xb += 8 * warps) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) { const int x = xb + u * warps; if (x < keep_words && x * 32 + lane < p.keep) v[u] = __ldcg(w + x * 32 + lane); }
+#pragma unroll
+            for (int u = 0; u < 8; u++) { const int x = xb + u * warps; if (x < keep_words && (above[x] & below(x)) >> lane & 1u) w_out[x * 32 + lane] = v[u]; }
+        }
 }
 
+// Four codes times ratio, rounded to the nearest whole number.  Whole numbers become FP32 and back by their place in the mantissa (2^23 + 128 + code; the
+// product + 1.5 x 2^23): conversions run at an eighth of the rate of sums, and half of the kernel was them.
 __device__ __forceinline__ uint32_t ev_scale(uint32_t c, float ratio) {
-    uint32_t r = 0;
+    const uint32_t u = c ^ 0x80808080u;
+    uint32_t r[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) r |= (uint32_t)(__float2int_rn((float)(int8_t)(c >> (8 * j)) * ratio) & 255) << (8 * j);
-    return r;
+    for (int j = 0; j < 4; j++) {
+        const float f = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + j)), 8388736.f);
+        r[j] = __float_as_uint(__fadd_rn(__fmul_rn(f, ratio), 12582912.f));
+    }
+    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
 }
 
 static constexpr int MV_THREADS = 256, MV_U = 8;                      // pieces of 16 codes on their way, a lane
