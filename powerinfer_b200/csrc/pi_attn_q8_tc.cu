@@ -119,6 +119,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         return ok;
     };
 
+    // ---- codes: keys and values in turn.  (Slots behind the cache are not read: their halves are of anything, and count nothing.)
+    auto ask = [&](int i) {
+        const int slot = i % AT_RAW, j0 = k0 + (i >> 1) * AT_KEYS;
+        const unsigned bytes = (unsigned)min(AT_KEYS, p.c.n_ctx - j0) * HD;
+        mbar_expect_tx(s_rfull + slot, bytes);
+        bulk_g2s(smem_raw + (raw - smem_u32(smem_raw)) + (size_t)slot * AT_KEYS * HD, (i & 1 ? p.c.v : p.c.k) + (head * p.c.n_ctx + j0) * HD, bytes, s_rfull + slot);
+    };
+    if (warp == 1 && lane == 0) for (int i = 0; i < min(AT_RAW, 2 * n_tiles); i++) ask(i);
     // ---- the halves of a tile: a warp takes 8 rows x 64 columns, so that what it stores together meets all banks
     const int ct = tid - 640, cr = (ct >> 2) & 63, cc = ct & 3;       // row (of 64), piece of 16 columns of a thread
     const uint32_t from0 = (uint32_t)(cr * HD + cc * 16), to0 = (uint32_t)cr * 128u + (uint32_t)(((2 * cc) ^ (cr & 7)) * 16);
@@ -142,18 +150,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         const bool mine = warp >= 4 && warp < 20;
         const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
         float * rows = reinterpret_cast<float *>(smem_raw + (kbuf - smem_u32(smem_raw)));
-        constexpr int RPW = 32 / LPR * 4;                             // rows of a warp's turn: four loads on their way
-#pragma unroll 1
-        for (int r0 = warp * RPW; r0 < AT_ROWS; r0 += AT_THREADS / 32 * RPW) {
-            float4 u[4];
+        constexpr int RPW = 8, NL = RPW / (32 / LPR);                 // rows of a warp, all on their way at once
+        if (warp < AT_ROWS / RPW) {
+            const int r0 = warp * RPW;
+            float4 u[NL];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < NL; k++) {
                 const int q = r0 + k * (32 / LPR) + lane / LPR, row = t.first + q, tok = row / p.group;
                 u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (q < t.n_rows) u[k] = aq_query(p.xtype, p.q, (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD + lane % LPR * 4);
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) *reinterpret_cast<float4 *>(rows + (r0 + k * (32 / LPR) + lane / LPR) * PITCH + lane % LPR * 4) = u[k];
+            for (int k = 0; k < NL; k++) *reinterpret_cast<float4 *>(rows + (r0 + k * (32 / LPR) + lane / LPR) * PITCH + lane % LPR * 4) = u[k];
         }
         __syncthreads();
         float4 v[NQ / 4];
@@ -242,16 +250,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             __syncwarp();
         } else if (warp == 1) {
             // ============================================================= codes
-            const int8_t * kc = p.c.k + (head * p.c.n_ctx + k0) * HD, * vc = p.c.v + (head * p.c.n_ctx + k0) * HD;
-            int i = 0;
-            for (; i < 2 * n_tiles; i++) {                            // (slots behind the cache are not read: their halves are of anything, and count nothing)
+            int i = min(AT_RAW, 2 * n_tiles);
+            for (; i < 2 * n_tiles; i++) {
                 const int slot = i % AT_RAW;
                 if (!wait(s_rempty + slot, i / AT_RAW & 1 ^ 1)) break;
-                if (lane == 0) {
-                    const unsigned bytes = (unsigned)min(AT_KEYS, p.c.n_ctx - k0 - (i >> 1) * AT_KEYS) * HD;
-                    mbar_expect_tx(s_rfull + slot, bytes);
-                    bulk_g2s(smem_raw + (raw - smem_u32(smem_raw)) + (size_t)slot * AT_KEYS * HD, (i & 1 ? vc : kc) + (size_t)(i >> 1) * AT_KEYS * HD, bytes, s_rfull + slot);
-                }
+                if (lane == 0) ask(i);
                 __syncwarp();
             }
             if (lane == 0) ring_land(s_rfull, i, AT_RAW);
@@ -282,11 +285,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             const float back = largest > 0.f ? AT_P / largest : 0.f, wv = sv == 0.f ? 0.f : sv * back, wk = sk;
             if (i + 2 < n_tiles) scales(i + 2, sk, sv);
             const bool masked = k0 + i * AT_KEYS + half * 64 + 64 > least;       // (of this warp's rows)
+            const int parts = max(0, min(4, (k1 - k0 - i * AT_KEYS - half * 64 + 15) >> 4));      // of 16 slots: the products take no more
             wait(s_qk + b, i >> 1 & 1);
             tc_fence_after();
             float m = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 2; c++) {
+            for (int c = 0; 2 * c < parts; c++) {
                 float x[32];
                 at_ld32(x, mine + 32 * c);
 #pragma unroll
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             float2 l[2] = {f2(0.f), f2(0.f)};
             auto exps = [&](auto with_mask) {
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < parts; c++) {
                     float x[16];
                     tc_ld16(x, mine + 16 * c);
                     uint32_t hl[16];                                  // upper parts of 16 slots, then lower parts
