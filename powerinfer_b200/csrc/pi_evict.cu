@@ -6,16 +6,17 @@
 // for the order of slots.  A block's scale becomes the largest of the scales of the rows that are in it now, and codes of other scales
 // rne(code * (scale / that)).
 //
-// k_evict_select, a CTA per sequence and KV head: the weights as ordered integers in shared memory; the threshold from three histograms of 11, 11 and 10
-// bits (whole numbers: their order does not matter); then bit maps of what is above it and of what equals it, sums over their words, and the holes' slots
-// as a list from which every mover takes its place.  k_evict_move, a warp per block: rows are gathered and scaled.  Bound by latency: the bytes are those of the
-// weights and of the moved rows.
+// k_evict_select, a CTA per sequence and KV head: the weights as ordered integers in registers, EV_REGS a thread (longer sequences: that many at a time, read
+// again); the threshold from three histograms of 11, 11 and 10 bits (whole numbers: their order does not matter); then bit maps of what is above it and of
+// what equals it, sums over their words, and the holes' slots as a list from which every mover takes its place.  k_evict_move, a warp per block: rows are gathered
+// and scaled.  Few heads: bound by the instructions that one SM issues for a head's slots.  (A cluster of eight SMs a head was slower: the histograms travel.)
+// Many: by the bytes of the moved rows.
 #include "pi_kv_q8.cuh"
 
 namespace pi {
 
-static constexpr int EV_THREADS = 1024;                               // at most
-static constexpr int EV_CACHED = 36864;                               // weights that shared memory holds beside the maps of 262144 slots
+static constexpr int EV_THREADS = 1024, EV_REGS = 16;                 // threads at most
+static constexpr int EV_LIST = 16384;                                 // holes that the list holds at a time
 static constexpr int EV_BINS = 2048;
 
 // order of weights as unsigned numbers: -0 as 0, what is not a number above all others; 0 is no weight's
@@ -37,15 +38,15 @@ __device__ __forceinline__ int ev_before(int v, int * s_red) {
     return before + incl - v;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, int cached) {
+__global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, int listed) {
     extern __shared__ uint32_t ev_smem[];
     __shared__ int s_red[32];
-    __shared__ int s_bin[EV_BINS];
+    __shared__ __align__(16) int s_bin[EV_BINS];
     __shared__ int s_found[2];
-    const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+    const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5, CHUNK = EV_REGS * nt;
     const int h = blockIdx.x, i = blockIdx.y, n_ctx = p.c.n_ctx, words_max = (n_ctx + 31) / 32;
     uint32_t * above = ev_smem, * equal = above + words_max;         // bit maps of the slots
-    uint32_t * keys = equal + words_max;                              // later the holes' slots
+    int * list = (int *)(equal + words_max);                          // the holes' slots
     pdl_launch();
     pdl_wait();
     int32_t * kept = p.kept + ((size_t)i * p.c.H + h) * p.keep;
@@ -69,25 +70,17 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
     }
     // ---- candidates: slots c0 .. c1 - 1, of which `need` stay.  Others have the key 0.
     const int c0 = p.n_sink, c1 = len - p.n_recent;
-    int need = p.keep - p.n_sink - p.n_recent;
-    const bool here = len <= cached;
-    auto slot_key = [&](int j, float x) { return j >= c0 && j < c1 ? ev_key(x) : 0u; };
-    if (here) {
-        int j = tid;
-        for (; j + 7 * nt < len; j += 8 * nt) {                       // (all on their way before the first is looked at)
-            float x[8];
+    int need = p.keep - p.n_sink - p.n_recent, have = -1;
+    uint32_t key[EV_REGS];                                            // of the slots have + u * nt + tid
+    auto load = [&](int from) {
+        if (from == have) return;
+        have = from;
+        float x[EV_REGS];
 #pragma unroll
-            for (int u = 0; u < 8; u++) x[u] = __ldcg(w + j + u * nt);
+        for (int u = 0; u < EV_REGS; u++) { const int j = from + u * nt + tid; x[u] = j >= c0 && j < c1 ? __ldcg(w + j) : 0.f; }
 #pragma unroll
-            for (int u = 0; u < 8; u++) keys[j + u * nt] = slot_key(j + u * nt, x[u]);
-        }
-        float x[8];
-#pragma unroll
-        for (int u = 0; u < 8; u++) x[u] = j + u * nt < len ? __ldcg(w + j + u * nt) : 0.f;
-#pragma unroll
-        for (int u = 0; u < 8; u++) if (j + u * nt < len) keys[j + u * nt] = slot_key(j + u * nt, x[u]);
-    }
-    auto key = [&](int j) { return here ? keys[j] : slot_key(j, __ldcg(w + j)); };
+        for (int u = 0; u < EV_REGS; u++) { const int j = from + u * nt + tid; key[u] = j >= c0 && j < c1 ? ev_key(x[u]) : 0u; }
+    };
     // ---- t, the need-th largest key, and how many of those that equal it stay
     uint32_t t = 0xffffffffu;
     if (need > 0) {
@@ -97,10 +90,13 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
             const int bins = shift ? EV_BINS : 1024, hi = shift == 21 ? 32 : shift == 10 ? 21 : 10;       // bits shift .. hi - 1
             for (int x = tid; x < EV_BINS; x += nt) s_bin[x] = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int j = tid; j < len; j += nt) {
-                const uint32_t k = key(j);
-                if (k != 0u && (hi == 32 || k >> hi == t >> hi)) atomicAdd(&s_bin[k >> shift & (uint32_t)(bins - 1)], 1);
+            for (int from = 0; from < len; from += CHUNK) {
+                load(from);
+#pragma unroll
+                for (int u = 0; u < EV_REGS; u++) {
+                    const uint32_t k = key[u];
+                    if (k != 0u && (hi == 32 || k >> hi == t >> hi)) atomicAdd(&s_bin[k >> shift & (uint32_t)(bins - 1)], 1);
+                }
             }
             __syncthreads();
             // thread x has the x-th bins from above: the bin in which the need-th key lies
@@ -121,17 +117,18 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
     }
     // ---- bit maps over the slots
     const int words = (len + 31) / 32;
-    for (int x = warp; x < words; x += warps) {
-        const int j = x * 32 + lane;
-        bool a = false, e = false;
-        if (j < len) {
-            if (j < c0 || j >= c1) a = true;
-            else if (need > 0) { const uint32_t k = key(j); a = k > t; e = k == t; }
+    for (int from = 0; from < len; from += CHUNK) {
+        load(from);
+#pragma unroll
+        for (int u = 0; u < EV_REGS; u++) {
+            const int k = (from + u * nt + tid) >> 5;
+            const uint32_t am = __ballot_sync(0xffffffffu, key[u] > t), em = __ballot_sync(0xffffffffu, key[u] == t);      // (t is never 0)
+            if (lane == 0 && k < words) { above[k] = am; equal[k] = em; }
         }
-        const uint32_t am = __ballot_sync(0xffffffffu, a), em = __ballot_sync(0xffffffffu, e);
-        if (lane == 0) { above[x] = am; equal[x] = em; }
     }
     __syncthreads();
+    // slots of word k that are below `end`
+    auto under = [&](int k, int end) { return k * 32 + 32 <= end ? 0xffffffffu : k * 32 >= end ? 0u : (1u << (end - k * 32)) - 1u; };
     // ---- of the equals the first ones; then `equal` takes the number of holes (below the budget) or movers (behind it) before each word
     const int per = (words + nt - 1) / nt, x0 = min(tid * per, words), x1 = min(x0 + per, words);
     int mine = 0;
@@ -142,10 +139,10 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
         const int n = __popc(e);
         if (n > left) { take = 0u; for (int k = 0; k < left; k++) { const uint32_t b = e & (0u - e); take |= b; e ^= b; } }
         left = max(0, left - n);
-        above[x] |= take;
+        above[x] |= take | under(x, c0) | (under(x, len) & ~under(x, c1));
     }
     const int keep_words = (p.keep + 31) / 32;
-    auto below = [&](int x) { return x * 32 + 32 <= p.keep ? 0xffffffffu : x * 32 >= p.keep ? 0u : (1u << (p.keep - x * 32)) - 1u; };
+    auto below = [&](int x) { return under(x, p.keep); };
     int holes = 0, movers = 0;
     for (int x = x0; x < x1; x++) { const uint32_t m = below(x); holes += __popc(~above[x] & m); movers += __popc(above[x] & ~m); }
     int before_h = ev_before(holes, s_red), before_m = ev_before(movers, s_red);
@@ -156,46 +153,46 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(const EvictArgs p, 
         before_h += __popc(~above[x] & m);
         before_m += __popc(above[x] & ~m);
     }
-    // ---- who takes which place: the holes of ranks `from` and on as a list, from which the movers of the same ranks read
+    // ---- who takes which place: the holes of ranks `first` and on as a list, from which the movers of the same ranks read
     __syncthreads();
-    for (int from = 0; from < p.keep; from += cached) {
-        for (int x = warp; x < keep_words; x += warps) {
-            const uint32_t m = below(x), e = ~above[x] & m;
-            const int rank = (int)equal[x] + __popc(e & ((1u << lane) - 1u)) - from, j = x * 32 + lane;
-            if (e >> lane & 1u) { if (rank >= 0 && rank < cached) keys[rank] = j; }
-            else if (from == 0 && m >> lane & 1u) kept[j] = j;
+    for (int first = 0; first < p.keep; first += listed) {
+        for (int k = warp; k < keep_words; k += warps) {
+            const uint32_t m = below(k), e = ~above[k] & m;
+            const int rank = (int)equal[k] + __popc(e & ((1u << lane) - 1u)) - first, j = k * 32 + lane;
+            if (e >> lane & 1u) { if (rank >= 0 && rank < listed) list[rank] = j; }
+            else if (first == 0 && m >> lane & 1u) kept[j] = j;
         }
         __syncthreads();
-        for (int xb = p.keep / 32 + warp; xb < words; xb += 8 * warps) {
+        for (int kb = p.keep / 32 + warp; kb < words; kb += 8 * warps) {
             int to[8]; float v[8];                                    // (eight words' weights on their way; nothing behind the budget is written)
 #pragma unroll
             for (int u = 0; u < 8; u++) {
-                const int x = xb + u * warps;
+                const int k = kb + u * warps;
                 to[u] = -1;
-                if (x >= words) continue;
-                const uint32_t m = below(x), e = above[x] & ~m;
-                const int rank = (m ? 0 : (int)equal[x]) + __popc(e & ((1u << lane) - 1u)) - from;
-                if ((e >> lane & 1u) && rank >= 0 && rank < cached) {
-                    to[u] = keys[rank];
-                    if (w_out) v[u] = __ldcg(w + x * 32 + lane);
+                if (k >= words) continue;
+                const uint32_t m = below(k), e = above[k] & ~m;
+                const int rank = (m ? 0 : (int)equal[k]) + __popc(e & ((1u << lane) - 1u)) - first;
+                if ((e >> lane & 1u) && rank >= 0 && rank < listed) {
+                    to[u] = list[rank];
+                    if (w_out) v[u] = __ldcg(w + k * 32 + lane);
                 }
             }
 #pragma unroll
             for (int u = 0; u < 8; u++)
                 if (to[u] >= 0) {
-                    kept[to[u]] = (xb + u * warps) * 32 + lane;
+                    kept[to[u]] = (kb + u * warps) * 32 + lane;
                     if (w_out) w_out[to[u]] = v[u];
                 }
         }
         __syncthreads();
     }
     if (w_out && w_out != w)
-        for (int xb = warp; xb < keep_words; xb += 8 * warps) {
+        for (int kb = warp; kb < keep_words; kb += 8 * warps) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) { const int x = xb + u * warps; if (x < keep_words && x * 32 + lane < p.keep) v[u] = __ldcg(w + x * 32 + lane); }
+            for (int u = 0; u < 8; u++) { const int j = (kb + u * warps) * 32 + lane; if (j < p.keep) v[u] = __ldcg(w + j); }
 #pragma unroll
-            for (int u = 0; u < 8; u++) { const int x = xb + u * warps; if (x < keep_words && (above[x] & below(x)) >> lane & 1u) w_out[x * 32 + lane] = v[u]; }
+            for (int u = 0; u < 8; u++) { const int j = (kb + u * warps) * 32 + lane; if (j < p.keep && above[j >> 5] >> lane & 1u) w_out[j] = v[u]; }
         }
 }
 
@@ -270,18 +267,18 @@ __global__ void __launch_bounds__(MV_THREADS) k_evict_move(const EvictArgs p) {
 }
 
 int launch_kv_evict_q8(const EvictArgs & a, cudaStream_t st) {
-    const int words = (a.c.n_ctx + 31) / 32, cached = a.c.n_ctx < EV_CACHED ? a.c.n_ctx : EV_CACHED;
-    const size_t smem = (size_t)words * 8 + (size_t)cached * 4;
+    const int words = (a.c.n_ctx + 31) / 32, listed = a.keep < EV_LIST ? a.keep : EV_LIST;
+    const size_t smem = (size_t)words * 8 + (size_t)listed * 4;
     // short sequences: smaller CTAs, of which an SM holds several
     const int threads = a.c.n_ctx <= 4096 ? 256 : EV_THREADS;
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        PI_CUDA(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024));
+        PI_CUDA(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_evict_select, dim3(a.c.H, a.n), dim3(threads), smem, st, true, a, cached));
+    PI_CUDA(launch_k(k_evict_select, dim3(a.c.H, a.n), dim3(threads), smem, st, true, a, listed));
     const int64_t units = (int64_t)2 * a.c.H * (a.keep >> a.c.shift);
     PI_CUDA(launch_k(k_evict_move, dim3((unsigned)((units + MV_THREADS / 32 - 1) / (MV_THREADS / 32)), a.n), dim3(MV_THREADS), 0, st, true, a));
     return PI_OK;
