@@ -209,7 +209,7 @@ __device__ __forceinline__ uint32_t ev_scale(uint32_t c, float ratio) {
     return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
 }
 
-static constexpr int MV_THREADS = 256, MV_U = 8;                      // pieces of 16 codes on their way, a lane
+static constexpr int MV_THREADS = 256, MV_U = 4;                      // pieces of 16 codes on their way, a lane
 
 __global__ void __launch_bounds__(MV_THREADS) k_evict_move(const EvictArgs p) {
     const int lane = threadIdx.x & 31, B = p.c.block, blocks = p.keep >> p.c.shift;
@@ -240,20 +240,26 @@ __global__ void __launch_bounds__(MV_THREADS) k_evict_move(const EvictArgs p) {
     const int hd = p.c.hd, per_row = hd / 16, n16 = B * per_row;
     __syncwarp();
     if (lane == 0 && now != old) scale[b] = now;
+    int row = lane / per_row, part = lane - row * per_row;            // of a lane's next piece; 32 pieces on
+    const int row_on = 32 / per_row, part_on = 32 - row_on * per_row;
     for (int e0 = 0; e0 < n16; e0 += MV_U * 32) {
         uint4 c[MV_U]; float ratio[MV_U]; int to[MV_U];
 #pragma unroll
         for (int u = 0; u < MV_U; u++) {
-            const int e = e0 + u * 32 + lane, r = min(e / per_row, B - 1), piece = e - r * per_row;
+            const int r = min(row, B - 1), piece = part;
+            const bool in = row < B;
+            row += row_on; part += part_on;
+            if (part >= per_row) { part -= per_row; row++; }
             int from = -1; float s = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
+                if (k * 32 >= B) break;
                 const int f = __shfl_sync(0xffffffffu, src[k], r & 31); const float o = __shfl_sync(0xffffffffu, of[k], r & 31);
                 if (r >> 5 == k) { from = f; s = o; }
             }
             to[u] = -1;
             // (a row that stays is written where the block's steps grew; behind the sequence's end nothing is)
-            if (e < n16 && from >= 0 && (from != b * B + r || now != s)) {
+            if (in && from >= 0 && (from != b * B + r || now != s)) {
                 to[u] = r * hd + piece * 16;
                 ratio[u] = s == now ? 1.f : s / now;
                 c[u] = *reinterpret_cast<const uint4 *>(codes + (size_t)from * hd + piece * 16);
@@ -270,7 +276,8 @@ int launch_kv_evict_q8(const EvictArgs & a, cudaStream_t st) {
     const int words = (a.c.n_ctx + 31) / 32, listed = a.keep < EV_LIST ? a.keep : EV_LIST;
     const size_t smem = (size_t)words * 8 + (size_t)listed * 4;
     // short sequences: smaller CTAs, of which an SM holds several
-    const int threads = a.c.n_ctx <= 4096 ? 256 : EV_THREADS;
+    int threads = 128;
+    while (threads < EV_THREADS && threads * EV_REGS < a.c.n_ctx) threads *= 2;
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
