@@ -276,11 +276,13 @@ def _here(*tensors):
 def _row_matrix(t: torch.Tensor, what: str, width: int = 0):
     """t [T, n] (or [T, heads, head_dim]) as rows that the kernels take, 16-byte aligned and a row's values side by side (a copy where it is not):
     (tensor, address, rows, values of a row, values between rows, type)"""
-    if t.dim() == 3:
+    shape = t.shape
+    if len(shape) == 3:
         t = t.flatten(1)
-    if t.dim() != 2:
+        shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{what} must have 2 or 3 dimensions: rows of heads")
-    T, n = t.shape
+    T, n = shape
     xtype = _ROW_TYPES.get(t.dtype)
     if xtype is None:
         raise ValueError(f"{what} is {t.dtype}: float32 or float16 is needed")
@@ -337,7 +339,7 @@ def rope_ext(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, freqs: 
         if q_at != q.data_ptr():
             raise ValueError("in place needs rows that are 16-byte aligned")
     else:
-        yq, yq_step = xq.new_empty((T, nq)), nq
+        yq, yq_step = torch.empty_like(xq), nq                       # (contiguous: xq's rows are, or lie apart)
         yq_at = yq.data_ptr()
     if k is None:
         _here(xq, pos, f)
@@ -352,7 +354,7 @@ def rope_ext(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, freqs: 
         if k_at != k.data_ptr():
             raise ValueError("in place needs rows that are 16-byte aligned")
     else:
-        yk, yk_step = xk.new_empty((T, nk)), nk
+        yk, yk_step = torch.empty_like(xk), nk
         yk_at = yk.data_ptr()
     _here(xq, xk, pos, f)
     check(lib.pi_rope_ext(xtype, q_at, q_step, nq // head_dim, yq_at, yq_step, k_at, k_step, nk // head_dim, yk_at, yk_step, T, head_dim, 2 * f.numel(),
@@ -410,8 +412,8 @@ def kv_load_q8(cache: KvCacheQ8, q_start: torch.Tensor, pos0: torch.Tensor, T: i
     width, xtype = cache.n_head_kv * cache.head_dim, _ROW_TYPES.get(dtype)
     if xtype is None:
         raise ValueError("values are read as float32 or float16")
-    k = cache.k.new_empty((T, width), dtype=dtype)
-    v = cache.k.new_empty((T, width), dtype=dtype)
+    k = cache.k_scale.new_empty(T, width) if dtype is torch.float32 else cache.k_scale.new_empty(T, width, dtype=dtype)
+    v = torch.empty_like(k)
     _here(cache.k, q_start, pos0, seq)
     check(lib.pi_kv_load_q8(cache.c, _batch(q_start, pos0, seq, T, max_new), xtype, k.data_ptr(), width, v.data_ptr(), width, _stream()))
     return k, v
@@ -436,14 +438,14 @@ def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0:
     if n % hd:
         raise ValueError(f"q has rows of {n} values: heads of {hd} are needed")
     if out is None:
-        out = q.new_empty((T, n))
+        out = torch.empty_like(q)
     elif out.shape != (T, n) or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and type")
     w_in, w_out = _slot_weights(weights_in, cache), _slot_weights(weights_out, cache)
     _here(cache.k, q, out, q_start, pos0, seq, weights_in, weights_out)
     b, most = _batch(q_start, pos0, seq, T, max_new), cache.n_ctx if max_kv is None else max_kv
     need = lib.pi_attention_q8_workspace_bytes(cache.c, b, n // hd, most, 0 if w_out is None else 1)
-    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    ws = cache.k.new_empty(need) if need else None
     check(lib.pi_attention_q8(cache.c, b, xtype, q_at, q_step, n // hd, most, hd ** -0.5 if scale is None else scale, out.data_ptr(), n, w_in, w_out,
                               None if ws is None else ws.data_ptr(), need, _stream()))
     return out
@@ -457,7 +459,7 @@ def kv_evict_q8(cache: KvCacheQ8, weights: torch.Tensor, lens: torch.Tensor, kee
     n = lens.numel()
     w, w_out = _slot_weights(weights, cache), _slot_weights(weights_out, cache)
     _here(cache.k, weights, weights_out, lens, seq)
-    kept = lens.new_empty((n, cache.n_head_kv, max(0, keep)))
+    kept = lens.new_empty(n, cache.n_head_kv, max(0, keep))
     check(lib.pi_kv_evict_q8(cache.c, _ints(lens, n, "lens"), None if seq is None else _ints(seq, n, "seq"), n, keep, n_sink, n_recent, w, w_out,
                              kept.data_ptr(), _stream()))
     return kept
