@@ -121,7 +121,7 @@ int pi_sparse_ffn(int wtype, const void * up, const void * gate, const void * do
  * overlap on the GPU (different streams, or different host threads) race on it, so serialise them. */
 size_t pi_axpy_static_max_bytes(void);
 
-/* Did the last pi_mul_mat / pi_predictor / pi_mul_mat_idx / pi_axpy / pi_sparse_ffn that used `workspace` (of at least
+/* Did the last pi_mul_mat / pi_predictor / pi_mul_mat_idx / pi_axpy / pi_sparse_ffn (or pi_attention_q8, see there) that used `workspace` (of at least
  * pi_workspace_bytes) finish all its bounded device-side waits (the
  * batch kernels stream rows through rings of bulk copies guarded by waits that give up after a limit rather than hang)?
  * PI_OK, or PI_ERR_TIMEOUT with the status bits in pi_last_error(): the call's result is then incomplete.  workspace NULL:
@@ -200,7 +200,8 @@ typedef struct {
 /* Consecutive tokens of n sequences, of different numbers: entry i is rows q_start[i] .. q_start[i + 1] - 1 of the row arrays (T rows), in slots
  * pos0[i] and on of sequence seq[i] (seq NULL: i).  q_start int32 [n + 1], seq and pos0 int32 [n], on the device.  max_new: an upper bound of the tokens
  * of an entry (tokens beyond it are not handled).  An entry whose sequence or first slot the cache lacks is not stored, attends to
- * nothing and reads zeros; so do tokens whose slots lie behind n_ctx.  Rows of no entry are left as they were. */
+ * nothing and reads zeros; so do tokens whose slots lie behind n_ctx.  Rows of no entry are left as they were; entries' rows must not overlap where
+ * something is written to them. */
 typedef struct {
     const int32_t * q_start, * seq, * pos0;
     int n, T, max_new;
@@ -222,7 +223,9 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
  * weights_out F32 [n_seq, n_head_kv, n_ctx] (NULL: none): for every slot that an entry's tokens see the sum of its probabilities over
  * those tokens and the heads of the group, plus weights_in (same shape, may be the same array; NULL: 0) for slots before pos0; the sums' order is
  * fixed.  Other elements are left as they were.  Of entries that name one sequence the last one with tokens counts.
- * workspace: pi_attention_q8_workspace_bytes with the same arguments (`weights`: whether weights_out is given), 256-byte aligned; 0 bytes may be NULL. */
+ * workspace: pi_attention_q8_workspace_bytes with the same arguments (`weights`: whether weights_out is given), 256-byte aligned; 0 bytes may be NULL.
+ * From 64 query rows a KV head on (head_dim 64 and 128), pi_op_status(workspace) tells whether all bounded waits inside the kernel completed; the rows of one that
+ * did not are NaN. */
 size_t pi_attention_q8_workspace_bytes(const pi_kv_q8 * cache, const pi_kv_batch * batch, int n_head, int max_kv, int weights);
 int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, const void * q, int64_t q_stride, int n_head, int max_kv, float scale,
                     void * out, int64_t out_stride, const float * weights_in, float * weights_out,

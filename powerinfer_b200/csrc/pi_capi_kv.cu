@@ -31,6 +31,15 @@ static int check_rows(const void * x, int64_t stride, int64_t width, int xtype, 
                "%s: %s must be 16-byte aligned, rows of %lld values at least, a multiple of 16 bytes apart", who, what, (long long)width);
     return PI_OK;
 }
+// whether rows of two arrays (T of them, `stride` values apart, `width` wide, `size` bytes a value) share memory; columns of one wider matrix need not
+static bool rows_meet(const void * a, int64_t sa, int64_t wa, const void * b, int64_t sb, int64_t wb, int64_t T, int64_t size) {
+    if (!a || !b || T <= 0) return false;
+    const int64_t a0 = (int64_t)(uintptr_t)a, b0 = (int64_t)(uintptr_t)b, a1 = a0 + ((T - 1) * sa + wa) * size, b1 = b0 + ((T - 1) * sb + wb) * size;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (sa != sb || T == 1) return true;
+    const int64_t pitch = sa * size, at = ((b0 - a0) % pitch + pitch) % pitch;      // where b's rows begin in a's
+    return at < wa * size || at + wb * size > pitch;
+}
 static int check_batch(const pi_kv_batch * b, RaggedB & o, const char * who) {
     PI_REQUIRE(b && b->T >= 0 && b->T <= KV_BIG && b->n >= 0 && b->n <= 65535 && b->max_new >= 0 && (b->n == 0 || (b->q_start && b->pos0)),
                "%s: bad batch (0 <= T <= 2^30, 0 <= n <= 65535, q_start and pos0 given)", who);
@@ -78,7 +87,7 @@ int pi_rope_ext(int xtype, const void * q, int64_t q_stride, int n_head, void * 
                "rope_ext: bad arguments (keys come with n_head_kv > 0, or neither)");
     if (T == 0) return PI_OK;
     PI_REQUIRE(pos && freqs && aligned(freqs, 8), "rope_ext: positions and frequencies are needed");
-    const size_t size = xtype == PI_TYPE_F16 ? 2 : 4;
+    const int64_t size = xtype == PI_TYPE_F16 ? 2 : 4;
     RopeExtArgs a;
     const void * x[2] = {q, k}; void * y[2] = {q_out, k_out};
     const int64_t xs[2] = {q_stride, k_stride}, ys[2] = {q_out_stride, k_out_stride};
@@ -90,11 +99,12 @@ int pi_rope_ext(int xtype, const void * q, int64_t q_stride, int n_head, void * 
         if ((rc = check_rows(x[i], xs[i], width, xtype, "rope_ext", i ? "k" : "q"))) return rc;
         if ((rc = check_rows(y[i], ys[i], width, xtype, "rope_ext", i ? "k_out" : "q_out"))) return rc;
         // in place, or apart: rows that overlap otherwise would be read after they were written
-        const char * x0 = (const char *)x[i], * y0 = (const char *)y[i];
-        const bool in_place = x0 == y0 && xs[i] == ys[i];
-        const char * x1 = x0 + ((size_t)(T - 1) * xs[i] + width) * size, * y1 = y0 + ((size_t)(T - 1) * ys[i] + width) * size;
-        PI_REQUIRE(in_place || x1 <= y0 || y1 <= x0, "rope_ext: %s overlaps its result (in place needs the same address and stride)", i ? "k" : "q");
+        const bool in_place = x[i] == y[i] && xs[i] == ys[i];
+        PI_REQUIRE(in_place || !rows_meet(x[i], xs[i], width, y[i], ys[i], width, T, size), "rope_ext: %s overlaps its result (in place needs the same address and stride)", i ? "k" : "q");
     }
+    const int64_t wq = (int64_t)n_head * head_dim, wk = (int64_t)n_head_kv * head_dim;
+    PI_REQUIRE(!k || (!rows_meet(q, q_stride, wq, k_out, k_out_stride, wk, T, size) && !rows_meet(k, k_stride, wk, q_out, q_out_stride, wq, T, size) &&
+                      !rows_meet(q_out, q_out_stride, wq, k_out, k_out_stride, wk, T, size)), "rope_ext: queries and keys overlap each other's results");
     a.xtype = xtype; a.T = T; a.hd = head_dim; a.n_rot = n_rot; a.halves = neox != 0; a.pos = pos; a.freqs = freqs; a.mscale = mscale;
     PI_REQUIRE((int64_t)T * ((int64_t)(n_head + n_head_kv) * head_dim / 1024 + 1) < (int64_t(1) << 31), "rope_ext: too many tokens for one call");
     return launch_rope_ext(a, (cudaStream_t)stream);
@@ -145,7 +155,7 @@ int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype
     if (b.n == 0 || b.T == 0 || b.max_new == 0) return PI_OK;
     const int64_t width = (int64_t)n_head * c.hd;
     if ((rc = check_rows(q, q_stride, width, xtype, "attention_q8", "q")) || (rc = check_rows(out, out_stride, width, xtype, "attention_q8", "out"))) return rc;
-    PI_REQUIRE(q != out, "attention_q8: q and out must be different");
+    PI_REQUIRE(!rows_meet(q, q_stride, width, out, out_stride, width, b.T, xtype == PI_TYPE_F16 ? 2 : 4), "attention_q8: q and out must be different");
     PI_REQUIRE(!weights_in || weights_out, "attention_q8: weights_in without weights_out");
     AttnQ8Args a;
     a.c = c; a.b = b; a.xtype = xtype; a.q = q; a.q_stride = q_stride; a.n_head = n_head; a.max_kv = max_kv;

@@ -56,6 +56,9 @@ def evict(c=None, lens=P, n=2, keep=128, sink=4, recent=32, w=P, w_out=None, kep
     (lambda: rope(qs=514), INVALID, "16 bytes apart"),
     (lambda: rope(qo=P + 2048), INVALID, "overlaps"),
     (lambda: rope(qo=P, qos=1024), INVALID, "overlaps"),
+    (lambda: rope(k=P + 512 * 4 * 8, ks=256, nk=2, ko=(1 << 24) + 16, kos=256), INVALID, "each other's"),
+    (lambda: rope(k=1 << 24, ks=512, nk=2, ko=1 << 25, kos=256), INVALID, "each other's"),
+    (lambda: rope(k=P + 1024, ks=512, nk=2, ko=P, kos=512), INVALID, "each other's"),
     (lambda: rope(nk=2), INVALID, "rope_ext"),
     (lambda: rope(pos=None), INVALID, "positions"),
     (lambda: store(cache(head_dim=80)), INVALID, "head_dim"),
@@ -73,6 +76,8 @@ def evict(c=None, lens=P, n=2, keep=128, sink=4, recent=32, w=P, w_out=None, kep
     (lambda: store(cache(head_dim=80), fn="pi_kv_load_q8"), INVALID, "head_dim"),
     (lambda: attention(n_head=6), INVALID, "multiple of n_head_kv"),
     (lambda: attention(out=P), INVALID, "different"),
+    (lambda: attention(out=P + 4096), INVALID, "different"),
+    (lambda: attention(out=P - 16), INVALID, "different"),
     (lambda: attention(w_in=P), INVALID, "weights_out"),
     (lambda: attention(qs=1026), INVALID, "q must be"),
     (lambda: attention(cache(n_ctx=4096), max_kv=4096, ws=None, wsn=0), WORKSPACE, "workspace"),
