@@ -144,8 +144,30 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         }
     };
 
-    // ---- queries into tensor memory: rows to shared memory (the halves' place) as they lie, then a row and a quarter of its columns a thread
-    {
+    // ---- queries into tensor memory.  Halves as they are: a row and a quarter of its columns a thread, straight from global memory.
+    if constexpr (!TWO_Q) {
+        if (warp >= 4 && warp < 20) {
+            constexpr int NQ = HD / 4;
+            const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = t.first + r, tok = row / p.group;
+            uint32_t u[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) u[j] = 0u;
+            if (r < t.n_rows) {
+                const uint4 * from = reinterpret_cast<const uint4 *>((const __half *)p.q + (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD + part * NQ);
+#pragma unroll
+                for (int j = 0; j < NQ / 8; j++) { const uint4 v = __ldg(from + j); u[4 * j] = v.x; u[4 * j + 1] = v.y; u[4 * j + 2] = v.z; u[4 * j + 3] = v.w; }
+            }
+            if (p.scale_log2 < 0.f) {                                 // (the factor of the scores is positive: maxima stay maxima)
+#pragma unroll
+                for (int j = 0; j < 16; j++) u[j] ^= 0x80008000u;
+            }
+            if (part == 0) s_f[r] = fabsf(p.scale_log2);
+            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q + (uint32_t)(part * NQ / 2);
+            if (NQ == 32) tc_st16(to, u); else at_st8(to, u);
+            tc_wait_st();
+        }
+    } else {
+        // FP32: whole rows to shared memory (the halves' place) as they lie, then a row and a quarter of its columns a thread, scaled and split
         constexpr int NQ = HD / 4, PITCH = HD + 4, LPR = HD / 4;      // lanes that read a row
         const bool mine = warp >= 4 && warp < 20;
         const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
@@ -186,8 +208,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 aq_split(v[j].x * up, v[j].y * up, hi[2 * j], lo[2 * j]);
                 aq_split(v[j].z * up, v[j].w * up, hi[2 * j + 1], lo[2 * j + 1]);
             }
-            if (NQ == 32) { tc_st16(to, hi); if (TWO_Q) tc_st16(to + HD / 2, lo); }
-            else          { at_st8(to, hi);  if (TWO_Q) at_st8(to + HD / 2, lo); }
+            if (NQ == 32) { tc_st16(to, hi); tc_st16(to + HD / 2, lo); }
+            else          { at_st8(to, hi);  at_st8(to + HD / 2, lo); }
             tc_wait_st();
         }
     }
