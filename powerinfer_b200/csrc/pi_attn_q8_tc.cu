@@ -10,7 +10,7 @@
 //
 // Precision.  FP32 rows: queries and probabilities as the sum of two halves each, i.e. two products in the place of one, 22 bits.  FP16 rows:
 // queries as they are, probabilities rounded to a half (2^-11 of each, beside the result's own rounding).  Values' scales ride on the probabilities, over the
-// tile's largest one; probabilities are held times 2^14.
+// power of two above the tile's largest one; probabilities are held times 2^14.
 //
 // Warps: 0 issues the products; 1 asks for the codes; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
 // their maxima); 20..27 make the halves and drain the sums, a row and half of the columns a thread.
@@ -27,7 +27,6 @@ namespace pi {
 #endif
 static constexpr int AT_THREADS = 896;
 static constexpr int AT_REGS_M = 24, AT_REGS_S = 64, AT_REGS_D = 104;  // 24 + 4 x 64 + 2 x 104 of the 7 x 72 of the launch
-static constexpr float AT_P = 16384.f;
 static constexpr uint32_t AT_SUB = AT_KEYS * 128;                     // bytes of 64 columns of a tile
 static constexpr int AT_RAW = 4;                                      // tiles of codes on their way: keys and values in turn
 
@@ -304,20 +303,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             float largest = fabsf(sv) <= FLT_MAX ? sv : 0.f;          // (of the finite ones)
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-            const float back = largest > 0.f ? AT_P / largest : 0.f, wv = sv == 0.f ? 0.f : sv * back, wk = sk;
+            // 2^14 over the power of two above it (exact; clamped where that is no normal number)
+            const int e = min(max((int)(__float_as_uint(largest) >> 23), 13), 253);
+            const float ref_v = __uint_as_float((uint32_t)(e - 13) << 23), wv = sv == 0.f ? 0.f : sv * __uint_as_float((uint32_t)(267 - e) << 23), wk = sk;
+            float fk[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) fk[c] = f * __shfl_sync(0xffffffffu, wk, half * 4 + c);
             if (i + 2 < n_tiles) scales(i + 2, sk, sv);
             const bool masked = k0 + i * AT_KEYS + half * 64 + 64 > least;       // (of this warp's rows)
             const int parts = max(0, min(4, (k1 - k0 - i * AT_KEYS - half * 64 + 15) >> 4));      // of 16 slots: the products take no more
             wait(s_qk + b, i >> 1 & 1);
             tc_fence_after();
             float m = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; 2 * c < parts; c++) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                if (2 * c >= parts) break;
                 float x[32];
                 at_ld32(x, mine + 32 * c);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float fk = f * __shfl_sync(0xffffffffu, wk, half * 4 + 2 * c + h);
                     float * y = x + h * 16;
                     if (masked) {
 #pragma unroll
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
 #pragma unroll
                     for (int j = 6; j < 14; j += 4) { a = max3(a, y[j], y[j + 1]); e = max3(e, y[j + 2], y[j + 3]); }
                     a = fmaxf(max3(a, y[14], y[15]), e);
-                    if (a > -INFINITY) m = fmaxf(m, a * fk);          // (-infinity times a factor of 0 is no number)
+                    if (a > -INFINITY) m = fmaxf(m, a * fk[2 * c + h]);      // (-infinity times a factor of 0 is no number)
                 }
             }
             s_max[b][half][r] = m;
@@ -341,10 +345,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                     float x[16];
                     tc_ld16(x, mine + 16 * c);
                     uint32_t hl[16];                                  // upper parts of 16 slots, then lower parts
-                    const float2 fk = f2(f * __shfl_sync(0xffffffffu, wk, half * 4 + c)), pv = f2(__shfl_sync(0xffffffffu, wv, half * 4 + c));
+                    const float2 fc = f2(c == 0 ? fk[0] : c == 1 ? fk[1] : c == 2 ? fk[2] : fk[3]), pv = f2(__shfl_sync(0xffffffffu, wv, half * 4 + c));
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float2 y = f2_fma(make_float2(x[j], x[j + 1]), fk, ref);
+                        const float2 y = f2_fma(make_float2(x[j], x[j + 1]), fc, ref);
                         float2 pr = make_float2(exp2_approx(y.x), exp2_approx(y.y)), w = f2_mul(pr, pv);
                         if (decltype(with_mask)::value) {             // (a masked slot counts nothing whatever its scores and its block's scales are)
                             if (c * 16 + j >= left) pr.x = w.x = 0.f;
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             if (i >= 2) wait(s_free + b, (i - 2) >> 1 & 1);           // the tile before has been drained: its sums are no more needed
             s_sum[b][half][r] = (l[0].x + l[0].y) + (l[1].x + l[1].y);
             if (half == 0) s_top[b][r] = m;
-            if (r == 0 && half == 0) s_ref[b] = largest * (1.f / AT_P);
+            if (r == 0 && half == 0) s_ref[b] = ref_v;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
