@@ -21,6 +21,7 @@ namespace pi {
 
 static constexpr int AQ_WARPS = 4, AQ_THREADS = AQ_WARPS * 32, AQ_STEP = AQ_WARPS * 16;
 static constexpr float AQ_RISE = 8.f, AQ_P = 128.f;                   // bits a maximum may lag; probabilities are held times this (2^8 * 128 < 65504)
+static constexpr float AQ_V_LEAST = 0x1p-119f;                        // values' scales below it count relative to it: AQ_P over a scale, and a scale over AQ_P, are normal numbers
 
 template <int HD> struct AqShape {
     static constexpr int KW = HD % 64 == 0 ? 16 : 8, KG = HD / (4 * KW);                   // codes a lane takes of a key row at once, and how often
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         for (int n = 0; n < S::NT; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) o[mt][n][j] = 0.f;
-    float v_ref = 0.f, v_inv = 0.f;                                   // scale of the value sums, and AQ_P over it
+    float v_ref = AQ_V_LEAST, v_inv = AQ_P / AQ_V_LEAST;              // scale of the value sums, and AQ_P over it
 
     const unsigned char * kt = ring + (ST - 1) * S::STAGE;
     for (int it = 0; it < steps; it++) {

@@ -8,9 +8,9 @@
 // drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer than a tile.
 // So every tile has its own maximum (no exchange between tiles; the two score buffers are two groups of warps' own): the drain joins tiles.
 //
-// Precision.  FP32 rows: queries and probabilities as the sum of two halves each, i.e. two products in the place of one, 22 bits.  FP16 rows:
-// queries as they are, probabilities rounded to a half (2^-11 of each, beside the result's own rounding).  Values' scales ride on the probabilities, over the
-// power of two above the tile's largest one; probabilities are held times 2^14.
+// Precision.  Probabilities, and queries of FP32 rows, as the sum of two halves each, i.e. two products in the place of one: 22 bits.  Queries of FP16 rows
+// as they are.  (Probabilities of FP16 rows as one half: 7 % less time for 11 bits.)  Values' scales ride on the probabilities, over the power of two above the tile's
+// largest one; probabilities are held times 2^14.
 //
 // Warps: 0 issues the products; 1 asks for the codes; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
 // their maxima); 20..27 make the halves and drain the sums, a row and half of the columns a thread.
@@ -22,9 +22,6 @@
 
 namespace pi {
 
-#ifndef AT_F16_P
-#define AT_F16_P true
-#endif
 static constexpr int AT_THREADS = 896;
 static constexpr int AT_REGS_M = 24, AT_REGS_S = 64, AT_REGS_D = 104;  // 24 + 4 x 64 + 2 x 104 of the 7 x 72 of the launch
 static constexpr uint32_t AT_SUB = AT_KEYS * 128;                     // bytes of 64 columns of a tile
@@ -66,8 +63,8 @@ __device__ __forceinline__ void f2_split(float2 x, uint32_t & hi, uint32_t & lo)
     lo = h2u(__floats2half2_rn(r.x, r.y));
 }
 
-// TWO_Q, TWO_P: two halves for each query, for each probability
-template <int HD, bool TWO_Q, bool TWO_P>
+// TWO_Q: two halves for each query
+template <int HD, bool TWO_Q>
 __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     constexpr int KS = HD / 16, SUBS = HD / 64, U = HD / 32;          // steps of 16 columns; pieces of 64 columns; chunks of 16 codes of a tile a thread
     constexpr uint32_t TILE = SUBS * AT_SUB;
@@ -252,16 +249,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                 const uint32_t a = tmem + T_S + (uint32_t)(b * AT_KEYS), d = tmem + T_O;
                 const uint64_t v = tc_desc_mn(vbuf + (uint32_t)b * TILE, AT_SUB);
                 if (steps == AT_KEYS / 16) {
-                    if (TWO_P) {
 #pragma unroll
-                        for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
-                    }
+                    for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
 #pragma unroll
-                    for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
+                    for (int j = 0; j < AT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, true);
                 } else {
-                    if (TWO_P)
-                        for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
-                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO_P || j > 0);
+                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
+                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, true);
                 }
                 tc_commit(s_pv + b);
                 if (i + 2 < tiles) scores(i + 2);
@@ -304,7 +298,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             // 2^14 over the power of two above it (exact; clamped where that is no normal number)
-            const int e = min(max((int)(__float_as_uint(largest) >> 23), 13), 253);
+            const int e = min(max((int)(__float_as_uint(largest) >> 23), 14), 253);
             const float ref_v = __uint_as_float((uint32_t)(e - 13) << 23), wv = sv == 0.f ? 0.f : sv * __uint_as_float((uint32_t)(267 - e) << 23), wk = sk;
             float fk[4];
 #pragma unroll
@@ -355,11 +349,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                             if (c * 16 + j + 1 >= left) pr.y = w.y = 0.f;
                         }
                         l[j >> 1 & 1] = f2_add(l[j >> 1 & 1], pr);
-                        if (TWO_P) f2_split(w, hl[j / 2], hl[8 + j / 2]);
-                        else       hl[j / 2] = h2u(__floats2half2_rn(w.x, w.y));
+                        f2_split(w, hl[j / 2], hl[8 + j / 2]);
                     }
-                    if (TWO_P) tc_st16(mine + 16 * c, hl);
-                    else       at_st8(mine + 16 * c, hl);
+                    tc_st16(mine + 16 * c, hl);
                 }
             };
             if (masked) exps(std::true_type()); else exps(std::false_type());
@@ -459,23 +451,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
 
 bool attn_q8_tc_takes(int hd, int64_t rows) { return (hd == 64 || hd == 128) && rows >= 64; }
 
-template <int HD, bool TWO_Q, bool TWO_P>
+template <int HD, bool TWO_Q>
 static int at_go(const AttnQ8P & p, cudaStream_t st) {
     constexpr size_t smem = (size_t)4 * (HD / 64) * AT_SUB + AT_RAW * AT_KEYS * HD + 1024;
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        PI_CUDA(cudaFuncSetAttribute(k_attn_q8_tc<HD, TWO_Q, TWO_P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        PI_CUDA(cudaFuncSetAttribute(k_attn_q8_tc<HD, TWO_Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q, TWO_P>, dim3(aq_grid(p)), dim3(AT_THREADS), smem, st, true, p));
+    PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q>, dim3(aq_grid(p)), dim3(AT_THREADS), smem, st, true, p));
     return PI_OK;
 }
 
 int launch_attn_q8_tc(const AttnQ8P & p, cudaStream_t st) {
-    if (p.c.hd == 64) return p.xtype == PI_TYPE_F16 ? at_go<64, false, AT_F16_P>(p, st) : at_go<64, true, true>(p, st);
-    return p.xtype == PI_TYPE_F16 ? at_go<128, false, AT_F16_P>(p, st) : at_go<128, true, true>(p, st);
+    if (p.c.hd == 64) return p.xtype == PI_TYPE_F16 ? at_go<64, false>(p, st) : at_go<64, true>(p, st);
+    return p.xtype == PI_TYPE_F16 ? at_go<128, false>(p, st) : at_go<128, true>(p, st);
 }
 
 }  // namespace pi

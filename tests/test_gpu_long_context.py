@@ -369,6 +369,24 @@ def test_attention_values_of_very_different_sizes(ops):
         run_attention(ops, p, rng, [0, T, 2 * T], [512 - T, 512 - T], 16, max_new=T)
 
 
+@pytest.mark.parametrize("T", [1, 140])
+def test_attention_values_of_the_smallest_scales(ops, T):
+    """Scales of values from the smallest normal number on.  Below 2^-119 probabilities are held relative to 2^-119, i.e. 2^7 and not 2^14 times: what their
+    lower halves leave out is 2^-25 of the largest value.  Sums near the smallest numbers are off by half of 2^-149 wherever they are rounded: once a tile
+    or warp, once a split, once where they are put out."""
+    rng = np.random.default_rng(T)
+    p = Pair(ops, 2, 2, 512, 128, 16, fill=rng)
+    p.c.scale["v"][0] = 2.0 ** -126
+    p.c.scale["v"][1] = 2.0 ** rng.integers(-126, -112, (2, 32)).astype(np.float32)
+    p.c.scale["v"][1, :, 0] = 2.0 ** -126
+    p.d.v_scale.copy_(dev(p.c.scale["v"]))
+    q, start, at, up = rows(rng, 2 * T, 16 * 128), [0, T, 2 * T], [512 - T, 512 - T], 2.0 ** 100
+    got = ops.attention_q8(p.d, dev(q), ints(start), ints(at)).cpu().numpy().astype(np.float64) * up
+    want, size, terms, most = p.c.attention(q, 16, 128 ** -0.5, start, at)
+    tol = attention_bound(size * up, terms, most * up * 2 ** 7, 128, 512, "f32", want) + 32 * 2.0 ** -149 * up
+    assert np.all(np.abs(got - want * up) <= tol)
+
+
 def test_attention_nan_and_inf_stay_in_their_rows(ops):
     """A query that is not a number gives rows of no number, its neighbours' are untouched; so does a scale that a row sees."""
     rng = np.random.default_rng(6)
@@ -435,6 +453,50 @@ def test_attention_refuses(ops):
         with pytest.raises((ValueError, RuntimeError)):
             ops.attention_q8(p.d, **a)
     assert ops.attention_q8(p.d, torch.zeros(0, 256, device="cuda"), ints([0, 0]), z).shape == (0, 256)
+
+
+def test_attention_of_a_prompt_leaves_a_clear_status(ops):
+    """Through the C entry, whose workspace is the caller's: full of ones before, the status word says that every wait completed."""
+    import ctypes as C
+    from powerinfer_b200 import _lib
+    rng = np.random.default_rng(5)
+    p = Pair(ops, 1, 2, 1024, 128, 64, fill=rng)
+    start, at = ints([0, 100]), ints([900])
+    q = dev(rows(rng, 100, 8 * 128))
+    out = torch.empty_like(q)
+    b = _lib.KvBatch(start.data_ptr(), None, at.data_ptr(), 1, 100, 100)
+    need = _lib.lib.pi_attention_q8_workspace_bytes(p.d.c, C.byref(b), 8, 1024, 0)
+    ws = torch.full((need,), -1, dtype=torch.int8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(2):
+        assert _lib.lib.pi_attention_q8(p.d.c, C.byref(b), _lib.PI_TYPE_F32, q.data_ptr(), 1024, 8, 1024, 128 ** -0.5, out.data_ptr(), 1024, None, None,
+                                        ws.data_ptr(), need, stream) == 0
+        assert _lib.lib.pi_op_status(ws.data_ptr(), stream) == 0
+    assert torch.equal(out, ops.attention_q8(p.d, q, start, at))
+
+
+def test_rows_of_heads_and_rows_that_lie_oddly(ops):
+    """Three dimensions, a single row of a wider matrix, rows that are no multiple of 16 bytes apart: the same results as contiguous rows."""
+    rng = np.random.default_rng(6)
+    p = Pair(ops, 2, 2, 64, 64, 16, fill=rng)
+    start, at = ints([0, 1, 3]), ints([20, 40])
+    q = dev(rows(rng, 3, 4 * 64))
+    plain = ops.attention_q8(p.d, q, start, at)
+    assert torch.equal(ops.attention_q8(p.d, q.view(3, 4, 64), start, at), plain)
+    odd = torch.zeros(3, 4 * 64 + 1, device="cuda")
+    odd[:, 1:] = q
+    assert torch.equal(ops.attention_q8(p.d, odd[:, 1:], start, at), plain)
+    assert torch.equal(ops.attention_q8(p.d, q.t().contiguous().t(), start, at), plain)
+    one = ops.attention_q8(p.d, q[:1], ints([0, 1]), ints([20]))
+    assert torch.equal(ops.attention_q8(p.d, odd[:1, 1:], ints([0, 1]), ints([20])), one)
+    f = ops.rope_freqs(64)
+    yq, _ = ops.rope_ext(q, None, ints([5, 6, 7]), f, 64)
+    assert torch.equal(ops.rope_ext(odd[:, 1:], None, ints([5, 6, 7]), f, 64)[0], yq)
+    assert torch.equal(ops.rope_ext(q.view(3, 4, 64), None, ints([5, 6, 7]), f, 64)[0], yq)
+    k, v = q[:, :128], q[:, 128:]
+    ops.kv_store_q8(p.d, k.reshape(3, 2, 64), odd[:, 129:], start, at)
+    p.c.store(k.cpu().numpy(), v.cpu().numpy(), [0, 1, 3], [20, 40])
+    p.same()
 
 
 # ------------------------------------------------------------------------------------------------ eviction
@@ -566,6 +628,48 @@ def test_calls_on_two_streams_and_in_graphs(ops):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(results[i][0], plain[i][at][0]) and torch.equal(results[i][1], plain[i][at][1])
+
+
+def test_a_step_as_a_graph_on_another_stream(ops):
+    """Rotation, store, attention of a prompt and of single tokens, eviction and read-back as one captured step, replayed with other lengths and rows on a
+    stream of its own: the same bits as the calls one by one."""
+    rng = np.random.default_rng(32)
+    H, group, hd, n_ctx, T = 2, 4, 64, 512, 42
+    names = ("k", "v", "k_scale", "v_scale")
+    a, b = (Pair(ops, 3, H, n_ctx, hd, 16) for _ in range(2))
+    f = ops.rope_freqs(hd)
+    step = [torch.empty(T, (H * group + 2 * H) * hd, device="cuda"), ints([0] * T), ints([0, 40, 41, 42]), ints([0] * 3), ints([0] * 3)]
+    weights = [torch.zeros(3, H, n_ctx, device="cuda") for _ in range(2)]
+
+    def run(c, w):
+        qkv, pos, start, at, lens = step
+        q, k = ops.rope_ext(qkv[:, :H * group * hd], qkv[:, H * group * hd:H * (group + 1) * hd], pos, f, hd)
+        ops.kv_store_q8(c, k, qkv[:, H * (group + 1) * hd:], start, at, max_new=40)
+        out = ops.attention_q8(c, q, start, at, max_new=40, weights_in=w, weights_out=w)
+        kept = ops.kv_evict_q8(c, w, lens, 128, 2, 16, weights_out=w)
+        return (out, kept) + tuple(ops.kv_load_q8(c, start, ints_of_graph, T, max_new=40))
+
+    ints_of_graph = ints([3, 0, 100])
+    side = torch.cuda.Stream()
+    step[0].copy_(dev(rows(rng, T, step[0].shape[1])))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = run(a.d, weights[0])
+    for at in ([0, 7, 200], [40, 8, 201], [80, 9, 128], [120, 511, 128], [128, 128, 128]):
+        step[0].copy_(dev(rows(rng, T, step[0].shape[1])))
+        step[1].copy_(ints([at[0] + i for i in range(40)] + at[1:]))
+        step[3].copy_(ints(at))
+        step[4].copy_(ints([at[0] + 40, min(at[1] + 1, n_ctx), at[2] + 1]))
+        want = run(b.d, weights[1])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for got, w in zip(captured, want):
+            assert torch.equal(got, w)
+        assert torch.equal(*weights)
+        for n in names:
+            assert torch.equal(getattr(a.d, n), getattr(b.d, n))
 
 
 @pytest.mark.parametrize("x", ["f32", "f16"])
