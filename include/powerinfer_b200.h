@@ -190,7 +190,7 @@ int pi_rope_ext(int xtype, const void * q, int64_t q_stride, int n_head, void * 
                 int T, int head_dim, int n_rot, int neox, const int32_t * pos, const double * freqs, float mscale, void * stream);
 
 /* A KV cache in 8 bits: codes int8 [n_seq, n_head_kv, n_ctx, head_dim], 16-byte aligned, and for every block of `block` slots of a sequence and KV
- * head a scale, F32 [n_seq, n_head_kv, n_ctx / block]; a value is code * scale.  head_dim 64, 96, 128, 192 or 256; block 16, 32, 64 or 128;
+ * head a scale, F32 [n_seq, n_head_kv, n_ctx / block], not negative; a value is code * scale.  head_dim 64, 96, 128, 192 or 256; block 16, 32, 64 or 128;
  * n_ctx a multiple of block.  A slot is a place in the cache; it equals the token's position until slots are evicted. */
 typedef struct {
     void * k, * v; float * k_scale, * v_scale;

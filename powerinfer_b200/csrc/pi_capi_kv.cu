@@ -40,6 +40,11 @@ static bool rows_meet(const void * a, int64_t sa, int64_t wa, const void * b, in
     const int64_t pitch = sa * size, at = ((b0 - a0) % pitch + pitch) % pitch;      // where b's rows begin in a's
     return at < wa * size || at + wb * size > pitch;
 }
+// whether two arrays of n values of four bytes are one and the same, or apart
+static bool same_or_apart(const void * a, const void * b, int64_t n) {
+    const int64_t a0 = (int64_t)(uintptr_t)a, b0 = (int64_t)(uintptr_t)b;
+    return !a || !b || a == b || a0 + 4 * n <= b0 || b0 + 4 * n <= a0;
+}
 static int check_batch(const pi_kv_batch * b, RaggedB & o, const char * who) {
     PI_REQUIRE(b && b->T >= 0 && b->T <= KV_BIG && b->n >= 0 && b->n <= 65535 && b->max_new >= 0 && (b->n == 0 || (b->q_start && b->pos0)),
                "%s: bad batch (0 <= T <= 2^30, 0 <= n <= 65535, q_start and pos0 given)", who);
@@ -117,6 +122,7 @@ int pi_kv_store_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype,
     if (b.n == 0 || b.T == 0 || b.max_new == 0) return PI_OK;
     const int64_t width = (int64_t)c.H * c.hd;
     if ((rc = check_rows(k, k_stride, width, xtype, "kv_store_q8", "k")) || (rc = check_rows(v, v_stride, width, xtype, "kv_store_q8", "v"))) return rc;
+    PI_REQUIRE(((int64_t)(b.max_new < c.n_ctx ? b.max_new : c.n_ctx) / c.block + 2) * 2 * c.H < (int64_t(1) << 31), "kv_store_q8: too many slots for one call");
     return launch_kv_store_q8(c, b, xtype, k, k_stride, v, v_stride, (cudaStream_t)stream);
 }
 
@@ -128,6 +134,7 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
     const int64_t width = (int64_t)c.H * c.hd;
     PI_REQUIRE((int64_t)(b.max_new / 16 + 1) * c.H < (int64_t(1) << 30), "kv_load_q8: too many slots for one call");
     if ((rc = check_rows(k, k_stride, width, xtype, "kv_load_q8", "k")) || (rc = check_rows(v, v_stride, width, xtype, "kv_load_q8", "v"))) return rc;
+    PI_REQUIRE(!rows_meet(k, k_stride, width, v, v_stride, width, b.T, xtype == PI_TYPE_F16 ? 2 : 4), "kv_load_q8: k and v overlap");
     return launch_kv_load_q8(c, b, xtype, k, k_stride, v, v_stride, (cudaStream_t)stream);
 }
 
@@ -157,6 +164,7 @@ int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype
     if ((rc = check_rows(q, q_stride, width, xtype, "attention_q8", "q")) || (rc = check_rows(out, out_stride, width, xtype, "attention_q8", "out"))) return rc;
     PI_REQUIRE(!rows_meet(q, q_stride, width, out, out_stride, width, b.T, xtype == PI_TYPE_F16 ? 2 : 4), "attention_q8: q and out must be different");
     PI_REQUIRE(!weights_in || weights_out, "attention_q8: weights_in without weights_out");
+    PI_REQUIRE(same_or_apart(weights_in, weights_out, (int64_t)c.n_seq * c.H * c.n_ctx), "attention_q8: weights_in and weights_out overlap (the same array, or apart)");
     AttnQ8Args a;
     a.c = c; a.b = b; a.xtype = xtype; a.q = q; a.q_stride = q_stride; a.n_head = n_head; a.max_kv = max_kv;
     a.scale = scale; a.out = out; a.out_stride = out_stride; a.w_in = weights_in; a.w_out = weights_out;
@@ -177,6 +185,7 @@ int pi_kv_evict_q8(const pi_kv_q8 * cache, const int32_t * len, const int32_t * 
     PI_REQUIRE(a.c.n_ctx <= 1 << 18, "kv_evict_q8: n_ctx=%d is more than 262144", a.c.n_ctx);
     if (n == 0) return PI_OK;
     PI_REQUIRE(len && weights && kept, "kv_evict_q8: len, weights and kept are needed");
+    PI_REQUIRE(same_or_apart(weights, weights_out, (int64_t)a.c.n_seq * a.c.H * a.c.n_ctx), "kv_evict_q8: weights and weights_out overlap (the same array, or apart)");
     a.len = len; a.seq = seq; a.n = n; a.keep = keep; a.n_sink = n_sink; a.n_recent = n_recent; a.w = weights; a.w_out = weights_out; a.kept = kept;
     return launch_kv_evict_q8(a, (cudaStream_t)stream);
 }

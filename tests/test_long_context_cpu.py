@@ -91,6 +91,11 @@ def evict(c=None, lens=P, n=2, keep=128, sink=4, recent=32, w=P, w_out=None, kep
     (lambda: evict(lens=None), INVALID, "needed"),
     (lambda: evict(kept=None), INVALID, "needed"),
     (lambda: evict(cache(n_ctx=1 << 19)), INVALID, "262144"),
+    (lambda: evict(w=P, w_out=P + 1024), INVALID, "the same array, or apart"),
+    (lambda: attention(w_in=P + 4, w_out=P), INVALID, "the same array, or apart"),
+    (lambda: store(fn="pi_kv_load_q8", k=P, v=P), INVALID, "k and v overlap"),
+    (lambda: store(fn="pi_kv_load_q8", k=P, ks=768, v=P + 256 * 4, vs=768), INVALID, "k and v overlap"),
+    (lambda: store(cache(n_head_kv=65535, n_ctx=1 << 30, block=16), batch(T=1 << 30, max_new=1 << 30), ks=65535 * 128, vs=65535 * 128), INVALID, "too many slots"),
 ])
 def test_bad_arguments_are_refused_before_any_launch(call, code, needle):
     rc = call()
