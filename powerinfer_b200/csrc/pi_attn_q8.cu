@@ -7,15 +7,18 @@
 // between warps), keep a maximum, a sum and all sums of values of their own, and join them at the end.  Long ranges are
 // split over CTAs, whose sums k_attn_q8_join joins.
 //
-// Precision.  A code is exact as a half.  A query row is scaled by a power of two and held as the sum of two halves, rows 0 .. 7 of the
-// tensor cores' tile the upper, rows 8 .. 15 the lower parts, so the tile that a group of up to 8 heads would leave half empty makes the products
-// with 22 bits; the sum of both is in one lane.  Probabilities go the same way, times vs over the largest vs so far (at most 1): out = sums *
-// that scale.  Maxima, sums and the exponents' arguments are FP32.
+// Precision.  Scores are products of whole numbers: the codes as they lie, and a query row of 23 bits and a sign as three digits of 8 bits, which are three rows
+// of the tensor cores' tile (24 rows for 8 queries, 48 for 16); their sums are exact.  A probability, times vs over the largest vs so far (at most 1), is the sum of
+// two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits, and a value's code is exact as a half: out = sums * that scale.  (Probabilities as
+// digits would spare the values' conversions, but their sums fill twice the registers, and whole numbers cannot follow a maximum that rises.)
+// Maxima, sums and the exponents' arguments are FP32.
 //
-// Layouts.  mma.m16n8k16 sums over 16 columns (scores) or slots (values) in any order that both operands share: a lane's piece of a key row is
+// Layouts.  mma sums over 32 columns (scores) or 16 slots (values) in any order that both operands share: a lane's piece of a key row is
 // 16 contiguous codes, of a value row hd / 8 of them, and every 4 codes are operands of one product.  The probabilities of the score tile's layout
 // are the value product's operand as they stand.  Where the maximum rises by less than 2^8, sums are not scaled anew.
 #include "pi_attn_q8.cuh"
+
+#include <cfloat>
 
 namespace pi {
 
@@ -45,13 +48,14 @@ template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], co
     else                       r[0] = *reinterpret_cast<const uint32_t *>(p);
 }
 
-// The query rows of a tile as A operands, scaled; e: by which power of two the scores have to be multiplied.  Lane (g, q) holds row g (upper
-// parts) and row g + 8 (lower parts) of every 4 of its 16 columns.
+// A query row as A operands: whole numbers of 24 bits in three digits to the base 256 (-128 .. 127), a[d] the d-th digits of every 4 of a lane's columns.  Returns by
+// which power of two the scores have to be multiplied; not a number where a value of the row is not finite, so that its scores are none either.
 template <int HD>
-__device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[HD / 16][4]) {
+__device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[3][HD / 16]) {
     using S = AqShape<HD>;
     float4 x[S::KS];
     float m = 0.f;
+    bool finite = true;
     const size_t at = there ? (size_t)(s.first + row / p.group) * p.q_stride + (size_t)(hk * p.group + row % p.group) * HD : 0;
 #pragma unroll
     for (int c = 0; c < S::KG; c++)
@@ -60,19 +64,56 @@ __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s
             float4 & v = x[c * (S::KW / 4) + w];
             v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (there) v = aq_query(p.xtype, p.q, at + c * 4 * S::KW + q * S::KW + w * 4);
-            m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            const float a0 = fabsf(v.x), a1 = fabsf(v.y), a2 = fabsf(v.z), a3 = fabsf(v.w);
+            finite = finite && a0 <= FLT_MAX && a1 <= FLT_MAX && a2 <= FLT_MAX && a3 <= FLT_MAX;
+            m = fmaxf(fmaxf(m, fmaxf(a0, a1)), fmaxf(a2, a3));
         }
+    if (!finite) m = INFINITY;
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25 (what is not finite stays that: the row's scores are)
-    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;
+    // the largest to 2^21 x 1.98 .. 2^22 x 1.98: three digits reach 2^22 x 1.992.  A value is off by half of 1, at most 2^-22 of the largest
+    const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -100), 127) - 22;
     const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
     for (int i = 0; i < S::KS; i++) {
-        aq_split(x[i].x * up, x[i].y * up, a[i][0], a[i][1]);
-        aq_split(x[i].z * up, x[i].w * up, a[i][2], a[i][3]);
+        const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t t[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) t[j] = (uint32_t)(__float2int_rn(v[j] * up) + 0x808080);       // digits + 128
+        const uint32_t t01 = __byte_perm(t[0], t[1], 0x5140), t23 = __byte_perm(t[2], t[3], 0x5140);
+        a[0][i] = __byte_perm(t01, t23, 0x5410) ^ 0x80808080u;
+        a[1][i] = __byte_perm(t01, t23, 0x7632) ^ 0x80808080u;
+        a[2][i] = __byte_perm(__byte_perm(t[0], t[1], 0x0062), __byte_perm(t[2], t[3], 0x0062), 0x5410) ^ 0x80808080u;
     }
-    return down;
+    return m <= FLT_MAX ? down : __int_as_float(0x7fc00000);
+}
+
+// Sums of products of digits and codes are whole numbers up to 2^22 (256 x 128 x 128): begun at 1.5 x 2^23's bits, they are that number plus the sum.
+static constexpr int AQ_ZERO = 0x4B400000;
+// d += (16 rows of 32 digits) x (32 codes of 8 slots)
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1),
+                   "r"(first ? AQ_ZERO : d[0]), "r"(first ? AQ_ZERO : d[1]), "r"(first ? AQ_ZERO : d[2]), "r"(first ? AQ_ZERO : d[3]));
+}
+__device__ __forceinline__ float aq_score(int d2, int d1, int d0) {
+    const float f2 = __int_as_float(d2) - 12582912.f, f1 = __int_as_float(d1) - 12582912.f, f0 = __int_as_float(d0) - 12582912.f;
+    return fmaf(fmaf(f2, 256.f, f1), 256.f, f0);
+}
+// products of 32 columns of 8 slots (b0, b1) and of the rows: x[digit 2 | 1], x[digit 0] for 8 rows, x[digit] for 16
+template <int HD, int MT, int NX>
+__device__ __forceinline__ void aq_products(int (&x)[NX][4], const uint32_t (&a)[MT][3][HD / 16], int s, uint32_t b0, uint32_t b1) {
+    if constexpr (MT == 1) {
+        mma16832(x[0], a[0][2][2 * s], a[0][1][2 * s], a[0][2][2 * s + 1], a[0][1][2 * s + 1], b0, b1, s == 0);
+        mma16832(x[1], a[0][0][2 * s], 0u, a[0][0][2 * s + 1], 0u, b0, b1, s == 0);
+    } else {
+#pragma unroll
+        for (int d = 0; d < 3; d++) mma16832(x[d], a[0][d][2 * s], a[1][d][2 * s], a[0][d][2 * s + 1], a[1][d][2 * s + 1], b0, b1, s == 0);
+    }
+}
+template <int MT, int NX> __device__ __forceinline__ float aq_score_of(const int (&x)[NX][4], int mt, int j) {
+    if constexpr (MT == 1) return aq_score(x[0][j], x[0][2 + j], x[1][j]);
+    else                   return aq_score(x[2][2 * mt + j], x[1][2 * mt + j], x[0][2 * mt + j]);
 }
 
 template <int HD, int MT>
@@ -117,7 +158,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
     for (int it = 0; it < ST - 1; it++) issue();
 
-    uint32_t a[MT][S::KS][4];
+    uint32_t a[MT][3][S::KS];
     float f[MT], m[MT], l[MT]; int sees[MT], score_row[MT], least = 0x7fffffff; bool there[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
@@ -150,27 +191,16 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         const float sk = __ldg(ks + (j0 >> p.c.shift)), sv = __ldg(vs + (j0 >> p.c.shift));
 
         // ---- scores of 16 slots
-        float x[MT][2][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) x[mt][n][j] = 0.f;
+        int x[2][MT + 1][4];
 #pragma unroll
         for (int c = 0; c < S::KG; c++) {
             uint32_t w[2][S::KW / 4];
 #pragma unroll
             for (int n = 0; n < 2; n++) aq_lds<S::KW>(w[n], kt + S::k_at(n * 8 + g, c * 4 * S::KW + q * S::KW));
 #pragma unroll
-            for (int i = 0; i < S::KW / 4; i++)
+            for (int i = 0; i < S::KW / 8; i++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const uint32_t u = w[n][i] ^ 0x80808080u, b0 = q8_lo(u), b1 = q8_hi(u);
-                    const int k = c * (S::KW / 4) + i;
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) mma16816(x[mt][n], a[mt][k][0], a[mt][k][1], a[mt][k][2], a[mt][k][3], b0, b1);
-                }
+                for (int n = 0; n < 2; n++) aq_products<HD, MT>(x[n], a, c * (S::KW / 8) + i, w[n][2 * i], w[n][2 * i + 1]);
         }
         // ---- probabilities, as A operands of the value products
         float ratio = 1.f;
@@ -184,7 +214,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) y[n][j] = (x[mt][n][j] + x[mt][n][j + 2]) * fk;
+                for (int j = 0; j < 2; j++) y[n][j] = aq_score_of<MT>(x[n], mt, j) * fk;
             const bool masked = j0 + 16 > least;
             if (masked) {
 #pragma unroll
@@ -467,7 +497,7 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
         }
         later = __any_sync(0xffffffffu, later);
     }
-    uint32_t a[S::KS][4];
+    uint32_t a[1][3][S::KS];
     float f = 0.f, lse = 0.f;
     int a_row = -1, sees = 0;
     if (later) return;
@@ -481,20 +511,17 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
                 const int row = r0 + g, tok = row / p.group;
                 const bool there = row < n_rows;
                 lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row % p.group) : 0.f;
-                f = aq_load_query<HD>(p, s, row, there, hk, q, a) * p.scale_log2;
+                f = aq_load_query<HD>(p, s, row, there, hk, q, a[0]) * p.scale_log2;
                 sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
                 a_row = r0;
             }
 #pragma unroll
             for (int n = 0; n < NK; n++) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                int x[2][4];
 #pragma unroll
-                for (int k = 0; k < S::KS; k++) {
-                    const uint32_t u = w[n][k / (S::KW / 4)][k % (S::KW / 4)] ^ 0x80808080u;
-                    mma16816(x, a[k][0], a[k][1], a[k][2], a[k][3], q8_lo(u), q8_hi(u));
-                }
+                for (int k = 0; k < HD / 32; k++) aq_products<HD, 1>(x, a, k, w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4)], w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4) + 1]);
 #pragma unroll
-                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx((x[j] + x[j + 2]) * (f * sk[n >> 1]) - lse);
+                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx(aq_score_of<1>(x, 0, j) * (f * sk[n >> 1]) - lse);
             }
         }
         const int at = j0;

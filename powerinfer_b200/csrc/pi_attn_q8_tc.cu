@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         __syncthreads();
         if (mine) {
             const float m = fmaxf(fmaxf(s_max[0][0][r], s_max[0][1][r]), fmaxf(s_max[1][0][r], s_max[1][1][r]));
-            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11, as there
+            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25
             const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
             if (part == 0) s_f[r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
             const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q + (uint32_t)(part * NQ / 2);
