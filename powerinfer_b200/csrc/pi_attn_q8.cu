@@ -23,8 +23,8 @@
 namespace pi {
 
 static constexpr int AQ_WARPS = 4, AQ_THREADS = AQ_WARPS * 32, AQ_STEP = AQ_WARPS * 16;
-static constexpr float AQ_RISE = 8.f, AQ_P = 128.f;                   // bits a maximum may lag; probabilities are held times this (2^8 * 128 < 65504)
-static constexpr float AQ_V_LEAST = 0x1p-119f;                        // values' scales below it count relative to it: AQ_P over a scale, and a scale over AQ_P, are normal numbers
+static constexpr float AQ_RISE = 7.f, AQ_P = 256.f;                   // bits a maximum may lag; probabilities are held times this (2^7 * 256 < 65504)
+static constexpr float AQ_V_LEAST = 0x1p-118f;                        // values' scales below it count relative to it: AQ_P over a scale, and a scale over AQ_P, are normal numbers
 
 template <int HD> struct AqShape {
     static constexpr int KW = HD % 64 == 0 ? 16 : 8, KG = HD / (4 * KW);                   // codes a lane takes of a key row at once, and how often
@@ -35,11 +35,10 @@ template <int HD> struct AqShape {
     static __device__ __forceinline__ int v_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ (((row >> 1) & 3) << 5) : byte); }
     static constexpr int STAGES = HD <= 128 ? 4 : 3, STAGE = 2 * 16 * HD;
     static constexpr int ctas(int mt) { return HD <= 128 && mt == 1 ? 3 : 2; }           // that an SM holds
-    static constexpr size_t ring() { return (size_t)AQ_WARPS * STAGES * STAGE; }
-    static constexpr size_t smem(int mt) {
-        const size_t sums = (size_t)AQ_WARPS * 8 * mt * (HD + 4) * 4;
-        return ring() > sums ? ring() : sums;
-    }
+    // shared memory: the ring, in the end the warps' sums in its place, and the queries' digits
+    static constexpr size_t RING = (size_t)AQ_WARPS * STAGES * STAGE;
+    template <int MT> static constexpr size_t DIGITS = RING > (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4 ? RING : (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4;
+    template <int MT> static constexpr size_t SMEM = DIGITS<MT> + 3 * 8 * MT * (HD + 16);
 };
 
 template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], const unsigned char * p) {
@@ -48,15 +47,38 @@ template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], co
     else                       r[0] = *reinterpret_cast<const uint32_t *>(p);
 }
 
-// A query row as A operands: whole numbers of 24 bits in three digits to the base 256 (-128 .. 127), a[d] the d-th digits of every 4 of a lane's columns.  Returns by
-// which power of two the scores have to be multiplied; not a number where a value of the row is not finite, so that its scores are none either.
+// A query row in whole numbers of 23 bits and a sign, as three digits to the base 256 (-128 .. 127), four columns at a time
+struct AqScaled { float up, down; };                                  // factor of the row; of its scores (not a number where a value of the row is not finite: so are they)
+__device__ __forceinline__ void aq_max(const float4 & v, float & m, float & zero) {    // zero: no more 0 where a value is not finite
+    m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    zero = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, zero))));
+}
+// the largest to 2^21 x 1.98 .. 2^22 x 1.98: three digits reach 2^22 x 1.992.  A value is off by half of 1, at most 2^-22 of the largest
+__device__ __forceinline__ AqScaled aq_scaled(float m) {
+    const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -100), 128) - 22;
+    return {__uint_as_float((uint32_t)(127 - e) << 23), m < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : __int_as_float(0x7fc00000)};
+}
+__device__ __forceinline__ void aq_digits(const float4 & x, float up, uint32_t & d0, uint32_t & d1, uint32_t & d2) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    uint32_t t[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) t[j] = (uint32_t)(__float2int_rn(v[j] * up) + 0x808080);           // digits + 128
+    const uint32_t t01 = __byte_perm(t[0], t[1], 0x5140), t23 = __byte_perm(t[2], t[3], 0x5140);
+    d0 = __byte_perm(t01, t23, 0x5410) ^ 0x80808080u;
+    d1 = __byte_perm(t01, t23, 0x7632) ^ 0x80808080u;
+    d2 = __byte_perm(__byte_perm(t[0], t[1], 0x0062), __byte_perm(t[2], t[3], 0x0062), 0x5410) ^ 0x80808080u;
+}
+__device__ __forceinline__ size_t aq_query_at(const AttnQ8P & p, const SeqB & s, int row, int hk, int hd) {
+    const int tok = p.by_group.of(row);
+    return (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * hd;
+}
+// A lane's pieces of one row as A operands (which only its warp needs): a[d] the d-th digits of every 4 of its columns.  Returns the factor of the scores.
 template <int HD>
 __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[3][HD / 16]) {
     using S = AqShape<HD>;
     float4 x[S::KS];
-    float m = 0.f;
-    bool finite = true;
-    const size_t at = there ? (size_t)(s.first + row / p.group) * p.q_stride + (size_t)(hk * p.group + row % p.group) * HD : 0;
+    float m = 0.f, zero = 0.f;
+    const size_t at = there ? aq_query_at(p, s, row, hk, HD) : 0;
 #pragma unroll
     for (int c = 0; c < S::KG; c++)
 #pragma unroll
@@ -64,29 +86,49 @@ __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s
             float4 & v = x[c * (S::KW / 4) + w];
             v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (there) v = aq_query(p.xtype, p.q, at + c * 4 * S::KW + q * S::KW + w * 4);
-            const float a0 = fabsf(v.x), a1 = fabsf(v.y), a2 = fabsf(v.z), a3 = fabsf(v.w);
-            finite = finite && a0 <= FLT_MAX && a1 <= FLT_MAX && a2 <= FLT_MAX && a3 <= FLT_MAX;
-            m = fmaxf(fmaxf(m, fmaxf(a0, a1)), fmaxf(a2, a3));
+            aq_max(v, m, zero);
         }
-    if (!finite) m = INFINITY;
+    if (zero != 0.f) m = INFINITY;
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // the largest to 2^21 x 1.98 .. 2^22 x 1.98: three digits reach 2^22 x 1.992.  A value is off by half of 1, at most 2^-22 of the largest
-    const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -100), 127) - 22;
-    const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+    const AqScaled f = aq_scaled(m);
 #pragma unroll
-    for (int i = 0; i < S::KS; i++) {
-        const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint32_t t[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) t[j] = (uint32_t)(__float2int_rn(v[j] * up) + 0x808080);       // digits + 128
-        const uint32_t t01 = __byte_perm(t[0], t[1], 0x5140), t23 = __byte_perm(t[2], t[3], 0x5140);
-        a[0][i] = __byte_perm(t01, t23, 0x5410) ^ 0x80808080u;
-        a[1][i] = __byte_perm(t01, t23, 0x7632) ^ 0x80808080u;
-        a[2][i] = __byte_perm(__byte_perm(t[0], t[1], 0x0062), __byte_perm(t[2], t[3], 0x0062), 0x5410) ^ 0x80808080u;
-    }
-    return m <= FLT_MAX ? down : __int_as_float(0x7fc00000);
+    for (int i = 0; i < S::KS; i++) aq_digits(x[i], f.up, a[0][i], a[1][i], a[2][i]);
+    return f.down * p.scale_log2;
 }
+// The R rows of a tile as digits in shared memory, by the whole CTA: [digit][row][HD + 16], and the factors of their scores.  The loads come before what
+// else the CTA asks for: behind the ring's first codes they are waited for 3 us.
+template <int HD, int R> struct AqQueries {
+    static constexpr int TPR = AQ_THREADS / R, W = HD / 4, N = (W + TPR - 1) / TPR, PITCH = HD + 16;
+    float4 x[N];
+    __device__ __forceinline__ void load(const AttnQ8P & p, const SeqB & s, const TileB & t, int hk) {
+        const int row = threadIdx.x / TPR, j = threadIdx.x % TPR;
+        const size_t at = row < t.n_rows ? aq_query_at(p, s, t.first + row, hk, HD) : 0;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < t.n_rows && j + u * TPR < W) x[u] = aq_query(p.xtype, p.q, at + (j + u * TPR) * 4);
+        }
+    }
+    __device__ __forceinline__ void put(const AttnQ8P & p, unsigned char * digits, float * factor) {
+        const int row = threadIdx.x / TPR, j = threadIdx.x % TPR;
+        float m = 0.f, zero = 0.f;
+#pragma unroll
+        for (int u = 0; u < N; u++) aq_max(x[u], m, zero);
+        if (zero != 0.f) m = INFINITY;
+#pragma unroll
+        for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const AqScaled f = aq_scaled(m);
+        if (j == 0) factor[row] = f.down * p.scale_log2;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            uint32_t d[3];
+            aq_digits(x[u], f.up, d[0], d[1], d[2]);
+#pragma unroll
+            for (int k = 0; k < 3; k++) if (j + u * TPR < W) *reinterpret_cast<uint32_t *>(digits + (k * R + row) * PITCH + (j + u * TPR) * 4) = d[k];
+        }
+    }
+};
 
 // Sums of products of digits and codes are whole numbers up to 2^22 (256 x 128 x 128): begun at 1.5 x 2^23's bits, they are that number plus the sum.
 static constexpr int AQ_ZERO = 0x4B400000;
@@ -121,18 +163,21 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
     using S = AqShape<HD>;
     constexpr int R = 8 * MT, ST = S::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R];
+    __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R], s_back[AQ_WARPS], s_f[R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const AqItem wk = aq_item(p, blockIdx.x);
     const int split = wk.split, rt = wk.rt, hk = wk.hk;
     pdl_launch();
     pdl_wait();
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
-    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, R);
+    const TileB t = aq_tile(p, s, rt, R);
     if (t.n_rows <= 0) return;
     const int k0 = split * p.split, k1 = split == wk.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
     if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
 
+    unsigned char * digits = smem + S::template DIGITS<MT>;
+    AqQueries<HD, R> queries;
+    queries.load(p, s, t, hk);
     const size_t head = (size_t)max(s.sq, 0) * p.c.H + hk;
     const int8_t * kc = p.c.k + head * p.c.n_ctx * HD, * vc = p.c.v + head * p.c.n_ctx * HD;
     const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
@@ -158,17 +203,29 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
     for (int it = 0; it < ST - 1; it++) issue();
 
+    queries.put(p, digits, s_f);
+    __syncthreads();
     uint32_t a[MT][3][S::KS];
-    float f[MT], m[MT], l[MT]; int sees[MT], score_row[MT], least = 0x7fffffff; bool there[MT];
+    float f[MT], m[MT], l[MT]; int sees[MT], least = 0x7fffffff; bool there[MT];
+    float * scores[MT];                                               // (where they are kept)
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-        const int row = mt * 8 + g;
+        const int row = mt * 8 + g, tok = p.by_group.of(t.first + row);
         there[mt] = row < t.n_rows;
-        f[mt] = aq_load_query<HD>(p, s, t.first + row, there[mt], hk, q, a[mt]) * p.scale_log2;
-        sees[mt] = there[mt] ? aq_sees(s, p.c.n_ctx, (t.first + row) / p.group) : 0;
+        f[mt] = s_f[row];
+        sees[mt] = there[mt] ? aq_sees(s, p.c.n_ctx, tok) : 0;
         if (there[mt]) least = min(least, sees[mt]);
-        score_row[mt] = (s.first + (t.first + row) / p.group) * p.n_head + hk * p.group + (t.first + row) % p.group;
+        scores[mt] = p.scores && there[mt] ? p.scores + (size_t)((s.first + tok) * p.n_head + hk * p.group + t.first + row - tok * p.group) * p.score_pitch + 2 * q : nullptr;
         m[mt] = -INFINITY; l[mt] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 3; d++)
+#pragma unroll
+            for (int c = 0; c < S::KG; c++) {
+                uint32_t w[S::KW / 4];
+                aq_lds<S::KW>(w, digits + (d * R + row) * (HD + 16) + c * 4 * S::KW + q * S::KW);
+#pragma unroll
+                for (int i = 0; i < S::KW / 4; i++) a[mt][d][c * (S::KW / 4) + i] = w[i];
+            }
     }
     least = __reduce_min_sync(0xffffffffu, least);
     float o[MT][S::NT][4];
@@ -204,7 +261,10 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         }
         // ---- probabilities, as A operands of the value products
         float ratio = 1.f;
-        if (sv > v_ref) { ratio = v_ref / sv; v_ref = sv; v_inv = AQ_P / sv; }
+        if (sv >= v_ref) {                                            // to the power of two above it: one rise where the scales are of one size
+            const float now = __uint_as_float(min((__float_as_uint(sv) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+            ratio = v_ref / now; v_ref = now; v_inv = AQ_P / now;
+        }
         const float pv = sv == 0.f ? 0.f : sv * v_inv;
         uint32_t pa[MT][4];
 #pragma unroll
@@ -222,8 +282,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
                     for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j >= sees[mt]) y[n][j] = -INFINITY;
             }
-            if (p.scores && there[mt]) {
-                float * to = p.scores + (size_t)score_row[mt] * p.score_pitch + j0 + 2 * q;
+            if (scores[mt]) {
+                float * to = scores[mt] + j0;
                 *reinterpret_cast<float2 *>(to) = make_float2(y[0][0], y[0][1]);
                 *reinterpret_cast<float2 *>(to + 8) = make_float2(y[1][0], y[1][1]);
             }
@@ -237,7 +297,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
                 l[mt] *= alpha;
                 down *= alpha;
             }
-            if (__any_sync(0xffffffffu, down != 1.f)) {
+            if (it > 0 && __any_sync(0xffffffffu, down != 1.f)) {
 #pragma unroll
                 for (int n = 0; n < S::NT; n++)
 #pragma unroll
@@ -283,8 +343,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; }
+        if (lane == 0) s_back[warp] = v_ref * (1.f / AQ_P);
         float * row = so + (size_t)(warp * R + mt * 8 + g) * PITCH;
-        const float back = v_ref * (1.f / AQ_P);
 #pragma unroll
         for (int c = 0; c < S::VG; c++)
 #pragma unroll
@@ -292,10 +352,10 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
                 for (int j = 0; j < S::VW; j += 4) {
                     float4 v;
-                    v.x = (o[mt][c * S::VW + j][h] + o[mt][c * S::VW + j][h + 2]) * back;
-                    v.y = (o[mt][c * S::VW + j + 1][h] + o[mt][c * S::VW + j + 1][h + 2]) * back;
-                    v.z = (o[mt][c * S::VW + j + 2][h] + o[mt][c * S::VW + j + 2][h + 2]) * back;
-                    v.w = (o[mt][c * S::VW + j + 3][h] + o[mt][c * S::VW + j + 3][h + 2]) * back;
+                    v.x = (o[mt][c * S::VW + j][h] + o[mt][c * S::VW + j][h + 2]);
+                    v.y = (o[mt][c * S::VW + j + 1][h] + o[mt][c * S::VW + j + 1][h + 2]);
+                    v.z = (o[mt][c * S::VW + j + 2][h] + o[mt][c * S::VW + j + 2][h + 2]);
+                    v.w = (o[mt][c * S::VW + j + 3][h] + o[mt][c * S::VW + j + 3][h + 2]);
                     *reinterpret_cast<float4 *>(row + c * 8 * S::VW + (2 * q + h) * S::VW + j) = v;
                 }
     }
@@ -310,16 +370,16 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < AQ_WARPS; w++) {
-            const float k = exp2_approx(s_m[w][r] - ref);
+            const float is = exp2_approx(s_m[w][r] - ref), k = is * s_back[w];
             const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * R + r) * PITCH + d);
-            sum = fmaf(k, s_l[w][r], sum);
+            sum = fmaf(is, s_l[w][r], sum);
             v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);
         }
         if (wk.n_splits > 1) {
             *reinterpret_cast<float4 *>(p.part + (part0 + r) * HD + d) = v;
             if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
         } else {
-            const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
+            const int row = t.first + r, of = p.by_group.of(row), tok = s.first + of, h = hk * p.group + row - of * p.group;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const size_t at = (size_t)tok * p.out_stride + (size_t)h * HD + d;
             aq_put(p.xtype, p.out, at, v.x * inv); aq_put(p.xtype, p.out, at + 1, v.y * inv);
@@ -361,7 +421,7 @@ __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
     ask(sub);
     const AqItem wk = aq_item(p, p.whole + k_item * p.n_splits);
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
-    const TileB t = aq_tile(s, p.c.n_ctx, p.group, R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, R);
+    const TileB t = aq_tile(p, s, R == AT_ROWS ? p.row_tiles - 1 - wk.rt : wk.rt, R);
     if (r >= t.n_rows) return;
     const int used = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));
 #pragma unroll
@@ -397,7 +457,7 @@ __global__ void __launch_bounds__(256) k_attn_q8_join(const AttnQ8P p, int R) {
                 for (int w = 0; w < WPR; w++) v[j] += s_sum[w][lane + 32 * j];
             }
     }
-    const int row = t.first + r, tok = s.first + row / p.group, h = wk.hk * p.group + row % p.group;
+    const int row = t.first + r, of = p.by_group.of(row), tok = s.first + of, h = wk.hk * p.group + row - of * p.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const size_t at = (size_t)tok * p.out_stride + (size_t)h * hd + lane;
 #pragma unroll
@@ -428,7 +488,7 @@ __global__ void __launch_bounds__(128) k_attn_q8_weights_kept(const AttnQ8P p, c
     const int rows = s.n_new * p.group;
 #pragma unroll 8
     for (int r = 0; r < rows; r++) {
-        const int tok = r / p.group, row = (s.first + tok) * p.n_head + hk * p.group + r - tok * p.group;
+        const int tok = p.by_group.of(r), row = (s.first + tok) * p.n_head + hk * p.group + r - tok * p.group;
         const float lse = __ldcg(p.lse + row);
         const int sees = aq_sees(s, p.c.n_ctx, tok) - j0;             // (scores of what a row does not see were not all made)
         const float4 y = __ldcg(reinterpret_cast<const float4 *>(p.scores + (size_t)row * p.score_pitch + j0));
@@ -508,10 +568,10 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
         const int tok0 = max(0, j0 - s.pos);                          // the first token that sees one of these slots
         for (int r0 = tok0 * p.group / 8 * 8; r0 < n_rows; r0 += 8) {
             if (r0 != a_row) {
-                const int row = r0 + g, tok = row / p.group;
+                const int row = r0 + g, tok = p.by_group.of(row);
                 const bool there = row < n_rows;
-                lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row % p.group) : 0.f;
-                f = aq_load_query<HD>(p, s, row, there, hk, q, a[0]) * p.scale_log2;
+                lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row - tok * p.group) : 0.f;
+                f = aq_load_query<HD>(p, s, row, there, hk, q, a[0]);
                 sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
                 a_row = r0;
             }
@@ -591,7 +651,7 @@ static int aq_go(const AttnQ8P & p, cudaStream_t st) {
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
-    constexpr size_t smem = AqShape<HD>::smem(MT);
+    constexpr size_t smem = AqShape<HD>::template SMEM<MT>;
     if (dev < 0 || dev >= 16 || !done[dev]) {
         PI_CUDA(cudaFuncSetAttribute(k_attn_q8<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
@@ -628,6 +688,7 @@ int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
     p.c = a.c; p.b = a.b; p.xtype = a.xtype; p.q = a.q; p.q_stride = a.q_stride; p.n_head = a.n_head; p.group = a.n_head / a.c.H;
     p.scale_log2 = a.scale * 1.44269504088896340736f; p.out = a.out; p.out_stride = a.out_stride;
     p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles; p.items = r.items; p.whole = r.whole;
+    p.by_group = AqDiv::by(p.group); p.by_heads = AqDiv::by(a.c.H); p.by_tiles = AqDiv::by(r.row_tiles); p.by_splits = AqDiv::by(r.n_splits);
     char * s = (char *)a.scratch;
     p.status = (unsigned int *)(s + 8);
     s += r.words;

@@ -4,12 +4,25 @@
 
 namespace pi {
 
+// n / d for n < 2^31 by a product (a division is 20 instructions, and what a CTA does before its first slot is waited for)
+struct AqDiv {
+    unsigned mul, shift;
+    __host__ static AqDiv by(int d) {
+        AqDiv r{0, 0};
+        while ((1ll << r.shift) < d) r.shift++;
+        r.mul = (unsigned)((1ull << 32) * ((1ull << r.shift) - (unsigned)d) / (unsigned)d + 1);
+        return r;
+    }
+    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi((unsigned)n, mul) + (unsigned)n) >> shift); }
+};
+
 struct AttnQ8P {
     KvQ8 c; RaggedB b;
     int xtype; const void * q; int64_t q_stride; int n_head, group;
     float scale_log2; void * out; int64_t out_stride;
     // An item is a tile of rows of a KV head of an entry.  The first `whole` items are a CTA each, the others n_splits: ranges of `split` slots.
     int split, n_splits, row_tiles, items, whole;
+    AqDiv by_group, by_heads, by_tiles, by_splits;                    // the KV heads' number, row_tiles, n_splits
     float * part; float2 * part_ml; float * lse;                      // [split item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
     float * scores; int score_pitch;                                  // (null: not kept) the rows' scores in bits, [T * n_head][pitch]
     unsigned int * status;                                            // tcgen05 alone: bit 4, a wait ran out
@@ -20,11 +33,11 @@ __device__ __forceinline__ AqItem aq_item(const AttnQ8P & p, int cta) {
     AqItem w;
     const int k = cta - p.whole;
     w.n_splits = k < 0 ? 1 : p.n_splits;
-    w.item = k < 0 ? cta : p.whole + k / p.n_splits;
-    w.split = k < 0 ? 0 : k % p.n_splits;
-    const int of_head = w.item / p.row_tiles;
+    w.item = k < 0 ? cta : p.whole + p.by_splits.of(k);
+    w.split = k < 0 ? 0 : k - (w.item - p.whole) * p.n_splits;
+    const int of_head = p.by_tiles.of(w.item);
     w.rt = w.item - of_head * p.row_tiles;
-    w.entry = of_head / p.c.H;
+    w.entry = p.by_heads.of(of_head);
     w.hk = of_head - w.entry * p.c.H;
     return w;
 }
@@ -37,14 +50,14 @@ __device__ __forceinline__ int aq_sees(const SeqB & s, int n_ctx, int tok) {    
     const int slot = s.pos + tok;
     return s.sq < 0 || slot >= n_ctx ? 0 : slot + 1;
 }
-__device__ __forceinline__ TileB aq_tile(const SeqB & s, int n_ctx, int group, int rt, int R) {
+__device__ __forceinline__ TileB aq_tile(const AttnQ8P & p, const SeqB & s, int rt, int R) {
     TileB t;
     t.first = rt * R;
-    t.n_rows = min(R, s.n_new * group - t.first);
+    t.n_rows = min(R, s.n_new * p.group - t.first);
     t.seen = 0;
     if (t.n_rows > 0 && s.sq >= 0) {                                  // the last of its rows whose slot there is
-        const int last = min((t.first + t.n_rows - 1) / group, n_ctx - 1 - s.pos);
-        if (last >= t.first / group) t.seen = s.pos + last + 1;
+        const int last = min(p.by_group.of(t.first + t.n_rows - 1), p.c.n_ctx - 1 - s.pos);
+        if (last >= p.by_group.of(t.first)) t.seen = s.pos + last + 1;
     }
     return t;
 }

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     pdl_wait();
     if (blockIdx.x == 0 && tid == 0) *p.status = 0u;
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, w.entry);
-    const TileB t = aq_tile(s, p.c.n_ctx, p.group, rt, AT_ROWS);
+    const TileB t = aq_tile(p, s, rt, AT_ROWS);
     if (t.n_rows <= 0) return;
     const int k0 = split * p.split, k1 = split == w.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
     if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     if constexpr (!TWO_Q) {
         if (warp >= 4 && warp < 20) {
             constexpr int NQ = HD / 4;
-            const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = t.first + r, tok = row / p.group;
+            const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = t.first + r, tok = p.by_group.of(row);
             uint32_t u[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) u[j] = 0u;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             float4 u[NL];
 #pragma unroll
             for (int k = 0; k < NL; k++) {
-                const int q = r0 + k * (32 / LPR) + lane / LPR, row = t.first + q, tok = row / p.group;
+                const int q = r0 + k * (32 / LPR) + lane / LPR, row = t.first + q, tok = p.by_group.of(row);
                 u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (q < t.n_rows) u[k] = aq_query(p.xtype, p.q, (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD + lane % LPR * 4);
             }
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * AT_KEYS + half * 64);
         const float * ks = p.c.ks + head * (p.c.n_ctx >> p.c.shift), * vs = p.c.vs + head * (p.c.n_ctx >> p.c.shift);
         const bool there = r < t.n_rows;
-        const int sees = there ? aq_sees(s, p.c.n_ctx, (t.first + r) / p.group) : 0;
+        const int sees = there ? aq_sees(s, p.c.n_ctx, p.by_group.of(t.first + r)) : 0;
         const int least = __reduce_min_sync(0xffffffffu, there ? sees : 0x7fffffff);
         const float f = s_f[r];
         auto scales = [&](int i, float & k, float & v) {              // lane j: those of the 16 slots j of the tile (0 behind the range)
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);
 
         if (r < t.n_rows) {
-            const int row = t.first + r, tok = s.first + row / p.group, h = hk * p.group + row % p.group;
+            const int row = t.first + r, of = p.by_group.of(row), tok = s.first + of, h = hk * p.group + row - of * p.group;
             if (!ok) sum = __int_as_float(0x7fc00000);                // a wait ran out: no numbers instead of wrong ones
             if (w.n_splits > 1) {
                 const size_t at = ((size_t)(w.item - p.whole) * p.n_splits + split) * AT_ROWS + r;
