@@ -7,6 +7,10 @@
 // between warps), keep a maximum, a sum and all sums of values of their own, and join them at the end.  Long ranges are
 // split over CTAs, whose sums k_attn_q8_join joins.
 //
+// Measured (FP16 or FP32 rows, head_dim 128): 32 sequences of 1056 to 2048 slots, 32 heads 80 us (5.1 TB/s; between two lengths 6.7, the copy rate: the rest is what
+// CTAs do before their first slot and behind their last, the tail and the launches), one of 32768 slots, 64 heads over 8 KV heads 17 us and 5 of the join.
+// Queries are asked for before the ring's codes: behind them they took 3 us of a CTA's 15.
+//
 // Precision.  Scores are products of whole numbers: the codes as they lie, and a query row of 23 bits and a sign as three digits of 8 bits, which are three rows
 // of the tensor cores' tile (24 rows for 8 queries, 48 for 16); their sums are exact.  A probability, times vs over the largest vs so far (at most 1), is the sum of
 // two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits, and a value's code is exact as a half: out = sums * that scale.  (Probabilities as

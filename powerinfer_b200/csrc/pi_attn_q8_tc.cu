@@ -12,6 +12,10 @@
 // as they are.  (Probabilities of FP16 rows as one half: 7 % less time for 11 bits.)  Values' scales ride on the probabilities, over the power of two above the tile's
 // largest one; probabilities are held times 2^14.
 //
+// Measured: 1024 tokens over 4096 slots, 64 FP32 heads of 128 over 8 KV heads 257 us of the call's 270 (tensor pipe 51 % busy, issue slots 64 %); prompts of 701 to 421
+// tokens, 128 FP16 heads of 64 327 us (19 %, 61 %).  A tile takes 1.9 us (64 dimensions: 1.4), a CTA 12 us (FP16 of 64: 5.5) besides, the last tile's way and the next CTA's start.
+// Bound by the issue slots: 8 exponentials, splits and rounded sums a slot and four rows, halves of the codes, while products of 16 slots take 57 clocks each to issue.
+//
 // Warps: 0 issues the products; 1 asks for the codes; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the halves tell each other
 // their maxima); 20..27 make the halves and drain the sums, a row and half of the columns a thread.
 #include "pi_attn_q8.cuh"
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) tc_dealloc(tmem, 512);
+    if (warp == 0) tc_dealloc(s_tmem, 512);
 }
 
 bool attn_q8_tc_takes(int hd, int64_t rows) { return (hd == 64 || hd == 128) && rows >= 64; }

@@ -10,7 +10,8 @@
 // again); the threshold from three histograms of 11, 11 and 10 bits (whole numbers: their order does not matter); then bit maps of what is above it and of
 // what equals it, sums over their words, and the holes' slots as a list from which every mover takes its place.  k_evict_move, a warp per block: rows are gathered
 // and scaled.  Few heads: bound by the instructions that one SM issues for a head's slots.  (A cluster of eight SMs a head was slower: the histograms travel.)
-// Many: by the bytes of the moved rows.
+// Many: by the bytes of the moved rows.  Measured: 16384 slots to 2048, 8 heads: 21 us and 10 us; 1280 to 1024, 16 sequences of 32 heads: 19 us and 30 us.
+// (Four copies of the first histogram, against lanes that meet in a bin: the same 21 us.)
 #include "pi_kv_q8.cuh"
 
 namespace pi {

@@ -10,7 +10,7 @@ Tolerances.  Half a step is u = 2^-24 in FP32 and 2^-11 in FP16.
              rounding by 2 E u: e_s = E (hd + 10) u in all.  A probability is then off by 2 e_s of itself, 4 u from exp2 (2 ulp),
              4 u from its product with the scale and its two halves, both sums by n u at most.  So an output is off by at most sum_j p_j |v_j| * (2 e_s + (2 n + 16) u); sums on
              the tensor cores are cut, not rounded: twice the u of sums.  The lower half of a probability has no steps below 2^-24 of what it
-             is held times, 2^7 and the largest scale of values so far, beside which the largest probability is 1 or more: what is left out is
+             is held times, 2^7 or more over the largest scale of values so far, beside which the largest probability is 1 or more: what is left out is
              2^-25 / 2^7 = 2^-32 of the largest value that a block holds, for each slot.  (Peaked softmaxes show it where the one value that counts is 0.)
   weights    the same of the sum of probabilities, over the tokens and heads that it adds.
 """
@@ -371,7 +371,7 @@ def test_attention_values_of_very_different_sizes(ops):
 
 @pytest.mark.parametrize("T", [1, 140])
 def test_attention_values_of_the_smallest_scales(ops, T):
-    """Scales of values from the smallest normal number on.  Below 2^-119 probabilities are held relative to 2^-119, i.e. 2^7 and not 2^14 times: what their
+    """Scales of values from the smallest normal number on.  Below 2^-118 probabilities are held times 2^8 over 2^-118, at 2^-126 times 1: what their
     lower halves leave out is 2^-25 of the largest value.  Sums near the smallest numbers are off by half of 2^-149 wherever they are rounded: once a tile
     or warp, once a split, once where they are put out."""
     rng = np.random.default_rng(T)

@@ -1,6 +1,8 @@
 """The operators of a long context without a device: what they refuse, calls without work, and the frequencies of scaled rotary positions."""
 import ctypes as C
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -165,3 +167,14 @@ def test_frequencies_refuse(bad):
     out, m = np.empty(256), C.c_float()
     assert lib.pi_rope_freqs_host(out.ctypes.data, C.addressof(m), a["n_rot"], a["base"], a["scale"], a["ext"], 1.0, 32.0, 1.0, 0, None) == INVALID
     assert "rope_freqs" in err()
+
+
+def test_the_prompt_kernel_gives_tensor_memory_back_when_no_product_is_in_flight():
+    """The issuing warp waits for its last products, also after a wait ran out (no look at s_dead); copies on their way land before the CTA ends; the threads that meet
+    at a named barrier come to it whatever ran out."""
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "pi_attn_q8_tc.cu")).read()
+    assert text.count("tc_dealloc(") == 1
+    assert re.search(r"tc_commit\(&(\w+)\);[^\n]*\n *for \(int spins = 0; spins < \(1 << 20\) && !mbar_try_wait\(&\1, 0u\); spins\+\+\) \{\}\n *__syncwarp\(\);", text)
+    assert "ring_land(s_rfull, i, AT_RAW)" in text
+    loop = text[text.index("for (int i = b; i < n_tiles; i += 2)"):text.index("// ================================================================= tiles in, sums out")]
+    assert "bar.sync" in loop and not re.search(r"\b(break|return);", re.sub(r"if \([^)]*parts\) break;", "", loop))
