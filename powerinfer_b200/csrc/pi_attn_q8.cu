@@ -612,8 +612,9 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
 struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole, pitch; size_t words, lse, ml, part, scores; };     // rows of a tile; bytes of each piece of scratch
 
 // CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split
-// into ranges of at least AQ_LEAST slots.  A CTA costs as much as its slots and AQ_TURN times 64 more, and so does the kernel that joins.
-static constexpr int AQ_LEAST = 256, AQ_TURN = 4;
+// into ranges of at least AQ_LEAST slots.  A CTA costs as much as its slots and AQ_TURN times 64 more (on tcgen05 AQ_TURN_TC), the kernel that joins
+// as AQ_TURN times 64.
+static constexpr int AQ_LEAST = 256, AQ_TURN = 4, AQ_TURN_TC = 10, AQ_ROUNDS = 4;        // (more rounds than that: room for the parts, and nothing gained)
 // Weights: scores of few rows are kept, if they take no more than this (8 sequences of 64 heads and 8000 slots, 16 MB: 28 us for reading the keys again, 6 so)
 static constexpr int64_t AQ_SCORES = int64_t(256) << 20;
 static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
@@ -626,9 +627,11 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
     const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd <= 128 && r.R == 8 ? 3 : 2), rest = items % slots, units = (keys + AQ_LEAST / 4 - 1) / (AQ_LEAST / 4);
     // parts of an item of the last round: the number for which its CTAs, in rounds of their own, take the least
+    const int64_t turn = r.tc ? AQ_TURN_TC : AQ_TURN;
     int64_t n = 1, least = -1;
     for (int64_t k = 1; rest && k <= 128 && (k == 1 || k * AQ_LEAST < keys + AQ_LEAST); k++) {
-        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + AQ_TURN) + (k > 1 ? AQ_TURN : 0);
+        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + turn) + (k > 1 ? AQ_TURN : 0);
+        if (rounds > AQ_ROUNDS) break;
         if (least < 0 || cost < least) { least = cost; n = k; }
     }
     const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;

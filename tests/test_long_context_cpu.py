@@ -125,6 +125,15 @@ def test_workspace_sizes():
     assert workspace(cache(), batch(), 6, 256) == 0 and "multiple" in err()
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("n,new,group", [(1, 1, 8), (50, 1, 8), (37, 1, 1), (3, 20, 4), (2, 1000, 8), (400, 1, 16)])
+def test_partial_sums_stay_small(hd, n, new, group):
+    """Partial sums are of the last round's items: a few rounds of 444 CTAs of 8 rows, or of 148 of 128, however long the context is."""
+    for n_ctx in (4096, 1 << 20):
+        got = workspace(cache(n_seq=1, head_dim=hd, n_ctx=n_ctx), batch(n=n, T=n * new, max_new=new), 4 * group, n_ctx)
+        assert got <= 4 * 444 * 16 * (hd * 4 + 8) * 3 + 4096
+
+
 def freqs(n_rot, base=10000.0, scale=1.0, ext=0.0, attn=1.0, fast=32.0, slow=1.0, orig=0, factors=None):
     out, m = np.empty(n_rot // 2), C.c_float()
     f = None if factors is None else np.asarray(factors, np.float32)
