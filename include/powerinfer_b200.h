@@ -224,6 +224,7 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
  * those tokens and the heads of the group, plus weights_in (same shape, may be the same array; NULL: 0) for slots before pos0; the sums' order is
  * fixed.  Other elements are left as they were.  Of entries that name one sequence the last one with tokens counts.
  * workspace: pi_attention_q8_workspace_bytes with the same arguments (`weights`: whether weights_out is given), 256-byte aligned; 0 bytes may be NULL.
+ * It serves one call at a time: calls of one stream, or captured graphs that are not replayed at once.
  * From 64 query rows a KV head on (head_dim 64 and 128), pi_op_status(workspace) tells whether all bounded waits inside the kernel completed; the rows of one that
  * did not are NaN. */
 size_t pi_attention_q8_workspace_bytes(const pi_kv_q8 * cache, const pi_kv_batch * batch, int n_head, int max_kv, int weights);
