@@ -455,6 +455,15 @@ def test_attention_refuses(ops):
     assert ops.attention_q8(p.d, torch.zeros(0, 256, device="cuda"), ints([0, 0]), z).shape == (0, 256)
 
 
+@pytest.mark.parametrize("hd", [64, 96, 192, 256])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+def test_weights_where_scores_are_not_kept(ops, hd, x):
+    """Scores of 300 tokens and 16 heads with room for 16384 slots are more than the workspace keeps: the keys are read a second time."""
+    rng = np.random.default_rng(hd)
+    p = Pair(ops, 2, 2, 16384, hd, 32, fill=rng)
+    run_attention(ops, p, rng, [0, 290, 300], [41, 7], 16, x, seq=[1, 0], max_kv=400, weights=True)
+
+
 def test_attention_of_a_prompt_leaves_a_clear_status(ops):
     """Through the C entry, whose workspace is the caller's: full of ones before, the status word says that every wait completed."""
     import ctypes as C
