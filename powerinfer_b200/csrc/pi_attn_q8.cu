@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
     using S = AqShape<HD>;
     constexpr int R = 8 * MT, ST = S::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R], s_back[AQ_WARPS], s_f[R];
+    __shared__ float s_m[AQ_WARPS][R], s_l[AQ_WARPS][R], s_back[AQ_WARPS][R], s_f[R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const AqItem wk = aq_item(p, blockIdx.x);
     const int split = wk.split, rt = wk.rt, hk = wk.hk;
@@ -239,7 +239,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         for (int n = 0; n < S::NT; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) o[mt][n][j] = 0.f;
-    float v_ref = AQ_V_LEAST, v_inv = AQ_P / AQ_V_LEAST;              // scale of the value sums, and AQ_P over it
+    float v_ref[MT], v_inv[MT];                                       // scale of a row's value sums, and AQ_P over it (of what the row sees: others' scales have no say in it)
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) { v_ref[mt] = AQ_V_LEAST; v_inv[mt] = AQ_P / AQ_V_LEAST; }
 
     const unsigned char * kt = ring + (ST - 1) * S::STAGE;
     for (int it = 0; it < steps; it++) {
@@ -264,15 +266,15 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
                 for (int n = 0; n < 2; n++) aq_products<HD, MT>(x[n], a, c * (S::KW / 8) + i, w[n][2 * i], w[n][2 * i + 1]);
         }
         // ---- probabilities, as A operands of the value products
-        float ratio = 1.f;
-        if (sv >= v_ref) {                                            // to the power of two above it: one rise where the scales are of one size
-            const float now = __uint_as_float(min((__float_as_uint(sv) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
-            ratio = v_ref / now; v_ref = now; v_inv = AQ_P / now;
-        }
-        const float pv = sv == 0.f ? 0.f : sv * v_inv;
         uint32_t pa[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
+            float down = 1.f;
+            if (sv >= v_ref[mt] && j0 < sees[mt]) {                   // to the power of two above it: one rise where the scales are of one size
+                const float now = __uint_as_float(min((__float_as_uint(sv) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+                down = v_ref[mt] / now; v_ref[mt] = now; v_inv[mt] = AQ_P / now;
+            }
+            const float pv = sv * v_inv[mt];
             float y[2][2];
             const float fk = f[mt] * sk;
 #pragma unroll
@@ -292,7 +294,6 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
                 *reinterpret_cast<float2 *>(to + 8) = make_float2(y[1][0], y[1][1]);
             }
             float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
-            float down = ratio;
             if (__any_sync(0xffffffffu, top > m[mt] + AQ_RISE)) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -346,8 +347,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         float sum = l[mt];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; }
-        if (lane == 0) s_back[warp] = v_ref * (1.f / AQ_P);
+        if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; s_back[warp][mt * 8 + g] = v_ref[mt] * (1.f / AQ_P); }
         float * row = so + (size_t)(warp * R + mt * 8 + g) * PITCH;
 #pragma unroll
         for (int c = 0; c < S::VG; c++)
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < AQ_WARPS; w++) {
-            const float is = exp2_approx(s_m[w][r] - ref), k = is * s_back[w];
+            const float is = exp2_approx(s_m[w][r] - ref), k = is * s_back[w][r];
             const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * R + r) * PITCH + d);
             sum = fmaf(is, s_l[w][r], sum);
             v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);

@@ -9,8 +9,8 @@
 // So every tile has its own maximum (no exchange between tiles; the two score buffers are two groups of warps' own): the drain joins tiles.
 //
 // Precision.  Probabilities, and queries of FP32 rows, as the sum of two halves each, i.e. two products in the place of one: 22 bits.  Queries of FP16 rows
-// as they are.  (Probabilities of FP16 rows as one half: 7 % less time for 11 bits.)  Values' scales ride on the probabilities, over the power of two above the tile's
-// largest one; probabilities are held times 2^14.
+// as they are.  (Probabilities of FP16 rows as one half: 7 % less time for 11 bits.)  Values' scales ride on the probabilities, over the power of two above the
+// largest one that the row sees in the tile; probabilities are held times 2^14.
 //
 // Measured: 1024 tokens over 4096 slots, 64 FP32 heads of 128 over 8 KV heads 257 us of the call's 270 (tensor pipe 51 % busy, issue slots 64 %); prompts of 701 to 421
 // tokens, 128 FP16 heads of 64 327 us (19 %, 61 %).  A tile takes 1.9 us (64 dimensions: 1.4), a CTA 12 us (FP16 of 64: 5.5) besides, the last tile's way and the next CTA's start.
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     __shared__ float s_f[AT_ROWS];                                    // factor of a row's scores
     __shared__ float s_max[2][2][AT_ROWS], s_sum[2][2][AT_ROWS];       // of a tile's halves: maximum, sum of the probabilities
     __shared__ float s_top[2][AT_ROWS];                               // maximum of a tile
-    __shared__ float s_ref[2];                                        // largest scale of its values
+    __shared__ float s_ref[2][AT_ROWS];                               // power of two that its values' scales are held over
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t kbuf = (smem_u32(smem_raw) + 1023u) & ~1023u, vbuf = kbuf + 2 * TILE, raw = vbuf + 2 * TILE;
     const AqItem w = aq_item(p, blockIdx.x);
@@ -298,12 +298,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
         if (b < n_tiles) scales(b, sk, sv);
         for (int i = b; i < n_tiles; i += 2) {                        // (to the end whatever waits ran out: the halves meet at a barrier)
             const int left = sees - (k0 + i * AT_KEYS + half * 64);   // slots of this half that the row sees
-            float largest = fabsf(sv) <= FLT_MAX ? sv : 0.f;          // (of the finite ones)
+            const float wv = sv, wk = sk, finite = fabsf(sv) <= FLT_MAX ? sv : 0.f;
+            float largest = finite;                                   // of the finite ones that the row sees (what others see has no say in it)
+            if (k0 + i * AT_KEYS + AT_KEYS > least) {                 // (decided by all eight pieces: the same in both halves)
+                largest = 0.f;
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                for (int c = 0; c < 8; c++) { const float v = __shfl_sync(0xffffffffu, finite, c); if (k0 + i * AT_KEYS + c * 16 < sees) largest = fmaxf(largest, v); }
+            } else {
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            }
             // 2^14 over the power of two above it (exact; clamped where that is no normal number)
             const int e = min(max((int)(__float_as_uint(largest) >> 23), 14), 253);
-            const float ref_v = __uint_as_float((uint32_t)(e - 13) << 23), wv = sv == 0.f ? 0.f : sv * __uint_as_float((uint32_t)(267 - e) << 23), wk = sk;
+            const float up = __uint_as_float((uint32_t)(267 - e) << 23);
             float fk[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) fk[c] = f * __shfl_sync(0xffffffffu, wk, half * 4 + c);
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
                     float x[16];
                     tc_ld16(x, mine + 16 * c);
                     uint32_t hl[16];                                  // upper parts of 16 slots, then lower parts
-                    const float2 fc = f2(c == 0 ? fk[0] : c == 1 ? fk[1] : c == 2 ? fk[2] : fk[3]), pv = f2(__shfl_sync(0xffffffffu, wv, half * 4 + c));
+                    const float2 fc = f2(c == 0 ? fk[0] : c == 1 ? fk[1] : c == 2 ? fk[2] : fk[3]), pv = f2(__shfl_sync(0xffffffffu, wv, half * 4 + c) * up);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const float2 y = f2_fma(make_float2(x[j], x[j + 1]), fc, ref);
@@ -361,8 +368,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             if (masked) exps(std::true_type()); else exps(std::false_type());
             if (i >= 2) wait(s_free + b, (i - 2) >> 1 & 1);           // the tile before has been drained: its sums are no more needed
             s_sum[b][half][r] = (l[0].x + l[0].y) + (l[1].x + l[1].y);
-            if (half == 0) s_top[b][r] = m;
-            if (r == 0 && half == 0) s_ref[b] = ref_v;
+            if (half == 0) { s_top[b][r] = m; s_ref[b][r] = __uint_as_float((254u << 23) - __float_as_uint(up)); }      // (1 / up)
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -381,8 +387,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
             const float was = top == now ? 1.f : exp2_approx(top - now), is = m == -INFINITY ? 0.f : exp2_approx(m - now);
             top = now;
             sum = fmaf(sum, was, (s_sum[b][0][r] + s_sum[b][1][r]) * is);
-            const float ref = s_ref[b];
-            const float k = is * ref;
+            const float k = is * s_ref[b][r];
             ok = wait(s_pv + b, i >> 1 & 1) && ok;
             tc_fence_after();
 #pragma unroll
