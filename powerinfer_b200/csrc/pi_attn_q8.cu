@@ -11,8 +11,8 @@
 // CTAs do before their first slot and behind their last, the tail and the launches), one of 32768 slots, 64 heads over 8 KV heads 17 us and 5 of the join.
 // Queries are asked for before the ring's codes: behind them they took 3 us of a CTA's 15.
 //
-// Precision.  Scores are products of whole numbers: the codes as they lie, and a query row of 23 bits and a sign as three digits of 8 bits, which are three rows
-// of the tensor cores' tile (24 rows for 8 queries, 48 for 16); their sums are exact.  A probability, times vs over the largest vs so far (at most 1), is the sum of
+// Precision.  Scores are products of whole numbers: the codes as they lie, and a query row of 31 bits and a sign as four digits of 8 bits, which are four rows
+// of the tensor cores' tile (32 rows for 8 queries, 64 for 16); their sums are exact.  A probability, times vs over the largest vs so far (at most 1), is the sum of
 // two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits, and a value's code is exact as a half: out = sums * that scale.  (Probabilities as
 // digits would spare the values' conversions, but their sums fill twice the registers, and whole numbers cannot follow a maximum that rises.)
 // Maxima, sums and the exponents' arguments are FP32.
@@ -42,7 +42,7 @@ template <int HD> struct AqShape {
     // shared memory: the ring, in the end the warps' sums in its place, and the queries' digits
     static constexpr size_t RING = (size_t)AQ_WARPS * STAGES * STAGE;
     template <int MT> static constexpr size_t DIGITS = RING > (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4 ? RING : (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4;
-    template <int MT> static constexpr size_t SMEM = DIGITS<MT> + 3 * 8 * MT * (HD + 16);
+    template <int MT> static constexpr size_t SMEM = DIGITS<MT> + 4 * 8 * MT * (HD + 16);
 };
 
 template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], const unsigned char * p) {
@@ -51,26 +51,29 @@ template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], co
     else                       r[0] = *reinterpret_cast<const uint32_t *>(p);
 }
 
-// A query row in whole numbers of 23 bits and a sign, as three digits to the base 256 (-128 .. 127), four columns at a time
+// A query row in whole numbers of 31 bits and a sign, as four digits to the base 256 (-128 .. 127), four columns at a time.  (Three digits, 23 bits, are too few: a value is off by
+// half of 1, whatever its size is, and queries with a channel tens of times larger than the others are usual.  With four, FP32 values within 2^-7 of the row's
+// largest and FP16 ones within 2^-20 are exact.)
 struct AqScaled { float up, down; };                                  // factor of the row; of its scores (not a number where a value of the row is not finite: so are they)
 __device__ __forceinline__ void aq_max(const float4 & v, float & m, float & zero) {    // zero: no more 0 where a value is not finite
     m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
     zero = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, zero))));
 }
-// the largest to 2^21 x 1.98 .. 2^22 x 1.98: three digits reach 2^22 x 1.992.  A value is off by half of 1, at most 2^-22 of the largest
+// the largest to 2^29 x 1.98 .. 2^30 x 1.98: four digits reach 2^30 x 1.992.  A value is off by half of 1, at most 2^-30.9 of the largest
 __device__ __forceinline__ AqScaled aq_scaled(float m) {
-    const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -100), 128) - 22;
+    const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -92), 128) - 30;
     return {__uint_as_float((uint32_t)(127 - e) << 23), m < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : __int_as_float(0x7fc00000)};
 }
-__device__ __forceinline__ void aq_digits(const float4 & x, float up, uint32_t & d0, uint32_t & d1, uint32_t & d2) {
+__device__ __forceinline__ void aq_digits(const float4 & x, float up, uint32_t (&d)[4]) {
     const float v[4] = {x.x, x.y, x.z, x.w};
     uint32_t t[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) t[j] = (uint32_t)(__float2int_rn(v[j] * up) + 0x808080);           // digits + 128
-    const uint32_t t01 = __byte_perm(t[0], t[1], 0x5140), t23 = __byte_perm(t[2], t[3], 0x5140);
-    d0 = __byte_perm(t01, t23, 0x5410) ^ 0x80808080u;
-    d1 = __byte_perm(t01, t23, 0x7632) ^ 0x80808080u;
-    d2 = __byte_perm(__byte_perm(t[0], t[1], 0x0062), __byte_perm(t[2], t[3], 0x0062), 0x5410) ^ 0x80808080u;
+    for (int j = 0; j < 4; j++) t[j] = (uint32_t)__float2int_rn(v[j] * up) + 0x80808080u;          // digits + 128
+    const uint32_t a = __byte_perm(t[0], t[1], 0x5140), b = __byte_perm(t[2], t[3], 0x5140), c = __byte_perm(t[0], t[1], 0x7362), e = __byte_perm(t[2], t[3], 0x7362);
+    d[0] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+    d[1] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+    d[2] = __byte_perm(c, e, 0x5410) ^ 0x80808080u;
+    d[3] = __byte_perm(c, e, 0x7632) ^ 0x80808080u;
 }
 __device__ __forceinline__ size_t aq_query_at(const AttnQ8P & p, const SeqB & s, int row, int hk, int hd) {
     const int tok = p.by_group.of(row);
@@ -78,7 +81,7 @@ __device__ __forceinline__ size_t aq_query_at(const AttnQ8P & p, const SeqB & s,
 }
 // A lane's pieces of one row as A operands (which only its warp needs): a[d] the d-th digits of every 4 of its columns.  Returns the factor of the scores.
 template <int HD>
-__device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[3][HD / 16]) {
+__device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s, int row, bool there, int hk, int q, uint32_t (&a)[4][HD / 16]) {
     using S = AqShape<HD>;
     float4 x[S::KS];
     float m = 0.f, zero = 0.f;
@@ -97,7 +100,12 @@ __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const AqScaled f = aq_scaled(m);
 #pragma unroll
-    for (int i = 0; i < S::KS; i++) aq_digits(x[i], f.up, a[0][i], a[1][i], a[2][i]);
+    for (int i = 0; i < S::KS; i++) {
+        uint32_t d[4];
+        aq_digits(x[i], f.up, d);
+#pragma unroll
+        for (int k = 0; k < 4; k++) a[k][i] = d[k];
+    }
     return f.down * p.scale_log2;
 }
 // The R rows of a tile as digits in shared memory, by the whole CTA: [digit][row][HD + 16], and the factors of their scores.  The loads come before what
@@ -126,10 +134,10 @@ template <int HD, int R> struct AqQueries {
         if (j == 0) factor[row] = f.down * p.scale_log2;
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            uint32_t d[3];
-            aq_digits(x[u], f.up, d[0], d[1], d[2]);
+            uint32_t d[4];
+            aq_digits(x[u], f.up, d);
 #pragma unroll
-            for (int k = 0; k < 3; k++) if (j + u * TPR < W) *reinterpret_cast<uint32_t *>(digits + (k * R + row) * PITCH + (j + u * TPR) * 4) = d[k];
+            for (int k = 0; k < 4; k++) if (j + u * TPR < W) *reinterpret_cast<uint32_t *>(digits + (k * R + row) * PITCH + (j + u * TPR) * 4) = d[k];
         }
     }
 };
@@ -142,24 +150,24 @@ __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, 
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1),
                    "r"(first ? AQ_ZERO : d[0]), "r"(first ? AQ_ZERO : d[1]), "r"(first ? AQ_ZERO : d[2]), "r"(first ? AQ_ZERO : d[3]));
 }
-__device__ __forceinline__ float aq_score(int d2, int d1, int d0) {
-    const float f2 = __int_as_float(d2) - 12582912.f, f1 = __int_as_float(d1) - 12582912.f, f0 = __int_as_float(d0) - 12582912.f;
-    return fmaf(fmaf(f2, 256.f, f1), 256.f, f0);
+__device__ __forceinline__ float aq_score(int d3, int d2, int d1, int d0) {
+    const float f3 = __int_as_float(d3) - 12582912.f, f2 = __int_as_float(d2) - 12582912.f, f1 = __int_as_float(d1) - 12582912.f, f0 = __int_as_float(d0) - 12582912.f;
+    return fmaf(fmaf(fmaf(f3, 256.f, f2), 256.f, f1), 256.f, f0);
 }
-// products of 32 columns of 8 slots (b0, b1) and of the rows: x[digit 2 | 1], x[digit 0] for 8 rows, x[digit] for 16
+// products of 32 columns of 8 slots (b0, b1) and of the rows: x[digits 3 | 2], x[digits 1 | 0] for 8 rows, x[digit] for 16
 template <int HD, int MT, int NX>
-__device__ __forceinline__ void aq_products(int (&x)[NX][4], const uint32_t (&a)[MT][3][HD / 16], int s, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void aq_products(int (&x)[NX][4], const uint32_t (&a)[MT][4][HD / 16], int s, uint32_t b0, uint32_t b1) {
     if constexpr (MT == 1) {
-        mma16832(x[0], a[0][2][2 * s], a[0][1][2 * s], a[0][2][2 * s + 1], a[0][1][2 * s + 1], b0, b1, s == 0);
-        mma16832(x[1], a[0][0][2 * s], 0u, a[0][0][2 * s + 1], 0u, b0, b1, s == 0);
+#pragma unroll
+        for (int d = 0; d < 2; d++) mma16832(x[d], a[0][3 - 2 * d][2 * s], a[0][2 - 2 * d][2 * s], a[0][3 - 2 * d][2 * s + 1], a[0][2 - 2 * d][2 * s + 1], b0, b1, s == 0);
     } else {
 #pragma unroll
-        for (int d = 0; d < 3; d++) mma16832(x[d], a[0][d][2 * s], a[1][d][2 * s], a[0][d][2 * s + 1], a[1][d][2 * s + 1], b0, b1, s == 0);
+        for (int d = 0; d < 4; d++) mma16832(x[d], a[0][d][2 * s], a[1][d][2 * s], a[0][d][2 * s + 1], a[1][d][2 * s + 1], b0, b1, s == 0);
     }
 }
 template <int MT, int NX> __device__ __forceinline__ float aq_score_of(const int (&x)[NX][4], int mt, int j) {
-    if constexpr (MT == 1) return aq_score(x[0][j], x[0][2 + j], x[1][j]);
-    else                   return aq_score(x[2][2 * mt + j], x[1][2 * mt + j], x[0][2 * mt + j]);
+    if constexpr (MT == 1) return aq_score(x[0][j], x[0][2 + j], x[1][j], x[1][2 + j]);
+    else                   return aq_score(x[3][2 * mt + j], x[2][2 * mt + j], x[1][2 * mt + j], x[0][2 * mt + j]);
 }
 
 template <int HD, int MT>
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 
     queries.put(p, digits, s_f);
     __syncthreads();
-    uint32_t a[MT][3][S::KS];
+    uint32_t a[MT][4][S::KS];
     float f[MT], m[MT], l[MT]; int sees[MT], least = 0x7fffffff; bool there[MT];
     float * scores[MT];                                               // (where they are kept)
 #pragma unroll
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         scores[mt] = p.scores && there[mt] ? p.scores + (size_t)((s.first + tok) * p.n_head + hk * p.group + t.first + row - tok * p.group) * p.score_pitch + 2 * q : nullptr;
         m[mt] = -INFINITY; l[mt] = 0.f;
 #pragma unroll
-        for (int d = 0; d < 3; d++)
+        for (int d = 0; d < 4; d++)
 #pragma unroll
             for (int c = 0; c < S::KG; c++) {
                 uint32_t w[S::KW / 4];
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         const float sk = __ldg(ks + (j0 >> p.c.shift)), sv = __ldg(vs + (j0 >> p.c.shift));
 
         // ---- scores of 16 slots
-        int x[2][MT + 1][4];
+        int x[2][2 * MT][4];
 #pragma unroll
         for (int c = 0; c < S::KG; c++) {
             uint32_t w[2][S::KW / 4];
@@ -561,7 +569,7 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
         }
         later = __any_sync(0xffffffffu, later);
     }
-    uint32_t a[1][3][S::KS];
+    uint32_t a[1][4][S::KS];
     float f = 0.f, lse = 0.f;
     int a_row = -1, sees = 0;
     if (later) return;

@@ -3,7 +3,7 @@ the same bits.  Half a step is u = 2^-24 in FP32, 2^-11 in FP16."""
 import numpy as np
 import pytest
 
-from test_gpu_long_context import Pair, dev, ints, ops, rows, run_attention  # noqa: F401
+from test_gpu_long_context import NP, Pair, U, dev, ints, ops, rows, run_attention  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -42,3 +42,65 @@ def test_prompt_rows_against_64_bits_beside_a_large_later_scale(ops):
         p.c.scale["v"][0, :, 14] = 1e12
         p.d.v_scale.copy_(dev(p.c.scale["v"]))
         run_attention(ops, p, rng, [0, 140], [100], 8)
+
+
+# ------------------------------------------------------------------------------------------------ queries with one large element
+
+def check_large(ops, p, q, start, pos, n_head, x, max_kv=None):
+    """A query is whole numbers of which the row's largest is 2^30 x 0.99 or more: a value is off by 2^-30.9 of it at most, products with codes and their sums are
+    exact.  Four sums become one number in FP32 steps (a sum is 2^22 at most: u of 2^30 each beside u of the score), then come two factors, the product and the
+    difference in the exponent: e_s = scale (2^-30.9 max |q| max_j sum_d |k_jd| + 2 u max |q| max_j s_j) + 10 u max_j |s_j|.  The rest as in
+    test_gpu_long_context.  Weights are sums of probabilities: 2 e_s + (4 n + 16) u of each, and u for each addition."""
+    T, hd, H, group = len(q), p.c.hd, p.c.H, n_head // p.c.H
+    scale, u = hd ** -0.5, U["f32"]
+    shape = (p.c.n_seq, H, p.c.n_ctx)
+    w_got, w_want = torch.zeros(shape, device="cuda"), np.zeros(shape)
+    got = ops.attention_q8(p.d, dev(q), ints(start), ints(pos), max_kv=max_kv, weights_out=w_got).float().cpu().numpy().astype(np.float64)
+    want, size, _, most = p.c.attention(q, n_head, scale, start, pos, w_out=w_want)
+    heads = q.astype(np.float64).reshape(T, n_head, hd)
+    e_s, n_max = np.zeros((T, n_head)), 1
+    for i, first, n, at, sq in p.c.entries(start, pos, None, T, T):
+        end = min(at + n, p.c.n_ctx)
+        n_max = max(n_max, end)
+        for h in range(H):
+            k = p.c.values("k", sq, h, end)
+            hs = slice(h * group, (h + 1) * group)
+            big = np.abs(heads[first:first + n, hs]).max(-1)
+            top = np.abs(np.einsum("tgd,jd->tgj", heads[first:first + n, hs], k)).max(-1)
+            e_s[first:first + n, hs] = scale * (big * (2.0 ** -30.9 * np.abs(k).sum(-1).max() + 2 * u * p.c.scale["k"][sq, h].max()) + 10 * u * top)
+    rel = 2 * e_s + (4 * n_max + 16) * u
+    tol = (size.reshape(T, n_head, hd) * rel[..., None] + 2.0 ** -32 * most[..., None]).reshape(T, -1) + 1e-30
+    if x == "f16":
+        tol = tol + U["f16"] * (np.abs(want) + tol) + 2.0 ** -25
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+    wt = w_want * (rel.max() + (T * group + 2) * u) + 1e-30
+    off = np.abs(w_got.cpu().numpy() - w_want)
+    assert np.all(off <= wt), float((off / wt).max())
+
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("group", [4, 16])
+@pytest.mark.parametrize("large", [30.0, 3000.0])
+def test_queries_with_one_large_element(ops, x, hd, group, large):
+    """A channel that is large in the queries and nothing in the keys: the other elements keep their bits."""
+    rng = np.random.default_rng(hd + group)
+    p = Pair(ops, 2, 2, 64, hd, 16, fill=rng)
+    p.c.codes["k"][..., 5] = 0
+    p.d.k.copy_(dev(p.c.codes["k"]))
+    q = rng.standard_normal((2, 2 * group, hd)).astype(np.float32)
+    q[..., 5] = np.sign(q[..., 5]) * large
+    check_large(ops, p, q.reshape(2, -1).astype(NP[x]), [0, 1, 2], [50, 63], 2 * group, x)
+
+
+@pytest.mark.parametrize("hd", [96, 256])
+def test_weights_of_queries_with_one_large_element(ops, hd):
+    """Where the keys are read a second time for the weights."""
+    rng = np.random.default_rng(hd)
+    p = Pair(ops, 1, 1, 16384, hd, 32, fill=rng)
+    p.c.codes["k"][..., 5] = 0
+    p.d.k.copy_(dev(p.c.codes["k"]))
+    T, n_head = 290, 16
+    q = rng.standard_normal((T, n_head, hd)).astype(np.float32)
+    q[..., 5] = np.sign(q[..., 5]) * 3000
+    check_large(ops, p, q.reshape(T, -1), [0, T], [41], n_head, "f32", max_kv=400)
