@@ -11,8 +11,10 @@
 // CTAs do before their first slot and behind their last, the tail and the launches), one of 32768 slots, 64 heads over 8 KV heads 17 us and 5 of the join.
 // Queries are asked for before the ring's codes: behind them they took 3 us of a CTA's 15.
 //
-// Precision.  Scores are products of whole numbers: the codes as they lie, and a query row of 31 bits and a sign as four digits of 8 bits, which are four rows
-// of the tensor cores' tile (32 rows for 8 queries, 64 for 16); their sums are exact.  A probability, times vs over the largest vs so far (at most 1), is the sum of
+// Precision.  Scores of 8 rows are products of whole numbers: the codes as they lie, and a query row of 31 bits and a sign as four digits of 8 bits, which are four rows
+// of the tensor cores' tile; their sums are exact.  16 rows have queries as halves, FP16 as they are and FP32 as the sum of two (22 bits), and the codes become halves
+// for them: digits are four products for all of the rows, 160 us where two halves take 149 and one 132 (8 sequences of 7 tokens, 8000 slots, 64 heads over 8).
+// A probability, times vs over the largest vs so far (at most 1), is the sum of
 // two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits, and a value's code is exact as a half: out = sums * that scale.  (Probabilities as
 // digits would spare the values' conversions, but their sums fill twice the registers, and whole numbers cannot follow a maximum that rises.)
 // Maxima, sums and the exponents' arguments are FP32.
@@ -39,10 +41,10 @@ template <int HD> struct AqShape {
     static __device__ __forceinline__ int v_at(int row, int byte) { return row * HD + (HD % 128 == 0 ? byte ^ (((row >> 1) & 3) << 5) : byte); }
     static constexpr int STAGES = HD <= 128 ? 4 : 3, STAGE = 2 * 16 * HD;
     static constexpr int ctas(int mt) { return HD <= 128 && mt == 1 ? 3 : 2; }           // that an SM holds
-    // shared memory: the ring, in the end the warps' sums in its place, and the queries' digits
+    // shared memory: the ring, in the end the warps' sums in its place, and the queries
     static constexpr size_t RING = (size_t)AQ_WARPS * STAGES * STAGE;
     template <int MT> static constexpr size_t DIGITS = RING > (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4 ? RING : (size_t)AQ_WARPS * 8 * MT * (HD + 4) * 4;
-    template <int MT> static constexpr size_t SMEM = DIGITS<MT> + 4 * 8 * MT * (HD + 16);
+    template <int MT> static constexpr size_t SMEM = DIGITS<MT> + (MT == 1 ? 4 * 8 * (HD + 16) : 2 * 16 * (2 * HD + 16));
 };
 
 template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], const unsigned char * p) {
@@ -51,7 +53,7 @@ template <int W> __device__ __forceinline__ void aq_lds(uint32_t (&r)[W / 4], co
     else                       r[0] = *reinterpret_cast<const uint32_t *>(p);
 }
 
-// A query row in whole numbers of 31 bits and a sign, as four digits to the base 256 (-128 .. 127), four columns at a time.  (Three digits, 23 bits, are too few: a value is off by
+// A query row of 8 in whole numbers of 31 bits and a sign, as four digits to the base 256 (-128 .. 127), four columns at a time.  (Three digits, 23 bits, are too few: a value is off by
 // half of 1, whatever its size is, and queries with a channel tens of times larger than the others are usual.  With four, FP32 values within 2^-7 of the row's
 // largest and FP16 ones within 2^-20 are exact.)
 struct AqScaled { float up, down; };                                  // factor of the row; of its scores (not a number where a value of the row is not finite: so are they)
@@ -62,6 +64,11 @@ __device__ __forceinline__ void aq_max(const float4 & v, float & m, float & zero
 // the largest to 2^29 x 1.98 .. 2^30 x 1.98: four digits reach 2^30 x 1.992.  A value is off by half of 1, at most 2^-30.9 of the largest
 __device__ __forceinline__ AqScaled aq_scaled(float m) {
     const int e = min(max((int)((__float_as_uint(m) + 0x20000u) >> 23) - 127, -92), 128) - 30;
+    return {__uint_as_float((uint32_t)(127 - e) << 23), m < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : __int_as_float(0x7fc00000)};
+}
+// the largest to 2^10 .. 2^11: a value as two halves is off by 2^-22 of itself, or by 2^-25 (lower parts have no steps below 2^-24)
+__device__ __forceinline__ AqScaled aq_scaled_halves(float m) {
+    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;
     return {__uint_as_float((uint32_t)(127 - e) << 23), m < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : __int_as_float(0x7fc00000)};
 }
 __device__ __forceinline__ void aq_digits(const float4 & x, float up, uint32_t (&d)[4]) {
@@ -108,10 +115,10 @@ __device__ __forceinline__ float aq_load_query(const AttnQ8P & p, const SeqB & s
     }
     return f.down * p.scale_log2;
 }
-// The R rows of a tile as digits in shared memory, by the whole CTA: [digit][row][HD + 16], and the factors of their scores.  The loads come before what
+// The R rows of a tile in shared memory, by the whole CTA: 8 as digits [digit][row][HD + 16], 16 as halves [upper, lower][row][HD + 8], and the factors of their scores.  The loads come before what
 // else the CTA asks for: behind the ring's first codes they are waited for 3 us.
 template <int HD, int R> struct AqQueries {
-    static constexpr int TPR = AQ_THREADS / R, W = HD / 4, N = (W + TPR - 1) / TPR, PITCH = HD + 16;
+    static constexpr int TPR = AQ_THREADS / R, W = HD / 4, N = (W + TPR - 1) / TPR, PITCH = R == 8 ? HD + 16 : 2 * HD + 16;
     float4 x[N];
     __device__ __forceinline__ void load(const AttnQ8P & p, const SeqB & s, const TileB & t, int hk) {
         const int row = threadIdx.x / TPR, j = threadIdx.x % TPR;
@@ -122,7 +129,7 @@ template <int HD, int R> struct AqQueries {
             if (row < t.n_rows && j + u * TPR < W) x[u] = aq_query(p.xtype, p.q, at + (j + u * TPR) * 4);
         }
     }
-    __device__ __forceinline__ void put(const AttnQ8P & p, unsigned char * digits, float * factor) {
+    template <bool TWO_Q> __device__ __forceinline__ void put(const AttnQ8P & p, unsigned char * to, float * factor) {
         const int row = threadIdx.x / TPR, j = threadIdx.x % TPR;
         float m = 0.f, zero = 0.f;
 #pragma unroll
@@ -130,14 +137,23 @@ template <int HD, int R> struct AqQueries {
         if (zero != 0.f) m = INFINITY;
 #pragma unroll
         for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const AqScaled f = aq_scaled(m);
+        const AqScaled f = R == 8 ? aq_scaled(m) : TWO_Q ? aq_scaled_halves(m) : AqScaled{1.f, m < INFINITY ? 1.f : __int_as_float(0x7fc00000)};
         if (j == 0) factor[row] = f.down * p.scale_log2;
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            uint32_t d[4];
-            aq_digits(x[u], f.up, d);
+            const bool mine = j + u * TPR < W;
+            if constexpr (R == 8) {
+                uint32_t d[4];
+                aq_digits(x[u], f.up, d);
 #pragma unroll
-            for (int k = 0; k < 4; k++) if (j + u * TPR < W) *reinterpret_cast<uint32_t *>(digits + (k * R + row) * PITCH + (j + u * TPR) * 4) = d[k];
+                for (int k = 0; k < 4; k++) if (mine) *reinterpret_cast<uint32_t *>(to + (k * R + row) * PITCH + (j + u * TPR) * 4) = d[k];
+            } else {
+                uint2 hi, lo;
+                aq_split(x[u].x * f.up, x[u].y * f.up, hi.x, lo.x);
+                aq_split(x[u].z * f.up, x[u].w * f.up, hi.y, lo.y);
+                if (mine) *reinterpret_cast<uint2 *>(to + row * PITCH + (j + u * TPR) * 8) = hi;
+                if (TWO_Q && mine) *reinterpret_cast<uint2 *>(to + (R + row) * PITCH + (j + u * TPR) * 8) = lo;
+            }
         }
     }
 };
@@ -154,23 +170,16 @@ __device__ __forceinline__ float aq_score(int d3, int d2, int d1, int d0) {
     const float f3 = __int_as_float(d3) - 12582912.f, f2 = __int_as_float(d2) - 12582912.f, f1 = __int_as_float(d1) - 12582912.f, f0 = __int_as_float(d0) - 12582912.f;
     return fmaf(fmaf(fmaf(f3, 256.f, f2), 256.f, f1), 256.f, f0);
 }
-// products of 32 columns of 8 slots (b0, b1) and of the rows: x[digits 3 | 2], x[digits 1 | 0] for 8 rows, x[digit] for 16
-template <int HD, int MT, int NX>
-__device__ __forceinline__ void aq_products(int (&x)[NX][4], const uint32_t (&a)[MT][4][HD / 16], int s, uint32_t b0, uint32_t b1) {
-    if constexpr (MT == 1) {
+// products of 32 columns of 8 slots (b0, b1) and of 8 rows: x[digits 3 | 2], x[digits 1 | 0]
+template <int HD>
+__device__ __forceinline__ void aq_products(int (&x)[2][4], const uint32_t (&a)[4][HD / 16], int s, uint32_t b0, uint32_t b1) {
 #pragma unroll
-        for (int d = 0; d < 2; d++) mma16832(x[d], a[0][3 - 2 * d][2 * s], a[0][2 - 2 * d][2 * s], a[0][3 - 2 * d][2 * s + 1], a[0][2 - 2 * d][2 * s + 1], b0, b1, s == 0);
-    } else {
-#pragma unroll
-        for (int d = 0; d < 4; d++) mma16832(x[d], a[0][d][2 * s], a[1][d][2 * s], a[0][d][2 * s + 1], a[1][d][2 * s + 1], b0, b1, s == 0);
-    }
+    for (int d = 0; d < 2; d++) mma16832(x[d], a[3 - 2 * d][2 * s], a[2 - 2 * d][2 * s], a[3 - 2 * d][2 * s + 1], a[2 - 2 * d][2 * s + 1], b0, b1, s == 0);
 }
-template <int MT, int NX> __device__ __forceinline__ float aq_score_of(const int (&x)[NX][4], int mt, int j) {
-    if constexpr (MT == 1) return aq_score(x[0][j], x[0][2 + j], x[1][j], x[1][2 + j]);
-    else                   return aq_score(x[3][2 * mt + j], x[2][2 * mt + j], x[1][2 * mt + j], x[0][2 * mt + j]);
-}
+__device__ __forceinline__ float aq_score_of(const int (&x)[2][4], int j) { return aq_score(x[0][j], x[0][2 + j], x[1][j], x[1][2 + j]); }
 
-template <int HD, int MT>
+// TWO_Q: of 16 rows two halves for each query; 8 rows are digits
+template <int HD, int MT, bool TWO_Q>
 __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(const AttnQ8P p) {
     using S = AqShape<HD>;
     constexpr int R = 8 * MT, ST = S::STAGES;
@@ -215,11 +224,10 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
     for (int it = 0; it < ST - 1; it++) issue();
 
-    queries.put(p, digits, s_f);
+    queries.template put<TWO_Q>(p, digits, s_f);
     __syncthreads();
-    uint32_t a[MT][4][S::KS];
     float f[MT], m[MT], l[MT]; int sees[MT], least = 0x7fffffff; bool there[MT];
-    float * scores[MT];                                               // (where they are kept)
+    int scores[MT];                                                   // place of its scores (-1: not kept)
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
         const int row = mt * 8 + g, tok = p.by_group.of(t.first + row);
@@ -227,17 +235,30 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         f[mt] = s_f[row];
         sees[mt] = there[mt] ? aq_sees(s, p.c.n_ctx, tok) : 0;
         if (there[mt]) least = min(least, sees[mt]);
-        scores[mt] = p.scores && there[mt] ? p.scores + (size_t)((s.first + tok) * p.n_head + hk * p.group + t.first + row - tok * p.group) * p.score_pitch + 2 * q : nullptr;
+        scores[mt] = p.scores && there[mt] ? ((s.first + tok) * p.n_head + hk * p.group + t.first + row - tok * p.group) * p.score_pitch + 2 * q : -1;
         m[mt] = -INFINITY; l[mt] = 0.f;
+    }
+    uint32_t a[4][S::KS];                                             // 8 rows: [digit]; 16 rows: [2 row / 8 + pair of columns] upper and, with two halves, lower parts
+    uint32_t a_low[TWO_Q && MT == 2 ? 4 : 1][S::KS];
 #pragma unroll
-        for (int d = 0; d < 4; d++)
+    for (int c = 0; c < S::KG; c++) {
+        const int col = c * 4 * S::KW + q * S::KW;
 #pragma unroll
-            for (int c = 0; c < S::KG; c++) {
+        for (int k = 0; k < 4; k++) {
+            if constexpr (MT == 1) {
                 uint32_t w[S::KW / 4];
-                aq_lds<S::KW>(w, digits + (d * R + row) * (HD + 16) + c * 4 * S::KW + q * S::KW);
+                aq_lds<S::KW>(w, digits + (k * R + g) * (HD + 16) + col);
 #pragma unroll
-                for (int i = 0; i < S::KW / 4; i++) a[mt][d][c * (S::KW / 4) + i] = w[i];
+                for (int i = 0; i < S::KW / 4; i++) a[k][c * (S::KW / 4) + i] = w[i];
+            } else {
+                const unsigned char * from = digits + ((k >> 1) * 8 + g) * (2 * HD + 16) + col * 2 + (k & 1) * 4;
+#pragma unroll
+                for (int i = 0; i < S::KW / 4; i++) {
+                    a[k][c * (S::KW / 4) + i] = *reinterpret_cast<const uint32_t *>(from + i * 8);
+                    if constexpr (TWO_Q && HD != 128) a_low[k][c * (S::KW / 4) + i] = *reinterpret_cast<const uint32_t *>(from + R * (2 * HD + 16) + i * 8);
+                }
             }
+        }
     }
     least = __reduce_min_sync(0xffffffffu, least);
     float o[MT][S::NT][4];
@@ -247,9 +268,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         for (int n = 0; n < S::NT; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) o[mt][n][j] = 0.f;
-    float v_ref[MT], v_inv[MT];                                       // scale of a row's value sums, and AQ_P over it (of what the row sees: others' scales have no say in it)
+    uint32_t v_ref[MT];                                               // scale of a row's value sums, a power of two, as bits (of what the row sees: others' scales have no say in it)
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) { v_ref[mt] = AQ_V_LEAST; v_inv[mt] = AQ_P / AQ_V_LEAST; }
+    for (int mt = 0; mt < MT; mt++) v_ref[mt] = __float_as_uint(AQ_V_LEAST);
 
     const unsigned char * kt = ring + (ST - 1) * S::STAGE;
     for (int it = 0; it < steps; it++) {
@@ -262,33 +283,71 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         const float sk = __ldg(ks + (j0 >> p.c.shift)), sv = __ldg(vs + (j0 >> p.c.shift));
 
         // ---- scores of 16 slots
-        int x[2][2 * MT][4];
+        float raw[MT][2][2];
+        if constexpr (MT == 1) {
+            int x[2][2][4];
 #pragma unroll
-        for (int c = 0; c < S::KG; c++) {
-            uint32_t w[2][S::KW / 4];
+            for (int c = 0; c < S::KG; c++) {
+                uint32_t w[2][S::KW / 4];
 #pragma unroll
-            for (int n = 0; n < 2; n++) aq_lds<S::KW>(w[n], kt + S::k_at(n * 8 + g, c * 4 * S::KW + q * S::KW));
+                for (int n = 0; n < 2; n++) aq_lds<S::KW>(w[n], kt + S::k_at(n * 8 + g, c * 4 * S::KW + q * S::KW));
 #pragma unroll
-            for (int i = 0; i < S::KW / 8; i++)
+                for (int i = 0; i < S::KW / 8; i++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) aq_products<HD, MT>(x[n], a, c * (S::KW / 8) + i, w[n][2 * i], w[n][2 * i + 1]);
+                    for (int n = 0; n < 2; n++) aq_products<HD>(x[n], a, c * (S::KW / 8) + i, w[n][2 * i], w[n][2 * i + 1]);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) raw[0][n][j] = aq_score_of(x[n], j);
+        } else {
+            float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < S::KG; c++) {
+                uint32_t w[2][S::KW / 4];
+#pragma unroll
+                for (int n = 0; n < 2; n++) aq_lds<S::KW>(w[n], kt + S::k_at(n * 8 + g, c * 4 * S::KW + q * S::KW));
+                if constexpr (TWO_Q && HD == 128) {                   // (lower parts anew in every step: in registers they spill, 159 us for 149)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 * from = reinterpret_cast<const uint4 *>(digits + (R + h * 8 + g) * (2 * HD + 16) + (c * 4 * S::KW + q * S::KW) * 2);
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint4 v = from[u];
+                            a_low[2 * h][c * 4 + 2 * u] = v.x; a_low[2 * h + 1][c * 4 + 2 * u] = v.y; a_low[2 * h][c * 4 + 2 * u + 1] = v.z; a_low[2 * h + 1][c * 4 + 2 * u + 1] = v.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < S::KW / 4; i++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const uint32_t u = w[n][i] ^ 0x80808080u, b0 = q8_lo(u), b1 = q8_hi(u);
+                        const int k = c * (S::KW / 4) + i;
+                        if constexpr (TWO_Q) mma16816(x[n], a_low[0][k], a_low[2][k], a_low[1][k], a_low[3][k], b0, b1);
+                        mma16816(x[n], a[0][k], a[2][k], a[1][k], a[3][k], b0, b1);
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) raw[j >> 1][n][j & 1] = x[n][j];
         }
         // ---- probabilities, as A operands of the value products
         uint32_t pa[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            float down = 1.f;
-            if (sv >= v_ref[mt] && j0 < sees[mt]) {                   // to the power of two above it: one rise where the scales are of one size
-                const float now = __uint_as_float(min((__float_as_uint(sv) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
-                down = v_ref[mt] / now; v_ref[mt] = now; v_inv[mt] = AQ_P / now;
-            }
-            const float pv = sv * v_inv[mt];
+            // to the power of two above it: one rise where the scales are of one size.  (In bits: a division in a branch that some rows take cost 20 us of 141.)
+            const uint32_t now = j0 < sees[mt] && sv >= __uint_as_float(v_ref[mt]) ? min((__float_as_uint(sv) & 0x7f800000u) + 0x00800000u, 0x7f000000u) : v_ref[mt];
+            float down = __int_as_float(max(0x3f800000 - (int)(now - v_ref[mt]), 0));
+            v_ref[mt] = now;
+            const float pv = sv * __uint_as_float((262u << 23) - now);                   // (AQ_P = 2^8 over it)
             float y[2][2];
             const float fk = f[mt] * sk;
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) y[n][j] = aq_score_of<MT>(x[n], mt, j) * fk;
+                for (int j = 0; j < 2; j++) y[n][j] = raw[mt][n][j] * fk;
             const bool masked = j0 + 16 > least;
             if (masked) {
 #pragma unroll
@@ -296,8 +355,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
 #pragma unroll
                     for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j >= sees[mt]) y[n][j] = -INFINITY;
             }
-            if (scores[mt]) {
-                float * to = scores[mt] + j0;
+            if (scores[mt] >= 0) {
+                float * to = p.scores + scores[mt] + j0;
                 *reinterpret_cast<float2 *>(to) = make_float2(y[0][0], y[0][1]);
                 *reinterpret_cast<float2 *>(to + 8) = make_float2(y[1][0], y[1][1]);
             }
@@ -355,7 +414,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
         float sum = l[mt];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; s_back[warp][mt * 8 + g] = v_ref[mt] * (1.f / AQ_P); }
+        if (q == 0) { s_m[warp][mt * 8 + g] = m[mt]; s_l[warp][mt * 8 + g] = sum; s_back[warp][mt * 8 + g] = __uint_as_float(v_ref[mt]) * (1.f / AQ_P); }
         float * row = so + (size_t)(warp * R + mt * 8 + g) * PITCH;
 #pragma unroll
         for (int c = 0; c < S::VG; c++)
@@ -569,7 +628,7 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
         }
         later = __any_sync(0xffffffffu, later);
     }
-    uint32_t a[1][4][S::KS];
+    uint32_t a[4][S::KS];
     float f = 0.f, lse = 0.f;
     int a_row = -1, sees = 0;
     if (later) return;
@@ -583,7 +642,7 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
                 const int row = r0 + g, tok = p.by_group.of(row);
                 const bool there = row < n_rows;
                 lse = there ? __ldcg(p.lse + (size_t)(s.first + tok) * p.n_head + hk * p.group + row - tok * p.group) : 0.f;
-                f = aq_load_query<HD>(p, s, row, there, hk, q, a[0]);
+                f = aq_load_query<HD>(p, s, row, there, hk, q, a);
                 sees = there ? aq_sees(s, p.c.n_ctx, tok) : 0;
                 a_row = r0;
             }
@@ -591,9 +650,9 @@ __global__ void __launch_bounds__(AQ_THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 2) 
             for (int n = 0; n < NK; n++) {
                 int x[2][4];
 #pragma unroll
-                for (int k = 0; k < HD / 32; k++) aq_products<HD, 1>(x, a, k, w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4)], w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4) + 1]);
+                for (int k = 0; k < HD / 32; k++) aq_products<HD>(x, a, k, w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4)], w[n][2 * k / (S::KW / 4)][2 * k % (S::KW / 4) + 1]);
 #pragma unroll
-                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx(aq_score_of<1>(x, 0, j) * (f * sk[n >> 1]) - lse);
+                for (int j = 0; j < 2; j++) if (j0 + n * 8 + 2 * q + j < sees) sum[n][j] += exp2_approx(aq_score_of(x, j) * (f * sk[n >> 1]) - lse);
             }
         }
         const int at = j0;
@@ -664,17 +723,17 @@ size_t attn_q8_scratch(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv
     return r.words + r.lse + r.ml + r.part + r.scores;
 }
 
-template <int HD, int MT>
+template <int HD, int MT, bool TWO_Q>
 static int aq_go(const AttnQ8P & p, cudaStream_t st) {
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
     constexpr size_t smem = AqShape<HD>::template SMEM<MT>;
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        PI_CUDA(cudaFuncSetAttribute(k_attn_q8<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        PI_CUDA(cudaFuncSetAttribute(k_attn_q8<HD, MT, TWO_Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_attn_q8<HD, MT>, dim3(aq_grid(p)), dim3(AQ_THREADS), smem, st, true, p));
+    PI_CUDA(launch_k(k_attn_q8<HD, MT, TWO_Q>, dim3(aq_grid(p)), dim3(AQ_THREADS), smem, st, true, p));
     return PI_OK;
 }
 
@@ -682,8 +741,8 @@ template <int HD>
 static int aq_run(const AttnQ8P & p, const AqPlan & r, const float * w_in, float * w_out, int max_kv, cudaStream_t st) {
     int rc;
     if (r.tc)                     rc = launch_attn_q8_tc(p, st);
-    else if constexpr (HD <= 128) rc = r.R == 8 ? aq_go<HD, 1>(p, st) : aq_go<HD, 2>(p, st);
-    else                          rc = aq_go<HD, 1>(p, st);
+    else if constexpr (HD <= 128) rc = r.R == 8 ? aq_go<HD, 1, true>(p, st) : p.xtype == PI_TYPE_F16 ? aq_go<HD, 2, false>(p, st) : aq_go<HD, 2, true>(p, st);
+    else                          rc = aq_go<HD, 1, true>(p, st);
     if (rc) return rc;
     if (p.items > p.whole) {
         const int64_t rows = (int64_t)(p.items - p.whole) * r.R;

@@ -47,10 +47,13 @@ def test_prompt_rows_against_64_bits_beside_a_large_later_scale(ops):
 # ------------------------------------------------------------------------------------------------ queries with one large element
 
 def check_large(ops, p, q, start, pos, n_head, x, max_kv=None):
-    """A query is whole numbers of which the row's largest is 2^30 x 0.99 or more: a value is off by 2^-30.9 of it at most, products with codes and their sums are
-    exact.  Four sums become one number in FP32 steps (a sum is 2^22 at most: u of 2^30 each beside u of the score), then come two factors, the product and the
-    difference in the exponent: e_s = scale (2^-30.9 max |q| max_j sum_d |k_jd| + 2 u max |q| max_j s_j) + 10 u max_j |s_j|.  The rest as in
-    test_gpu_long_context.  Weights are sums of probabilities: 2 e_s + (4 n + 16) u of each, and u for each addition."""
+    """Up to 8 rows a KV head, and any number with head_dim above 128 or where the weights' kernel reads the keys again: a query is whole numbers of which the
+    row's largest is 2^30 x 0.99 or more.  A value is off by 2^-30.9 of it at most, products with codes and their sums are exact.  Four sums become one number in FP32
+    steps (a sum is 2^22 at most: u of 2^30 each beside u of the score), then come two factors, the product and the difference in the exponent:
+        e_s = scale (2^-30.9 max |q| max_j sum_d |k_jd| + 2 u max |q| max_j s_j) + 10 u max_j |s_j|.
+    9 to 63 rows: FP16 as they are; FP32 as two halves, off by 2^-22 of the value or 2^-35 of the row's largest; sums are cut, 2 hd u of their terms' sizes at most:
+        e_s = scale max_j sum_d |q_d k_jd| (2^-22 + (2 hd + 10) u) + scale 2^-35 max |q| max_j sum_d |k_jd|.
+    The rest as in test_gpu_long_context.  Weights are sums of probabilities: 2 e_s + (4 n + 16) u of each, and u for each addition."""
     T, hd, H, group = len(q), p.c.hd, p.c.H, n_head // p.c.H
     scale, u = hd ** -0.5, U["f32"]
     shape = (p.c.n_seq, H, p.c.n_ctx)
@@ -67,7 +70,11 @@ def check_large(ops, p, q, start, pos, n_head, x, max_kv=None):
             hs = slice(h * group, (h + 1) * group)
             big = np.abs(heads[first:first + n, hs]).max(-1)
             top = np.abs(np.einsum("tgd,jd->tgj", heads[first:first + n, hs], k)).max(-1)
-            e_s[first:first + n, hs] = scale * (big * (2.0 ** -30.9 * np.abs(k).sum(-1).max() + 2 * u * p.c.scale["k"][sq, h].max()) + 10 * u * top)
+            sums = np.abs(k).sum(-1).max()
+            terms = np.einsum("tgd,jd->tgj", np.abs(heads[first:first + n, hs]), np.abs(k)).max(-1)
+            whole = scale * (big * (2.0 ** -30.9 * sums + 2 * u * p.c.scale["k"][sq, h].max()) + 10 * u * top)
+            halves = scale * (terms * ((2.0 ** -22 if x == "f32" else 0.0) + (2 * hd + 10) * u) + 2.0 ** -35 * big * sums)
+            e_s[first:first + n, hs] = halves if 8 < T * group < 64 and hd <= 128 else whole
     rel = 2 * e_s + (4 * n_max + 16) * u
     tol = (size.reshape(T, n_head, hd) * rel[..., None] + 2.0 ** -32 * most[..., None]).reshape(T, -1) + 1e-30
     if x == "f16":
