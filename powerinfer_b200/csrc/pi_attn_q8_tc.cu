@@ -157,6 +157,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
 #pragma unroll
                 for (int j = 0; j < NQ / 8; j++) { const uint4 v = __ldg(from + j); u[4 * j] = v.x; u[4 * j + 1] = v.y; u[4 * j + 2] = v.z; u[4 * j + 3] = v.w; }
             }
+            // a value that is not finite: the row's scores are no numbers (an infinity alone may make them all the lowest value, as if the row saw nothing)
+            const __half2 none = __floats2half2_rn(0.f, 0.f);
+            __half2 zero[4] = {none, none, none, none};
+#pragma unroll
+            for (int j = 0; j < NQ / 2; j++) zero[j & 3] = __hfma2(*reinterpret_cast<const __half2 *>(&u[j]), none, zero[j & 3]);
+            if (!__hbeq2(__hadd2(__hadd2(zero[0], zero[1]), __hadd2(zero[2], zero[3])), none)) u[0] = 0x7fff7fffu;
             if (p.scale_log2 < 0.f) {                                 // (the factor of the scores is positive: maxima stay maxima)
 #pragma unroll
                 for (int j = 0; j < 16; j++) u[j] ^= 0x80008000u;

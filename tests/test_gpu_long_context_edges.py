@@ -111,3 +111,22 @@ def test_weights_of_queries_with_one_large_element(ops, hd):
     q = rng.standard_normal((T, n_head, hd)).astype(np.float32)
     q[..., 5] = np.sign(q[..., 5]) * 3000
     check_large(ops, p, q.reshape(T, -1), [0, T], [41], n_head, "f32", max_kv=400)
+
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("T", [1, 3, 140])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_infinite_queries_against_keys_of_one_sign(ops, x, hd, T, sign):
+    """Scores that are all minus infinity are no mask: their row has no numbers, as a row of plus infinities has."""
+    rng = np.random.default_rng(hd + T)
+    p = Pair(ops, 1, 2, 256, hd, 16, fill=rng)
+    p.c.codes["k"][..., 5] = rng.integers(1, 100, p.c.codes["k"].shape[:-1])
+    p.d.k.copy_(dev(p.c.codes["k"]))
+    q = rows(rng, T, 8 * hd, x)
+    clean = ops.attention_q8(p.d, dev(q), ints([0, T]), ints([40]))
+    q[T // 2, 3 * hd + 5] = sign * np.inf
+    got = ops.attention_q8(p.d, dev(q), ints([0, T]), ints([40]))
+    hurt = torch.zeros_like(got, dtype=torch.bool)
+    hurt[T // 2, 3 * hd:4 * hd] = True
+    assert torch.isnan(got[hurt]).all() and torch.equal(got[~hurt], clean[~hurt])
