@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
 
         if (r < t.n_rows) {
             const int row = t.first + r, of = p.by_group.of(row), tok = s.first + of, h = hk * p.group + row - of * p.group;
-            if (!ok) sum = __int_as_float(0x7fc00000);                // a wait ran out: no numbers instead of wrong ones
+            if (!ok || s_dead) sum = __int_as_float(0x7fc00000);      // a wait ran out, here or in a warp that came to s_pfull all the same: no numbers instead of wrong ones
             if (w.n_splits > 1) {
                 const size_t at = ((size_t)(w.item - p.whole) * p.n_splits + split) * AT_ROWS + r;
 #pragma unroll

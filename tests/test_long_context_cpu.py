@@ -187,3 +187,13 @@ def test_the_prompt_kernel_gives_tensor_memory_back_when_no_product_is_in_flight
     assert "ring_land(s_rfull, i, AT_RAW)" in text
     loop = text[text.index("for (int i = b; i < n_tiles; i += 2)"):text.index("// ================================================================= tiles in, sums out")]
     assert "bar.sync" in loop and not re.search(r"\b(break|return);", re.sub(r"if \([^)]*parts\) break;", "", loop))
+
+
+def test_the_prompt_kernel_writes_no_numbers_after_any_wait_ran_out():
+    """(A wait cannot be made to run out on the device without a broken kernel.)  The warps that make probabilities go on behind a wait that ran out and arrive at the
+    barrier that the draining warps wait for, so these look at the flag that the others have set before."""
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "pi_attn_q8_tc.cu")).read()
+    give_up = text[text.index("auto wait = [&]"):text.index("// ---- codes: keys and values in turn")]
+    assert give_up.index("s_dead = 1") < give_up.index("return ok;")
+    out = text[text.index("for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);"):]
+    assert "s_dead) sum = __int_as_float(0x7fc00000);" in out[:out.index("p.part")]
