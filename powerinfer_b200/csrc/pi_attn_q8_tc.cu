@@ -89,7 +89,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     const int split = w.split, hk = w.hk, rt = p.row_tiles - 1 - w.rt;      // (the longest rows first)
     pdl_launch();
     pdl_wait();
-    if (blockIdx.x == 0 && tid == 0) *p.status = 0u;
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, w.entry);
     const TileB t = aq_tile(p, s, rt, AT_ROWS);
     if (t.n_rows <= 0) return;
@@ -464,6 +463,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1) k_attn_q8_tc(const AttnQ8P p) {
     if (warp == 0) tc_dealloc(s_tmem, 512);
 }
 
+// Clears the status word in front of the kernel: no CTA of its own can, as another one's wait may have run out by then.  (A copy of zeros instead took 4.5 us a call.)
+__global__ void k_attn_q8_clear(unsigned int * status) {
+    pdl_launch();
+    pdl_wait();
+    if (threadIdx.x == 0) *status = 0u;
+}
+
 bool attn_q8_tc_takes(int hd, int64_t rows) { return (hd == 64 || hd == 128) && rows >= 64; }
 
 template <int HD, bool TWO_Q>
@@ -476,6 +482,7 @@ static int at_go(const AttnQ8P & p, cudaStream_t st) {
         PI_CUDA(cudaFuncSetAttribute(k_attn_q8_tc<HD, TWO_Q>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
+    PI_CUDA(launch_k(k_attn_q8_clear, dim3(1), dim3(32), 0, st, true, p.status));
     PI_CUDA(launch_k(k_attn_q8_tc<HD, TWO_Q>, dim3(aq_grid(p)), dim3(AT_THREADS), smem, st, true, p));
     return PI_OK;
 }

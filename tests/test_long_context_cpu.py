@@ -197,3 +197,10 @@ def test_the_prompt_kernel_writes_no_numbers_after_any_wait_ran_out():
     assert give_up.index("s_dead = 1") < give_up.index("return ok;")
     out = text[text.index("for (int i = max(0, n_tiles - 2); i < n_tiles && ok; i++) drain(i);"):]
     assert "s_dead) sum = __int_as_float(0x7fc00000);" in out[:out.index("p.part")]
+
+
+def test_the_status_word_of_a_prompt_is_cleared_before_its_launch():
+    """No CTA clears what another one may have set by then."""
+    text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "pi_attn_q8_tc.cu")).read()
+    assert not re.search(r"\*p\.status\s*=", text)
+    assert text.index("launch_k(k_attn_q8_clear") < text.index("launch_k(k_attn_q8_tc")
