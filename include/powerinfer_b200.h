@@ -225,8 +225,8 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
  * fixed.  Other elements are left as they were.  Of entries that name one sequence the last one with tokens counts.
  * workspace: pi_attention_q8_workspace_bytes with the same arguments (`weights`: whether weights_out is given), 256-byte aligned; 0 bytes may be NULL.
  * It serves one call at a time: calls of one stream, or captured graphs that are not replayed at once.
- * From 64 query rows a KV head on (head_dim 64 and 128), pi_op_status(workspace) tells whether all bounded waits inside the kernel completed; the rows of one that
- * did not are NaN. */
+ * pi_op_status(workspace) tells whether all bounded waits inside the kernels completed (there are some from 64 query rows a KV head on, head_dim 64 and 128); the
+ * rows of one that did not are NaN.  Where 0 bytes are needed, 256 take the status word, if they are given. */
 size_t pi_attention_q8_workspace_bytes(const pi_kv_q8 * cache, const pi_kv_batch * batch, int n_head, int max_kv, int weights);
 int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, const void * q, int64_t q_stride, int n_head, int max_kv, float scale,
                     void * out, int64_t out_stride, const float * weights_in, float * weights_out,

@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD>::ctas(MT)) k_attn_q8(c
     const int split = wk.split, rt = wk.rt, hk = wk.hk;
     pdl_launch();
     pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.status) *p.status = 0u;          // (no wait of this kernel runs out)
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
     const TileB t = aq_tile(p, s, rt, R);
     if (t.n_rows <= 0) return;
@@ -706,7 +707,6 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     r.items = (int)items;
     r.whole = (int)(r.n_splits == 1 ? items : items - rest);
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
-    r.words = r.tc ? 256 : 0;                                         // (the status word where pi_op_status looks for it)
     r.lse = weights ? up((size_t)b.T * n_head * 4) : 0;
     r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
     r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
@@ -715,6 +715,7 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     const bool kept = weights && !r.tc && bytes <= AQ_SCORES;
     r.pitch = kept ? c.n_ctx : 0;
     r.scores = kept ? up((size_t)bytes) : 0;
+    r.words = r.tc || r.lse + r.ml + r.part + r.scores ? 256 : 0;     // (the status word where pi_op_status looks for it)
     return r;
 }
 
@@ -767,7 +768,7 @@ int launch_attention_q8(const AttnQ8Args & a, cudaStream_t st) {
     p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles; p.items = r.items; p.whole = r.whole;
     p.by_group = AqDiv::by(p.group); p.by_heads = AqDiv::by(a.c.H); p.by_tiles = AqDiv::by(r.row_tiles); p.by_splits = AqDiv::by(r.n_splits);
     char * s = (char *)a.scratch;
-    p.status = (unsigned int *)(s + 8);
+    p.status = s ? (unsigned int *)(s + 8) : nullptr;
     s += r.words;
     p.lse = a.w_out ? (float *)s : nullptr;
     p.part_ml = (float2 *)(s + r.lse); p.part = (float *)(s + r.lse + r.ml);

@@ -25,7 +25,7 @@ struct AttnQ8P {
     AqDiv by_group, by_heads, by_tiles, by_splits;                    // the KV heads' number, row_tiles, n_splits
     float * part; float2 * part_ml; float * lse;                      // [split item][split][R][hd], (max, sum) beside them; log2 of the rows' normalisers [T][n_head]
     float * scores; int score_pitch;                                  // (null: not kept) the rows' scores in bits, [T * n_head][pitch]
-    unsigned int * status;                                            // tcgen05 alone: bit 4, a wait ran out
+    unsigned int * status;                                            // (null: no workspace) tcgen05 alone: bit 4, a wait ran out; others clear it
 };
 
 struct AqItem { int item, entry, hk, rt, split, n_splits; };

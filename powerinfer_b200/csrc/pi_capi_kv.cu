@@ -170,7 +170,7 @@ int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype
     a.scale = scale; a.out = out; a.out_stride = out_stride; a.w_in = weights_in; a.w_out = weights_out;
     const size_t need = attn_q8_scratch(c, b, n_head, max_kv, weights_out != nullptr);
     if (need && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) { set_error("attention_q8: workspace too small or misaligned"); return PI_ERR_WORKSPACE; }
-    a.scratch = (float *)workspace;
+    a.scratch = need || (workspace && aligned(workspace, 256) && workspace_bytes >= 256) ? (float *)workspace : nullptr;       // (for the status word, where nothing else is needed)
     return launch_attention_q8(a, (cudaStream_t)stream);
 }
 

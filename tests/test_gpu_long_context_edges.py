@@ -1,5 +1,7 @@
 """Calls of the long-context operators that their documentation allows and where they went wrong once, against long_context_oracle or against a call that has to give
 the same bits.  Half a step is u = 2^-24 in FP32, 2^-11 in FP16."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -130,3 +132,26 @@ def test_infinite_queries_against_keys_of_one_sign(ops, x, hd, T, sign):
     hurt = torch.zeros_like(got, dtype=torch.bool)
     hurt[T // 2, 3 * hd:4 * hd] = True
     assert torch.isnan(got[hurt]).all() and torch.equal(got[~hurt], clean[~hurt])
+
+
+# ------------------------------------------------------------------------------------------------ status of a call
+
+@pytest.mark.parametrize("hd,T,n_head,n_ctx,weights", [(128, 1, 16, 16384, False), (128, 1, 16, 256, True), (96, 100, 8, 512, True), (192, 3, 4, 16384, False), (64, 1, 4, 64, False),
+                                                       (128, 100, 8, 1024, False)])
+def test_status_after_any_call(ops, hd, T, n_head, n_ctx, weights):
+    """pi_op_status of a workspace that held anything before: the call's, whichever kernels it took and whether it needed the workspace."""
+    from powerinfer_b200 import _lib
+    rng = np.random.default_rng(5)
+    p = Pair(ops, 1, 2, n_ctx, hd, 64, fill=rng)
+    start, at = ints([0, T]), ints([n_ctx - T - 3])
+    q = dev(rows(rng, T, n_head * hd))
+    out, w = torch.empty_like(q), torch.zeros(1, 2, n_ctx, device="cuda")
+    b = _lib.KvBatch(start.data_ptr(), None, at.data_ptr(), 1, T, T)
+    need = _lib.lib.pi_attention_q8_workspace_bytes(p.d.c, C.byref(b), n_head, n_ctx, int(weights))
+    ws = torch.full((max(need, 256),), -1, dtype=torch.int8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(2):
+        assert _lib.lib.pi_attention_q8(p.d.c, C.byref(b), _lib.PI_TYPE_F32, q.data_ptr(), n_head * hd, n_head, n_ctx, hd ** -0.5, out.data_ptr(), n_head * hd, None,
+                                        w.data_ptr() if weights else None, ws.data_ptr(), ws.numel(), stream) == 0
+        assert _lib.lib.pi_op_status(ws.data_ptr(), stream) == 0
+    assert torch.equal(out, ops.attention_q8(p.d, q, start, at, weights_out=torch.zeros_like(w) if weights else None))
