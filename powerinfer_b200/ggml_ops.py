@@ -73,6 +73,7 @@ class Workspace:
         self.buf = None
         self.at = self.size = 0
         self.need: dict = {}                 # (ncols, nrows, T) -> bytes
+        self.asked = None                    # where the last operator's status word is: (address, the tensor that holds it); None: it has none
 
     def get(self, ncols: int, nrows: int, T: int):
         need = self.need.get((ncols, nrows, T))
@@ -84,6 +85,7 @@ class Workspace:
             self.buf = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
             off = (-self.buf.data_ptr()) % 256
             self.at, self.size = self.buf.data_ptr() + off, self.buf.numel() - off
+        self.asked = self.at, self.buf
         return self.at, self.size
 
 
@@ -92,9 +94,9 @@ _ws = Workspace()
 
 def last_op_status() -> int:
     """Status of the last operator issued through this module (pi_op_status): 0, or 5 (a bounded device-side wait ran out)."""
-    if _ws.buf is None:
+    if _ws.asked is None:
         return 0
-    return int(lib.pi_op_status(_ws.at, _stream()))
+    return int(lib.pi_op_status(_ws.asked[0], _stream()))
 
 
 def upload_weight(host: np.ndarray, wtype: int, nrows: int, ncols: int) -> Weight:
@@ -445,9 +447,13 @@ def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0:
     _here(cache.k, q, out, q_start, pos0, seq, weights_in, weights_out)
     b, most = _batch(q_start, pos0, seq, T, max_new), cache.n_ctx if max_kv is None else max_kv
     need = lib.pi_attention_q8_workspace_bytes(cache.c, b, n // hd, most, 0 if w_out is None else 1)
-    ws = cache.k.new_empty(need) if need else None
-    check(lib.pi_attention_q8(cache.c, b, xtype, q_at, q_step, n // hd, most, hd ** -0.5 if scale is None else scale, out.data_ptr(), n, w_in, w_out,
-                              None if ws is None else ws.data_ptr(), need, _stream()))
+    _ws.asked = ws_at = None                                          # (the former call's scratch goes back first)
+    if need:
+        ws = cache.k.new_empty(need)
+        ws_at = ws.data_ptr()
+        if (hd == 64 or hd == 128) and min(T, T if max_new is None else max_new) * (n // hd // cache.n_head_kv) >= 64:
+            _ws.asked = ws_at, ws                                     # (the calls with bounded waits; kept until the next operator, for last_op_status)
+    check(lib.pi_attention_q8(cache.c, b, xtype, q_at, q_step, n // hd, most, hd ** -0.5 if scale is None else scale, out.data_ptr(), n, w_in, w_out, ws_at, need, _stream()))
     return out
 
 

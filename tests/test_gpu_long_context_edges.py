@@ -155,3 +155,23 @@ def test_status_after_any_call(ops, hd, T, n_head, n_ctx, weights):
                                         w.data_ptr() if weights else None, ws.data_ptr(), ws.numel(), stream) == 0
         assert _lib.lib.pi_op_status(ws.data_ptr(), stream) == 0
     assert torch.equal(out, ops.attention_q8(p.d, q, start, at, weights_out=torch.zeros_like(w) if weights else None))
+
+
+def test_last_op_status_is_that_of_the_attention(ops):
+    """The status word that last_op_status reads is the last operator's: of a prompt's attention, then of another operator."""
+    rng = np.random.default_rng(6)
+    p = Pair(ops, 1, 2, 1024, 128, 64, fill=rng)
+    x = torch.randn(2, 256, device="cuda")
+    w = ops.upload_weight(rng.standard_normal((64, 256)).astype(np.float16), ops.PI_TYPE_F16, 64, 256)
+    ops.ggml_mul_mat(w, x)
+    assert ops.last_op_status() == 0
+    q = dev(rows(rng, 100, 8 * 128))
+    ops.attention_q8(p.d, q, ints([0, 100]), ints([900]))
+    assert ops.last_op_status() == 0
+    ops._ws.asked[1][8:12] = torch.tensor([16, 0, 0, 0], dtype=torch.int8, device="cuda")     # as if a wait had run out
+    assert ops.last_op_status() == 5
+    ops.attention_q8(p.d, q[:1], ints([0, 1]), ints([30]), max_kv=64)
+    assert ops.last_op_status() == 0
+    ops.attention_q8(p.d, q, ints([0, 100]), ints([900]))
+    ops.ggml_mul_mat(w, x)
+    assert ops.last_op_status() == 0
