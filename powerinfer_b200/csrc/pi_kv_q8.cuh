@@ -48,11 +48,10 @@ struct SeqB { int first, n_new, pos, sq; };                           // first r
 __device__ __forceinline__ SeqB seq_entry(const RaggedB & b, int n_seq, int n_ctx, int i) {
     SeqB s;
     s.first = b.q_start[i];
-    s.n_new = min(b.q_start[i + 1] - s.first, b.max_new);
+    const int end = b.q_start[i + 1];
     s.pos = b.pos0[i];
     s.sq = b.seq ? b.seq[i] : i;
-    if (s.first < 0 || s.first > b.T) s.n_new = 0;
-    s.n_new = max(0, min(s.n_new, b.T - s.first));
+    s.n_new = s.first < 0 || s.first > b.T || end <= s.first ? 0 : min(min(end, b.T) - s.first, b.max_new);      // (no difference that 32 bits do not hold)
     if (s.sq < 0 || s.sq >= n_seq || s.pos < 0 || s.pos >= n_ctx) s.sq = -1;
     return s;
 }

@@ -175,3 +175,16 @@ def test_last_op_status_is_that_of_the_attention(ops):
     ops.attention_q8(p.d, q, ints([0, 100]), ints([900]))
     ops.ggml_mul_mat(w, x)
     assert ops.last_op_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ batches
+
+def test_ends_far_below_zero_are_no_tokens(ops):
+    """An end so far below its start that the difference does not fit 32 bits."""
+    rng = np.random.default_rng(7)
+    p = Pair(ops, 2, 2, 128, 64, 16, fill=rng)
+    k = rows(rng, 8, 128)
+    for end in (-2 ** 31, -2 ** 31 + 4, -1):
+        p.store(k, k, [5, end], [0])
+        p.same()
+        run_attention(ops, p, rng, [5, end], [20], 4, T=8)
