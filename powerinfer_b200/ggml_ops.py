@@ -385,6 +385,8 @@ class KvCacheQ8:
 
     @classmethod
     def empty(cls, n_seq: int, n_ctx: int, n_head_kv: int, head_dim: int, block: int = 64) -> "KvCacheQ8":
+        if block <= 0 or n_ctx <= 0 or n_ctx % block:
+            raise ValueError(f"n_ctx={n_ctx} must be a multiple of block={block}")
         codes = [torch.zeros(n_seq, n_head_kv, n_ctx, head_dim, dtype=torch.int8, device="cuda") for _ in range(2)]
         return cls(*codes, *(torch.zeros(n_seq, n_head_kv, n_ctx // block, device="cuda") for _ in range(2)))
 

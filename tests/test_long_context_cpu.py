@@ -204,3 +204,11 @@ def test_the_status_word_of_a_prompt_is_cleared_before_its_launch():
     text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "pi_attn_q8_tc.cu")).read()
     assert not re.search(r"\*p\.status\s*=", text)
     assert text.index("launch_k(k_attn_q8_clear") < text.index("launch_k(k_attn_q8_tc")
+
+
+@pytest.mark.parametrize("n_ctx,block", [(128, 96), (96, 64), (160, 64), (100, 64), (0, 64), (128, 0), (128, -64)])
+def test_an_empty_cache_has_the_block_that_was_asked_for(n_ctx, block):
+    """(128 slots in blocks of 96 made a cache with one block of 128.)"""
+    ggml_ops = pytest.importorskip("powerinfer_b200.ggml_ops")
+    with pytest.raises(ValueError, match="multiple of block"):
+        ggml_ops.KvCacheQ8.empty(1, n_ctx, 1, 64, block)
