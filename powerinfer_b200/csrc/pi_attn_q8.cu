@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(128) k_attn_q8_weights_kept(const AttnQ8P p, c
     const float4 had = before ? make_float4(w_in[at], w_in[at + 1], w_in[at + 2], w_in[at + 3]) : sum;
     const int rows = s.n_new * p.group;
 #pragma unroll 8
-    for (int r = 0; r < rows; r++) {
+    for (int r = max(0, j0 - s.pos) * p.group; r < rows; r++) {      // (from the first token that sees one of these slots)
         const int tok = p.by_group.of(r), row = (s.first + tok) * p.n_head + hk * p.group + r - tok * p.group;
         const float lse = __ldcg(p.lse + row);
         const int sees = aq_sees(s, p.c.n_ctx, tok) - j0;             // (scores of what a row does not see were not all made)
@@ -685,6 +685,11 @@ struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole, pitch;
 static constexpr int AQ_LEAST = 256, AQ_TURN = 4, AQ_TURN_TC = 10, AQ_ROUNDS = 4;        // (more rounds than that: room for the parts, and nothing gained)
 // Weights: scores of few rows are kept, if they take no more than this (8 sequences of 64 heads and 8000 slots, 16 MB: 28 us for reading the keys again, 6 so)
 static constexpr int64_t AQ_SCORES = int64_t(256) << 20;
+// ... and if there are no more than AQ_KEEP_ROWS, or their keys in all sequences are AQ_KEEP_WORK bytes: one thread adds a slot's rows one after the other, 0.4 to 0.8 us a row
+// however few slots there are, where reading the keys again takes 0.04 us a row and million of bytes (one sequence of 4096 slots and 1 KV head of 96, 1680 rows: 600 us
+// kept, 252 read again, 16 rows: the same; 8 sequences of 8000 slots and 8 heads of 96, 64 rows: 53 us and 125)
+static constexpr int AQ_KEEP_ROWS = 16;
+static constexpr int64_t AQ_KEEP_WORK = int64_t(16) << 20;
 static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv, bool weights) {
     AqPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
@@ -712,7 +717,7 @@ static AqPlan aq_plan(const KvQ8 & c, const RaggedB & b, int n_head, int max_kv,
     r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
     // (a sequence may see more slots than expected: their scores need room too)
     const int64_t bytes = (int64_t)b.T * n_head * c.n_ctx * 4;
-    const bool kept = weights && !r.tc && bytes <= AQ_SCORES;
+    const bool kept = weights && !r.tc && bytes <= AQ_SCORES && (rows <= AQ_KEEP_ROWS || (int64_t)b.n * c.H * keys * c.hd >= AQ_KEEP_WORK);
     r.pitch = kept ? c.n_ctx : 0;
     r.scores = kept ? up((size_t)bytes) : 0;
     r.words = r.tc || r.lse + r.ml + r.part + r.scores ? 256 : 0;     // (the status word where pi_op_status looks for it)

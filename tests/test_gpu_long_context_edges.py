@@ -188,3 +188,15 @@ def test_ends_far_below_zero_are_no_tokens(ops):
         p.store(k, k, [5, end], [0])
         p.same()
         run_attention(ops, p, rng, [5, end], [20], 4, T=8)
+
+
+# ------------------------------------------------------------------------------------------------ sizes that the other tests do not reach
+
+@pytest.mark.parametrize("max_kv", [1024, 1000, 300])
+def test_weights_of_chunks_of_wide_heads(ops, max_kv):
+    """64 rows a KV head of 256 dimensions: scores kept (keys of 16 MB and more are expected), and keys read a second time."""
+    rng = np.random.default_rng(21)
+    p = Pair(ops, 8, 8, 1024, 256, 64, fill=rng)
+    lens = [8, 3, 8, 1, 8, 8, 0, 5]
+    start = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    run_attention(ops, p, rng, start, [1016, 0, 500, 1023, 1020, 7, 5, 300], 64, seq=[3, 1, 0, 7, 2, 6, 5, 4], max_new=8, max_kv=max_kv, weights=True)
