@@ -5,7 +5,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from test_gpu_long_context import NP, Pair, U, dev, ints, ops, rows, run_attention  # noqa: F401
+from test_gpu_long_context import NP, Pair, U, dev, ints, ops, rows, run_attention, run_evict  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -191,6 +191,36 @@ def test_ends_far_below_zero_are_no_tokens(ops):
 
 
 # ------------------------------------------------------------------------------------------------ sizes that the other tests do not reach
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_with_more_places_than_the_list_holds(ops, in_place):
+    """A budget above 16384 slots: the holes are listed in several turns."""
+    rng = np.random.default_rng(15)
+    p = Pair(ops, 1, 2, 53248, 64, 128, fill=rng)
+    w = np.exp(rng.standard_normal((1, 2, 53248)) * 2).astype(np.float32)
+    w[0, 1, :40960] = 0                                                # every place but the first ones and the last ones is a hole
+    run_evict(ops, p, w, [53240], 40960, 4, 100, in_place=in_place)
+
+
+@pytest.mark.parametrize("hd,x", [(64, "f16"), (128, "f32")])
+def test_prompt_over_many_parts(ops, hd, x):
+    """Few tiles of 128 rows over a long range: more than 8 parts of each are joined."""
+    rng = np.random.default_rng(hd)
+    p = Pair(ops, 1, 1, 16384, hd, 64, fill=rng)
+    run_attention(ops, p, rng, [0, 20], [15990], 8, x)
+
+
+def test_codes_of_minus_128(ops):
+    """The store makes codes of +-127, a caller's own cache may hold -128."""
+    rng = np.random.default_rng(18)
+    for T, hd in ((1, 128), (3, 96), (140, 64), (140, 128)):
+        p = Pair(ops, 1, 2, 256, hd, 16, fill=rng)
+        for n, codes in (("k", p.d.k), ("v", p.d.v)):
+            p.c.codes[n][rng.random(p.c.codes[n].shape) < 0.3] = -128
+            codes.copy_(dev(p.c.codes[n]))
+        run_attention(ops, p, rng, [0, T], [100], 8, weights=True)
+    run_evict(ops, p, rng.random((1, 2, 256), dtype=np.float32), [256], 64, 2, 9)
+
 
 @pytest.mark.parametrize("max_kv", [1024, 1000, 300])
 def test_weights_of_chunks_of_wide_heads(ops, max_kv):
