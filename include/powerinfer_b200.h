@@ -238,7 +238,9 @@ int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype
  * the largest).  Kept slots below `keep` stay; the others, ascending, take the places of the evicted ones below `keep`, ascending.  A block that takes rows in
  * gets the largest scale of its rows, codes of other scales rne(code * (scale / that)).  kept int32 [n, n_head_kv, keep]: the slot that each slot's
  * row came from, -1 behind the end.  weights_out (NULL: none; may be `weights`): the weights in the new order.  The sequence then has
- * min(len, keep) slots.  With len - keep >= n_recent the last n_recent slots are the newest tokens, also after earlier evictions.
+ * min(len, keep) slots.  n_recent names slots, not tokens: evictions of at least n_recent slots each (len - keep >= n_recent) keep the n_recent newest tokens.  One of fewer
+ * slots leaves kept tokens of the last n_recent below `keep`, in places where the next call does not know them as recent: a sequence that is cut at
+ * every token has no recent window.
  * Of entries that name one sequence the last one counts, the others' kept are -1.  n_ctx up to 262144. */
 int pi_kv_evict_q8(const pi_kv_q8 * cache, const int32_t * len, const int32_t * seq, int n, int keep, int n_sink, int n_recent,
                    const float * weights, float * weights_out, int32_t * kept, void * stream);

@@ -463,7 +463,9 @@ def kv_evict_q8(cache: KvCacheQ8, weights: torch.Tensor, lens: torch.Tensor, kee
                 weights_out: torch.Tensor | None = None) -> torch.Tensor:
     """Sequences of lens[i] slots cut to `keep` by their accumulated weights (float32 [n_seq, n_head_kv, n_ctx], as attention_q8 leaves them): the first
     n_sink slots, the last n_recent and the heaviest others stay, for every KV head its own.  Returns the slot that each kept row came from,
-    int32 [n, n_head_kv, keep] (-1: none); weights_out (may be `weights`) takes the weights in the new order."""
+    int32 [n, n_head_kv, keep] (-1: none); weights_out (may be `weights`) takes the weights in the new order.
+    Kept slots behind `keep` move into the places of evicted ones below it.  So the last n_recent slots are the newest tokens only if every eviction takes n_recent
+    slots or more (lens[i] - keep >= n_recent): let a sequence grow to keep + n_recent before it is cut.  Cut at every token, it has no recent window."""
     n = lens.numel()
     w, w_out = _slot_weights(weights, cache), _slot_weights(weights_out, cache)
     _here(cache.k, weights, weights_out, lens, seq)

@@ -230,3 +230,23 @@ def test_weights_of_chunks_of_wide_heads(ops, max_kv):
     lens = [8, 3, 8, 1, 8, 8, 0, 5]
     start = np.concatenate([[0], np.cumsum(lens)]).tolist()
     run_attention(ops, p, rng, start, [1016, 0, 500, 1023, 1020, 7, 5, 300], 64, seq=[3, 1, 0, 7, 2, 6, 5, 4], max_new=8, max_kv=max_kv, weights=True)
+
+
+# ------------------------------------------------------------------------------------------------ recent tokens
+
+def test_recent_tokens_stay_where_as_many_slots_go_at_a_time(ops):
+    """Evictions of n_recent slots and more keep the n_recent newest tokens, whatever their weights are; what moved has left the end."""
+    rng = np.random.default_rng(19)
+    keep, recent, n_ctx = 64, 24, 128
+    cache = ops.KvCacheQ8.empty(1, n_ctx, 2, 64, 16)
+    token = [np.arange(keep) for _ in range(2)]                        # which token a slot holds, for each head
+    n = keep
+    for more in (24, 40, 24, 64, 30):
+        token = [np.concatenate([t, np.arange(n, n + more)]) for t in token]
+        n += more
+        w = rng.random((1, 2, n_ctx), dtype=np.float32)
+        w[:, :, -(n_ctx - keep):] = 0                                  # the new tokens have collected nothing yet
+        kept = ops.kv_evict_q8(cache, dev(w), ints([keep + more]), keep, 2, recent).cpu().numpy()
+        token = [t[kept[0, h]] for h, t in enumerate(token)]
+        for t in token:
+            assert set(range(n - recent, n)) <= set(t.tolist())
