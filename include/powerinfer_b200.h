@@ -218,8 +218,10 @@ int pi_kv_load_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype, 
 
 /* llm_build_kqv (llama.cpp:4764-4850) over the 8-bit cache, the new tokens' keys and values in it already: token t of entry i sees slots
  * 0 .. pos0[i] + t; out = softmax(scale * q . k) v for every query head, heads h of group h / (n_head / n_head_kv).  q, out [T, n_head * head_dim]
- * (F32 or F16); products are made with 22 bits of queries and probabilities and summed in FP32, whatever the type.  max_kv: the slots that the longest
- * sequence is expected to see (it sets how the work is cut; more slots are read too, more slowly).  A token that sees nothing has zeros.
+ * (F32 or F16).  Queries: F16 as they are and F32 to 22 bits; to 2^-31 of its row's largest value where a KV head has up to 8 query rows in all (max_new * n_head / n_head_kv) or
+ * head_dim is 192 or 256, and for weights_out where keys are read again.  A probability over the row's largest one, times the scale of its value, has 22 bits down to 2^-10 of the
+ * largest scale of values that the row has met, and an error of 2^-32 of that scale below.  Sums are FP32.  max_kv: the slots that the longest sequence is expected to see (it sets how the work is cut;
+ * more slots are read too, more slowly).  A token that sees nothing has zeros; what it does not see has no part in its row, whatever is there.
  * weights_out F32 [n_seq, n_head_kv, n_ctx] (NULL: none): for every slot that an entry's tokens see the sum of its probabilities over
  * those tokens and the heads of the group, plus weights_in (same shape, may be the same array; NULL: 0) for slots before pos0; the sums' order is
  * fixed.  Other elements are left as they were.  Of entries that name one sequence the last one with tokens counts.

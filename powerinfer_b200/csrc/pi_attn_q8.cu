@@ -7,7 +7,7 @@
 // between warps), keep a maximum, a sum and all sums of values of their own, and join them at the end.  Long ranges are
 // split over CTAs, whose sums k_attn_q8_join joins.
 //
-// Measured (FP16 or FP32 rows, head_dim 128): 32 sequences of 1056 to 2048 slots, 32 heads 80 us (5.1 TB/s; between two lengths 6.7, the copy rate: the rest is what
+// Measured (FP16 or FP32 rows, head_dim 128): 32 sequences of 1056 to 2048 slots, 32 heads 79 us (5.2 TB/s; between two lengths 6.7, the copy rate: the rest is what
 // CTAs do before their first slot and behind their last, the tail and the launches), one of 32768 slots, 64 heads over 8 KV heads 17 us and 5 of the join.
 // Queries are asked for before the ring's codes: behind them they took 3 us of a CTA's 15.
 //
@@ -15,13 +15,14 @@
 // of the tensor cores' tile; their sums are exact.  16 rows have queries as halves, FP16 as they are and FP32 as the sum of two (22 bits), and the codes become halves
 // for them: digits are four products for all of the rows, 160 us where two halves take 149 and one 132 (8 sequences of 7 tokens, 8000 slots, 64 heads over 8).
 // A probability, times vs over the largest vs so far (at most 1), is the sum of
-// two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits, and a value's code is exact as a half: out = sums * that scale.  (Probabilities as
+// two halves, rows 0 .. 7 the upper and rows 8 .. 15 the lower parts, 22 bits down to 2^-10 of the largest vs (held times 2^8 over the power of two
+// above it, steps of 2^-24: an error of 2^-32 of that vs below), and a value's code is exact as a half: out = sums * that scale.  The scale is a row's own, of what it sees.  (Probabilities as
 // digits would spare the values' conversions, but their sums fill twice the registers, and whole numbers cannot follow a maximum that rises.)
 // Maxima, sums and the exponents' arguments are FP32.
 //
 // Layouts.  mma sums over 32 columns (scores) or 16 slots (values) in any order that both operands share: a lane's piece of a key row is
 // 16 contiguous codes, of a value row hd / 8 of them, and every 4 codes are operands of one product.  The probabilities of the score tile's layout
-// are the value product's operand as they stand.  Where the maximum rises by less than 2^8, sums are not scaled anew.
+// are the value product's operand as they stand.  Where the maximum rises by less than 2^7, sums are not scaled anew.
 #include "pi_attn_q8.cuh"
 
 #include <cfloat>

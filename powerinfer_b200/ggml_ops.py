@@ -331,7 +331,7 @@ def rope_freqs(n_rot: int, freq_base: float = 10000.0, freq_scale: float = 1.0, 
 
 def rope_ext(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, freqs: RopeFreqs, head_dim: int, mode: int = 0, inplace: bool = False):
     """Queries [T, n_head * head_dim] and keys [T, n_head_kv * head_dim] rotated to pos int32 [T]; mode 0 (pairs (2i, 2i+1)) or 2 (neox).  The first
-    2 * len(freqs) dimensions of each head turn.  Returns (q, k), new tensors, or the same ones with inplace."""
+    2 * len(freqs) dimensions of each head turn.  Returns (q, k): new tensors of rows (two dimensions, also for [T, heads, head_dim]), or the same ones with inplace."""
     xq, q_at, T, nq, q_step, xtype = _row_matrix(q, "q")
     f = freqs.freqs
     if nq % head_dim:
@@ -434,7 +434,7 @@ def _slot_weights(w: torch.Tensor | None, cache: KvCacheQ8):
 def attention_q8(cache: KvCacheQ8, q: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None, max_new: int | None = None,
                  max_kv: int | None = None, scale: float | None = None, weights_in: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
-    """The KQV block over the 8-bit cache, the batch's own keys and values stored before: q [T, n_head * head_dim] -> the same shape and type.  Token t
+    """The KQV block over the 8-bit cache, the batch's own keys and values stored before: q [T, n_head * head_dim] (or [T, n_head, head_dim]) -> rows of q's type.  Token t
     of entry i sees the slots up to pos0[i] + t.  max_kv: slots that the longest sequence sees (None: all).  weights_out float32 [n_seq,
     n_head_kv, n_ctx] takes each seen slot's probabilities, plus weights_in for slots before pos0.  Rows of no entry are left as `out` has them."""
     hd = cache.head_dim
