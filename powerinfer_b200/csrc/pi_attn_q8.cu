@@ -682,7 +682,8 @@ struct AqPlan { bool tc; int R, row_tiles, split, n_splits, items, whole, pitch;
 
 // CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split
 // into ranges of at least AQ_LEAST slots.  A CTA costs as much as its slots and AQ_TURN times 64 more (on tcgen05 AQ_TURN_TC), the kernel that joins
-// as AQ_TURN times 64.
+// as AQ_TURN times 64.  Measured on both sides (us): with 1 and 3 for 4 and 10, 40 sequences of 1000 slots, 64 heads over 8 of 128, 30 for 22, 512 tokens over 4096 slots 168 for
+// 132; with 12 and 30 the same, but 3 prompts of 300 tokens over 3000 slots, 32 heads over 8, 99 for 117.  AQ_ROUNDS 2 and 8: the same within 3 %.
 static constexpr int AQ_LEAST = 256, AQ_TURN = 4, AQ_TURN_TC = 10, AQ_ROUNDS = 4;        // (more rounds than that: room for the parts, and nothing gained)
 // Weights: scores of few rows are kept, if they take no more than this (8 sequences of 64 heads and 8000 slots, 16 MB: 28 us for reading the keys again, 6 so)
 static constexpr int64_t AQ_SCORES = int64_t(256) << 20;
