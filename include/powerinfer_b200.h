@@ -121,7 +121,7 @@ int pi_sparse_ffn(int wtype, const void * up, const void * gate, const void * do
  * overlap on the GPU (different streams, or different host threads) race on it, so serialise them. */
 size_t pi_axpy_static_max_bytes(void);
 
-/* Did the last pi_mul_mat / pi_predictor / pi_mul_mat_idx / pi_axpy / pi_sparse_ffn (or pi_attention_q8, see there) that used `workspace` (of at least
+/* Did the last pi_mul_mat / pi_predictor / pi_mul_mat_idx / pi_axpy / pi_sparse_ffn (or pi_attention_q8, pi_attention_tree, see there) that used `workspace` (of at least
  * pi_workspace_bytes) finish all its bounded device-side waits (the
  * batch kernels stream rows through rings of bulk copies guarded by waits that give up after a limit rather than hang)?
  * PI_OK, or PI_ERR_TIMEOUT with the status bits in pi_last_error(): the call's result is then incomplete.  workspace NULL:
@@ -246,6 +246,56 @@ int pi_attention_q8(const pi_kv_q8 * cache, const pi_kv_batch * batch, int xtype
  * Of entries that name one sequence the last one counts, the others' kept are -1.  n_ctx up to 262144. */
 int pi_kv_evict_q8(const pi_kv_q8 * cache, const int32_t * len, const int32_t * seq, int n, int keep, int n_sink, int n_recent,
                    const float * weights, float * weights_out, int32_t * kept, void * stream);
+
+/* ---- drafted tokens over a paged cache: trees, keys and values into pages, their attention, the path that stays ----------------------- */
+
+/* A cache of pages: k, v F16 [n_layer, n_pages, n_head_kv, page, head_dim], 16-byte aligned; table int32 [n_seq, max_pages] on the device: slot j of a sequence is
+ * row j % page of the page that its row of the table names at j / page.  A number outside 0 .. n_pages - 1 is a page that is not there: nothing is
+ * stored in its slots and nobody sees them.  A sequence has n_ctx = max_pages * page slots at most.  Sequences may share pages that they only read;
+ * what a call writes to a row that two of its sequences share is either's, in pieces of 16 bytes.  head_dim 64, 96, 128, 192 or 256; page 16, 32, 64 or 128.
+ * (Sequences over one pool are the reference's cells with sequence ids, llama.cpp:1573-1693.) */
+typedef struct {
+    void * k, * v; const int32_t * table;
+    int n_layer, n_pages, n_seq, max_pages, n_head_kv, page, head_dim;
+} pi_kv_paged;
+
+/* A tree of drafted tokens is an entry of a pi_kv_batch: its tokens lie in the order of their numbers 0 .. m - 1 (m up to 4096), parents int32 [T] has the
+ * number of each one's parent, which is smaller than its own; any other number: it has none.
+ * mask [T, words] of 64 bits: bit u % 64 of word u / 64 of a token's row is set where token u of its entry is the token itself or one of its ancestors (those behind
+ * 64 * words have no bit).  pos int32 [T]: pos0 of the entry plus the number of the token's ancestors, the position that it is rotated to.  pos may be NULL.  seq is not
+ * read, and pos0 has no limit here.  Rows of no entry are left as they were. */
+int pi_tree_mask(const pi_kv_batch * batch, const int32_t * parents, uint64_t * mask, int words, int32_t * pos, void * stream);
+
+/* The path of a tree that a target model agrees with: from token 0 of an entry, whose next one is the lowest child u of the last one c with tokens[u] == choice[c]; tokens, parents,
+ * choice int32 [T] (choice: the target's token behind each one).  path int32 [n, batch->max_new]: the numbers of its tokens, token 0 the first, -1 behind the end;
+ * n_path int32 [n] how many; next int32 [n]: choice of the last one (of an entry without tokens: n_path 0, next -1).  seq and pos0 are not read (pos0 may be NULL). */
+int pi_tree_accept(const pi_kv_batch * batch, const int32_t * tokens, const int32_t * parents, const int32_t * choice, int32_t * path, int32_t * n_path, int32_t * next, void * stream);
+
+/* llm_build_kv_store behind ggml_rope_custom (llama.cpp:4383-4418, ggml.c:11163-11325) into pages of layer `layer`: k rotated to pos int32 [T] (NULL: the slots' numbers) and v, [T, n_head_kv * head_dim]
+ * (F32 or F16), each rounded once to F16; and q [T, n_head * head_dim] rotated to the same positions into q_out, of q's type (q NULL: none).  Rotation as in
+ * pi_rope_ext: n_rot, neox, freqs F64 [n_rot / 2], mscale; freqs NULL: keys as they are, and no q.  q_out may be q (same address and stride).  Slots behind n_ctx and of
+ * pages that are not there are not stored.  Of entries that name one sequence the last one with tokens is stored; every entry's queries are rotated. */
+int pi_kv_append_paged(const pi_kv_paged * cache, const pi_kv_batch * batch, int layer, int xtype, const void * k, int64_t k_stride, const void * v, int64_t v_stride,
+                       const void * q, int64_t q_stride, int n_head, void * q_out, int64_t q_out_stride,
+                       const int32_t * pos, const double * freqs, int n_rot, int neox, float mscale, void * stream);
+
+/* llm_build_kqv (llama.cpp:4764-4850) over the pages of layer `layer`, the new tokens' keys and values in them already: token t of entry i sees the slots 0 .. pos0[i] - 1 and
+ * pos0[i] + u for those new tokens u of its entry that its row of mask [T, mask_words] names (pi_tree_mask's, or any other; mask NULL: u <= t), where the cache has
+ * them; out = softmax(scale * q . k) v for every query head, heads h of group h / (n_head / n_head_kv).  q, out [T, n_head * head_dim] (F32 or F16).  A token that sees nothing has
+ * zeros, so has one whose own slot lies behind n_ctx; what it does not see has no part in its row, whatever is there.  (What it sees has to be finite numbers: a row that sees others is not.)
+ * F32 rows: queries to 2^-22 of their row's largest value, probabilities to 22 bits down to 2^-12 of the row's largest; F16 rows: queries as they are, probabilities to 11 bits.  Sums are FP32.
+ * max_kv: the slots that the longest sequence is expected to have (it sets how the work is cut; more slots are read too, more slowly).
+ * workspace: pi_attention_tree_workspace_bytes with the same arguments, 256-byte aligned; 0 bytes may be NULL.  It serves one call at a time: calls of one stream, or
+ * captured graphs that are not replayed at once.  pi_op_status(workspace) tells whether all bounded waits inside the kernels completed; the rows of one that did not are NaN.
+ * (Without a workspace there are none.) */
+size_t pi_attention_tree_workspace_bytes(const pi_kv_paged * cache, const pi_kv_batch * batch, int xtype, int n_head, int max_kv);
+int pi_attention_tree(const pi_kv_paged * cache, const pi_kv_batch * batch, int layer, int xtype, const void * q, int64_t q_stride, int n_head, const uint64_t * mask, int mask_words,
+                      int max_kv, float scale, void * out, int64_t out_stride, void * workspace, size_t workspace_bytes, void * stream);
+
+/* The path that stays (llama_kv_cache_seq_cp and llama_kv_cache_seq_rm of a speculative step in one, llama.cpp:1573-1693): in all layers the rows of slots pos0[i] + path[i][r] move to slots pos0[i] + r of
+ * sequence seq[i] (NULL: i), r < n_path[i].  path int32 [n, max_path], ascending: it ends where a number is not larger than the one before it or is negative.  Rows whose page is not there, or that
+ * lie behind n_ctx, do not move.  The other slots are left as they were.  Of entries that name one sequence the last one with a path counts. */
+int pi_kv_keep_paged(const pi_kv_paged * cache, const int32_t * path, int max_path, const int32_t * n_path, const int32_t * pos0, const int32_t * seq, int n, void * stream);
 
 /* ---- the decode token loop ------------------------------------------------------------------------------ */
 

@@ -26,6 +26,10 @@ class KvBatch(C.Structure):               # pi_kv_batch
     _fields_ = [(n, C.c_void_p) for n in ("q_start", "seq", "pos0")] + [(n, C.c_int) for n in ("n", "T", "max_new")]
 
 
+class KvPaged(C.Structure):               # pi_kv_paged
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "table")] + [(n, C.c_int) for n in ("n_layer", "n_pages", "n_seq", "max_pages", "n_head_kv", "page", "head_dim")]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} not built: run `python -m powerinfer_b200.build` (needs nvcc)")
@@ -59,6 +63,12 @@ def _load():
         "pi_attention_q8_workspace_bytes": (sz, [vp, vp, i32, i32, i32]),
         "pi_attention_q8": (i32, [vp, vp, i32, vp, i64, i32, i32, f32, vp, i64, vp, vp, vp, sz, vp]),
         "pi_kv_evict_q8": (i32, [vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]),
+        "pi_tree_mask": (i32, [vp, vp, vp, i32, vp, vp]),
+        "pi_tree_accept": (i32, [vp, vp, vp, vp, vp, vp, vp, vp]),
+        "pi_kv_append_paged": (i32, [vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, vp, i32, i32, f32, vp]),
+        "pi_attention_tree_workspace_bytes": (sz, [vp, vp, i32, i32, i32]),
+        "pi_attention_tree": (i32, [vp, vp, i32, i32, vp, i64, i32, vp, i32, i32, f32, vp, i64, vp, sz, vp]),
+        "pi_kv_keep_paged": (i32, [vp, vp, i32, vp, vp, vp, i32, vp]),
         "pi_attention_decode": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     }
     for name, (res, args) in sig.items():
@@ -72,7 +82,8 @@ EXPORTS = ["pi_last_error", "pi_version", "pi_row_bytes", "pi_workspace_bytes", 
            "pi_dequantize_q4_0", "pi_quantize_q8_0", "pi_mul_mat_idx", "pi_axpy", "pi_sparse_ffn", "pi_axpy_static_max_bytes", "pi_axpy_static", "pi_op_status",
            "pi_mul_mat", "pi_predictor",
            "pi_active_list", "pi_norm", "pi_rope", "pi_rope_table_host", "pi_attention_decode",
-           "pi_rope_freqs_host", "pi_rope_ext", "pi_kv_store_q8", "pi_kv_load_q8", "pi_attention_q8_workspace_bytes", "pi_attention_q8", "pi_kv_evict_q8"]
+           "pi_rope_freqs_host", "pi_rope_ext", "pi_kv_store_q8", "pi_kv_load_q8", "pi_attention_q8_workspace_bytes", "pi_attention_q8", "pi_kv_evict_q8",
+           "pi_tree_mask", "pi_tree_accept", "pi_kv_append_paged", "pi_attention_tree_workspace_bytes", "pi_attention_tree", "pi_kv_keep_paged"]
 
 
 def check(rc: int) -> None:

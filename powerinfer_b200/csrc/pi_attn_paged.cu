@@ -1,0 +1,457 @@
+// Attention over a paged cache for a ragged batch of trees of drafted tokens: token t of entry i sees the slots before pos0[i], and of the entry's new ones those
+// that its mask names (or those up to its own).
+//
+//     s_j = scale * (q . k_j)     p_j = exp(s_j - max s)     out = sum_j p_j v_j / sum_j p_j     over the slots j that the token sees
+//
+// Bound by the bytes of keys and values.  A CTA takes 16 query rows that read one KV head (the query heads of a group, of one or more tokens) and a range of slots; its
+// four warps take 16 slots each in turn, a part of one page, copied ahead into a ring of their own (cp.async; no barrier between warps), keep a maximum, a sum and all
+// sums of values of their own, and join them at the end.  Long ranges are split over CTAs, whose sums k_attn_paged_join joins.
+//
+// Precision.  Queries of FP32 rows, over a power of two of their row's largest value, and their probabilities are the sum of two halves each, 22 bits, i.e. two products in the place
+// of one; queries of FP16 rows are halves as they are, and their probabilities one half, 11 bits like the result's own rounding.  Probabilities are held times 2^8: their steps
+// end 2^-32 (FP16 rows: 2^-32 too) below the largest one.  Maxima, sums and the exponents' arguments are FP32.
+//
+// What a row does not see: scores are set to -infinity by the mask's bits, whatever the keys are; slots behind the entry's last and pages that are not there come as zeros; and where a step that not
+// every row sees whole holds a value that is not finite, its slots are added one by one to the rows that see them.
+//
+// Layouts.  A slot's row has 16-byte pieces permuted by its number, so that ldmatrix meets all banks.  The probabilities of the score tile's layout are the value product's
+// operand as they stand.  Where the maximum rises by less than 2^7, sums are not scaled anew.
+#include "pi_attn_paged.cuh"
+
+#include <cfloat>
+
+namespace pi {
+
+static constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, PA_STEP = PA_WARPS * 16, PA_R = 16;
+static constexpr float PA_RISE = 7.f, PA_P = 256.f;                   // bits a maximum may lag; probabilities are held times this (2^7 * 256 < 65504)
+
+template <int HD> struct PaShape {
+    static constexpr int KS = HD / 16, NT = HD / 8, PIECES = HD / 8;  // steps of 16 columns, tiles of 8 columns, 16-byte pieces of a row
+    static __device__ __forceinline__ uint32_t at(int row, int piece) {
+        return (uint32_t)(row * PIECES + (HD % 64 == 0 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3))) * 16u;
+    }
+    static constexpr int STAGES = HD <= 96 ? 4 : 3, STAGE = 2 * 16 * HD * 2;
+    static constexpr int CTAS = HD == 64 ? 3 : HD <= 128 ? 2 : 1;     // that an SM holds
+    static constexpr size_t RING = (size_t)PA_WARPS * STAGES * STAGE, JOIN = (size_t)PA_WARPS * PA_R * (HD + 4) * 4, QUERIES = 2 * PA_R * (2 * HD + 16);
+    static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + QUERIES;
+};
+
+// 16 rows in shared memory as halves [upper, lower][row][HD + 8], and the factors of their scores
+template <int HD, bool TWO> struct PaQueries {
+    static constexpr int TPR = PA_THREADS / PA_R, W = HD / 4, N = W / TPR, PITCH = 2 * HD + 16;
+    float4 x[N];
+    __device__ __forceinline__ void load(const AttnPagedP & p, const SeqB & s, const TileP & t, int hk) {
+        const int r = threadIdx.x / TPR, j = threadIdx.x % TPR, row = t.first + r, tok = p.by_group.of(row);
+        const size_t at = r < t.n_rows ? (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD : 0;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < t.n_rows) x[u] = aq_query(p.xtype, p.q, at + (j + u * TPR) * 4);
+        }
+    }
+    __device__ __forceinline__ void put(const AttnPagedP & p, unsigned char * to, float * factor) {
+        const int r = threadIdx.x / TPR, j = threadIdx.x % TPR;
+        float m = 0.f, zero = 0.f;                                    // zero: no more 0 where a value is not finite
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(x[u].x), fabsf(x[u].y))), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
+            zero = fmaf(x[u].x, 0.f, fmaf(x[u].y, 0.f, fmaf(x[u].z, 0.f, fmaf(x[u].w, 0.f, zero))));
+        }
+        if (zero != 0.f) m = INFINITY;
+#pragma unroll
+        for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        // two halves: the largest to 2^10 .. 2^11, a value is then off by 2^-22 of itself, or by 2^-25 (lower parts have no steps below 2^-24)
+        const int e = TWO ? min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10 : 0;
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = m < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : __int_as_float(0x7fc00000);
+        if (j == 0) factor[r] = down * p.scale_log2;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            uint2 hi, lo;
+            aq_split(x[u].x * up, x[u].y * up, hi.x, lo.x);
+            aq_split(x[u].z * up, x[u].w * up, hi.y, lo.y);
+            *reinterpret_cast<uint2 *>(to + r * PITCH + (j + u * TPR) * 8) = hi;
+            if (TWO) *reinterpret_cast<uint2 *>(to + (PA_R + r) * PITCH + (j + u * TPR) * 8) = lo;
+        }
+    }
+};
+
+// TWO: two halves for queries and probabilities (FP32 rows)
+template <int HD, bool TWO>
+__global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(const AttnPagedP p) {
+    using S = PaShape<HD>;
+    using Q = PaQueries<HD, TWO>;
+    constexpr int ST = S::STAGES;
+    constexpr bool Q_REGS = HD <= 128;                                // queries stay in registers
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float s_m[PA_WARPS][PA_R], s_l[PA_WARPS][PA_R], s_f[PA_R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const AqItem wk = ap_item(p, blockIdx.x);
+    const int split = wk.split, hk = wk.hk;
+    pdl_launch();
+    pdl_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && p.status) *p.status = 0u;          // (no wait of this kernel runs out)
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
+    const TileP t = ap_tile(p, s, wk.rt, PA_R);
+    if (t.n_rows <= 0) return;
+    const int k0 = split * p.split, k1 = split == wk.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
+    if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
+    unsigned char * queries = smem + (S::SMEM - S::QUERIES);
+    Q qs;
+    qs.load(p, s, t, hk);
+    const __half * kc = p.c.k + page_at(p.c, 0, hk), * vc = p.c.v + page_at(p.c, 0, hk);
+    const size_t of_page = page_at(p.c, 1, 0);                        // halves from page to page
+    const int first = k0 + warp * 16, steps = first < k1 ? (k1 - first + PA_STEP - 1) / PA_STEP : 0;
+    const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * ST * S::STAGE);
+    // pages of the next 32 steps, one a lane, and of the 32 behind them
+    auto pages = [&](int it) { const int j = first + (it + lane) * PA_STEP; return j < k1 ? page_of(p.c, s.sq, j >> p.c.shift) : -1; };
+    int page_now = steps ? pages(0) : -1, page_then = steps > 32 ? pages(32) : -1;
+    uint32_t valid = 0;                                               // bit it & 31: step `it`'s page is there
+    int asked = 0;
+    auto issue = [&]() {
+        if (asked < steps) {
+            if (asked > 0 && (asked & 31) == 0) { page_now = page_then; page_then = asked + 32 < steps ? pages(asked + 32) : -1; }
+            const int page = __shfl_sync(0xffffffffu, page_now, asked & 31), j0 = first + asked * PA_STEP;
+            valid = page >= 0 ? valid | 1u << (asked & 31) : valid & ~(1u << (asked & 31));
+            if (page >= 0) {
+                const size_t at = (size_t)page * of_page + (size_t)(j0 & (p.c.page - 1)) * HD;
+                const uint32_t fill = ring + (uint32_t)(asked % ST) * S::STAGE;
+#pragma unroll
+                for (int u = 0; u < HD / 16; u++) {
+                    const int e = u * 32 + lane, row = e / S::PIECES, piece = e - row * S::PIECES, bytes = j0 + row < t.there ? 16 : 0;      // (behind the entry's slots: zeros)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(fill + S::at(row, piece)), "l"(kc + at + e * 8), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(fill + 16 * HD * 2 + S::at(row, piece)), "l"(vc + at + e * 8), "r"(bytes) : "memory");
+                }
+            }
+            asked++;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int it = 0; it < ST - 1; it++) issue();
+
+    qs.put(p, queries, s_f);
+    __syncthreads();
+    float f[2], m[2], l[2]; int tok[2]; bool any[2];                  // of rows g and g + 8
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = g + 8 * h;
+        tok[h] = r < t.n_rows ? p.by_group.of(t.first + r) : 0x7fffffff;
+        f[h] = s_f[r]; m[h] = -INFINITY; l[h] = 0.f; any[h] = false;
+    }
+    // ldmatrix: a lane names a row of one of four 8 x 8 pieces
+    const uint32_t q_at = smem_u32(queries) + (uint32_t)((lane & 15) * Q::PITCH + (lane >> 4) * 16);
+    uint32_t a[Q_REGS ? S::KS : 1][4], a_low[Q_REGS && TWO ? S::KS : 1][4];
+    if constexpr (Q_REGS) {
+#pragma unroll
+        for (int k = 0; k < S::KS; k++) {
+            ldsm4(a[k], q_at + k * 32);
+            if constexpr (TWO) ldsm4(a_low[k], q_at + PA_R * Q::PITCH + k * 32);
+        }
+    }
+    float o[S::NT][4];
+#pragma unroll
+    for (int n = 0; n < S::NT; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[n][j] = 0.f;
+    const int k_row = (lane & 7) + (lane >> 4) * 8, k_piece = lane >> 3 & 1, v_row = lane & 15, v_piece = lane >> 4;
+
+    for (int it = 0; it < steps; it++) {
+        asm volatile("cp.async.wait_group %0;" :: "n"(ST - 2) : "memory");
+        __syncwarp();                                                 // the stage is there for all lanes, and all have read the last one
+        const bool there = valid >> (it & 31) & 1;
+        issue();                                                      // (into which this goes)
+        if (!there) continue;                                         // nobody sees the slots of a page that is not there
+        const uint32_t kt = ring + (uint32_t)(it % ST) * S::STAGE, vt = kt + 16 * HD * 2;
+        const int j0 = first + it * PA_STEP;
+        const bool masked = j0 + 16 > s.pos;                          // not wholly of the context, which every row sees
+        // ---- scores of 16 slots
+        float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int k = 0; k < S::KS; k++) {
+            uint32_t b[4];
+            ldsm4(b, kt + S::at(k_row, 2 * k + k_piece));
+            if constexpr (Q_REGS) {
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    if constexpr (TWO) mma16816(x[n], a_low[k][0], a_low[k][1], a_low[k][2], a_low[k][3], b[2 * n], b[2 * n + 1]);
+                    mma16816(x[n], a[k][0], a[k][1], a[k][2], a[k][3], b[2 * n], b[2 * n + 1]);
+                }
+            } else {
+                uint32_t w[4];
+                if constexpr (TWO) {
+                    ldsm4(w, q_at + PA_R * Q::PITCH + k * 32);
+#pragma unroll
+                    for (int n = 0; n < 2; n++) mma16816(x[n], w[0], w[1], w[2], w[3], b[2 * n], b[2 * n + 1]);
+                }
+                ldsm4(w, q_at + k * 32);
+#pragma unroll
+                for (int n = 0; n < 2; n++) mma16816(x[n], w[0], w[1], w[2], w[3], b[2 * n], b[2 * n + 1]);
+            }
+        }
+        // ---- probabilities, as A operands of the value products
+        uint32_t sees[2] = {0xffffu, 0xffffu};
+        if (masked) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) sees[h] = ap_sees(p, s, tok[h], j0 - s.pos) & 0xffffu;
+        }
+        uint32_t pa[4], pl[4];
+        float alpha[2] = {1.f, 1.f};
+        bool moved = false;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            any[h] |= sees[h] != 0;
+            float y[2][2];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    y[n][j] = x[n][2 * h + j] * f[h];
+                    if (masked && !(sees[h] >> (n * 8 + 2 * q + j) & 1)) y[n][j] = -INFINITY;
+                }
+            float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
+            if (__any_sync(0xffffffffu, top > m[h] + PA_RISE)) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float now = fmaxf(m[h], top);
+                alpha[h] = now == m[h] ? 1.f : exp2_approx(m[h] - now);
+                m[h] = now;
+                l[h] *= alpha[h];
+                moved = true;
+            }
+            const float ref = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float p0 = exp2_approx(y[n][0] - ref), p1 = exp2_approx(y[n][1] - ref);
+                l[h] += p0 + p1;
+                aq_split(p0 * PA_P, p1 * PA_P, pa[2 * n + h], pl[2 * n + h]);
+            }
+        }
+        if (moved && it > 0) {
+#pragma unroll
+            for (int n = 0; n < S::NT; n++) { o[n][0] *= alpha[0]; o[n][1] *= alpha[0]; o[n][2] *= alpha[1]; o[n][3] *= alpha[1]; }
+        }
+        // ---- values
+        bool odd = false;                                             // a value that is not finite, where not every row sees every slot
+        if (masked) {
+            __half2 zero = __floats2half2_rn(0.f, 0.f);
+            const __half2 none = zero;
+#pragma unroll
+            for (int u = 0; u < HD / 16; u++) {
+                uint4 w;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(vt + (uint32_t)(u * 32 + lane) * 16u) : "memory");
+                const __half2 * v = reinterpret_cast<const __half2 *>(&w);
+#pragma unroll
+                for (int j = 0; j < 4; j++) zero = __hfma2(v[j], none, zero);
+            }
+            odd = __any_sync(0xffffffffu, !__hbeq2(zero, none));
+        }
+        if (!odd) {
+#pragma unroll
+            for (int n = 0; n < S::NT; n += 2) {
+                uint32_t b[4];
+                ldsm4_t(b, vt + S::at(v_row, n + v_piece));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (TWO) mma16816(o[n + h], pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
+                    mma16816(o[n + h], pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
+                }
+            }
+        } else {
+            // slot by slot: the products of one slot's value and all rows' probabilities, kept by the rows that see it.  (Lower parts of probabilities would make no number of an infinity
+            // times 0: they count where the value is finite.)
+#pragma unroll 1
+            for (int j = 0; j < 16; j++) {
+                const bool mine = (j >> 1 & 3) == q;                  // this lane's slots are 2q, 2q + 1, 8 + 2q, 9 + 2q
+                const uint32_t keep = mine ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+                const uint32_t lo8 = j < 8 ? keep : 0u, hi8 = j < 8 ? 0u : keep;
+                const bool see0 = sees[0] >> j & 1, see1 = sees[1] >> j & 1;
+#pragma unroll
+                for (int n = 0; n < S::NT; n += 2) {
+                    uint32_t b[4];
+                    ldsm4_t(b, vt + S::at(v_row, n + v_piece));
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t b0 = b[2 * h] & lo8, b1 = b[2 * h + 1] & hi8;
+                        float w[4] = {0.f, 0.f, 0.f, 0.f}, wl[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma16816(w, pa[0], pa[1], pa[2], pa[3], b0, b1);
+                        if constexpr (TWO) mma16816(wl, pl[0], pl[1], pl[2], pl[3], b0, b1);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (e < 2 ? see0 : see1) o[n + h][e] += fabsf(w[e]) <= FLT_MAX ? w[e] + wl[e] : w[e];
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- the four warps' sums together
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    constexpr int PITCH = HD + 4;
+    float * so = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float sum = l[h];
+        if (any[h] && m[h] == -INFINITY) sum = __int_as_float(0x7fc00000);         // (every score that it sees is -infinity: no number)
+        const bool none = tok[h] >= p.c.n_ctx - s.pos;                // a token without a slot of its own
+        if (none) { m[h] = -INFINITY; sum = 0.f; }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int r = g + 8 * h;
+        if (q == 0) { s_m[warp][r] = m[h]; s_l[warp][r] = sum; }
+        float * row = so + (size_t)(warp * PA_R + r) * PITCH + 2 * q;
+#pragma unroll
+        for (int n = 0; n < S::NT; n++) *reinterpret_cast<float2 *>(row + n * 8) = none ? make_float2(0.f, 0.f) : make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    __syncthreads();
+    const size_t part0 = ((size_t)(wk.item - p.whole) * p.n_splits + split) * PA_R;
+    for (int e = threadIdx.x; e < t.n_rows * (HD / 4); e += PA_THREADS) {
+        const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
+        float top = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < PA_WARPS; w++) top = fmaxf(top, s_m[w][r]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; w++) {
+            const float is = exp2_approx(s_m[w][r] - ref), k = is * (1.f / PA_P);
+            const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * PA_R + r) * PITCH + d);
+            sum = fmaf(is, s_l[w][r], sum);
+            v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);
+        }
+        if (wk.n_splits > 1) {
+            *reinterpret_cast<float4 *>(p.part + (part0 + r) * HD + d) = v;
+            if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
+        } else {
+            const int row = t.first + r, of = p.by_group.of(row), h = hk * p.group + row - of * p.group;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const size_t at = (size_t)(s.first + of) * p.out_stride + (size_t)h * HD + d;
+            if (p.xtype == PI_TYPE_F16) *reinterpret_cast<uint2 *>((__half *)p.out + at) = make_uint2(h2u(__floats2half2_rn(v.x * inv, v.y * inv)), h2u(__floats2half2_rn(v.z * inv, v.w * inv)));
+            else                        *reinterpret_cast<float4 *>((float *)p.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        }
+    }
+}
+
+// The splits of a tile joined, in their order.  A CTA has one row: its groups of HD / 4 threads take splits in turn.
+static constexpr int PJ_THREADS = 128;
+
+template <int HD>
+__global__ void __launch_bounds__(PJ_THREADS) k_attn_paged_join(const AttnPagedP p, int R) {
+    constexpr int W = HD / 4, G = PJ_THREADS / W > 0 ? PJ_THREADS / W : 1;
+    __shared__ float4 s_v[G][W]; __shared__ float s_sum[G];
+    const int k = blockIdx.x / R, r = blockIdx.x - k * R, item = p.whole + k, d = threadIdx.x % W, gr = threadIdx.x / W;
+    pdl_launch();
+    pdl_wait();
+    const int of_head = p.by_tiles.of(item), rt = item - of_head * p.row_tiles, entry = p.by_heads.of(of_head), hk = of_head - entry * p.c.H;
+    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, entry);
+    const TileP t = ap_tile(p, s, rt, R);
+    if (r >= t.n_rows) return;
+    const int n = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));       // parts that were written
+    const size_t at0 = (size_t)k * p.n_splits * R + r;
+    float top = -INFINITY;
+    for (int i = 0; i < n; i++) top = fmaxf(top, __ldcg(&p.part_ml[at0 + (size_t)i * R]).x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (gr < G) {
+        for (int i = gr; i < n; i += G) {
+            const float2 ml = __ldcg(&p.part_ml[at0 + (size_t)i * R]);
+            const float4 u = __ldcg(reinterpret_cast<const float4 *>(p.part + (at0 + (size_t)i * R) * HD) + d);
+            const float is = exp2_approx(ml.x - ref);
+            sum = fmaf(is, ml.y, sum);
+            v.x = fmaf(is, u.x, v.x); v.y = fmaf(is, u.y, v.y); v.z = fmaf(is, u.z, v.z); v.w = fmaf(is, u.w, v.w);
+        }
+        s_v[gr][d] = v;
+        if (d == 0) s_sum[gr] = sum;
+    }
+    __syncthreads();
+    if (gr > 0) return;
+#pragma unroll
+    for (int i = 1; i < G; i++) { const float4 u = s_v[i][d]; v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w; sum += s_sum[i]; }
+    const int row = t.first + r, of = p.by_group.of(row), h = hk * p.group + row - of * p.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t at = (size_t)(s.first + of) * p.out_stride + (size_t)h * HD + d * 4;
+    if (p.xtype == PI_TYPE_F16) *reinterpret_cast<uint2 *>((__half *)p.out + at) = make_uint2(h2u(__floats2half2_rn(v.x * inv, v.y * inv)), h2u(__floats2half2_rn(v.z * inv, v.w * inv)));
+    else                        *reinterpret_cast<float4 *>((float *)p.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+}
+
+// ---- how the work is cut
+struct PaPlan { int R, row_tiles, split, n_splits, items, whole; size_t words, ml, part; };
+
+// CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split into ranges of at least PA_LEAST
+// slots: into the number of parts for which its CTAs, in rounds of their own, take the least.  A CTA costs as much as its slots and PA_TURN times 64 more, the kernel that joins as
+// PA_TURN times 64.
+static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_ROUNDS = 4;
+static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int n_head, int max_kv) {
+    PaPlan r;
+    const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
+    r.R = PA_R;
+    r.row_tiles = (int)((rows + r.R - 1) / r.R);
+    const int step = PA_STEP;
+    const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
+    const int64_t slots = (int64_t)sm_count() * (c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), rest = items % slots, units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
+    int64_t n = 1, least = -1;
+    for (int64_t k = 1; rest && k <= 128 && (k == 1 || k * PA_LEAST < keys + PA_LEAST); k++) {
+        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + PA_TURN) + (k > 1 ? PA_TURN : 0);
+        if (rounds > PA_ROUNDS) break;
+        if (least < 0 || cost < least) { least = cost; n = k; }
+    }
+    const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;
+    r.split = (int)per; r.n_splits = (int)((keys + per - 1) / per);
+    r.items = (int)items;
+    r.whole = (int)(r.n_splits == 1 ? items : items - rest);
+    auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+    r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
+    r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
+    r.words = r.ml + r.part ? 256 : 0;                                // (the status word where pi_op_status looks for it)
+    return r;
+}
+
+size_t attn_paged_scratch(const KvPaged & c, const RaggedB & b, int xtype, int n_head, int max_kv) {
+    const PaPlan r = pa_plan(c, b, n_head, max_kv);
+    return r.words + r.ml + r.part;
+}
+
+template <int HD, bool TWO>
+static int pa_go(const AttnPagedP & p, cudaStream_t st) {
+    static bool done[16] = {false};
+    int dev = 0;
+    PI_CUDA(cudaGetDevice(&dev));
+    constexpr size_t smem = PaShape<HD>::SMEM;
+    if (dev < 0 || dev >= 16 || !done[dev]) {
+        PI_CUDA(cudaFuncSetAttribute(k_attn_paged<HD, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 16) done[dev] = true;
+    }
+    PI_CUDA(launch_k(k_attn_paged<HD, TWO>, dim3(ap_grid(p)), dim3(PA_THREADS), smem, st, true, p));
+    return PI_OK;
+}
+
+template <int HD>
+static int pa_run(const AttnPagedP & p, const PaPlan & r, cudaStream_t st) {
+    const int rc = p.xtype == PI_TYPE_F16 ? pa_go<HD, false>(p, st) : pa_go<HD, true>(p, st);
+    if (rc) return rc;
+    if (p.items > p.whole) PI_CUDA(launch_k(k_attn_paged_join<HD>, dim3((unsigned)((p.items - p.whole) * r.R)), dim3(PJ_THREADS), 0, st, true, p, r.R));
+    return PI_OK;
+}
+
+int launch_attention_paged(const AttnPagedArgs & a, cudaStream_t st) {
+    const PaPlan r = pa_plan(a.c, a.b, a.n_head, a.max_kv);
+    AttnPagedP p;
+    p.c = a.c; p.b = a.b; p.xtype = a.xtype; p.q = a.q; p.q_stride = a.q_stride; p.n_head = a.n_head; p.group = a.n_head / a.c.H;
+    p.mask = a.mask; p.words = a.words;
+    p.scale_log2 = a.scale * 1.44269504088896340736f; p.out = a.out; p.out_stride = a.out_stride;
+    p.split = r.split; p.n_splits = r.n_splits; p.row_tiles = r.row_tiles; p.items = r.items; p.whole = r.whole;
+    p.by_group = AqDiv::by(p.group); p.by_heads = AqDiv::by(a.c.H); p.by_tiles = AqDiv::by(r.row_tiles); p.by_splits = AqDiv::by(r.n_splits);
+    char * s = (char *)a.scratch;
+    p.status = s ? (unsigned int *)(s + 8) : nullptr;
+    s += r.words;
+    p.part_ml = (float2 *)s; p.part = (float *)(s + r.ml);
+    switch (a.c.hd) {
+        case 64:  return pa_run<64>(p, r, st);
+        case 96:  return pa_run<96>(p, r, st);
+        case 128: return pa_run<128>(p, r, st);
+        case 192: return pa_run<192>(p, r, st);
+        default:  return pa_run<256>(p, r, st);
+    }
+}
+
+}  // namespace pi

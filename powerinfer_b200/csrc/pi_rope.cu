@@ -8,6 +8,7 @@
 // thread requests its vectors first, the angles of the token are made while they travel (n_rot / 2 of them, once for all heads).
 // Bound by the bytes of x and y for many tokens, by the launch for one.  Measured: 1901 tokens of 128 + 8 FP16 heads of 64 15 us (66 MB, 4.3 TB/s), one token 4 us.
 #include "pi_kv_q8.cuh"
+#include "pi_rope.cuh"
 
 namespace pi {
 
@@ -31,22 +32,6 @@ template <> struct RopeVec<__half> {
         return u;
     }
 };
-__device__ __forceinline__ float rope_get(const float * p) { return *p; }
-__device__ __forceinline__ float rope_get(const __half * p) { return __half2float(*p); }
-__device__ __forceinline__ void rope_put(float * p, float v) { *p = v; }
-__device__ __forceinline__ void rope_put(__half * p, float v) { *p = __float2half_rn(v); }
-
-// cosine and sine of pos * f
-__device__ __forceinline__ float2 rope_angle(int pos, double f, float mscale) {
-    const double a = (double)pos * f, n = rint(a * 0.63661977236758134308);               // quarter turns
-    double r = fma(n, -1.57079632679489655800, a);                                        // pi / 2 in two parts
-    r = fma(n, -6.12323399573676603587e-17, r);
-    const float s0 = sinf((float)r), c0 = cosf((float)r);
-    const int k = (int)((long long)n & 3);
-    const float c = k & 1 ? s0 : c0, s = k & 1 ? c0 : s0;
-    return make_float2((k == 1 || k == 2 ? -c : c) * mscale, (k >= 2 ? -s : s) * mscale);
-}
-
 // UNIT: what a thread takes at once.  0: 32 bytes of a row (whole pairs); 1: 16 bytes of the first half and those of the second, or 32 of
 // the dimensions that pass; 2: one pair, where a half is no multiple of 16 bytes.
 template <typename T, int UNIT>
