@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(PJ_THREADS) k_attn_paged_join(const AttnPagedP
     const int k = blockIdx.x / R, r = blockIdx.x - k * R, item = p.whole + k, d = threadIdx.x % W, gr = threadIdx.x / W;
     pdl_launch();
     pdl_wait();
-    const int of_head = p.by_tiles.of(item), rt = item - of_head * p.row_tiles, entry = p.by_heads.of(of_head), hk = of_head - entry * p.c.H;
+    const int of_head = p.by_tiles.of(item), nt = item - of_head * p.row_tiles, rt = R == PT_ROWS ? p.row_tiles - 1 - nt : nt, entry = p.by_heads.of(of_head), hk = of_head - entry * p.c.H;
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, entry);
     const TileP t = ap_tile(p, s, rt, R);
     if (r >= t.n_rows) return;
@@ -375,23 +375,25 @@ __global__ void __launch_bounds__(PJ_THREADS) k_attn_paged_join(const AttnPagedP
 }
 
 // ---- how the work is cut
-struct PaPlan { int R, row_tiles, split, n_splits, items, whole; size_t words, ml, part; };
+struct PaPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, ml, part; };
 
 // CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split into ranges of at least PA_LEAST
-// slots: into the number of parts for which its CTAs, in rounds of their own, take the least.  A CTA costs as much as its slots and PA_TURN times 64 more, the kernel that joins as
+// slots: into the number of parts for which its CTAs, in rounds of their own, take the least.  A CTA costs as much as its slots and PA_TURN times 64 more (on tcgen05 PA_TURN_TC), the kernel that joins as
 // PA_TURN times 64.
-static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_ROUNDS = 4;
+static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 10, PA_ROUNDS = 4;
 static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int n_head, int max_kv) {
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
-    r.R = PA_R;
+    r.tc = attn_paged_tc_takes(c.hd, rows);
+    r.R = r.tc ? PT_ROWS : PA_R;
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
-    const int step = PA_STEP;
+    const int step = r.tc ? PT_KEYS : PA_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    const int64_t slots = (int64_t)sm_count() * (c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), rest = items % slots, units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
+    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), rest = items % slots, units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
+    const int64_t turn = r.tc ? PA_TURN_TC : PA_TURN;
     int64_t n = 1, least = -1;
     for (int64_t k = 1; rest && k <= 128 && (k == 1 || k * PA_LEAST < keys + PA_LEAST); k++) {
-        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + PA_TURN) + (k > 1 ? PA_TURN : 0);
+        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + turn) + (k > 1 ? PA_TURN : 0);
         if (rounds > PA_ROUNDS) break;
         if (least < 0 || cost < least) { least = cost; n = k; }
     }
@@ -402,7 +404,7 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int n_head, int max_
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
     r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
     r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
-    r.words = r.ml + r.part ? 256 : 0;                                // (the status word where pi_op_status looks for it)
+    r.words = r.tc || r.ml + r.part ? 256 : 0;                                // (the status word where pi_op_status looks for it)
     return r;
 }
 
@@ -427,7 +429,7 @@ static int pa_go(const AttnPagedP & p, cudaStream_t st) {
 
 template <int HD>
 static int pa_run(const AttnPagedP & p, const PaPlan & r, cudaStream_t st) {
-    const int rc = p.xtype == PI_TYPE_F16 ? pa_go<HD, false>(p, st) : pa_go<HD, true>(p, st);
+    const int rc = r.tc ? launch_attn_paged_tc(p, st) : p.xtype == PI_TYPE_F16 ? pa_go<HD, false>(p, st) : pa_go<HD, true>(p, st);
     if (rc) return rc;
     if (p.items > p.whole) PI_CUDA(launch_k(k_attn_paged_join<HD>, dim3((unsigned)((p.items - p.whole) * r.R)), dim3(PJ_THREADS), 0, st, true, p, r.R));
     return PI_OK;
