@@ -60,6 +60,28 @@ __device__ __forceinline__ uint32_t ap_sees(const AttnPagedP & p, const SeqB & s
     return there & (u0 < 0 ? (uint32_t)x << -u0 | ap_ones(-u0) : (uint32_t)x);
 }
 
+// The same for 128 slots: the words of the mask that hold them are on their way at once
+__device__ __forceinline__ void ap_sees128(const AttnPagedP & p, const SeqB & s, int tok, int u0, uint32_t (&sees)[4]) {
+    const int n_new = min(s.n_new, p.c.n_ctx - s.pos);
+    const bool none = s.sq < 0 || tok >= n_new;
+    const int end = none ? -0x40000000 : (p.mask ? n_new : tok + 1) - u0;
+    uint64_t x[3] = {0, 0, 0};
+    const int lo = max(u0, 0), w = lo >> 6, sh = lo & 63;
+    if (p.mask && !none) {
+        const uint64_t * row = p.mask + (size_t)(s.first + tok) * p.words;
+#pragma unroll
+        for (int i = 0; i < 3; i++) if (w + i < p.words) x[i] = __ldg(row + w + i);
+    }
+    // bits from lo on, then ones in front of them for the slots before the new ones
+    uint64_t a = x[0] >> sh | (sh ? x[1] << (64 - sh) : 0), b = x[1] >> sh | (sh ? x[2] << (64 - sh) : 0);
+    const int before = min(max(-u0, 0), 128);
+    if (before >= 128)     { a = b = ~0ull; }
+    else if (before >= 64) { b = a << (before - 64) | ((1ull << (before - 64)) - 1); a = ~0ull; }
+    else if (before > 0)   { b = b << before | a >> (64 - before); a = a << before | ((1ull << before) - 1); }
+    if (!p.mask) a = b = ~0ull;
+    sees[0] = (uint32_t)a & ap_ones(end); sees[1] = (uint32_t)(a >> 32) & ap_ones(end - 32); sees[2] = (uint32_t)b & ap_ones(end - 64); sees[3] = (uint32_t)(b >> 32) & ap_ones(end - 96);
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }

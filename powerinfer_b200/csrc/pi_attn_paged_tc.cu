@@ -1,20 +1,21 @@
 // Attention over a paged cache for more than a few query rows of a KV head (trees of a group's heads, prompts) on tcgen05; formulas and rows as in pi_attn_paged.cu.
 //
-// A CTA takes 128 query rows (the lanes) of one KV head and walks over its slots in tiles of 128.  Queries lie in tensor memory for the whole walk.  A tile's keys and
-// values come as tensor copies of one page's rows each into a ring of 128-byte swizzled rows of 64 halves, which is K-major for the scores and MN-major for the
-// values.  Scores S = Q K^T are made into one of two buffers in tensor memory; the probabilities take their place; sums of values O = P V of ONE tile go to a third buffer, which is
-// drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer than a tile.
-// So every tile has its own maximum (no exchange between tiles; the two score buffers are two groups of warps' own): the drain joins tiles.
+// A piece of work is 128 query rows (the lanes) of one KV head and a range of its slots, in tiles of 128.  A CTA an SM takes one piece after the other (a counter in
+// the workspace: pieces are of unequal lengths), and each of its roles goes on to the next as soon as its own part is done, so that the ends of a piece overlap.
+// A tile's keys and values come as tensor copies of one page's rows each into a ring of 128-byte swizzled rows of 64 halves, which is K-major for the scores and MN-major for the
+// values; queries lie beside them in the same layout.  Scores S = Q K^T are made into one of three buffers in tensor memory; the probabilities take their place; sums of values O = P V
+// of ONE tile go to one or two more, which are drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer
+// than a tile.  So every tile has its own maximum (no exchange between tiles; the score buffers are groups of warps' own): the drain joins tiles.
 //
-// A tile is special where not every row of the CTA sees all of its slots: then two warps go over its values before they are used.  Rows of slots that are not there
-// become zeros, values that are not finite too, and whoever sees such a slot has a row of no numbers; scores of slots that a row does not see are replaced by what its
+// A tile is special where not every row of the piece sees all of its slots: then a warp goes over its values before they are used.  Rows of slots that are not there
+// become zeros, rows with a value that is not finite too, and whoever sees such a slot has a row of no numbers; scores of slots that a row does not see are replaced by what its
 // mask says.
 //
 // Precision.  FP32 rows: queries and probabilities are the sum of two halves each, 22 bits, i.e. two products in the place of one.  FP16 rows: queries as they are, probabilities
 // one half, 11 bits like the result's own rounding.  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
 //
-// Warps: 0 issues the products; 1 asks for the tiles; 2 and 3 go over special tiles; 4..11 and 12..19 have the even and the odd tiles' probabilities, a row and half of the slots a thread (the
-// halves tell each other their maxima); 20..27 drain the sums, a row and half of the columns a thread.
+// Warps: 0 issues the products of scores and 2 those of values; 1 asks for the tiles; 3 goes over special ones; 4..7 take work and lay out its queries; 8..19 have the
+// probabilities, three groups a tile each in turn, a row a thread; 20..27 drain the sums, a row and half of the columns a thread.
 #include "pi_attn_paged.cuh"
 #include "pi_tc.cuh"
 #include "pi_tc_math.cuh"
@@ -24,419 +25,634 @@
 
 namespace pi {
 
-static constexpr int PT_THREADS = 896;
-static constexpr int PT_REGS_M = 40, PT_REGS_S = 64, PT_REGS_D = 104;  // 40 + 4 x 64 + 2 x 104 of the 7 x 72 of the launch
+static constexpr int PT_THREADS = 896, PT_GROUPS = 3;                  // groups of warps with tiles of probabilities
+static constexpr int PT_REGS_M = 40, PT_REGS_Q = 64, PT_REGS_S = 80, PT_REGS_D = 80;  // 40 + 64 + 3 x 80 + 2 x 80 of the 7 x 72 of the launch
 static constexpr uint32_t PT_SUB = PT_KEYS * 128;                     // bytes of 64 columns of a tile
 static constexpr int PT_BOX = 64;                                     // rows of a tensor copy, or a page's if it has fewer
+static constexpr int PT_WORK = 4;                                     // pieces of work that a CTA has in hand
+static constexpr int PT_AHEAD = 2;                                    // tiles that keys are ahead of values in the ring
+static constexpr int PT_INFO = 8;                                     // tiles whose description is kept: more than the ring holds, whose tiles warps 1 to 3 may be ahead
 
-struct PtP { AttnPagedP a; int box; CUtensorMap m_k, m_v; };
+struct PtP { AttnPagedP a; int box, units; unsigned int * next; CUtensorMap m_k, m_v; };
+
+// what is in shared memory besides the ring: queries' buffers (upper and, of FP32 rows, lower halves), tiles in the ring
+template <int HD, bool TWO> struct PtShape {
+    static constexpr int SUBS = (HD + 63) / 64;
+    static constexpr uint32_t TILE = SUBS * PT_SUB, QUERIES = TILE * (TWO ? 2 : 1);
+    static constexpr int QB = HD <= 64 ? 2 : 1, NS = (int)((196608u - QB * QUERIES) / TILE);
+    static constexpr size_t SMEM = QB * QUERIES + NS * TILE + 1024;
+};
+
+// A piece of work: 128 rows of one KV head and a range of slots
+struct PtWork { int tiles, k0, k1, first, n_rows, hk, there, clear, dst; SeqB s; };      // tiles -1: there is no more; dst: number of the part that it makes, -1: results
+
+// Barriers by their addresses in shared memory.  Code is kept short: seven roles run at once, and warps that waited for instructions were a third of the time.
+// A wait of up to some 20 us at a time (warps that ask again and again take issue slots), some 65536 times, or until another one of the CTA ran out.
+__device__ __forceinline__ bool pt_wait(uint32_t bar, unsigned parity, uint32_t dead) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p, q;\n .reg .u32 n, d;\n mov.u32 n, 0;\nWAIT:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n @p bra DONE;\n"
+                 " ld.volatile.shared.u32 d, [%4];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, 65536, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%4], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u), "r"(dead) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
+__device__ __forceinline__ void pt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
+__device__ __forceinline__ void pt_commit(uint32_t bar) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" :: "r"(bar) : "memory");
+}
+// N products of 16 steps of K each, both operands in shared memory, 32 bytes on from one to the next (64 columns of a piece are four); the first one adds to D if `add`
+template <int N> __device__ __forceinline__ void pt_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    static_assert(N == 2 || N == 4, "");
+    if constexpr (N == 4)
+        asm volatile("{\n .reg .pred e, p, t;\n .reg .b64 a, b;\n elect.sync _|e, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n setp.eq.u32 t, 0, 0;\n"
+                     " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+                     " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}"
+                     :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
+    else
+        asm volatile("{\n .reg .pred e, p, t;\n .reg .b64 a, b;\n elect.sync _|e, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n setp.eq.u32 t, 0, 0;\n"
+                     " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}"
+                     :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
+}
+// Four products of 16 slots each, probabilities in tensor memory, 16 columns on from one to the next, values 2048 bytes on
+__device__ __forceinline__ void pt_values(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n .reg .pred e, p, t;\n .reg .b32 a;\n .reg .b64 b;\n elect.sync _|e, 0xffffffff;\n setp.ne.u32 p, %4, 0;\n setp.eq.u32 t, 0, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n add.u32 a, %1, 16;\n add.s64 b, %2, 128;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+                 " add.u32 a, %1, 32;\n add.s64 b, %2, 256;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n add.u32 a, %1, 48;\n add.s64 b, %2, 384;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
+}
+// A place in a ring of barriers, and the parity of its phase
+struct PtRing {
+    uint32_t bar; unsigned at, parity;
+    __device__ __forceinline__ PtRing(uint64_t * bars) : bar(smem_u32(bars)), at(0), parity(0) {}
+    template <int N> __device__ __forceinline__ void step() { at++; if (at == N) { at = 0; parity ^= 1; } }
+    __device__ __forceinline__ uint32_t here() const { return bar + at * 8u; }
+};
 
 // TWO: two halves for queries and probabilities
 template <int HD, bool TWO>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_constant__ PtP pp) {
-    constexpr int KS = HD / 16, SUBS = (HD + 63) / 64, NV = SUBS * 64, NQ = HD / 4;       // steps of 16 columns; pieces of 64 columns; columns of the sums (behind HD: zeros); columns of a thread that loads queries
-    constexpr uint32_t TILE = SUBS * PT_SUB;
-    constexpr int NS = HD <= 64 ? 12 : 6, NP = NS / 2;                // tiles in the ring, keys and values in turn
-    constexpr uint32_t T_Q = 0, T_S = NV, T_O = NV + 2 * PT_KEYS;     // tensor memory: queries (upper, lower), two buffers of scores, sums
-    static_assert(T_O + NV <= 512 && PT_REGS_M + 4 * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
+    using Z = PtShape<HD, TWO>;
+    constexpr int KS = HD / 16, SUBS = Z::SUBS, NV = SUBS * 64;       // steps of 16 columns; pieces of 64 columns; columns of the sums (behind HD: zeros)
+    constexpr uint32_t TILE = Z::TILE;
+    constexpr int NS = Z::NS, QB = Z::QB;
+    constexpr int OB = (512 - PT_GROUPS * PT_KEYS) / NV;              // buffers of sums
+    constexpr uint32_t T_S = 0, T_O = PT_GROUPS * PT_KEYS;            // tensor memory: three buffers of scores, one or two of sums
+    static_assert(NS / 2 + 2 < PT_INFO && OB >= 1 && PT_REGS_M + PT_REGS_Q + PT_GROUPS * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
     const AttnPagedP & p = pp.a;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ uint64_t s_full[NS], s_empty[NS], s_vok[NP];
-    __shared__ uint64_t s_qk[2], s_pv[2], s_pfull[2], s_free[2], s_fin;
-    __shared__ uint32_t s_tmem;
-    __shared__ volatile int s_dead;
-    __shared__ uint32_t s_odd[NP][4];                                 // slots of a special tile with a value that is not finite
-    __shared__ float s_f[PT_ROWS];                                    // factor of a row's scores
-    __shared__ float s_max[2][2][PT_ROWS], s_sum[2][2][PT_ROWS];       // of a tile's halves: maximum, sum of the probabilities
-    __shared__ float s_top[2][PT_ROWS];                               // maximum of a tile
+    __shared__ uint64_t s_full[NS], s_empty[NS], s_vok[PT_INFO];
+    __shared__ uint64_t s_wfull[PT_WORK], s_wempty[PT_WORK], s_qfull[QB], s_qempty[QB];
+    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_ofree[OB], s_fin[2];
+    __shared__ PtWork s_work[PT_WORK];
+    __shared__ uint32_t s_tmem, s_info[PT_INFO];                      // of a tile: which groups of 16 slots are there; bit 8: special
+    __shared__ volatile unsigned s_dead;
+    __shared__ uint32_t s_odd[PT_INFO][4];                            // slots of a special tile with a value that is not finite
+    __shared__ float s_f[PT_WORK][PT_ROWS];                           // factor of a row's scores
+    __shared__ float s_top[PT_GROUPS][PT_ROWS], s_sum[PT_GROUPS][PT_ROWS];         // of a tile: maximum, sum of the probabilities
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const AqItem w = ap_item(p, blockIdx.x);
-    const int split = w.split, hk = w.hk, rt = p.row_tiles - 1 - w.rt;      // (the longest rows first)
-    pdl_launch();
-    pdl_wait();
-    const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, w.entry);
-    const TileP t = ap_tile(p, s, rt, PT_ROWS);
-    if (t.n_rows <= 0) return;
-    const int k0 = split * p.split, k1 = split == w.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
-    if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
-    const int n_tiles = k0 < k1 ? (k1 - k0 + PT_KEYS - 1) / PT_KEYS : 0;
-    const int clear = p.mask ? s.pos : s.pos + p.by_group.of(t.first) + 1;      // every row sees the slots before it
+    const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = queries + QB * Z::QUERIES;
 
     if (tid < NS) { mbar_init(s_full + tid, 1); mbar_init(s_empty + tid, 1); }
-    if (tid < NP) mbar_init(s_vok + tid, 2);
-    if (tid < 2) { mbar_init(s_qk + tid, 1); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 16); mbar_init(s_free + tid, 8); }
-    if (tid == 0) { mbar_init(&s_fin, 1); s_dead = 0; }
+    if (tid < PT_INFO) mbar_init(s_vok + tid, 1);
+    if (tid < PT_WORK) { mbar_init(s_wfull + tid, 1); mbar_init(s_wempty + tid, PT_THREADS / 32); }
+    if (tid < QB) { mbar_init(s_qfull + tid, 4); mbar_init(s_qempty + tid, 1); }
+    if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 4); mbar_init(s_stat + tid, 8); }
+    if (tid < OB) mbar_init(s_ofree + tid, 8);
+    if (tid < 2) mbar_init(s_fin + tid, 1);
+    if (tid == 0) s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    auto wait = [&](uint64_t * bar, unsigned parity) -> bool {        // warp-uniform; false: the wait ran out, here or elsewhere
-        bool ok = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
-        if (__builtin_expect(ok, 1)) return true;
-        for (int spins = 0; spins < (1 << 20) && !ok && !s_dead; spins++) ok = mbar_try_wait(bar, parity);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok && lane == 0) { s_dead = 1; atomicOr(p.status, 16u); }
-        return ok;
-    };
-    // which of a tile's eight groups of 16 slots are there
-    auto present = [&](int i) -> uint32_t {
-        const int j = k0 + i * PT_KEYS + (lane & 7) * 16;
-        return __ballot_sync(0xffffffffu, lane < 8 && j < t.there && page_of(p.c, s.sq, j >> p.c.shift) >= 0);
-    };
-    auto special = [&](int i, uint32_t there) { return there != 0xffu || k0 + (i + 1) * PT_KEYS > clear; };
+    if (tid == 32) { tma_map(&pp.m_k); tma_map(&pp.m_v); }
+    pdl_launch();
+    pdl_wait();
+    const uint32_t dead = smem_u32((const void *)&s_dead);
+    auto wait_at = [&](uint32_t bar, unsigned parity) { return pt_wait(bar, parity, dead); };      // warp-uniform; false: the wait ran out, here or elsewhere in the CTA
+    auto wait = [&](uint64_t * bar, unsigned parity) { return wait_at(smem_u32(bar), parity); };
+    auto work_of = [&](int n) { return s_work + n % PT_WORK; };
+    auto done_with = [&](int n) { __syncwarp(); if (lane == 0) mbar_arrive(s_wempty + n % PT_WORK); };
 
-    // ---- tiles: the n-th is keys (even) or values (odd) of tile n / 2
-    auto ask = [&](int n) {                                           // a whole warp: a lane takes a copy
-        const int slot = n % NS, j = k0 + (n >> 1) * PT_KEYS + lane * pp.box;
-        int page = -1;
-        if (lane * pp.box < PT_KEYS && j < t.there) page = page_of(p.c, s.sq, j >> p.c.shift);
-        const unsigned boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        if (lane == 0) mbar_expect_tx(s_full + slot, boxes * SUBS * pp.box * 128u);
-        __syncwarp();
-        if (page >= 0) {
-            const int y = ((page * p.c.H + hk) << p.c.shift) + (j & (p.c.page - 1));
-#pragma unroll
-            for (int u = 0; u < SUBS; u++) tma_tile(ring + (uint32_t)slot * TILE + u * PT_SUB + (uint32_t)(lane * pp.box) * 128u, n & 1 ? &pp.m_v : &pp.m_k, u * 64, y, s_full + slot);
-        }
-        __syncwarp();
-    };
-    if (warp == 1) for (int n = 0; n < min(NS, 2 * n_tiles); n++) ask(n);
-
-    // ---- queries into tensor memory: a row and a quarter of its columns a thread, straight from global memory
-    if (warp >= 4 && warp < 20) {
-        const int part = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, row = t.first + r, tok = p.by_group.of(row);
-        const size_t from = (size_t)(s.first + tok) * p.q_stride + (size_t)(hk * p.group + row - tok * p.group) * HD + part * NQ;
-        const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_Q + (uint32_t)(part * NQ / 2);
-        if constexpr (!TWO) {
-            uint32_t u[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) u[j] = 0u;
-            if (r < t.n_rows) {
-                const uint4 * at = reinterpret_cast<const uint4 *>((const __half *)p.q + from);
-#pragma unroll
-                for (int j = 0; j < NQ / 8; j++) { const uint4 v = __ldg(at + j); u[4 * j] = v.x; u[4 * j + 1] = v.y; u[4 * j + 2] = v.z; u[4 * j + 3] = v.w; }
-            }
-            // a value that is not finite: the row's scores are no numbers (an infinity alone may make them all the lowest value, as if the row saw nothing)
-            const __half2 none = __floats2half2_rn(0.f, 0.f);
-            __half2 zero[4] = {none, none, none, none};
-#pragma unroll
-            for (int j = 0; j < NQ / 2; j++) zero[j & 3] = __hfma2(*reinterpret_cast<const __half2 *>(&u[j]), none, zero[j & 3]);
-            if (!__hbeq2(__hadd2(__hadd2(zero[0], zero[1]), __hadd2(zero[2], zero[3])), none)) u[0] = 0x7fff7fffu;
-            if (p.scale_log2 < 0.f) {                                 // (the factor of the scores is positive: maxima stay maxima)
-#pragma unroll
-                for (int j = 0; j < 16; j++) u[j] ^= 0x80008000u;
-            }
-            if (part == 0) s_f[r] = fabsf(p.scale_log2);
-            tc_put<NQ / 2>(to, u);
-            tc_wait_st();
-        } else {
-            float4 v[NQ / 4];
-            float m = 0.f;
-#pragma unroll
-            for (int j = 0; j < NQ / 4; j++) {
-                v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < t.n_rows) v[j] = __ldg(reinterpret_cast<const float4 *>((const float *)p.q + from) + j);
-            }
-#pragma unroll
-            for (int j = 0; j < NQ / 4; j++) m = fmaxf(fmaxf(m, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
-            s_max[part >> 1][part & 1][r] = m;
-            asm volatile("bar.sync 3, 512;" ::: "memory");
-            m = fmaxf(fmaxf(s_max[0][0][r], s_max[0][1][r]), fmaxf(s_max[1][0][r], s_max[1][1][r]));
-            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25
-            const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
-            if (part == 0) s_f[r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) hi[j] = lo[j] = 0u;
-#pragma unroll
-            for (int j = 0; j < NQ / 4; j++) {
-                aq_split(v[j].x * up, v[j].y * up, hi[2 * j], lo[2 * j]);
-                aq_split(v[j].z * up, v[j].w * up, hi[2 * j + 1], lo[2 * j + 1]);
-            }
-            tc_put<NQ / 2>(to, hi);
-            tc_put<NQ / 2>(to + HD / 2, lo);
-            tc_wait_st();
-        }
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-
-    float top = -INFINITY, sum = 0.f;                                 // of a draining thread's row
-    float acc[HD / 2];
-#pragma unroll
-    for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PT_REGS_M));
         if (warp == 0) {
-            // ============================================================= products
-            constexpr uint32_t idesc_v = tc_idesc(NV, true);
-            const int tiles = __shfl_sync(0xffffffffu, n_tiles, 0), span = __shfl_sync(0xffffffffu, k1 - k0, 0);      // (uniform for the compiler)
+            // ============================================================= scores
             bool ok = true;
-            auto scores = [&](int i) {
-                const int b = i & 1, n = min(PT_KEYS, (span - i * PT_KEYS + 15) / 16 * 16), slot = 2 * i % NS;
-                ok = wait(s_full + slot, 2 * i / NS & 1) && ok;
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t idesc = tc_idesc(n, false), d = tmem + T_S + (uint32_t)(b * PT_KEYS);
-                const uint64_t k = tc_desc_k(ring + (uint32_t)slot * TILE);
-                if (TWO) {
-#pragma unroll
-                    for (int j = 0; j < KS; j++) tc_mma_f16_ta(d, tmem + T_Q + HD / 2 + 8 * j, k + (j >> 2) * (PT_SUB >> 4) + 2 * (j & 3), idesc, j > 0);
-                }
-#pragma unroll
-                for (int j = 0; j < KS; j++) tc_mma_f16_ta(d, tmem + T_Q + 8 * j, k + (j >> 2) * (PT_SUB >> 4) + 2 * (j & 3), idesc, TWO || j > 0);
-                tc_commit(s_empty + slot);
-                tc_commit(s_qk + b);
-            };
-            if (tiles > 0) scores(0);
-            if (tiles > 1) scores(1);
-            for (int i = 0; i < tiles && ok; i++) {
-                const int b = i & 1, steps = min(PT_KEYS / 16, (span - i * PT_KEYS + 15) / 16), slot = (2 * i + 1) % NS;
-                ok = wait(s_vok + (slot >> 1), (2 * i + 1) / NS & 1) && ok;
-                ok = wait(s_pfull + b, i >> 1 & 1) && ok;             // (the sums before are drained too)
+            PtRing work(s_wfull), qs(s_qfull), buf(s_qk), slot_k(s_full);
+            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_empty), qempty = smem_u32(s_qempty);
+            int g = 0;                                                // tiles in all
+            for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
+                ok = wait_at(work.here(), work.parity);
                 if (!ok) break;
-                tc_fence_after();
-                const uint32_t a = tmem + T_S + (uint32_t)(b * PT_KEYS), d = tmem + T_O;
-                const uint64_t v = tc_desc_mn(ring + (uint32_t)slot * TILE, PT_SUB);
-                if (steps == PT_KEYS / 16) {
-                    if (TWO) {
+                const int tiles = __shfl_sync(0xffffffffu, s_work[work.at].tiles, 0), span = __shfl_sync(0xffffffffu, s_work[work.at].k1 - s_work[work.at].k0, 0);      // (uniform for the compiler)
+                if (tiles < 0) break;
+                if (tiles > 0) {
+                    ok = wait_at(qs.here(), qs.parity);
+                    const uint64_t q = tc_desc_k(queries + qs.at * Z::QUERIES);
+                    for (int i = 0, left = span; i < tiles && ok; i++, g++, left -= PT_KEYS) {
+                        const uint32_t idesc = tc_idesc(left >= PT_KEYS ? PT_KEYS : (left + 15) / 16 * 16, false), d = tmem + T_S + buf.at * PT_KEYS;
+                        const uint64_t k = tc_desc_k(ring + slot_k.at * TILE);
+                        if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1);       // the buffer's probabilities have been used
+                        ok = wait_at(slot_k.here(), slot_k.parity) && ok;
+                        if (!ok) break;
+                        tc_fence_after();
+                        // (lower halves of the queries first)
+#pragma unroll 1
+                        for (int low = TWO ? 1 : 0; low >= 0; low--) {
 #pragma unroll
-                        for (int j = 0; j < PT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
+                            for (int c = 0; c < SUBS; c++) {
+                                const uint64_t at = q + (uint64_t)low * (TILE >> 4) + c * (PT_SUB >> 4);
+                                if (KS - 4 * c >= 4) pt_scores<4>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
+                                else                 pt_scores<2>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
+                            }
+                        }
+                        pt_commit(buf.here());
+                        if (lane == 0) pt_arrive(buf.here());         // (what this warp has seen others write is seen by whoever waits)
+                        __syncwarp();
+                        pt_commit(empty + slot_k.at * 8);
+                        if (i + 1 == tiles) pt_commit(qempty + qs.at * 8);
+                        buf.template step<PT_GROUPS>();
+                        // (the order of the ring: keys of two tiles, then keys of one more and values of the first that is left, in turn)
+                        slot_k.template step<NS>();
+                        if (g >= PT_AHEAD) slot_k.template step<NS>();
                     }
-#pragma unroll
-                    for (int j = 0; j < PT_KEYS / 16; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO || j > 0);
-                } else {
-                    if (TWO) for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + 8), v + 128 * j, idesc_v, j > 0);
-                    for (int j = 0; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16), v + 128 * j, idesc_v, TWO || j > 0);
+                    qs.template step<QB>();
                 }
-                tc_commit(s_empty + slot);
-                tc_commit(s_pv + b);
-                if (i + 2 < tiles) scores(i + 2);
+                if (ok) done_with(n);
             }
-            tc_commit(&s_fin);                                        // nothing is in flight when tensor memory is given back
-            for (int spins = 0; spins < (1 << 20) && !mbar_try_wait(&s_fin, 0u); spins++) {}
-            __syncwarp();
+            tc_commit(s_fin);                                         // nothing is in flight when tensor memory is given back
+            wait(s_fin, 0u);
+        } else if (warp == 2) {
+            // ============================================================= sums of values
+            constexpr uint32_t idesc_v = tc_idesc(NV, true);
+            bool ok = true;
+            PtRing work(s_wfull), buf(s_pfull), checked(s_vok), sums(s_ofree), slot_v(s_full);
+            for (int i = 0; i < PT_AHEAD + 1; i++) slot_v.template step<NS>();
+            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_empty);
+            int g = 0;
+            for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
+                ok = wait_at(work.here(), work.parity);
+                if (!ok) break;
+                const int tiles = __shfl_sync(0xffffffffu, s_work[work.at].tiles, 0), span = __shfl_sync(0xffffffffu, s_work[work.at].k1 - s_work[work.at].k0, 0);
+                if (tiles < 0) break;
+                for (int i = 0, left = span; i < tiles; i++, g++, left -= PT_KEYS) {
+                    const uint32_t a = tmem + T_S + buf.at * PT_KEYS, d = tmem + T_O + sums.at * NV;
+                    const uint64_t v = tc_desc_mn(ring + slot_v.at * TILE, PT_SUB);
+                    ok = wait_at(checked.here(), checked.parity);
+                    if (g >= OB) ok = wait_at(sums.here(), sums.parity ^ 1) && ok;
+                    ok = wait_at(buf.here(), buf.parity) && ok;
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int steps = left >= PT_KEYS ? PT_KEYS / 16 : (left + 15) / 16;
+#pragma unroll 1
+                    for (int low = TWO ? 1 : 0; low >= 0; low--) {    // (lower halves of the probabilities first)
+                        int j = 0;
+#pragma unroll 1
+                        for (; j + 4 <= steps; j += 4) pt_values(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, (TWO && low == 0) || j > 0);
+#pragma unroll 1
+                        for (; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, (TWO && low == 0) || j > 0);
+                    }
+                    pt_commit(pv + buf.at * 8);
+                    pt_commit(empty + slot_v.at * 8);
+                    buf.template step<PT_GROUPS>();
+                    checked.template step<PT_INFO>();
+                    sums.template step<OB>();
+                    slot_v.template step<NS>();
+                    slot_v.template step<NS>();
+                }
+                if (ok) done_with(n);
+            }
+            tc_commit(s_fin + 1);
+            wait(s_fin + 1, 0u);
         } else if (warp == 1) {
-            // ============================================================= tiles
-            int n = min(NS, 2 * n_tiles);
-            for (; n < 2 * n_tiles; n++) {
-                if (!wait(s_empty + n % NS, n / NS & 1 ^ 1)) break;
-                ask(n);
+            // ============================================================= tiles, in the order in which they are used: keys are PT_AHEAD tiles ahead of values.  A lane takes a copy.
+            PtRing slot(s_full);
+            const uint32_t empty = smem_u32(s_empty);
+            int at = 0;                                               // copies of tiles in all
+            bool ok = true;
+            int kn = -1, ki = 0, kt = 0, kg = 0, vn = -1, vi = 0, vt = 0;       // piece, tile in it, its tiles, of keys and of values; tiles of keys in all
+            int y = -1, y0 = -1, y1 = -1, y2 = -1;                    // a lane's row in the pools (-1: not there) of the next tile of keys, and of the last three
+            auto look = [&](int n, int i) {
+                const PtWork * w = work_of(n);
+                const int j = w->k0 + i * PT_KEYS + lane * pp.box;
+                if (lane * pp.box >= PT_KEYS || j >= w->there) return -1;
+                const int page = page_of(p.c, w->s.sq, j >> p.c.shift);
+                return page < 0 ? -1 : ((page * p.c.H + w->hk) << p.c.shift) + (j & (p.c.page - 1));
+            };
+            auto ask = [&](const CUtensorMap * map, int row) {
+                const unsigned copies = __ballot_sync(0xffffffffu, row >= 0);
+                if (lane == 0) mbar_expect_tx(s_full + slot.at, (unsigned)__popc(copies) * SUBS * pp.box * 128u);
+                __syncwarp();
+                if (row >= 0) {
+#pragma unroll
+                    for (int u = 0; u < SUBS; u++) tma_tile(ring + slot.at * TILE + u * PT_SUB + (uint32_t)(lane * pp.box) * 128u, map, u * 64, row, s_full + slot.at);
+                }
+                __syncwarp();
+            };
+            while (ok) {
+                while (kt >= 0 && ki == kt) {                         // the next piece that has tiles; kt -1: there is none
+                    kn++;
+                    if (!(ok = wait(s_wfull + kn % PT_WORK, kn / PT_WORK & 1))) break;
+                    ki = 0; kt = work_of(kn)->tiles;
+                    if (kt > 0) y = look(kn, 0);
+                }
+                if (!ok) break;
+                y0 = y1; y1 = y2; y2 = y;
+                if (kt > 0) {
+                    const PtWork * w = work_of(kn);
+                    const int j0 = w->k0 + ki * PT_KEYS, of = __shfl_sync(0xffffffffu, y, (lane & 7) * 16 / pp.box);
+                    const uint32_t groups = __ballot_sync(0xffffffffu, lane < 8 && j0 + lane * 16 < w->there && of >= 0);
+                    if (lane == 0) s_info[kg % PT_INFO] = groups | (groups != 0xffu || j0 + PT_KEYS > w->clear ? 256u : 0u);
+                    if (at >= NS && !(ok = wait_at(empty + slot.at * 8, slot.parity ^ 1))) break;
+                    ask(&pp.m_k, y);
+                    ki++;
+                    if (ki < kt) y = look(kn, ki);
+                }                                                     // (no more keys: their places stay empty, and are not used again)
+                slot.template step<NS>(); at++; kg++;
+                if (kg <= PT_AHEAD) continue;
+                while (vt >= 0 && vi == vt) {
+                    if (vn >= 0) done_with(vn);
+                    vn++;
+                    if (!(ok = wait(s_wfull + vn % PT_WORK, vn / PT_WORK & 1))) break;
+                    vi = 0; vt = work_of(vn)->tiles;
+                }
+                if (!ok || vt < 0) break;
+                if (at >= NS && !(ok = wait_at(empty + slot.at * 8, slot.parity ^ 1))) break;
+                ask(&pp.m_v, y0);
+                vi++;
+                slot.template step<NS>(); at++;
             }
-            if (lane == 0) ring_land(s_full, n, NS);
+            if (!ok && lane == 0) ring_land(s_full, at, NS);          // (else all have been waited for)
             __syncwarp();
         } else {
             // ============================================================= special tiles' values
-            for (int i = 0; i < n_tiles; i++) {
-                const int n = 2 * i + 1, slot = n % NS;
-                const uint32_t groups = present(i);
-                if (!wait(s_full + slot, n / NS & 1)) break;
-                if (special(i, groups)) {
-                    const int j0 = k0 + i * PT_KEYS;
-                    for (int h = 0; h < 2; h++) {                     // rows 0 .. 31 and 64 .. 95, or the others
-                        const int r = h * 64 + (warp - 2) * 32 + lane;
-                        const bool there = groups >> (r >> 4) & 1 && j0 + r < t.there;
-                        bool odd = false;
-                        for (int u = 0; u < SUBS * 8; u++) {
-                            const uint32_t at = ring + (uint32_t)slot * TILE + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)r * 128u + (uint32_t)((u + lane) & 7) * 16u;
-                            uint32_t x[4] = {0u, 0u, 0u, 0u};
-                            bool bad = !there;
-                            if (there) {
-                                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+            int g = 0;
+            bool ok = true;
+            PtRing slot_v(s_full);
+            for (int i = 0; i < PT_AHEAD + 1; i++) slot_v.template step<NS>();
+            for (int n = 0; ok; n++) {
+                ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
+                if (!ok) break;
+                const PtWork * w = work_of(n);
+                const int tiles = w->tiles, k0 = w->k0, there = w->there;
+                if (tiles < 0) break;
+                for (int i = 0; i < tiles; i++, g++) {
+                    if (!(ok = wait_at(slot_v.here(), slot_v.parity))) break;
+                    const uint32_t groups = s_info[g % PT_INFO], tile = ring + slot_v.at * TILE;
+                    slot_v.template step<NS>(); slot_v.template step<NS>();
+                    if (groups & 256u) {
+                        const int j0 = k0 + i * PT_KEYS;
+                        for (int h = 0; h < PT_ROWS / 32; h++) {      // a row a thread
+                            const int r = h * 32 + lane;
+                            const bool is = groups >> (r >> 4) & 1 && j0 + r < there;
+                            const uint32_t row = tile + (uint32_t)r * 128u;
+                            const __half2 none = __floats2half2_rn(0.f, 0.f);
+                            __half2 zero[4] = {none, none, none, none};          // no more 0 where a value is not finite
+                            if (is) {
+#pragma unroll 2
+                                for (int u = 0; u < SUBS * 8; u++) {
+                                    uint4 x;
+                                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u));
+                                    const __half2 * v = reinterpret_cast<const __half2 *>(&x);
 #pragma unroll
-                                for (int c = 0; c < 4; c++) {
-                                    if ((x[c] & 0x7c00u) == 0x7c00u) { bad = odd = true; x[c] &= 0xffff0000u; }
-                                    if ((x[c] & 0x7c000000u) == 0x7c000000u) { bad = odd = true; x[c] &= 0x0000ffffu; }
+                                    for (int c = 0; c < 4; c++) zero[c] = __hfma2(v[c], none, zero[c]);
                                 }
                             }
-                            if (bad) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+                            const bool odd = !__hbeq2(__hadd2(__hadd2(zero[0], zero[1]), __hadd2(zero[2], zero[3])), none);
+                            if (!is || odd) {                         // (the whole row: whoever sees it has no numbers)
+#pragma unroll 2
+                                for (int u = 0; u < SUBS * 8; u++)
+                                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u), "r"(0u) : "memory");
+                            }
+                            const uint32_t word = __ballot_sync(0xffffffffu, odd);
+                            if (lane == 0) s_odd[g % PT_INFO][h] = word;
                         }
-                        const uint32_t word = __ballot_sync(0xffffffffu, odd);
-                        if (lane == 0) s_odd[slot >> 1][h * 2 + warp - 2] = word;
+                        tc_fence_smem();
                     }
-                    tc_fence_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_vok + g % PT_INFO);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_vok + (slot >> 1));
+                if (ok) done_with(n);
             }
         }
-    } else if (warp < 20) {
-        // ================================================================= probabilities
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PT_REGS_S));
-        const int b = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, r = (warp & 3) * 32 + lane;
-        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * PT_KEYS + half * 64);
-        const bool idle = (warp & 3) * 32 >= t.n_rows;                // no rows: their probabilities may be anything
-        const int tok = r < t.n_rows ? p.by_group.of(t.first + r) : 0x7fffffff;
-        const float f = s_f[r];
-        uint32_t next = b < n_tiles ? present(b) : 0u;
-        for (int i = b; i < n_tiles; i += 2) {                        // (to the end whatever waits ran out: the halves meet at a barrier)
-            const uint32_t groups = next;
-            const bool masked = special(i, groups);
-            const int j0 = k0 + i * PT_KEYS + half * 64;
-            if (i + 2 < n_tiles) next = present(i + 2);
-            uint32_t sees[2] = {0xffffffffu, 0xffffffffu};
-            if (masked && !idle) {
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const uint32_t g = groups >> (half * 4 + c * 2);
-                    sees[c] = ap_sees(p, s, tok, j0 + c * 32 - s.pos) & ((g & 1 ? 0x0000ffffu : 0u) | (g & 2 ? 0xffff0000u : 0u));
+    } else if (warp < 8) {
+        // ================================================================= work and its queries
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PT_REGS_Q));
+        int unit = blockIdx.x, u = 0;
+        bool ok = true;
+        for (int n = 0; ok; n++) {
+            if (warp == 4) {                                          // the next piece that has something to do
+                if (n >= PT_WORK && !(ok = wait(s_wempty + n % PT_WORK, n / PT_WORK & 1 ^ 1))) break;
+                PtWork w;
+                w.tiles = -1;
+                while (unit < pp.units) {
+                    const AqItem it = ap_item(p, unit);
+                    const int nth = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1, rt = p.row_tiles - 1 - it.rt;      // (the longest rows first)
+                    w.s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, it.entry);
+                    const TileP t = ap_tile(p, w.s, rt, PT_ROWS);
+                    w.k0 = it.split * p.split; w.k1 = it.split == it.n_splits - 1 ? t.seen : min(t.seen, w.k0 + p.split);
+                    w.first = t.first; w.n_rows = t.n_rows; w.hk = it.hk; w.there = t.there; w.dst = nth;
+                    w.clear = p.mask ? w.s.pos : w.s.pos + p.by_group.of(t.first) + 1;      // every row sees the slots before it
+                    if (t.n_rows > 0 && (w.k0 < w.k1 || it.split == 0)) w.tiles = w.k0 < w.k1 ? (w.k1 - w.k0 + PT_KEYS - 1) / PT_KEYS : 0;      // (split 0 answers for rows that see nothing)
+                    int then = 0;
+                    if (lane == 0) then = (int)gridDim.x + (int)atomicAdd(pp.next, 1u);
+                    unit = __shfl_sync(0xffffffffu, then, 0);
+                    if (w.tiles >= 0) break;
                 }
+                if (lane == 0) { *work_of(n) = w; mbar_arrive(s_wfull + n % PT_WORK); }
+                __syncwarp();
             }
-            const int parts = idle ? 0 : max(0, min(4, (k1 - j0 + 15) >> 4));      // of 16 slots: the products take no more
-            wait(s_qk + b, i >> 1 & 1);
-            tc_fence_after();
-            float m = -INFINITY;
+            ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
+            if (!ok) break;
+            const PtWork * w = work_of(n);
+            const int tiles = w->tiles;
+            if (tiles < 0) break;
+            if (tiles > 0) {
+                const int qb = u % QB, part = lane & 7, r0 = (warp - 4) * 4 + (lane >> 3);
+                const uint32_t to = queries + (uint32_t)qb * Z::QUERIES;
+                const bool flip = p.scale_log2 < 0.f;                 // (the factor of the scores is positive: maxima stay maxima)
+                // Eight threads take a row, and have AT rows each on their way at a time.  The first ones are asked for before the buffer is free.
+                constexpr int AT = TWO ? 1 : 2, N = TWO ? HD / 32 : (HD / 8 + 7) / 8;
+                uint4 x[AT][N];
+                auto load = [&](int i) {
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                if (2 * c >= parts) break;
-                float x[32];
-                tc_ld32(x, mine + 32 * c);
-                if (masked) {
+                    for (int k = 0; k < AT; k++) {
+                        const int r = r0 + (i + k) * 16, row = w->first + r, tok = p.by_group.of(row);
+                        const bool there = r < w->n_rows;
+                        const size_t from = (size_t)(w->s.first + tok) * p.q_stride + (size_t)(w->hk * p.group + row - tok * p.group) * HD;
+                        const uint4 * at = reinterpret_cast<const uint4 *>((const char *)p.q + from * (TWO ? 4 : 2)) + part;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) if (!(sees[c] >> j & 1)) x[j] = -INFINITY;
-                }
-                float a[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) a[j] = max3(x[j], x[4 + j], x[8 + j]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[12 + j], x[16 + j]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[20 + j], x[24 + j]);
-#pragma unroll
-                for (int j = 0; j < 4; j++) a[j] = fmaxf(a[j], x[28 + j]);
-                m = fmaxf(m, max3(a[0], a[1], fmaxf(a[2], a[3])));
-            }
-            s_max[b][half][r] = m;
-            asm volatile("bar.sync %0, 256;" :: "r"(1 + b) : "memory");
-            m = fmaxf(m, s_max[b][half ^ 1][r]);
-            const bool none = m == -INFINITY;
-            m = none ? -INFINITY : m * f;                             // (-infinity times a factor of 0 is no number)
-            const float2 ref = f2(none ? 14.f : 14.f - m), fc = f2(f);
-            float2 l[2] = {f2(0.f), f2(0.f)};
-            auto exps = [&](auto with_mask) {
-#pragma unroll 1
-                for (int c = 0; c < parts; c++) {
-                    float x[16];
-                    tc_ld16(x, mine + 16 * c);
-                    uint32_t hl[16];                                  // upper parts of 16 slots, then lower parts
-                    const uint32_t see = (c < 2 ? sees[0] : sees[1]) >> ((c & 1) * 16);
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float2 y = f2_fma(make_float2(x[j], x[j + 1]), fc, ref);
-                        float2 pr = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                        if (decltype(with_mask)::value) {
-                            if (!(see >> j & 1)) pr.x = 0.f;
-                            if (!(see >> (j + 1) & 1)) pr.y = 0.f;
+                        for (int j = 0; j < N; j++) {
+                            x[k][j] = make_uint4(0u, 0u, 0u, 0u);
+                            if (there && (j * 8 + part) * (TWO ? 4 : 8) < HD) x[k][j] = __ldg(at + j * 8);
                         }
-                        l[j >> 1 & 1] = f2_add(l[j >> 1 & 1], pr);
-                        if constexpr (TWO) f2_split(pr, hl[j / 2], hl[8 + j / 2]);
-                        else               hl[j / 2] = h2u(__floats2half2_rn(pr.x, pr.y));
                     }
-                    if constexpr (TWO) tc_st16(mine + 16 * c, hl); else tc_put<8>(mine + 16 * c, hl);
+                };
+                load(0);
+                if (u >= QB && !(ok = wait(s_qempty + qb, u / QB & 1 ^ 1))) break;
+                u++;
+#pragma unroll 1
+                for (int i = 0; i < PT_ROWS / 16; i += AT) {
+                    uint4 y[AT][N];
+#pragma unroll
+                    for (int k = 0; k < AT; k++)
+#pragma unroll
+                        for (int j = 0; j < N; j++) y[k][j] = x[k][j];
+                    if (i + AT < PT_ROWS / 16) load(i + AT);
+#pragma unroll
+                    for (int k = 0; k < AT; k++) {
+                        const int r = r0 + (i + k) * 16;
+                        // where the 8 columns of piece c of a row lie
+                        auto place = [&](int c) { return to + (uint32_t)(c >> 3) * PT_SUB + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) * 16); };
+                        if constexpr (!TWO) {
+                            // a value that is not finite: the row's scores are no numbers (an infinity alone may make them all the lowest value, as if the row saw nothing)
+                            const __half2 none = __floats2half2_rn(0.f, 0.f);
+                            __half2 zero[N];
+#pragma unroll
+                            for (int j = 0; j < N; j++) {
+                                const __half2 * h = reinterpret_cast<const __half2 *>(&y[k][j]);
+                                zero[j] = __hfma2(h[0], none, __hfma2(h[1], none, __hfma2(h[2], none, __hmul2(h[3], none))));
+                            }
+                            bool odd = false;
+#pragma unroll
+                            for (int j = 0; j < N; j++) odd |= !__hbeq2(zero[j], none);
+                            if (odd) y[k][0].x = 0x7fff7fffu;
+                            const uint32_t sign = flip ? 0x80008000u : 0u;
+                            if (part == 0) s_f[n % PT_WORK][r] = fabsf(p.scale_log2);
+#pragma unroll
+                            for (int j = 0; j < N; j++) {
+                                const int c = j * 8 + part;
+                                if (c < HD / 8) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(place(c)), "r"(y[k][j].x ^ sign), "r"(y[k][j].y ^ sign), "r"(y[k][j].z ^ sign), "r"(y[k][j].w ^ sign) : "memory");
+                            }
+                        } else {
+                            float m = 0.f;
+                            auto value = [&](int j) { return make_float4(__uint_as_float(y[k][j].x), __uint_as_float(y[k][j].y), __uint_as_float(y[k][j].z), __uint_as_float(y[k][j].w)); };
+#pragma unroll
+                            for (int j = 0; j < N; j++) { const float4 v = value(j); m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w))); }
+#pragma unroll
+                            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25
+                            const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
+                            if (part == 0) s_f[n % PT_WORK][r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                            for (int j = 0; j < N; j++) {
+                                const float4 v = value(j);
+                                const uint32_t at = place((j * 8 + part) >> 1) + (uint32_t)(part & 1) * 8u;
+                                uint2 hi, lo;
+                                aq_split(v.x * up, v.y * up, hi.x, lo.x);
+                                aq_split(v.z * up, v.w * up, hi.y, lo.y);
+                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(at), "r"(hi.x), "r"(hi.y) : "memory");
+                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(at + TILE), "r"(lo.x), "r"(lo.y) : "memory");
+                            }
+                        }
+                    }
                 }
-            };
-            if (masked) exps(std::true_type()); else exps(std::false_type());
-            float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);
-            if (masked) {
-                const int slot = (2 * i + 1) % NS;
-                wait(s_vok + (slot >> 1), (2 * i + 1) / NS & 1);
-                if ((sees[0] & s_odd[slot >> 1][half * 2]) | (sees[1] & s_odd[slot >> 1][half * 2 + 1])) total = __int_as_float(0x7fc00000);
+                tc_fence_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_qfull + qb);
             }
-            if (none && (sees[0] | sees[1])) total = __int_as_float(0x7fc00000);         // (every score that it sees is -infinity)
-            if (i >= 2) wait(s_free + b, (i - 2) >> 1 & 1);           // the tile before has been drained: its sums are no more needed
-            s_sum[b][half][r] = total;
-            if (half == 0) s_top[b][r] = m;
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_pfull + b);
+            done_with(n);
+        }
+    } else if (warp < 8 + 4 * PT_GROUPS) {
+        // ================================================================= probabilities: a row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PT_REGS_S));
+        const int b = (warp - 8) >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * PT_KEYS);
+        const uint32_t qk = smem_u32(s_qk + b), stat = smem_u32(s_stat + b), pfull = smem_u32(s_pfull + b);
+        int g = 0, at = b;                                            // tiles in all; the group's next one
+        unsigned parity = 0;
+        bool ok = true;
+        for (int n = 0; ok; n++) {
+            ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
+            if (!ok) break;
+            const PtWork * w = work_of(n);
+            const int tiles = w->tiles, span = w->k1 - w->k0;
+            if (tiles < 0) break;
+            const bool idle = (warp & 3) * 32 >= w->n_rows;           // no rows: their probabilities may be anything
+            for (; at < g + tiles; at += PT_GROUPS, parity ^= 1) {
+                const int i = at - g;
+                if (!(ok = wait_at(qk, parity))) break;
+                tc_fence_after();
+                const uint32_t info = s_info[at % PT_INFO];
+                const bool masked = info & 256u;
+                const float f = fmaxf(s_f[n % PT_WORK][r], 0x1p-126f);            // (-infinity times 0 would be no number)
+                uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                if (masked && !idle) {
+                    ap_sees128(p, w->s, r < w->n_rows ? p.by_group.of(w->first + r) : 0x7fffffff, w->k0 + i * PT_KEYS - w->s.pos, sees);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sees[c] &= ((info >> (2 * c) & 1 ? 0x0000ffffu : 0u) | (info >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
+                }
+                const int chunks = idle ? 0 : min(4, (span - i * PT_KEYS + 31) >> 5);         // of 32 slots
+                float m = -INFINITY;
+                // (the scores of slots that a row does not see are put back as -infinity: their probabilities are 0)
+                auto largest = [&](auto with_mask) {
+#pragma unroll 1
+                    for (int c = 0; c < chunks; c++) {
+                        float x[32];
+                        tc_ld32(x, mine + 32 * c);
+                        if (decltype(with_mask)::value) {
+                            const uint32_t see = c == 0 ? sees[0] : c == 1 ? sees[1] : c == 2 ? sees[2] : sees[3];
+#pragma unroll
+                            for (int j = 0; j < 32; j++) if (!(see >> j & 1)) x[j] = -INFINITY;
+                            tc_st32(mine + 32 * c, x);
+                        }
+                        float a[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) a[j] = max3(x[j], x[4 + j], x[8 + j]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[12 + j], x[16 + j]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[20 + j], x[24 + j]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) a[j] = fmaxf(a[j], x[28 + j]);
+                        m = fmaxf(m, max3(a[0], a[1], fmaxf(a[2], a[3])));
+                    }
+                };
+                if (masked) { largest(std::true_type()); tc_wait_st(); } else largest(std::false_type());
+                const bool none = m == -INFINITY;
+                m *= f;
+                const float2 ref = f2(none ? 14.f : 14.f - m), fc = f2(f);
+                float2 l[2] = {f2(0.f), f2(0.f)};
+#pragma unroll 1
+                for (int c = 0; c < chunks; c++) {
+                    float x[32];
+                    tc_ld32(x, mine + 32 * c);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t hl[16];                              // upper parts of 16 slots, then lower parts
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const float2 y = f2_fma(make_float2(x[h * 16 + j], x[h * 16 + j + 1]), fc, ref), pr = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                            l[j >> 1 & 1] = f2_add(l[j >> 1 & 1], pr);
+                            if constexpr (TWO) f2_split(pr, hl[j / 2], hl[8 + j / 2]);
+                            else               hl[j / 2] = h2u(__floats2half2_rn(pr.x, pr.y));
+                        }
+                        if constexpr (TWO) tc_st16(mine + 32 * c + 16 * h, hl); else tc_put<8>(mine + 32 * c + 16 * h, hl);
+                    }
+                }
+                float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);
+                if (masked) {
+                    if (!(ok = wait(s_vok + at % PT_INFO, at / PT_INFO & 1))) break;
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) odd |= sees[c] & s_odd[at % PT_INFO][c];
+                    if (odd) total = __int_as_float(0x7fc00000);
+                }
+                if (none && (sees[0] | sees[1] | sees[2] | sees[3])) total = __int_as_float(0x7fc00000);         // (every score that it sees is -infinity)
+                if (at >= PT_GROUPS && !(ok = wait_at(stat, parity ^ 1))) break;                // what was there before has been read
+                s_sum[b][r] = total;
+                s_top[b][r] = m;
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) pt_arrive(pfull);
+            }
+            g += tiles;
+            if (ok) done_with(n);
         }
     } else {
         // ================================================================= sums out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PT_REGS_D));
         const int r = (warp & 3) * 32 + lane, d0 = warp >= 24 ? HD / 2 : 0;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_O + (uint32_t)d0;
+        PtRing buf(s_pfull), sums(s_ofree);
+        const uint32_t pv = smem_u32(s_pv), stat = smem_u32(s_stat);
         bool ok = true;
-        if (lane == 0) mbar_arrive(s_pfull);                          // (no sums before the first tile's)
-        for (int i = 0; i < n_tiles && ok; i++) {
-            const int b = i & 1;
-            ok = wait(s_pfull + b, i >> 1 & 1) && ok;
-            const float m = s_top[b][r], now = fmaxf(top, m);
-            const float was = top == now ? 1.f : exp2_approx(top - now), is = m == -INFINITY ? 0.f : exp2_approx(m - now);
-            top = now;
-            sum = fmaf(sum, was, (s_sum[b][0][r] + s_sum[b][1][r]) * is);
-            ok = wait(s_pv + b, i >> 1 & 1) && ok;
-            tc_fence_after();
+        for (int n = 0; ; n++) {
+            // (after a wait that ran out: the rows of the work in hand are no numbers)
+            if (ok) ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
+            else if (!__all_sync(0xffffffffu, mbar_try_wait(s_wfull + n % PT_WORK, n / PT_WORK & 1))) break;
+            if (!ok && !__all_sync(0xffffffffu, mbar_try_wait(s_wfull + n % PT_WORK, n / PT_WORK & 1))) break;
+            const PtWork * w = work_of(n);
+            const int tiles = w->tiles;
+            if (tiles < 0) break;
+            float top = -INFINITY, sum = 0.f;
+            float acc[HD / 2];
 #pragma unroll
-            for (int c = 0; c < HD / 2; c += 16) {
-                float v[16];
-                tc_ld16(v, mine + c);
-                if (c + 16 == HD / 2) {                               // the buffer goes back
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) { mbar_arrive(s_free + b); mbar_arrive(s_pfull + (b ^ 1)); }
-                }
+            for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
+            for (int i = 0; i < tiles && ok; i++) {
+                const int b = buf.at;
+                ok = wait_at(buf.here(), buf.parity);
+                const float m = s_top[b][r], of = s_sum[b][r], now = fmaxf(top, m);
+                __syncwarp();
+                if (lane == 0) pt_arrive(stat + b * 8);
+                const float was = top == now ? 1.f : exp2_approx(top - now), is = m == -INFINITY ? 0.f : exp2_approx(m - now);
+                top = now;
+                sum = fmaf(sum, was, of * is);
+                ok = wait_at(pv + b * 8, buf.parity) && ok;
+                tc_fence_after();
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float2 o = f2_fma(make_float2(v[j], v[j + 1]), f2(is), f2_mul(make_float2(acc[c + j], acc[c + j + 1]), f2(was)));
-                    acc[c + j] = o.x; acc[c + j + 1] = o.y;
-                }
-            }
-        }
-        if (r < t.n_rows) {
-            const int row = t.first + r, of = p.by_group.of(row), h = hk * p.group + row - of * p.group;
-            if (of >= p.c.n_ctx - s.pos) {                            // a token without a slot of its own
-                top = -INFINITY; sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
-            }
-            if (!ok || s_dead) sum = __int_as_float(0x7fc00000);      // a wait ran out, here or in a warp that came to s_pfull all the same: no numbers instead of wrong ones
-            if (w.n_splits > 1) {
-                const size_t at = ((size_t)(w.item - p.whole) * p.n_splits + split) * PT_ROWS + r;
-#pragma unroll
-                for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>(p.part + at * HD + d0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-                if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
-            } else {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const size_t at = (size_t)(s.first + of) * p.out_stride + (size_t)h * HD + d0;
-                if (p.xtype == PI_TYPE_F16) {
-#pragma unroll
-                    for (int j = 0; j < HD / 2; j += 8) {
-                        uint4 u;
-                        u.x = h2u(__floats2half2_rn(acc[j] * inv, acc[j + 1] * inv)); u.y = h2u(__floats2half2_rn(acc[j + 2] * inv, acc[j + 3] * inv));
-                        u.z = h2u(__floats2half2_rn(acc[j + 4] * inv, acc[j + 5] * inv)); u.w = h2u(__floats2half2_rn(acc[j + 6] * inv, acc[j + 7] * inv));
-                        *reinterpret_cast<uint4 *>((__half *)p.out + at + j) = u;
+                for (int c = 0; c < HD / 2; c += 8) {
+                    float v[8];
+                    tc_ld8(v, mine + sums.at * NV + c);
+                    if (c + 8 == HD / 2) {                           // the buffer goes back
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) pt_arrive(sums.here());
                     }
-                } else {
 #pragma unroll
-                    for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>((float *)p.out + at + j) = make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
+                    for (int j = 0; j < 8; j += 2) {
+                        const float2 o = f2_fma(make_float2(v[j], v[j + 1]), f2(is), f2_mul(make_float2(acc[c + j], acc[c + j + 1]), f2(was)));
+                        acc[c + j] = o.x; acc[c + j + 1] = o.y;
+                    }
+                }
+                buf.template step<PT_GROUPS>();
+                sums.template step<OB>();
+            }
+            if (r < w->n_rows) {
+                const int row = w->first + r, of = p.by_group.of(row), h = w->hk * p.group + row - of * p.group;
+                if (of >= p.c.n_ctx - w->s.pos) {                     // a token without a slot of its own
+                    top = -INFINITY; sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
+                }
+                if (!ok || s_dead) sum = __int_as_float(0x7fc00000);  // a wait ran out, here or in a warp that came to s_pfull all the same: no numbers instead of wrong ones
+                if (w->dst >= 0) {
+                    const size_t at = (size_t)w->dst * PT_ROWS + r;
+#pragma unroll
+                    for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>(p.part + at * HD + d0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                    if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
+                } else {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const size_t at = (size_t)(w->s.first + of) * p.out_stride + (size_t)h * HD + d0;
+                    if constexpr (!TWO) {
+#pragma unroll
+                        for (int j = 0; j < HD / 2; j += 8) {
+                            uint4 u;
+                            u.x = h2u(__floats2half2_rn(acc[j] * inv, acc[j + 1] * inv)); u.y = h2u(__floats2half2_rn(acc[j + 2] * inv, acc[j + 3] * inv));
+                            u.z = h2u(__floats2half2_rn(acc[j + 4] * inv, acc[j + 5] * inv)); u.w = h2u(__floats2half2_rn(acc[j + 6] * inv, acc[j + 7] * inv));
+                            *reinterpret_cast<uint4 *>((__half *)p.out + at + j) = u;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>((float *)p.out + at + j) = make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
+                    }
                 }
             }
+            if (ok) done_with(n);
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 0) tc_dealloc(s_tmem, 512);
+    if (tid == 0 && s_dead) atomicOr(p.status, 16u);
 }
 
-// Clears the status word in front of the kernel: no CTA of its own can, as another one's wait may have run out by then.
-__global__ void k_attn_paged_clear(unsigned int * status) {
+// Clears the status word and the number of the next piece of work in front of the kernel: no CTA of its own can, as another one may have been at them by then.
+__global__ void k_attn_paged_clear(unsigned int * status, unsigned int * next) {
     pdl_launch();
     pdl_wait();
-    if (threadIdx.x == 0) *status = 0u;
+    if (threadIdx.x == 0) { *status = 0u; *next = 0u; }
 }
 
 bool attn_paged_tc_takes(int hd, int64_t rows) { return hd <= 128 && rows > 16; }
 
 template <int HD, bool TWO>
 static int pt_go(const AttnPagedP & a, cudaStream_t st) {
-    constexpr int SUBS = (HD + 63) / 64;
-    constexpr size_t smem = (size_t)(HD <= 64 ? 12 : 6) * SUBS * PT_SUB + 1024;
+    constexpr size_t smem = PtShape<HD, TWO>::SMEM;
     static bool done[16] = {false};
     int dev = 0, rc;
     PI_CUDA(cudaGetDevice(&dev));
@@ -450,8 +666,10 @@ static int pt_go(const AttnPagedP & a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.c.n_pages * a.c.H * a.c.page;
     if ((rc = tensor_map(&p.m_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.k, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B)) ||
         (rc = tensor_map(&p.m_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.v, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-    PI_CUDA(launch_k(k_attn_paged_clear, dim3(1), dim3(32), 0, st, true, a.status));
-    PI_CUDA(launch_k(k_attn_paged_tc<HD, TWO>, dim3(ap_grid(a)), dim3(PT_THREADS), smem, st, true, p));
+    p.units = (int)ap_grid(a);
+    p.next = a.status + 8;
+    PI_CUDA(launch_k(k_attn_paged_clear, dim3(1), dim3(32), 0, st, true, a.status, p.next));
+    PI_CUDA(launch_k(k_attn_paged_tc<HD, TWO>, dim3((unsigned)(p.units < sm_count() ? p.units : sm_count())), dim3(PT_THREADS), smem, st, true, p));
     return PI_OK;
 }
 
