@@ -7,14 +7,14 @@
 // of ONE tile go to one or two more, which are drained and added with rounding in registers: the tensor cores cut FP32 sums at every step, so that no sum stays with them for longer
 // than a tile.  So every tile has its own maximum (no exchange between tiles; the score buffers are groups of warps' own): the drain joins tiles.
 //
-// A tile is special where not every row of the piece sees all of its slots: then a warp goes over its values before they are used.  Rows of slots that are not there
+// A tile is special where not every row of the piece sees all of its slots: then its group goes over its values before they are used.  Rows of slots that are not there
 // become zeros, rows with a value that is not finite too, and whoever sees such a slot has a row of no numbers; scores of slots that a row does not see are replaced by what its
 // mask says.
 //
 // Precision.  FP32 rows: queries and probabilities are the sum of two halves each, 22 bits, i.e. two products in the place of one.  FP16 rows: queries as they are, probabilities
 // one half, 11 bits like the result's own rounding.  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
 //
-// Warps: 0 issues the products of scores and 2 those of values; 1 asks for the tiles; 3 goes over special ones; 4..7 take work and lay out its queries; 8..19 have the
+// Warps: 0 issues the products of scores and 2 those of values; 1 asks for keys and 3 for values; 4..7 take work and lay out its queries; 8..19 have the
 // probabilities, three groups a tile each in turn, a row a thread; 20..27 drain the sums, a row and half of the columns a thread.
 #include "pi_attn_paged.cuh"
 #include "pi_tc.cuh"
@@ -30,8 +30,7 @@ static constexpr int PT_REGS_M = 40, PT_REGS_Q = 64, PT_REGS_S = 80, PT_REGS_D =
 static constexpr uint32_t PT_SUB = PT_KEYS * 128;                     // bytes of 64 columns of a tile
 static constexpr int PT_BOX = 64;                                     // rows of a tensor copy, or a page's if it has fewer
 static constexpr int PT_WORK = 4;                                     // pieces of work that a CTA has in hand
-static constexpr int PT_AHEAD = 2;                                    // tiles that keys are ahead of values in the ring
-static constexpr int PT_INFO = 8;                                     // tiles whose description is kept: more than the ring holds, whose tiles warps 1 to 3 may be ahead
+static constexpr int PT_INFO = 16;                                    // tiles whose description is kept: more than keys may be ahead of probabilities
 
 struct PtP { AttnPagedP a; int box, units; unsigned int * next; CUtensorMap m_k, m_v; };
 
@@ -39,7 +38,7 @@ struct PtP { AttnPagedP a; int box, units; unsigned int * next; CUtensorMap m_k,
 template <int HD, bool TWO> struct PtShape {
     static constexpr int SUBS = (HD + 63) / 64;
     static constexpr uint32_t TILE = SUBS * PT_SUB, QUERIES = TILE * (TWO ? 2 : 1);
-    static constexpr int QB = HD <= 64 ? 2 : 1, NS = (int)((196608u - QB * QUERIES) / TILE);
+    static constexpr int QB = HD <= 64 ? 2 : 1, NS = (int)((196608u - QB * QUERIES) / TILE), NK = NS / 2, NW = NS - NK;       // of keys, of values
     static constexpr size_t SMEM = QB * QUERIES + NS * TILE + 1024;
 };
 
@@ -94,30 +93,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     using Z = PtShape<HD, TWO>;
     constexpr int KS = HD / 16, SUBS = Z::SUBS, NV = SUBS * 64;       // steps of 16 columns; pieces of 64 columns; columns of the sums (behind HD: zeros)
     constexpr uint32_t TILE = Z::TILE;
-    constexpr int NS = Z::NS, QB = Z::QB;
+    constexpr int NK = Z::NK, NW = Z::NW, QB = Z::QB;
     constexpr int OB = (512 - PT_GROUPS * PT_KEYS) / NV;              // buffers of sums
     constexpr uint32_t T_S = 0, T_O = PT_GROUPS * PT_KEYS;            // tensor memory: three buffers of scores, one or two of sums
-    static_assert(NS / 2 + 2 < PT_INFO && OB >= 1 && PT_REGS_M + PT_REGS_Q + PT_GROUPS * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
+    static_assert(NK + PT_GROUPS < PT_INFO && OB >= 1 && PT_REGS_M + PT_REGS_Q + PT_GROUPS * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
     const AttnPagedP & p = pp.a;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ uint64_t s_full[NS], s_empty[NS], s_vok[PT_INFO];
+    __shared__ uint64_t s_kfull[NK], s_kempty[NK], s_vfull[NW], s_vempty[NW];
     __shared__ uint64_t s_wfull[PT_WORK], s_wempty[PT_WORK], s_qfull[QB], s_qempty[QB];
-    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_ofree[OB], s_fin[2];
+    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_scan[PT_GROUPS], s_fin[2];
     __shared__ PtWork s_work[PT_WORK];
     __shared__ uint32_t s_tmem, s_info[PT_INFO];                      // of a tile: which groups of 16 slots are there; bit 8: special
     __shared__ volatile unsigned s_dead;
-    __shared__ uint32_t s_odd[PT_INFO][4];                            // slots of a special tile with a value that is not finite
+    __shared__ uint32_t s_odd[PT_GROUPS][4];                           // slots of a special tile with a value that is not finite
     __shared__ float s_f[PT_WORK][PT_ROWS];                           // factor of a row's scores
     __shared__ float s_top[PT_GROUPS][PT_ROWS], s_sum[PT_GROUPS][PT_ROWS];         // of a tile: maximum, sum of the probabilities
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = queries + QB * Z::QUERIES;
+    const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, keys = queries + QB * Z::QUERIES, values = keys + NK * TILE;
 
-    if (tid < NS) { mbar_init(s_full + tid, 1); mbar_init(s_empty + tid, 1); }
-    if (tid < PT_INFO) mbar_init(s_vok + tid, 1);
+    if (tid < NK) { mbar_init(s_kfull + tid, 1); mbar_init(s_kempty + tid, 1); }
+    if (tid < NW) { mbar_init(s_vfull + tid, 1); mbar_init(s_vempty + tid, 1); }
     if (tid < PT_WORK) { mbar_init(s_wfull + tid, 1); mbar_init(s_wempty + tid, PT_THREADS / 32); }
     if (tid < QB) { mbar_init(s_qfull + tid, 4); mbar_init(s_qempty + tid, 1); }
-    if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 4); mbar_init(s_stat + tid, 8); }
-    if (tid < OB) mbar_init(s_ofree + tid, 8);
+    if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 12); mbar_init(s_stat + tid, 8); mbar_init(s_scan + tid, 4); }
     if (tid < 2) mbar_init(s_fin + tid, 1);
     if (tid == 0) s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -140,8 +138,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
         if (warp == 0) {
             // ============================================================= scores
             bool ok = true;
-            PtRing work(s_wfull), qs(s_qfull), buf(s_qk), slot_k(s_full);
-            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_empty), qempty = smem_u32(s_qempty);
+            PtRing work(s_wfull), qs(s_qfull), buf(s_qk), slot_k(s_kfull);
+            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_kempty), qempty = smem_u32(s_qempty);
             int g = 0;                                                // tiles in all
             for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
                 ok = wait_at(work.here(), work.parity);
@@ -153,7 +151,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     const uint64_t q = tc_desc_k(queries + qs.at * Z::QUERIES);
                     for (int i = 0, left = span; i < tiles && ok; i++, g++, left -= PT_KEYS) {
                         const uint32_t idesc = tc_idesc(left >= PT_KEYS ? PT_KEYS : (left + 15) / 16 * 16, false), d = tmem + T_S + buf.at * PT_KEYS;
-                        const uint64_t k = tc_desc_k(ring + slot_k.at * TILE);
+                        const uint64_t k = tc_desc_k(keys + slot_k.at * TILE);
                         if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1);       // the buffer's probabilities have been used
                         ok = wait_at(slot_k.here(), slot_k.parity) && ok;
                         if (!ok) break;
@@ -174,9 +172,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                         pt_commit(empty + slot_k.at * 8);
                         if (i + 1 == tiles) pt_commit(qempty + qs.at * 8);
                         buf.template step<PT_GROUPS>();
-                        // (the order of the ring: keys of two tiles, then keys of one more and values of the first that is left, in turn)
-                        slot_k.template step<NS>();
-                        if (g >= PT_AHEAD) slot_k.template step<NS>();
+                        slot_k.template step<NK>();
                     }
                     qs.template step<QB>();
                 }
@@ -188,21 +184,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             // ============================================================= sums of values
             constexpr uint32_t idesc_v = tc_idesc(NV, true);
             bool ok = true;
-            PtRing work(s_wfull), buf(s_pfull), checked(s_vok), sums(s_ofree), slot_v(s_full);
-            for (int i = 0; i < PT_AHEAD + 1; i++) slot_v.template step<NS>();
-            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_empty);
-            int g = 0;
+            PtRing work(s_wfull), buf(s_pfull), slot_v(s_vfull);
+            const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_vempty);
+            unsigned ob = 0;                                          // buffer of sums
             for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
                 ok = wait_at(work.here(), work.parity);
                 if (!ok) break;
                 const int tiles = __shfl_sync(0xffffffffu, s_work[work.at].tiles, 0), span = __shfl_sync(0xffffffffu, s_work[work.at].k1 - s_work[work.at].k0, 0);
                 if (tiles < 0) break;
-                for (int i = 0, left = span; i < tiles; i++, g++, left -= PT_KEYS) {
-                    const uint32_t a = tmem + T_S + buf.at * PT_KEYS, d = tmem + T_O + sums.at * NV;
-                    const uint64_t v = tc_desc_mn(ring + slot_v.at * TILE, PT_SUB);
-                    ok = wait_at(checked.here(), checked.parity);
-                    if (g >= OB) ok = wait_at(sums.here(), sums.parity ^ 1) && ok;
-                    ok = wait_at(buf.here(), buf.parity) && ok;
+                for (int i = 0, left = span; i < tiles; i++, left -= PT_KEYS) {
+                    const uint32_t a = tmem + T_S + buf.at * PT_KEYS, d = tmem + T_O + ob * NV;
+                    const uint64_t v = tc_desc_mn(values + slot_v.at * TILE, PT_SUB);
+                    ok = wait_at(slot_v.here(), slot_v.parity);
+                    ok = wait_at(buf.here(), buf.parity) && ok;       // (the buffer of sums has been drained too)
                     if (!ok) break;
                     tc_fence_after();
                     const int steps = left >= PT_KEYS ? PT_KEYS / 16 : (left + 15) / 16;
@@ -217,125 +211,58 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     pt_commit(pv + buf.at * 8);
                     pt_commit(empty + slot_v.at * 8);
                     buf.template step<PT_GROUPS>();
-                    checked.template step<PT_INFO>();
-                    sums.template step<OB>();
-                    slot_v.template step<NS>();
-                    slot_v.template step<NS>();
+                    slot_v.template step<NW>();
+                    if (++ob == OB) ob = 0;
                 }
                 if (ok) done_with(n);
             }
             tc_commit(s_fin + 1);
             wait(s_fin + 1, 0u);
-        } else if (warp == 1) {
-            // ============================================================= tiles, in the order in which they are used: keys are PT_AHEAD tiles ahead of values.  A lane takes a copy.
-            PtRing slot(s_full);
-            const uint32_t empty = smem_u32(s_empty);
-            int at = 0;                                               // copies of tiles in all
-            bool ok = true;
-            int kn = -1, ki = 0, kt = 0, kg = 0, vn = -1, vi = 0, vt = 0;       // piece, tile in it, its tiles, of keys and of values; tiles of keys in all
-            int y = -1, y0 = -1, y1 = -1, y2 = -1;                    // a lane's row in the pools (-1: not there) of the next tile of keys, and of the last three
-            auto look = [&](int n, int i) {
-                const PtWork * w = work_of(n);
-                const int j = w->k0 + i * PT_KEYS + lane * pp.box;
-                if (lane * pp.box >= PT_KEYS || j >= w->there) return -1;
-                const int page = page_of(p.c, w->s.sq, j >> p.c.shift);
-                return page < 0 ? -1 : ((page * p.c.H + w->hk) << p.c.shift) + (j & (p.c.page - 1));
-            };
-            auto ask = [&](const CUtensorMap * map, int row) {
-                const unsigned copies = __ballot_sync(0xffffffffu, row >= 0);
-                if (lane == 0) mbar_expect_tx(s_full + slot.at, (unsigned)__popc(copies) * SUBS * pp.box * 128u);
-                __syncwarp();
-                if (row >= 0) {
-#pragma unroll
-                    for (int u = 0; u < SUBS; u++) tma_tile(ring + slot.at * TILE + u * PT_SUB + (uint32_t)(lane * pp.box) * 128u, map, u * 64, row, s_full + slot.at);
-                }
-                __syncwarp();
-            };
-            while (ok) {
-                while (kt >= 0 && ki == kt) {                         // the next piece that has tiles; kt -1: there is none
-                    kn++;
-                    if (!(ok = wait(s_wfull + kn % PT_WORK, kn / PT_WORK & 1))) break;
-                    ki = 0; kt = work_of(kn)->tiles;
-                    if (kt > 0) y = look(kn, 0);
-                }
-                if (!ok) break;
-                y0 = y1; y1 = y2; y2 = y;
-                if (kt > 0) {
-                    const PtWork * w = work_of(kn);
-                    const int j0 = w->k0 + ki * PT_KEYS, of = __shfl_sync(0xffffffffu, y, (lane & 7) * 16 / pp.box);
-                    const uint32_t groups = __ballot_sync(0xffffffffu, lane < 8 && j0 + lane * 16 < w->there && of >= 0);
-                    if (lane == 0) s_info[kg % PT_INFO] = groups | (groups != 0xffu || j0 + PT_KEYS > w->clear ? 256u : 0u);
-                    if (at >= NS && !(ok = wait_at(empty + slot.at * 8, slot.parity ^ 1))) break;
-                    ask(&pp.m_k, y);
-                    ki++;
-                    if (ki < kt) y = look(kn, ki);
-                }                                                     // (no more keys: their places stay empty, and are not used again)
-                slot.template step<NS>(); at++; kg++;
-                if (kg <= PT_AHEAD) continue;
-                while (vt >= 0 && vi == vt) {
-                    if (vn >= 0) done_with(vn);
-                    vn++;
-                    if (!(ok = wait(s_wfull + vn % PT_WORK, vn / PT_WORK & 1))) break;
-                    vi = 0; vt = work_of(vn)->tiles;
-                }
-                if (!ok || vt < 0) break;
-                if (at >= NS && !(ok = wait_at(empty + slot.at * 8, slot.parity ^ 1))) break;
-                ask(&pp.m_v, y0);
-                vi++;
-                slot.template step<NS>(); at++;
-            }
-            if (!ok && lane == 0) ring_land(s_full, at, NS);          // (else all have been waited for)
-            __syncwarp();
         } else {
-            // ============================================================= special tiles' values
-            int g = 0;
+            // ============================================================= tiles of keys (warp 1) and of values (warp 3): a lane takes a copy of 64 columns of a box's rows
+            const bool is_k = warp == 1;
+            const CUtensorMap * map = is_k ? &pp.m_k : &pp.m_v;
+            const uint32_t full = smem_u32(is_k ? s_kfull : s_vfull), empty = smem_u32(is_k ? s_kempty : s_vempty), lot = is_k ? keys : values;
+            const unsigned slots = is_k ? NK : NW;
+            const int box = SUBS == 2 ? lane >> 1 : lane, x = SUBS == 2 ? (lane & 1) * 64 : 0;
+            const bool mine = box * pp.box < PT_KEYS;
+            const uint32_t place = (uint32_t)(x >> 6) * PT_SUB + (uint32_t)(box * pp.box) * 128u;
+            unsigned slot = 0, parity = 0;
+            int at = 0;                                               // tiles in all
             bool ok = true;
-            PtRing slot_v(s_full);
-            for (int i = 0; i < PT_AHEAD + 1; i++) slot_v.template step<NS>();
             for (int n = 0; ok; n++) {
                 ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
                 if (!ok) break;
                 const PtWork * w = work_of(n);
-                const int tiles = w->tiles, k0 = w->k0, there = w->there;
+                const int tiles = w->tiles;
                 if (tiles < 0) break;
-                for (int i = 0; i < tiles; i++, g++) {
-                    if (!(ok = wait_at(slot_v.here(), slot_v.parity))) break;
-                    const uint32_t groups = s_info[g % PT_INFO], tile = ring + slot_v.at * TILE;
-                    slot_v.template step<NS>(); slot_v.template step<NS>();
-                    if (groups & 256u) {
-                        const int j0 = k0 + i * PT_KEYS;
-                        for (int h = 0; h < PT_ROWS / 32; h++) {      // a row a thread
-                            const int r = h * 32 + lane;
-                            const bool is = groups >> (r >> 4) & 1 && j0 + r < there;
-                            const uint32_t row = tile + (uint32_t)r * 128u;
-                            const __half2 none = __floats2half2_rn(0.f, 0.f);
-                            __half2 zero[4] = {none, none, none, none};          // no more 0 where a value is not finite
-                            if (is) {
-#pragma unroll 2
-                                for (int u = 0; u < SUBS * 8; u++) {
-                                    uint4 x;
-                                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u));
-                                    const __half2 * v = reinterpret_cast<const __half2 *>(&x);
-#pragma unroll
-                                    for (int c = 0; c < 4; c++) zero[c] = __hfma2(v[c], none, zero[c]);
-                                }
-                            }
-                            const bool odd = !__hbeq2(__hadd2(__hadd2(zero[0], zero[1]), __hadd2(zero[2], zero[3])), none);
-                            if (!is || odd) {                         // (the whole row: whoever sees it has no numbers)
-#pragma unroll 2
-                                for (int u = 0; u < SUBS * 8; u++)
-                                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u), "r"(0u) : "memory");
-                            }
-                            const uint32_t word = __ballot_sync(0xffffffffu, odd);
-                            if (lane == 0) s_odd[g % PT_INFO][h] = word;
-                        }
-                        tc_fence_smem();
+                auto look = [&](int i) {                              // this lane's row in the pool, -1: not there
+                    const int j = w->k0 + i * PT_KEYS + box * pp.box;
+                    if (!mine || j >= w->there) return -1;
+                    const int page = page_of(p.c, w->s.sq, j >> p.c.shift);
+                    return page < 0 ? -1 : ((page * p.c.H + w->hk) << p.c.shift) + (j & (p.c.page - 1));
+                };
+                int y = tiles > 0 ? look(0) : -1;
+                for (int i = 0; i < tiles; i++, at++) {
+                    const int row = y;
+                    const unsigned copies = __ballot_sync(0xffffffffu, row >= 0);
+                    if (is_k) {                                       // which groups of 16 slots are there; whether the tile is special
+                        const int j0 = w->k0 + i * PT_KEYS, of = (lane & 7) * 16 / pp.box * SUBS;
+                        const uint32_t groups = __ballot_sync(0xffffffffu, lane < 8 && j0 + lane * 16 < w->there && (copies >> of & 1));
+                        if (lane == 0) s_info[at % PT_INFO] = groups | (groups != 0xffu || j0 + PT_KEYS > w->clear ? 256u : 0u);
                     }
+                    if (at >= (int)slots && !(ok = wait_at(empty + slot * 8, parity ^ 1))) break;
+                    if (lane == 0) mbar_expect_tx((is_k ? s_kfull : s_vfull) + slot, (unsigned)__popc(copies) * pp.box * 128u);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(s_vok + g % PT_INFO);
+                    if (row >= 0) tma_tile(lot + slot * TILE + place, map, x, row, (is_k ? s_kfull : s_vfull) + slot);
+                    if (i + 1 < tiles) y = look(i + 1);
+                    __syncwarp();
+                    if (++slot == slots) { slot = 0; parity ^= 1; }
                 }
                 if (ok) done_with(n);
             }
+            if (!ok && lane == 0) ring_land(is_k ? s_kfull : s_vfull, at, (int)slots);          // (else all have been waited for)
+            __syncwarp();
         }
     } else if (warp < 8) {
         // ================================================================= work and its queries
@@ -462,7 +389,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_S + (uint32_t)(b * PT_KEYS);
         const uint32_t qk = smem_u32(s_qk + b), stat = smem_u32(s_stat + b), pfull = smem_u32(s_pfull + b);
         int g = 0, at = b;                                            // tiles in all; the group's next one
-        unsigned parity = 0;
+        unsigned parity = 0, scans = 0;                               // of the group's barriers; special tiles so far
         bool ok = true;
         for (int n = 0; ok; n++) {
             ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
@@ -534,11 +461,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);
                 if (masked) {
-                    if (!(ok = wait(s_vok + at % PT_INFO, at / PT_INFO & 1))) break;
-                    uint32_t odd = 0;
+                    // the tile's values: a row a thread.  Rows of slots that are not there become zeros; so do those with a value that is not finite, and who sees them has no numbers
+                    const int slot = at % NW;
+                    if (!(ok = wait(s_vfull + slot, at / NW & 1))) break;
+                    const bool is = info >> (r >> 4) & 1 && w->k0 + i * PT_KEYS + r < w->there;
+                    const uint32_t row = values + (uint32_t)slot * TILE + (uint32_t)r * 128u;
+                    const __half2 null = __floats2half2_rn(0.f, 0.f);
+                    __half2 zero[4] = {null, null, null, null};       // no more 0 where a value is not finite
+                    if (is) {
+#pragma unroll 2
+                        for (int u = 0; u < SUBS * 8; u++) {
+                            uint4 x;
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u));
+                            const __half2 * v = reinterpret_cast<const __half2 *>(&x);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) odd |= sees[c] & s_odd[at % PT_INFO][c];
-                    if (odd) total = __int_as_float(0x7fc00000);
+                            for (int c = 0; c < 4; c++) zero[c] = __hfma2(v[c], null, zero[c]);
+                        }
+                    }
+                    const bool odd = !__hbeq2(__hadd2(__hadd2(zero[0], zero[1]), __hadd2(zero[2], zero[3])), null);
+                    if (!is || odd) {
+#pragma unroll 2
+                        for (int u = 0; u < SUBS * 8; u++)
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u), "r"(0u) : "memory");
+                    }
+                    tc_fence_smem();
+                    const uint32_t word = __ballot_sync(0xffffffffu, odd);
+                    if (lane == 0) { s_odd[b][warp & 3] = word; mbar_arrive(s_scan + b); }
+                    if (!(ok = wait(s_scan + b, scans & 1))) break;   // the group's other warps have their words there
+                    scans++;
+                    uint32_t none_of = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) none_of |= sees[c] & s_odd[b][c];
+                    if (none_of) total = __int_as_float(0x7fc00000);
                 }
                 if (none && (sees[0] | sees[1] | sees[2] | sees[3])) total = __int_as_float(0x7fc00000);         // (every score that it sees is -infinity)
                 if (at >= PT_GROUPS && !(ok = wait_at(stat, parity ^ 1))) break;                // what was there before has been read
@@ -557,9 +511,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PT_REGS_D));
         const int r = (warp & 3) * 32 + lane, d0 = warp >= 24 ? HD / 2 : 0;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_O + (uint32_t)d0;
-        PtRing buf(s_pfull), sums(s_ofree);
-        const uint32_t pv = smem_u32(s_pv), stat = smem_u32(s_stat);
+        PtRing buf(s_pfull);
+        const uint32_t pfull = smem_u32(s_pfull), pv = smem_u32(s_pv), stat = smem_u32(s_stat);
+        unsigned ob = 0;                                              // buffer of sums
         bool ok = true;
+        if (lane == 0) for (int i = 0; i < OB; i++) pt_arrive(pfull + i * 8);       // (nothing to drain before the first tiles)
         for (int n = 0; ; n++) {
             // (after a wait that ran out: the rows of the work in hand are no numbers)
             if (ok) ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
@@ -586,11 +542,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
 #pragma unroll
                 for (int c = 0; c < HD / 2; c += 8) {
                     float v[8];
-                    tc_ld8(v, mine + sums.at * NV + c);
+                    tc_ld8(v, mine + ob * NV + c);
                     if (c + 8 == HD / 2) {                           // the buffer goes back
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) pt_arrive(sums.here());
+                        if (lane == 0) pt_arrive(pfull + (buf.at + OB >= PT_GROUPS ? buf.at + OB - PT_GROUPS : buf.at + OB) * 8);
                     }
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
@@ -599,7 +555,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     }
                 }
                 buf.template step<PT_GROUPS>();
-                sums.template step<OB>();
+                if (++ob == OB) ob = 0;
             }
             if (r < w->n_rows) {
                 const int row = w->first + r, of = p.by_group.of(row), h = w->hk * p.group + row - of * p.group;
