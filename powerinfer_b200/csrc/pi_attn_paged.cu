@@ -332,56 +332,85 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
     }
 }
 
-// The splits of a tile joined, in their order.  A CTA has one row: its groups of HD / 4 threads take splits in turn.
-static constexpr int PJ_THREADS = 128;
+// The parts of a tile joined, in their order.  A warp has a row: a lane finds the weight of one part, then all parts' sums come with PJ_AT of them on their way at once.
+static constexpr int PJ_WARPS = 8, PJ_AT = 4;
 
 template <int HD>
-__global__ void __launch_bounds__(PJ_THREADS) k_attn_paged_join(const AttnPagedP p, int R) {
-    constexpr int W = HD / 4, G = PJ_THREADS / W > 0 ? PJ_THREADS / W : 1;
-    __shared__ float4 s_v[G][W]; __shared__ float s_sum[G];
-    const int k = blockIdx.x / R, r = blockIdx.x - k * R, item = p.whole + k, d = threadIdx.x % W, gr = threadIdx.x / W;
+__global__ void __launch_bounds__(PJ_WARPS * 32) k_attn_paged_join(const AttnPagedP p, int R) {
+    constexpr int W = HD % 128 == 0 ? 4 : HD % 64 == 0 ? 2 : 1, N = HD / (32 * W);       // values of a lane side by side, and how often
+    const int lane = threadIdx.x & 31, at = blockIdx.x * PJ_WARPS + (threadIdx.x >> 5), k = at / R, r = at - k * R, item = p.whole + k;
     pdl_launch();
     pdl_wait();
+    if (item >= p.items) return;
     const int of_head = p.by_tiles.of(item), nt = item - of_head * p.row_tiles, rt = R == PT_ROWS ? p.row_tiles - 1 - nt : nt, entry = p.by_heads.of(of_head), hk = of_head - entry * p.c.H;
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, entry);
     const TileP t = ap_tile(p, s, rt, R);
     if (r >= t.n_rows) return;
     const int n = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));       // parts that were written
-    const size_t at0 = (size_t)k * p.n_splits * R + r;
-    float top = -INFINITY;
-    for (int i = 0; i < n; i++) top = fmaxf(top, __ldcg(&p.part_ml[at0 + (size_t)i * R]).x);
+    const size_t first = (size_t)k * p.n_splits * R + r;
+    float top = -INFINITY, sum = 0.f, v[N * W];
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(&p.part_ml[first + (size_t)i * R]).x);
+    top = warp_max(top);
     const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f; float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (gr < G) {
-        for (int i = gr; i < n; i += G) {
-            const float2 ml = __ldcg(&p.part_ml[at0 + (size_t)i * R]);
-            const float4 u = __ldcg(reinterpret_cast<const float4 *>(p.part + (at0 + (size_t)i * R) * HD) + d);
-            const float is = exp2_approx(ml.x - ref);
-            sum = fmaf(is, ml.y, sum);
-            v.x = fmaf(is, u.x, v.x); v.y = fmaf(is, u.y, v.y); v.z = fmaf(is, u.z, v.z); v.w = fmaf(is, u.w, v.w);
-        }
-        s_v[gr][d] = v;
-        if (d == 0) s_sum[gr] = sum;
-    }
-    __syncthreads();
-    if (gr > 0) return;
 #pragma unroll
-    for (int i = 1; i < G; i++) { const float4 u = s_v[i][d]; v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w; sum += s_sum[i]; }
+    for (int j = 0; j < N * W; j++) v[j] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        float is = 0.f;
+        if (i0 + lane < n) {
+            const float2 ml = __ldcg(&p.part_ml[first + (size_t)(i0 + lane) * R]);
+            is = exp2_approx(ml.x - ref);
+            sum = fmaf(is, ml.y, sum);
+        }
+        const int here = min(32, n - i0);
+        for (int i = 0; i < here; i += PJ_AT) {
+            float u[PJ_AT][N * W];
+#pragma unroll
+            for (int c = 0; c < PJ_AT; c++) {
+                const float * from = p.part + (first + (size_t)(i0 + min(i + c, here - 1)) * R) * HD + lane * W;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    if constexpr (W == 4)      { const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + j * 128)); u[c][4 * j] = x.x; u[c][4 * j + 1] = x.y; u[c][4 * j + 2] = x.z; u[c][4 * j + 3] = x.w; }
+                    else if constexpr (W == 2) { const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + j * 64)); u[c][2 * j] = x.x; u[c][2 * j + 1] = x.y; }
+                    else                       u[c][j] = __ldcg(from + j * 32);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < PJ_AT; c++) {
+                const float w = __shfl_sync(0xffffffffu, is, min(i + c, 31));
+                if (i + c >= here) break;
+#pragma unroll
+                for (int j = 0; j < N * W; j++) v[j] = fmaf(w, u[c][j], v[j]);
+            }
+        }
+    }
+    sum = warp_sum(sum);
     const int row = t.first + r, of = p.by_group.of(row), h = hk * p.group + row - of * p.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const size_t at = (size_t)(s.first + of) * p.out_stride + (size_t)h * HD + d * 4;
-    if (p.xtype == PI_TYPE_F16) *reinterpret_cast<uint2 *>((__half *)p.out + at) = make_uint2(h2u(__floats2half2_rn(v.x * inv, v.y * inv)), h2u(__floats2half2_rn(v.z * inv, v.w * inv)));
-    else                        *reinterpret_cast<float4 *>((float *)p.out + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    const size_t to = (size_t)(s.first + of) * p.out_stride + (size_t)h * HD + lane * W;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        if (p.xtype == PI_TYPE_F16) {
+            __half * o = (__half *)p.out + to + j * 32 * W;
+            if constexpr (W == 4)      *reinterpret_cast<uint2 *>(o) = make_uint2(h2u(__floats2half2_rn(v[4 * j] * inv, v[4 * j + 1] * inv)), h2u(__floats2half2_rn(v[4 * j + 2] * inv, v[4 * j + 3] * inv)));
+            else if constexpr (W == 2) *reinterpret_cast<uint32_t *>(o) = h2u(__floats2half2_rn(v[2 * j] * inv, v[2 * j + 1] * inv));
+            else                       *o = __float2half_rn(v[j] * inv);
+        } else {
+            float * o = (float *)p.out + to + j * 32 * W;
+            if constexpr (W == 4)      *reinterpret_cast<float4 *>(o) = make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+            else if constexpr (W == 2) *reinterpret_cast<float2 *>(o) = make_float2(v[2 * j] * inv, v[2 * j + 1] * inv);
+            else                       *o = v[j] * inv;
+        }
+    }
 }
 
 // ---- how the work is cut
-struct PaPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, ml, part; };
+struct PaPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, q, factor, ml, part; };
 
 // CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split into ranges of at least PA_LEAST
 // slots: into the number of parts for which its CTAs, in rounds of their own, take the least.  A CTA costs as much as its slots and PA_TURN times 64 more (on tcgen05 PA_TURN_TC), the kernel that joins as
 // PA_TURN times 64.
 static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 10, PA_ROUNDS = 4;
-static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int n_head, int max_kv) {
+static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_head, int max_kv) {
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
     r.tc = attn_paged_tc_takes(c.hd, rows);
@@ -404,13 +433,15 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int n_head, int max_
     auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
     r.ml = up((size_t)(items - r.whole) * r.n_splits * r.R * 8);
     r.part = up((size_t)(items - r.whole) * r.n_splits * r.R * c.hd * 4);
+    r.q = r.tc ? up((size_t)b.T * n_head * c.hd * (xtype == PI_TYPE_F16 ? 2 : 4)) : 0;
+    r.factor = r.tc && xtype == PI_TYPE_F32 ? up((size_t)b.T * n_head * 4) : 0;
     r.words = r.tc || r.ml + r.part ? 256 : 0;                                // (the status word where pi_op_status looks for it)
     return r;
 }
 
 size_t attn_paged_scratch(const KvPaged & c, const RaggedB & b, int xtype, int n_head, int max_kv) {
-    const PaPlan r = pa_plan(c, b, n_head, max_kv);
-    return r.words + r.ml + r.part;
+    const PaPlan r = pa_plan(c, b, xtype, n_head, max_kv);
+    return r.words + r.q + r.factor + r.ml + r.part;
 }
 
 template <int HD, bool TWO>
@@ -431,12 +462,12 @@ template <int HD>
 static int pa_run(const AttnPagedP & p, const PaPlan & r, cudaStream_t st) {
     const int rc = r.tc ? launch_attn_paged_tc(p, st) : p.xtype == PI_TYPE_F16 ? pa_go<HD, false>(p, st) : pa_go<HD, true>(p, st);
     if (rc) return rc;
-    if (p.items > p.whole) PI_CUDA(launch_k(k_attn_paged_join<HD>, dim3((unsigned)((p.items - p.whole) * r.R)), dim3(PJ_THREADS), 0, st, true, p, r.R));
+    if (p.items > p.whole) PI_CUDA(launch_k(k_attn_paged_join<HD>, dim3((unsigned)(((int64_t)(p.items - p.whole) * r.R + PJ_WARPS - 1) / PJ_WARPS)), dim3(PJ_WARPS * 32), 0, st, true, p, r.R));
     return PI_OK;
 }
 
 int launch_attention_paged(const AttnPagedArgs & a, cudaStream_t st) {
-    const PaPlan r = pa_plan(a.c, a.b, a.n_head, a.max_kv);
+    const PaPlan r = pa_plan(a.c, a.b, a.xtype, a.n_head, a.max_kv);
     AttnPagedP p;
     p.c = a.c; p.b = a.b; p.xtype = a.xtype; p.q = a.q; p.q_stride = a.q_stride; p.n_head = a.n_head; p.group = a.n_head / a.c.H;
     p.mask = a.mask; p.words = a.words;
@@ -446,6 +477,8 @@ int launch_attention_paged(const AttnPagedArgs & a, cudaStream_t st) {
     char * s = (char *)a.scratch;
     p.status = s ? (unsigned int *)(s + 8) : nullptr;
     s += r.words;
+    p.queries = (__half *)s; p.factor = (float *)(s + r.q);
+    s += r.q + r.factor;
     p.part_ml = (float2 *)s; p.part = (float *)(s + r.ml);
     switch (a.c.hd) {
         case 64:  return pa_run<64>(p, r, st);

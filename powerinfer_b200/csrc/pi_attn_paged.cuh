@@ -13,6 +13,7 @@ struct AttnPagedP {
     // An item is a tile of rows of a KV head of an entry.  The first `whole` items are a CTA each, the others n_splits: ranges of `split` slots.
     int split, n_splits, row_tiles, items, whole;
     AqDiv by_group, by_heads, by_tiles, by_splits;                    // the KV heads' number, row_tiles, n_splits
+    __half * queries; float * factor;                                 // tcgen05 alone: the queries as halves, the factors of their scores
     float * part; float2 * part_ml;                                   // [split item][split][R][hd], (max, sum) beside them
     unsigned int * status;                                            // (null: no workspace) tcgen05 alone: bit 4, a wait ran out; others clear it
 };

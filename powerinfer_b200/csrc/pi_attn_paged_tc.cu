@@ -26,13 +26,13 @@
 namespace pi {
 
 static constexpr int PT_THREADS = 896, PT_GROUPS = 3;                  // groups of warps with tiles of probabilities
-static constexpr int PT_REGS_M = 40, PT_REGS_Q = 64, PT_REGS_S = 80, PT_REGS_D = 80;  // 40 + 64 + 3 x 80 + 2 x 80 of the 7 x 72 of the launch
+static constexpr int PT_REGS_M = 40, PT_REGS_Q = 40, PT_REGS_S = 72, PT_REGS_D = 104;  // 40 + 40 + 3 x 72 + 2 x 104 of the 7 x 72 of the launch
 static constexpr uint32_t PT_SUB = PT_KEYS * 128;                     // bytes of 64 columns of a tile
 static constexpr int PT_BOX = 64;                                     // rows of a tensor copy, or a page's if it has fewer
 static constexpr int PT_WORK = 4;                                     // pieces of work that a CTA has in hand
 static constexpr int PT_INFO = 16;                                    // tiles whose description is kept: more than keys may be ahead of probabilities
 
-struct PtP { AttnPagedP a; int box, units; unsigned int * next; CUtensorMap m_k, m_v; };
+struct PtP { AttnPagedP a; int box, units, wide; unsigned int * next; CUtensorMap m_q, m_k, m_v; };
 
 // what is in shared memory besides the ring: queries' buffers (upper and, of FP32 rows, lower halves), tiles in the ring
 template <int HD, bool TWO> struct PtShape {
@@ -79,6 +79,9 @@ __device__ __forceinline__ void pt_values(uint32_t d, uint32_t a, uint64_t b, ui
                  " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n}"
                  :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
 }
+__device__ __forceinline__ void pt_store8(float * p, const float * v) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
 // A place in a ring of barriers, and the parity of its phase
 struct PtRing {
     uint32_t bar; unsigned at, parity;
@@ -94,7 +97,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     constexpr int KS = HD / 16, SUBS = Z::SUBS, NV = SUBS * 64;       // steps of 16 columns; pieces of 64 columns; columns of the sums (behind HD: zeros)
     constexpr uint32_t TILE = Z::TILE;
     constexpr int NK = Z::NK, NW = Z::NW, QB = Z::QB;
-    constexpr int OB = (512 - PT_GROUPS * PT_KEYS) / NV;              // buffers of sums
+    constexpr int OB = (512 - PT_GROUPS * PT_KEYS) / NV;              // buffers of sums.  (Two halves of 64 columns, of which one is drained while the other is made: products of 64 columns take as long as those of 128)
+    constexpr int DH = HD / 2, DC = HD == 96 ? 16 : 32;               // columns of a thread that drains, and at a time
     constexpr uint32_t T_S = 0, T_O = PT_GROUPS * PT_KEYS;            // tensor memory: three buffers of scores, one or two of sums
     static_assert(NK + PT_GROUPS < PT_INFO && OB >= 1 && PT_REGS_M + PT_REGS_Q + PT_GROUPS * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
     const AttnPagedP & p = pp.a;
@@ -106,15 +110,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     __shared__ uint32_t s_tmem, s_info[PT_INFO];                      // of a tile: which groups of 16 slots are there; bit 8: special
     __shared__ volatile unsigned s_dead;
     __shared__ uint32_t s_odd[PT_GROUPS][4];                           // slots of a special tile with a value that is not finite
-    __shared__ float s_f[PT_WORK][PT_ROWS];                           // factor of a row's scores
     __shared__ float s_top[PT_GROUPS][PT_ROWS], s_sum[PT_GROUPS][PT_ROWS];         // of a tile: maximum, sum of the probabilities
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, keys = queries + QB * Z::QUERIES, values = keys + NK * TILE;
 
     if (tid < NK) { mbar_init(s_kfull + tid, 1); mbar_init(s_kempty + tid, 1); }
     if (tid < NW) { mbar_init(s_vfull + tid, 1); mbar_init(s_vempty + tid, 1); }
-    if (tid < PT_WORK) { mbar_init(s_wfull + tid, 1); mbar_init(s_wempty + tid, PT_THREADS / 32); }
-    if (tid < QB) { mbar_init(s_qfull + tid, 4); mbar_init(s_qempty + tid, 1); }
+    if (tid < PT_WORK) { mbar_init(s_wfull + tid, 1); mbar_init(s_wempty + tid, PT_THREADS / 32 - 3); }
+    if (tid < QB) { mbar_init(s_qfull + tid, 1); mbar_init(s_qempty + tid, 1); }
     if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 12); mbar_init(s_stat + tid, 8); mbar_init(s_scan + tid, 4); }
     if (tid < 2) mbar_init(s_fin + tid, 1);
     if (tid == 0) s_dead = 0;
@@ -124,9 +127,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    if (tid == 32) { tma_map(&pp.m_k); tma_map(&pp.m_v); }
+    if (tid == 32) { tma_map(&pp.m_q); tma_map(&pp.m_k); tma_map(&pp.m_v); }
     pdl_launch();
     pdl_wait();
+    asm volatile("fence.proxy.async;" ::: "memory");                // (what kernels before wrote is read by tensor copies)
     const uint32_t dead = smem_u32((const void *)&s_dead);
     auto wait_at = [&](uint32_t bar, unsigned parity) { return pt_wait(bar, parity, dead); };      // warp-uniform; false: the wait ran out, here or elsewhere in the CTA
     auto wait = [&](uint64_t * bar, unsigned parity) { return wait_at(smem_u32(bar), parity); };
@@ -195,11 +199,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 for (int i = 0, left = span; i < tiles; i++, left -= PT_KEYS) {
                     const uint32_t a = tmem + T_S + buf.at * PT_KEYS, d = tmem + T_O + ob * NV;
                     const uint64_t v = tc_desc_mn(values + slot_v.at * TILE, PT_SUB);
+                    const int steps = left >= PT_KEYS ? PT_KEYS / 16 : (left + 15) / 16;
                     ok = wait_at(slot_v.here(), slot_v.parity);
                     ok = wait_at(buf.here(), buf.parity) && ok;       // (the buffer of sums has been drained too)
                     if (!ok) break;
                     tc_fence_after();
-                    const int steps = left >= PT_KEYS ? PT_KEYS / 16 : (left + 15) / 16;
 #pragma unroll 1
                     for (int low = TWO ? 1 : 0; low >= 0; low--) {    // (lower halves of the probabilities first)
                         int j = 0;
@@ -265,22 +269,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             __syncwarp();
         }
     } else if (warp < 8) {
-        // ================================================================= work and its queries
+        // ================================================================= work and its queries (warp 4; 5..7 have nothing to do)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PT_REGS_Q));
-        int unit = blockIdx.x, u = 0;
-        bool ok = true;
-        for (int n = 0; ok; n++) {
-            if (warp == 4) {                                          // the next piece that has something to do
+        if (warp == 4) {
+            int unit = blockIdx.x;
+            PtRing qs(s_qfull);
+            const uint32_t qempty = smem_u32(s_qempty);
+            bool ok = true;
+            for (int n = 0, u = 0; ok; n++) {
                 if (n >= PT_WORK && !(ok = wait(s_wempty + n % PT_WORK, n / PT_WORK & 1 ^ 1))) break;
                 PtWork w;
                 w.tiles = -1;
-                while (unit < pp.units) {
+                while (unit < pp.units) {                             // the next piece that has something to do
                     const AqItem it = ap_item(p, unit);
-                    const int nth = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1, rt = p.row_tiles - 1 - it.rt;      // (the longest rows first)
                     w.s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, it.entry);
-                    const TileP t = ap_tile(p, w.s, rt, PT_ROWS);
+                    const TileP t = ap_tile(p, w.s, p.row_tiles - 1 - it.rt, PT_ROWS);      // (the longest rows first)
                     w.k0 = it.split * p.split; w.k1 = it.split == it.n_splits - 1 ? t.seen : min(t.seen, w.k0 + p.split);
-                    w.first = t.first; w.n_rows = t.n_rows; w.hk = it.hk; w.there = t.there; w.dst = nth;
+                    w.first = t.first; w.n_rows = t.n_rows; w.hk = it.hk; w.there = t.there;
+                    w.dst = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1;
                     w.clear = p.mask ? w.s.pos : w.s.pos + p.by_group.of(t.first) + 1;      // every row sees the slots before it
                     if (t.n_rows > 0 && (w.k0 < w.k1 || it.split == 0)) w.tiles = w.k0 < w.k1 ? (w.k1 - w.k0 + PT_KEYS - 1) / PT_KEYS : 0;      // (split 0 answers for rows that see nothing)
                     int then = 0;
@@ -290,97 +296,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 if (lane == 0) { *work_of(n) = w; mbar_arrive(s_wfull + n % PT_WORK); }
                 __syncwarp();
-            }
-            ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
-            if (!ok) break;
-            const PtWork * w = work_of(n);
-            const int tiles = w->tiles;
-            if (tiles < 0) break;
-            if (tiles > 0) {
-                const int qb = u % QB, part = lane & 7, r0 = (warp - 4) * 4 + (lane >> 3);
-                const uint32_t to = queries + (uint32_t)qb * Z::QUERIES;
-                const bool flip = p.scale_log2 < 0.f;                 // (the factor of the scores is positive: maxima stay maxima)
-                // Eight threads take a row, and have AT rows each on their way at a time.  The first ones are asked for before the buffer is free.
-                constexpr int AT = TWO ? 1 : 2, N = TWO ? HD / 32 : (HD / 8 + 7) / 8;
-                uint4 x[AT][N];
-                auto load = [&](int i) {
-#pragma unroll
-                    for (int k = 0; k < AT; k++) {
-                        const int r = r0 + (i + k) * 16, row = w->first + r, tok = p.by_group.of(row);
-                        const bool there = r < w->n_rows;
-                        const size_t from = (size_t)(w->s.first + tok) * p.q_stride + (size_t)(w->hk * p.group + row - tok * p.group) * HD;
-                        const uint4 * at = reinterpret_cast<const uint4 *>((const char *)p.q + from * (TWO ? 4 : 2)) + part;
-#pragma unroll
-                        for (int j = 0; j < N; j++) {
-                            x[k][j] = make_uint4(0u, 0u, 0u, 0u);
-                            if (there && (j * 8 + part) * (TWO ? 4 : 8) < HD) x[k][j] = __ldg(at + j * 8);
-                        }
+                if (w.tiles < 0) break;
+                if (w.tiles > 0) {
+                    if (u >= QB && !(ok = wait_at(qempty + qs.at * 8, qs.parity ^ 1))) break;
+                    u++;
+                    if (lane == 0) {
+                        mbar_expect_tx(s_qfull + qs.at, Z::QUERIES);
+                        const int row = (w.hk * p.b.T + w.s.first) * p.group + w.first;
+                        for (int low = 0; low <= (TWO ? 1 : 0); low++)
+                            for (int c = 0; c < SUBS; c++)
+                                tma_tile(queries + qs.at * Z::QUERIES + low * TILE + c * PT_SUB, &pp.m_q, c * 64, row + low * p.c.H * p.b.T * p.group, s_qfull + qs.at);
                     }
-                };
-                load(0);
-                if (u >= QB && !(ok = wait(s_qempty + qb, u / QB & 1 ^ 1))) break;
-                u++;
-#pragma unroll 1
-                for (int i = 0; i < PT_ROWS / 16; i += AT) {
-                    uint4 y[AT][N];
-#pragma unroll
-                    for (int k = 0; k < AT; k++)
-#pragma unroll
-                        for (int j = 0; j < N; j++) y[k][j] = x[k][j];
-                    if (i + AT < PT_ROWS / 16) load(i + AT);
-#pragma unroll
-                    for (int k = 0; k < AT; k++) {
-                        const int r = r0 + (i + k) * 16;
-                        // where the 8 columns of piece c of a row lie
-                        auto place = [&](int c) { return to + (uint32_t)(c >> 3) * PT_SUB + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) * 16); };
-                        if constexpr (!TWO) {
-                            // a value that is not finite: the row's scores are no numbers (an infinity alone may make them all the lowest value, as if the row saw nothing)
-                            const __half2 none = __floats2half2_rn(0.f, 0.f);
-                            __half2 zero[N];
-#pragma unroll
-                            for (int j = 0; j < N; j++) {
-                                const __half2 * h = reinterpret_cast<const __half2 *>(&y[k][j]);
-                                zero[j] = __hfma2(h[0], none, __hfma2(h[1], none, __hfma2(h[2], none, __hmul2(h[3], none))));
-                            }
-                            bool odd = false;
-#pragma unroll
-                            for (int j = 0; j < N; j++) odd |= !__hbeq2(zero[j], none);
-                            if (odd) y[k][0].x = 0x7fff7fffu;
-                            const uint32_t sign = flip ? 0x80008000u : 0u;
-                            if (part == 0) s_f[n % PT_WORK][r] = fabsf(p.scale_log2);
-#pragma unroll
-                            for (int j = 0; j < N; j++) {
-                                const int c = j * 8 + part;
-                                if (c < HD / 8) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(place(c)), "r"(y[k][j].x ^ sign), "r"(y[k][j].y ^ sign), "r"(y[k][j].z ^ sign), "r"(y[k][j].w ^ sign) : "memory");
-                            }
-                        } else {
-                            float m = 0.f;
-                            auto value = [&](int j) { return make_float4(__uint_as_float(y[k][j].x), __uint_as_float(y[k][j].y), __uint_as_float(y[k][j].z), __uint_as_float(y[k][j].w)); };
-#pragma unroll
-                            for (int j = 0; j < N; j++) { const float4 v = value(j); m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w))); }
-#pragma unroll
-                            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25
-                            const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
-                            if (part == 0) s_f[n % PT_WORK][r] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                            for (int j = 0; j < N; j++) {
-                                const float4 v = value(j);
-                                const uint32_t at = place((j * 8 + part) >> 1) + (uint32_t)(part & 1) * 8u;
-                                uint2 hi, lo;
-                                aq_split(v.x * up, v.y * up, hi.x, lo.x);
-                                aq_split(v.z * up, v.w * up, hi.y, lo.y);
-                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(at), "r"(hi.x), "r"(hi.y) : "memory");
-                                asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(at + TILE), "r"(lo.x), "r"(lo.y) : "memory");
-                            }
-                        }
-                    }
+                    __syncwarp();
+                    qs.template step<QB>();
                 }
-                tc_fence_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_qfull + qb);
+                done_with(n);
             }
-            done_with(n);
+            // (copies of queries in flight when a wait ran out: those of the last piece at most)
+            if (!ok && lane == 0) for (int i = 0; i < QB; i++) for (int spins = 0; spins < 1024 && !mbar_try_wait(s_qfull + i, 0u) && !mbar_try_wait(s_qfull + i, 1u); spins++) {}
+            __syncwarp();
         }
     } else if (warp < 8 + 4 * PT_GROUPS) {
         // ================================================================= probabilities: a row a thread
@@ -397,6 +331,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             const PtWork * w = work_of(n);
             const int tiles = w->tiles, span = w->k1 - w->k0;
             if (tiles < 0) break;
+            // (-infinity times 0 would be no number)
+            const float f = fmaxf(TWO ? (r < w->n_rows ? __ldg(p.factor + (size_t)(w->hk * p.b.T + w->s.first) * p.group + w->first + r) : 0.f) : fabsf(p.scale_log2), 0x1p-126f);
             const bool idle = (warp & 3) * 32 >= w->n_rows;           // no rows: their probabilities may be anything
             for (; at < g + tiles; at += PT_GROUPS, parity ^= 1) {
                 const int i = at - g;
@@ -404,7 +340,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 tc_fence_after();
                 const uint32_t info = s_info[at % PT_INFO];
                 const bool masked = info & 256u;
-                const float f = fmaxf(s_f[n % PT_WORK][r], 0x1p-126f);            // (-infinity times 0 would be no number)
                 uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
                 if (masked && !idle) {
                     ap_sees128(p, w->s, r < w->n_rows ? p.by_group.of(w->first + r) : 0x7fffffff, w->k0 + i * PT_KEYS - w->s.pos, sees);
@@ -509,7 +444,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     } else {
         // ================================================================= sums out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PT_REGS_D));
-        const int r = (warp & 3) * 32 + lane, d0 = warp >= 24 ? HD / 2 : 0;
+        const int r = (warp & 3) * 32 + lane, d0 = warp >= 24 ? DH : 0;
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T_O + (uint32_t)d0;
         PtRing buf(s_pfull);
         const uint32_t pfull = smem_u32(s_pfull), pv = smem_u32(s_pv), stat = smem_u32(s_stat);
@@ -525,9 +460,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             const int tiles = w->tiles;
             if (tiles < 0) break;
             float top = -INFINITY, sum = 0.f;
-            float acc[HD / 2];
+            float acc[DH];
 #pragma unroll
-            for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
+            for (int j = 0; j < DH; j++) acc[j] = 0.f;
             for (int i = 0; i < tiles && ok; i++) {
                 const int b = buf.at;
                 ok = wait_at(buf.here(), buf.parity);
@@ -540,16 +475,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 ok = wait_at(pv + b * 8, buf.parity) && ok;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 8) {
-                    float v[8];
-                    tc_ld8(v, mine + ob * NV + c);
-                    if (c + 8 == HD / 2) {                           // the buffer goes back
+                for (int c = 0; c < DH; c += DC) {
+                    float v[DC];
+                    if constexpr (DC == 32) tc_ld32(v, mine + ob * NV + c); else tc_ld16(v, mine + ob * NV + c);
+                    if (c + DC == DH) {                           // the buffer goes back
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) pt_arrive(pfull + (buf.at + OB >= PT_GROUPS ? buf.at + OB - PT_GROUPS : buf.at + OB) * 8);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
+                    for (int j = 0; j < DC; j += 2) {
                         const float2 o = f2_fma(make_float2(v[j], v[j + 1]), f2(is), f2_mul(make_float2(acc[c + j], acc[c + j + 1]), f2(was)));
                         acc[c + j] = o.x; acc[c + j + 1] = o.y;
                     }
@@ -562,28 +497,34 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 if (of >= p.c.n_ctx - w->s.pos) {                     // a token without a slot of its own
                     top = -INFINITY; sum = 0.f;
 #pragma unroll
-                    for (int j = 0; j < HD / 2; j++) acc[j] = 0.f;
+                    for (int j = 0; j < DH; j++) acc[j] = 0.f;
                 }
                 if (!ok || s_dead) sum = __int_as_float(0x7fc00000);  // a wait ran out, here or in a warp that came to s_pfull all the same: no numbers instead of wrong ones
+                // (32 bytes a store where rows lie so: a row a thread meets a line of its own at every store)
                 if (w->dst >= 0) {
                     const size_t at = (size_t)w->dst * PT_ROWS + r;
 #pragma unroll
-                    for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>(p.part + at * HD + d0 + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                    for (int j = 0; j < DH; j += 8) pt_store8(p.part + at * HD + d0 + j, acc + j);
                     if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
                 } else {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     const size_t at = (size_t)(w->s.first + of) * p.out_stride + (size_t)h * HD + d0;
+#pragma unroll
+                    for (int j = 0; j < DH; j++) acc[j] *= inv;
                     if constexpr (!TWO) {
 #pragma unroll
-                        for (int j = 0; j < HD / 2; j += 8) {
+                        for (int j = 0; j < DH; j += 8) {
                             uint4 u;
-                            u.x = h2u(__floats2half2_rn(acc[j] * inv, acc[j + 1] * inv)); u.y = h2u(__floats2half2_rn(acc[j + 2] * inv, acc[j + 3] * inv));
-                            u.z = h2u(__floats2half2_rn(acc[j + 4] * inv, acc[j + 5] * inv)); u.w = h2u(__floats2half2_rn(acc[j + 6] * inv, acc[j + 7] * inv));
+                            u.x = h2u(__floats2half2_rn(acc[j], acc[j + 1])); u.y = h2u(__floats2half2_rn(acc[j + 2], acc[j + 3]));
+                            u.z = h2u(__floats2half2_rn(acc[j + 4], acc[j + 5])); u.w = h2u(__floats2half2_rn(acc[j + 6], acc[j + 7]));
                             *reinterpret_cast<uint4 *>((__half *)p.out + at + j) = u;
                         }
+                    } else if (pp.wide) {
+#pragma unroll
+                        for (int j = 0; j < DH; j += 8) pt_store8((float *)p.out + at + j, acc + j);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < HD / 2; j += 4) *reinterpret_cast<float4 *>((float *)p.out + at + j) = make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv);
+                        for (int j = 0; j < DH; j += 4) *reinterpret_cast<float4 *>((float *)p.out + at + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
                     }
                 }
             }
@@ -597,11 +538,62 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     if (tid == 0 && s_dead) atomicOr(p.status, 16u);
 }
 
-// Clears the status word and the number of the next piece of work in front of the kernel: no CTA of its own can, as another one may have been at them by then.
-__global__ void k_attn_paged_clear(unsigned int * status, unsigned int * next) {
+// In front of the kernel: its queries as it takes them, halves [low][KV head][row of the group's tokens][HD], and of FP32 rows the factors of their scores; and the status word and the number of the next
+// piece cleared (no CTA of the kernel can, as another one may have been at them by then).  A row, over a power of two of its largest value where it is FP32, is one or the sum of two halves; negative
+// where the scale is (the factor of the scores is positive: maxima stay maxima).  Eight threads take a row.
+template <int HD, bool TWO>
+__global__ void __launch_bounds__(256) k_attn_paged_queries(const AttnPagedP p, __half * to, float * factor, unsigned int * next) {
+    const int part = threadIdx.x & 7, head = p.n_head, at = blockIdx.x * 32 + (threadIdx.x >> 3);
     pdl_launch();
     pdl_wait();
-    if (threadIdx.x == 0) { *status = 0u; *next = 0u; }
+    if (at == 0 && part == 0) { *p.status = 0u; *next = 0u; }
+    if (at >= p.b.T * head) return;                                   // (the same for the eight)
+    const int tok = at / head, h = at - tok * head, hk = h / p.group, rows = p.b.T * p.group;
+    const size_t row = (size_t)hk * rows + (size_t)tok * p.group + (h - hk * p.group);
+    const unsigned mine = 0xffu << (threadIdx.x & 24);
+    if constexpr (!TWO) {
+        constexpr int N = (HD / 8 + 7) / 8;
+        const uint4 * from = reinterpret_cast<const uint4 *>((const __half *)p.q + (size_t)tok * p.q_stride + (size_t)h * HD);
+        uint4 x[N];
+        const __half2 none = __floats2half2_rn(0.f, 0.f);
+        __half2 zero = none;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            x[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (j * 8 + part < HD / 8) x[j] = __ldg(from + j * 8 + part);
+            const __half2 * v = reinterpret_cast<const __half2 *>(x + j);
+#pragma unroll
+            for (int c = 0; c < 4; c++) zero = __hfma2(v[c], none, zero);
+        }
+        // a value that is not finite: the row's scores are no numbers (an infinity alone may make them all the lowest value, as if the row saw nothing)
+        if (!__hbeq2(zero, none)) x[0].x = 0x7fff7fffu;
+        const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (j * 8 + part < HD / 8) reinterpret_cast<uint4 *>(to + row * HD)[j * 8 + part] = make_uint4(x[j].x ^ sign, x[j].y ^ sign, x[j].z ^ sign, x[j].w ^ sign);
+    } else {
+        constexpr int N = HD / 32;
+        const float4 * from = reinterpret_cast<const float4 *>((const float *)p.q + (size_t)tok * p.q_stride + (size_t)h * HD);
+        float4 v[N];
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = __ldg(from + j * 8 + part);
+#pragma unroll
+        for (int j = 0; j < N; j++) m = fmaxf(fmaxf(m, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(mine, m, o));
+        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127) - 10;     // the largest to 2^10 .. 2^11: lower parts are then exact to 2^-25
+        const float up = copysignf(__uint_as_float((uint32_t)(127 - e) << 23), p.scale_log2);
+        if (part == 0) factor[row] = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            uint2 hi, lo;
+            aq_split(v[j].x * up, v[j].y * up, hi.x, lo.x);
+            aq_split(v[j].z * up, v[j].w * up, hi.y, lo.y);
+            reinterpret_cast<uint2 *>(to + row * HD)[j * 8 + part] = hi;
+            reinterpret_cast<uint2 *>(to + ((size_t)p.c.H * rows + row) * HD)[j * 8 + part] = lo;
+        }
+    }
 }
 
 bool attn_paged_tc_takes(int hd, int64_t rows) { return hd <= 128 && rows > 16; }
@@ -622,9 +614,12 @@ static int pt_go(const AttnPagedP & a, cudaStream_t st) {
     const int64_t rows = (int64_t)a.c.n_pages * a.c.H * a.c.page;
     if ((rc = tensor_map(&p.m_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.k, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B)) ||
         (rc = tensor_map(&p.m_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.v, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * 4 % 32 == 0;
     p.units = (int)ap_grid(a);
     p.next = a.status + 8;
-    PI_CUDA(launch_k(k_attn_paged_clear, dim3(1), dim3(32), 0, st, true, a.status, p.next));
+    const int64_t q_rows = (int64_t)a.b.T * a.n_head;
+    if ((rc = tensor_map(&p.m_q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.queries, HD, q_rows * (TWO ? 2 : 1), HD * 2, 64, PT_ROWS, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
+    PI_CUDA(launch_k(k_attn_paged_queries<HD, TWO>, dim3((unsigned)((q_rows + 31) / 32)), dim3(256), 0, st, true, a, a.queries, a.factor, p.next));
     PI_CUDA(launch_k(k_attn_paged_tc<HD, TWO>, dim3((unsigned)(p.units < sm_count() ? p.units : sm_count())), dim3(PT_THREADS), smem, st, true, p));
     return PI_OK;
 }

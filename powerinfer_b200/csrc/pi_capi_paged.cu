@@ -95,7 +95,7 @@ static int check_attention_tree(const pi_kv_paged * cache, const pi_kv_batch * b
     int rc;
     if ((rc = check_paged(cache, c, who)) || (rc = check_batch(batch, b, who)) || (rc = check_type(xtype, who))) return rc;
     PI_REQUIRE(n_head > 0 && n_head % c.H == 0 && n_head <= KV_BIG / c.hd, "attention_tree: n_head=%d must be a multiple of n_head_kv=%d", n_head, c.H);
-    PI_REQUIRE((int64_t)b.max_new * n_head < (int64_t(1) << 27) && (int64_t)b.n * ((int64_t)b.max_new * (n_head / c.H) / 16 + 1) * c.H < (int64_t(1) << 28),
+    PI_REQUIRE((int64_t)b.T * n_head < (int64_t(1) << 30) && (int64_t)b.max_new * n_head < (int64_t(1) << 27) && (int64_t)b.n * ((int64_t)b.max_new * (n_head / c.H) / 16 + 1) * c.H < (int64_t(1) << 28),
                "attention_tree: %d sequences of %d tokens of %d heads are too many for a call", b.n, b.max_new, n_head);
     return PI_OK;
 }
