@@ -14,18 +14,21 @@ static constexpr int AP_THREADS = 256;
 struct AppendP {
     AppendArgs a;
     int heads[3];                                                     // queries (0: none), keys, values
-    int parts, per_head, pairs;                                       // CTAs of a token; units of a head; whether a unit of queries and keys is one pair
+    int parts, per_head;                                              // CTAs of a token; units of a head (of queries and keys)
 };
 
-// 8 values of a row
-template <typename T> __device__ __forceinline__ void load8(const T * p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float * p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// 8 values of a row, as they are stored
+template <typename T> struct Eight { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ void load8(const T * p, Eight<T> & e) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) e.w[i] = reinterpret_cast<const uint4 *>(p)[i];
 }
-template <> __device__ __forceinline__ void load8<__half>(const __half * p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const float2 a = h2f(u.x), b = h2f(u.y), c = h2f(u.z), d = h2f(u.w);
+__device__ __forceinline__ void open8(const Eight<float> & e, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) { v[4 * i] = __uint_as_float(e.w[i].x); v[4 * i + 1] = __uint_as_float(e.w[i].y); v[4 * i + 2] = __uint_as_float(e.w[i].z); v[4 * i + 3] = __uint_as_float(e.w[i].w); }
+}
+__device__ __forceinline__ void open8(const Eight<__half> & e, float (&v)[8]) {
+    const float2 a = h2f(e.w[0].x), b = h2f(e.w[0].y), c = h2f(e.w[0].z), d = h2f(e.w[0].w);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
 }
 __device__ __forceinline__ void store8(float * p, const float (&v)[8]) {
@@ -41,9 +44,8 @@ __device__ __forceinline__ void store8(__half * p, const float (&v)[8]) {
 
 // A unit is 16 values of a head: 8 at d0 and 8 at d1.  KIND 0: pairs (2i, 2i + 1), 16 in a row; 1: pairs (i, i + half), 8 of each half, or 16 in a row of the dimensions
 // that pass; 2: the same where a half is no multiple of 8, pair by pair (values still 16 in a row).  In place is fine: a unit is read and written by one thread.
-template <typename T, int KIND>
+template <typename T, int KIND, int U>
 __global__ void __launch_bounds__(AP_THREADS) k_kv_append(const AppendP p) {
-    constexpr int U = KIND == 2 ? 4 : 2;
     __shared__ float2 cs[128];
     const AppendArgs & a = p.a;
     const int t = blockIdx.x / p.parts, part = blockIdx.x - t * p.parts, i = blockIdx.y, half = a.n_rot >> 1, hd = a.c.hd, lane = threadIdx.x & 31;
@@ -52,22 +54,20 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(const AppendP p) {
     const SeqB s = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, i);
     if (t >= s.n_new) return;
     const int slot = s.pos + t;
-    int page = -1;
-    if (s.sq >= 0 && slot < a.c.n_ctx) page = page_of(a.c, s.sq, slot >> a.c.shift);
-    if (a.b.seq && page >= 0) {                                       // of entries that name one sequence the last one counts
-        bool later = false;
-        for (int j = i + 1 + lane; j < a.b.n; j += 32) {
-            const SeqB o = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, j);
-            later |= o.sq == s.sq && o.n_new > 0;
-        }
-        if (__any_sync(0xffffffffu, later)) page = -1;                // (the same in every warp)
-    }
     const size_t row_in = (size_t)(s.first + t);
+    // ---- values on their way
     const int turning = (p.heads[0] + p.heads[1]) * p.per_head, units = turning + p.heads[2] * (hd >> 4);
-    float v[U][2][8]; int which[U], at[U], head[U];
+    Eight<T> v[U][KIND == 2 ? 1 : 2]; T pair[KIND == 2 ? U : 1][2]; int which[U], at[U], head[U];
+    (void)pair;
+    // first and second 8 of unit `at`: of queries and keys, of values
+    auto places = [&](int which, int at, bool & turns, int & d0, int & d1) {
+        turns = KIND == 1 && which < 2 && at * 8 < half;
+        d0 = KIND != 1 || which == 2 ? at * 16 : turns ? at * 8 : a.n_rot + (at * 8 - half) * 2;
+        d1 = turns ? d0 + half : d0 + 8;
+    };
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int n = (part * U + u) * AP_THREADS + threadIdx.x;
+        const int n = (part * U + u) * (int)blockDim.x + (int)threadIdx.x;
         which[u] = -1;
         if (n >= units) continue;
         const int per = n < turning ? p.per_head : hd >> 4, m = n < turning ? n : n - turning;
@@ -76,80 +76,122 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(const AppendP p) {
         which[u] = n >= turning ? 2 : h < p.heads[0] ? 0 : 1;
         if (which[u] == 1) h -= p.heads[0];
         head[u] = h;
-        if (which[u] > 0 && page < 0) { which[u] = -1; continue; }
         const T * x = (const T *)a.x[which[u]] + row_in * a.x_stride[which[u]] + (size_t)h * hd;
-        if (KIND == 2 && which[u] < 2) {
-            const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
-            v[u][0][0] = rope_get(x + d0); v[u][1][0] = rope_get(x + d1);
+        if constexpr (KIND == 2) {
+            if (which[u] < 2) {
+                const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
+                pair[u][0] = x[d0]; pair[u][1] = x[d1];
+            }
         } else {
-            const bool turns = KIND == 1 && which[u] < 2 && at[u] * 8 < half;
-            const int d0 = KIND != 1 || which[u] == 2 ? at[u] * 16 : turns ? at[u] * 8 : a.n_rot + (at[u] * 8 - half) * 2, d1 = turns ? d0 + half : d0 + 8;
+            bool turns; int d0, d1;
+            places(which[u], at[u], turns, d0, d1);
             load8(x + d0, v[u][0]);
-            load8(x + d1, v[u][1]);
+            load8(x + d1, v[u][KIND == 2 ? 0 : 1]);
         }
     }
+    // ---- meanwhile where they go, and the angles
+    int page = -1;
+    if (s.sq >= 0 && slot < a.c.n_ctx) page = page_of(a.c, s.sq, slot >> a.c.shift);
     const int pos = a.pos ? a.pos[row_in] : slot;
-    for (int j = threadIdx.x; j < half; j += AP_THREADS) cs[j] = rope_angle(pos, a.freqs[j], a.mscale);
+    for (int j = threadIdx.x; j < half; j += blockDim.x) cs[j] = rope_angle(pos, a.freqs[j], a.mscale);
+    if (a.b.seq && page >= 0) {                                       // of entries that name one sequence the last one counts
+        bool later = false;
+        for (int j = i + 1 + lane; j < a.b.n; j += 32) {
+            const SeqB o = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, j);
+            later |= o.sq == s.sq && o.n_new > 0;
+        }
+        if (__any_sync(0xffffffffu, later)) page = -1;                // (the same in every warp)
+    }
     __syncthreads();
+    auto put = [&](int which, int head, int d, const float (&y)[8]) {
+        if (which == 0)     store8((T *)a.q_out + row_in * a.q_out_stride + (size_t)head * hd + d, y);
+        else if (page >= 0) store8((which == 1 ? a.c.k : a.c.v) + page_at(a.c, page, head) + (size_t)(slot & (a.c.page - 1)) * hd + d, y);
+    };
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (which[u] < 0) continue;
-        __half * to = nullptr; T * q = nullptr;
-        if (which[u] == 0) q = (T *)a.q_out + row_in * a.q_out_stride + (size_t)head[u] * hd;
-        else               to = (which[u] == 1 ? a.c.k : a.c.v) + page_at(a.c, page, head[u]) + (size_t)(slot & (a.c.page - 1)) * hd;
-        if (KIND == 2 && which[u] < 2) {
-            const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
-            float y0 = v[u][0][0], y1 = v[u][1][0];
-            if (at[u] < half) {
-                const float2 c = cs[at[u]];
-                const float x0 = y0, x1 = y1;
-                y0 = x0 * c.x - x1 * c.y; y1 = x0 * c.y + x1 * c.x;
-            }
-            if (which[u] == 0) { rope_put(q + d0, y0); rope_put(q + d1, y1); }
-            else               { rope_put(to + d0, y0); rope_put(to + d1, y1); }
-            continue;
-        }
-        const bool turns = KIND == 1 && which[u] < 2 && at[u] * 8 < half;
-        const int d0 = KIND != 1 || which[u] == 2 ? at[u] * 16 : turns ? at[u] * 8 : a.n_rot + (at[u] * 8 - half) * 2, d1 = turns ? d0 + half : d0 + 8;
-        if (KIND == 0 && which[u] < 2) {
+        if constexpr (KIND == 2) {
+            if (which[u] < 2) {
+                const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
+                float y0 = rope_get(&pair[u][0]), y1 = rope_get(&pair[u][1]);
+                if (at[u] < half) {
+                    const float2 c = cs[at[u]];
+                    const float x0 = y0, x1 = y1;
+                    y0 = x0 * c.x - x1 * c.y; y1 = x0 * c.y + x1 * c.x;
+                }
+                if (which[u] == 0) {
+                    T * to = (T *)a.q_out + row_in * a.q_out_stride + (size_t)head[u] * hd;
+                    rope_put(to + d0, y0); rope_put(to + d1, y1);
+                } else if (page >= 0) {
+                    __half * to = a.c.k + page_at(a.c, page, head[u]) + (size_t)(slot & (a.c.page - 1)) * hd;
+                    rope_put(to + d0, y0); rope_put(to + d1, y1);
+                }
+            } else {
+                const T * x = (const T *)a.x[2] + row_in * a.x_stride[2] + (size_t)head[u] * hd + at[u] * 16;
 #pragma unroll
-            for (int w = 0; w < 2; w++)
+                for (int w = 0; w < 2; w++) {
+                    float y[8];
+                    load8(x + 8 * w, v[u][0]);
+                    open8(v[u][0], y);
+                    put(2, head[u], at[u] * 16 + 8 * w, y);
+                }
+            }
+        } else {
+            bool turns; int d0, d1;
+            places(which[u], at[u], turns, d0, d1);
+            float x0[8], x1[8];
+            open8(v[u][0], x0);
+            open8(v[u][1], x1);
+            if (KIND == 0 && which[u] < 2) {
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                    const int k = (d0 + w * 8 + j) >> 1;
-                    if (k < half) {
-                        const float2 c = cs[k];
-                        const float x0 = v[u][w][j], x1 = v[u][w][j + 1];
-                        v[u][w][j] = x0 * c.x - x1 * c.y; v[u][w][j + 1] = x0 * c.y + x1 * c.x;
-                    }
+                    const int k = (d0 + j) >> 1;
+                    if (k < half) { const float2 c = cs[k]; const float a0 = x0[j], a1 = x0[j + 1]; x0[j] = a0 * c.x - a1 * c.y; x0[j + 1] = a0 * c.y + a1 * c.x; }
+                    if (k + 4 < half) { const float2 c = cs[k + 4]; const float a0 = x1[j], a1 = x1[j + 1]; x1[j] = a0 * c.x - a1 * c.y; x1[j + 1] = a0 * c.y + a1 * c.x; }
                 }
-        } else if (turns) {
+            } else if (turns) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float2 c = cs[d0 + j];
-                const float x0 = v[u][0][j], x1 = v[u][1][j];
-                v[u][0][j] = x0 * c.x - x1 * c.y; v[u][1][j] = x0 * c.y + x1 * c.x;
+                for (int j = 0; j < 8; j++) {
+                    const float2 c = cs[d0 + j];
+                    const float a0 = x0[j], a1 = x1[j];
+                    x0[j] = a0 * c.x - a1 * c.y; x1[j] = a0 * c.y + a1 * c.x;
+                }
             }
+            put(which[u], head[u], d0, x0);
+            put(which[u], head[u], d1, x1);
         }
-        if (which[u] == 0) { store8(q + d0, v[u][0]); store8(q + d1, v[u][1]); }
-        else               { store8(to + d0, v[u][0]); store8(to + d1, v[u][1]); }
     }
 }
 
+template <typename T, int KIND>
+static int append_run(const AppendP & p, int U, int threads, cudaStream_t st) {
+    const dim3 grid((unsigned)((int64_t)p.parts * p.a.b.max_new), p.a.b.n), block(threads);
+    if (U == 1)      PI_CUDA(launch_k(k_kv_append<T, KIND, 1>, grid, block, 0, st, true, p));
+    else if (U == 2 || sizeof(T) == 4) PI_CUDA(launch_k(k_kv_append<T, KIND, 2>, grid, block, 0, st, true, p));
+    else if (U == 3) PI_CUDA(launch_k(k_kv_append<T, KIND, 3>, grid, block, 0, st, true, p));
+    else             PI_CUDA(launch_k(k_kv_append<T, KIND, 4>, grid, block, 0, st, true, p));
+    return PI_OK;
+}
+
+// Few tokens: a unit a thread, so that there are threads for all SMs.  Many: two to four units a thread (FP32: one or two, 64 bytes each), the number of units and threads that leaves the fewest without one (of 576 units of the
+// falcon shape 2 x 256 and a second CTA of 64 took 40 us for 3329 tokens).
 template <typename T>
 static int append_go(const AppendArgs & a, cudaStream_t st) {
     AppendP p;
     p.a = a;
     p.heads[0] = a.x[0] ? a.n_head : 0; p.heads[1] = p.heads[2] = a.c.H;
     const int half = a.n_rot / 2, kind = !a.halves || half == 0 ? 0 : half % 8 == 0 ? 1 : 2;
-    p.per_head = kind == 2 ? a.c.hd / 2 : a.c.hd / 16; p.pairs = kind == 2;
-    const int64_t units = (int64_t)(p.heads[0] + p.heads[1]) * p.per_head + (int64_t)p.heads[2] * (a.c.hd / 16), of_cta = (int64_t)AP_THREADS * (kind == 2 ? 4 : 2);
-    p.parts = (int)((units + of_cta - 1) / of_cta);
-    const dim3 grid((unsigned)((int64_t)p.parts * a.b.max_new), a.b.n);
-    if (kind == 0)      PI_CUDA(launch_k(k_kv_append<T, 0>, grid, dim3(AP_THREADS), 0, st, true, p));
-    else if (kind == 1) PI_CUDA(launch_k(k_kv_append<T, 1>, grid, dim3(AP_THREADS), 0, st, true, p));
-    else                PI_CUDA(launch_k(k_kv_append<T, 2>, grid, dim3(AP_THREADS), 0, st, true, p));
-    return PI_OK;
+    p.per_head = kind == 2 ? a.c.hd / 2 : a.c.hd / 16;
+    const int64_t units = (int64_t)(p.heads[0] + p.heads[1]) * p.per_head + (int64_t)p.heads[2] * (a.c.hd / 16);
+    int U = 1; int64_t least = -1;
+    for (int u = 1; u <= 4; u++) {
+        const bool many = (int64_t)a.b.n * a.b.max_new * units >= (int64_t)sm_count() * 8 * AP_THREADS;
+        if (many ? (sizeof(T) == 2 ? u == 1 : u > 2) : u > 1) continue;
+        const int64_t parts = (units + (int64_t)u * AP_THREADS - 1) / ((int64_t)u * AP_THREADS), threads = ((units + parts * u - 1) / (parts * u) + 31) / 32 * 32;
+        if (least < 0 || parts * threads * u <= least) { least = parts * threads * u; U = u; p.parts = (int)parts; }
+    }
+    const int threads = (int)(((units + (int64_t)p.parts * U - 1) / ((int64_t)p.parts * U) + 31) / 32 * 32);
+    return kind == 0 ? append_run<T, 0>(p, U, threads, st) : kind == 1 ? append_run<T, 1>(p, U, threads, st) : append_run<T, 2>(p, U, threads, st);
 }
 
 int launch_kv_append_paged(const AppendArgs & a, cudaStream_t st) {
