@@ -476,9 +476,24 @@ def kv_evict_q8(cache: KvCacheQ8, weights: torch.Tensor, lens: torch.Tensor, kee
 
 
 # ---- drafted tokens over a paged cache: trees, keys and values into pages, their attention, the path that stays.
+# (A call with few tokens lasts 3 us on the device: type, length, order and device of a tensor are asked for in one place, names are looked up once.)
 
 _KV_PAGED = struct.Struct("@3P7i4x")       # pi_kv_paged
 assert _KV_PAGED.size == C.sizeof(_lib.KvPaged)
+_I32, _I64, _F16 = torch.int32, torch.int64, torch.float16
+
+
+def _device() -> int:
+    return torch.cuda.current_device() if _raw_device is None else _raw_device()
+
+
+def _whole(t: torch.Tensor, n: int, device: int, what: str) -> int:
+    """Address of a contiguous int32 tensor of n on the device."""
+    if t.dtype is not _I32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, the current device is cuda:{device}")
+    return t.data_ptr()
 
 
 class KvCachePaged:
@@ -486,20 +501,21 @@ class KvCachePaged:
     slot j of a sequence is row j % page of the page that table[sequence, j // page] names (outside 0 .. n_pages - 1: a page that is not there).  The tensors are the caller's, who hands
     pages out by writing to the table."""
 
-    __slots__ = ("k", "v", "table", "n_layer", "n_pages", "n_seq", "max_pages", "n_head_kv", "page", "head_dim", "c")
+    __slots__ = ("k", "v", "table", "n_layer", "n_pages", "n_seq", "max_pages", "n_head_kv", "page", "head_dim", "device", "c")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
-        shape = k.shape
-        if k.dtype is not torch.float16 or v.dtype is not torch.float16 or table.dtype is not torch.int32:
+        shape, rows, self.device = k.shape, table.shape, _device()
+        if k.dtype is not _F16 or v.dtype is not _F16 or table.dtype is not _I32:
             raise ValueError("the pools are float16, the table int32")
-        if v.shape != shape or not 4 <= len(shape) <= 5 or table.dim() != 2:
+        if v.shape != shape or not 4 <= len(shape) <= 5 or len(rows) != 2:
             raise ValueError("the pools are [n_layer, n_pages, n_head_kv, page, head_dim], of one shape, the table [n_seq, max_pages]")
         if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous()):
             raise ValueError("the pools and the table must be contiguous")
-        _here(k, v, table)
+        if not k.get_device() == v.get_device() == table.get_device() == self.device:
+            raise ValueError(f"the pools and the table must be on the current device, cuda:{self.device}")
         self.k, self.v, self.table = k, v, table
         self.n_layer, self.n_pages, self.n_head_kv, self.page, self.head_dim = shape if len(shape) == 5 else (1, *shape)
-        self.n_seq, self.max_pages = table.shape
+        self.n_seq, self.max_pages = rows
         self.c = _KV_PAGED.pack(k.data_ptr(), v.data_ptr(), table.data_ptr(), self.n_layer, self.n_pages, self.n_seq, self.max_pages, self.n_head_kv, self.page, self.head_dim)
 
     @classmethod
@@ -509,31 +525,42 @@ class KvCachePaged:
         return cls(*pools, torch.full((n_seq, max_pages), -1, dtype=torch.int32, device="cuda"))
 
 
+def _on(cache: KvCachePaged) -> int:
+    """The current device, which has to be the cache's."""
+    device = _device()
+    if device != cache.device:
+        raise ValueError(f"the cache is on cuda:{cache.device}, the current device is cuda:{device}")
+    return device
+
+
+def _entries(q_start, pos0, seq, T: int, max_new, device: int) -> bytes:
+    n = pos0.numel()
+    return _KV_BATCH.pack(_whole(q_start, n + 1, device, "q_start"), 0 if seq is None else _whole(seq, n, device, "seq"), _whole(pos0, n, device, "pos0"), n, T,
+                          T if max_new is None else max_new)
+
+
 def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, max_new: int | None = None, words: int | None = None):
     """Trees of drafted tokens, parents int32 [T] (rows q_start[i] .. q_start[i + 1] are tree i; a token's parent is the number, in its tree, of one before it, any
     other number: it has none), as attention_tree and kv_append_paged take them: mask int64 [T, words] (bit u % 64 of word u // 64: token u of the tree is the row's token or an ancestor of it) and
     positions int32 [T] (pos0[i] and the number of ancestors).  max_new: tokens of the largest tree (None: T); words: by max_new where it is None."""
-    T, n = parents.numel(), pos0.numel()
-    most = T if max_new is None else max_new
+    T, device = parents.numel(), _device()
     if words is None:
-        words = max(1, -(-most // 64))
-    mask, pos = parents.new_empty((T, words), dtype=torch.int64), torch.empty_like(parents)
-    _here(parents, q_start, pos0)
-    check(lib.pi_tree_mask(_KV_BATCH.pack(_ints(q_start, n + 1, "q_start"), 0, _ints(pos0, n, "pos0"), n, T, most), _ints(parents, T, "parents"), mask.data_ptr(), words,
-                           pos.data_ptr(), _stream()))
+        words = -(-(T if max_new is None else max_new) // 64) or 1
+    at, b = _whole(parents, T, device, "parents"), _entries(q_start, pos0, None, T, max_new, device)
+    mask, pos = parents.new_empty((T, max(0, words)), dtype=_I64), parents.new_empty(T)
+    check(lib.pi_tree_mask(b, at, mask.data_ptr(), words, pos.data_ptr(), _stream()))
     return mask, pos
 
 
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tensor, q_start: torch.Tensor, max_new: int | None = None):
     """The path of each tree that the target model agrees with: it begins at token 0, and behind c comes the lowest child u of c with tokens[u] == choice[c] (choice int32 [T]: the target's
     token behind each one).  Returns (path int32 [n, max_new], the numbers of its tokens and -1 behind them; n_path int32 [n]; next int32 [n], choice of the last one)."""
-    T, n = tokens.numel(), q_start.numel() - 1
+    T, n, device = tokens.numel(), q_start.numel() - 1, _device()
     most = T if max_new is None else max_new
-    path, n_path = tokens.new_empty((n, max(0, most))), tokens.new_empty(n)
-    then = torch.empty_like(n_path)
-    _here(tokens, parents, choice, q_start)
-    check(lib.pi_tree_accept(_KV_BATCH.pack(_ints(q_start, n + 1, "q_start"), 0, 0, n, T, most), _ints(tokens, T, "tokens"), _ints(parents, T, "parents"), _ints(choice, T, "choice"),
-                             path.data_ptr(), n_path.data_ptr(), then.data_ptr(), _stream()))
+    a, b, c = _whole(tokens, T, device, "tokens"), _whole(parents, T, device, "parents"), _whole(choice, T, device, "choice")
+    of = _KV_BATCH.pack(_whole(q_start, n + 1, device, "q_start"), 0, 0, n, T, most)
+    path, n_path, then = tokens.new_empty((n, max(0, most))), tokens.new_empty(n), tokens.new_empty(n)
+    check(lib.pi_tree_accept(of, a, b, c, path.data_ptr(), n_path.data_ptr(), then.data_ptr(), _stream()))
     return path, n_path, then
 
 
@@ -542,28 +569,32 @@ def kv_append_paged(cache: KvCachePaged, k: torch.Tensor, v: torch.Tensor, q_sta
     """k, v [T, n_head_kv * head_dim] into the cache, keys rotated to pos int32 [T] on the way (None: to their slots' numbers; freqs None: not at all): rows
     q_start[i] .. q_start[i + 1] to the slots pos0[i] and on of sequence seq[i] (None: i); at most max_new rows of an entry (None: T).  mode 0 (pairs (2i, 2i+1)) or 2 (neox).
     q [T, n_head * head_dim]: returned rotated to the same positions, a new tensor (rows of no entry hold anything); without it None."""
-    hd = cache.head_dim
+    hd, device = cache.head_dim, _on(cache)
     width = cache.n_head_kv * hd
     k, k_at, T, _, k_step, xtype = _row_matrix(k, "k", width)
     v, v_at, Tv, _, v_step, vtype = _row_matrix(v, "v", width)
     if Tv != T or vtype != xtype:
         raise ValueError("k and v must have the same rows and type")
-    q_out, q_at, q_step, out_at, nq = None, None, 0, None, 0
+    if k.get_device() != device or v.get_device() != device:
+        raise ValueError(f"k and v must be on the current device, cuda:{device}")
+    q_out = q_at = out_at = f_at = None
+    q_step = nq = n_rot = 0
+    mscale = 1.0
+    if freqs is not None:
+        f, mscale = freqs.freqs, freqs.mscale
+        if f.get_device() != device:
+            raise ValueError(f"the frequencies must be on the current device, cuda:{device}")
+        f_at, n_rot = f.data_ptr(), 2 * f.numel()
     if q is not None:
         if freqs is None:
             raise ValueError("queries are returned rotated: frequencies are needed")
         q, q_at, Tq, nq, q_step, qtype = _row_matrix(q, "q")
-        if Tq != T or qtype != xtype or nq % hd:
-            raise ValueError(f"q must be of k's type, {T} rows of heads of {hd}")
+        if Tq != T or qtype != xtype or nq % hd or q.get_device() != device:
+            raise ValueError(f"q must be of k's type and device, {T} rows of heads of {hd}")
         q_out = torch.empty_like(q)
         out_at = q_out.data_ptr()
-    f, f_at, n_rot, mscale = None, None, 0, 1.0
-    if freqs is not None:
-        f = freqs.freqs
-        f_at, n_rot, mscale = f.data_ptr(), 2 * f.numel(), freqs.mscale
-    _here(cache.k, k, v, q, q_start, pos0, seq, pos, f)
-    check(lib.pi_kv_append_paged(cache.c, _batch(q_start, pos0, seq, T, max_new), layer, xtype, k_at, k_step, v_at, v_step, q_at, q_step, nq // hd, out_at, nq,
-                                 None if pos is None else _ints(pos, T, "pos"), f_at, n_rot, 1 if mode & 2 else 0, mscale, _stream()))
+    check(lib.pi_kv_append_paged(cache.c, _entries(q_start, pos0, seq, T, max_new, device), layer, xtype, k_at, k_step, v_at, v_step, q_at, q_step, nq // hd, out_at, nq,
+                                 None if pos is None else _whole(pos, T, device, "pos"), f_at, n_rot, 1 if mode & 2 else 0, mscale, _stream()))
     return q_out
 
 
@@ -572,25 +603,25 @@ def attention_tree(cache: KvCachePaged, q: torch.Tensor, q_start: torch.Tensor, 
     """The KQV block over a paged cache, the batch's own keys and values stored before: q [T, n_head * head_dim] (or [T, n_head, head_dim]) -> rows of q's type.  Token t of entry i sees the slots
     before pos0[i], and pos0[i] + u for the tokens u of its entry whose bit of mask int64 [T, words] is set (tree_mask's; None: u <= t).  max_kv: slots that the longest
     sequence has (None: all).  Rows of no entry are left as `out` has them."""
-    hd = cache.head_dim
+    hd, device = cache.head_dim, _on(cache)
     q, q_at, T, n, q_step, xtype = _row_matrix(q, "q")
-    if n % hd:
-        raise ValueError(f"q has rows of {n} values: heads of {hd} are needed")
+    if n % hd or q.get_device() != device:
+        raise ValueError(f"q must have rows of heads of {hd}, on the current device, cuda:{device}")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != (T, n) or out.dtype is not q.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape and type")
+    elif out.shape != (T, n) or out.dtype is not q.dtype or not out.is_contiguous() or out.get_device() != device:
+        raise ValueError("out must be contiguous, of q's shape, type and device")
     mask_at, words = None, 0
     if mask is not None:
-        if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != T or not mask.is_contiguous():
-            raise ValueError(f"mask must be contiguous int64 [{T}, words]")
-        mask_at, words = mask.data_ptr(), mask.shape[1]
-    _here(cache.k, q, out, q_start, pos0, seq, mask)
-    b, most, n_head = _batch(q_start, pos0, seq, T, max_new), cache.max_pages * cache.page if max_kv is None else max_kv, n // hd
+        shape = mask.shape
+        if mask.dtype is not _I64 or len(shape) != 2 or shape[0] != T or not mask.is_contiguous() or mask.get_device() != device:
+            raise ValueError(f"mask must be contiguous int64 [{T}, words], on the current device, cuda:{device}")
+        mask_at, words = mask.data_ptr(), shape[1]
+    b, most, n_head = _entries(q_start, pos0, seq, T, max_new, device), cache.max_pages * cache.page if max_kv is None else max_kv, n // hd
     need = lib.pi_attention_tree_workspace_bytes(cache.c, b, xtype, n_head, most)
     _ws.asked = ws_at = None                                          # (the former call's scratch goes back first)
     if need:
-        ws = cache.table.new_empty(need // 4)
+        ws = q_start.new_empty(need // 4)
         ws_at = ws.data_ptr()
         if hd <= 128 and min(T, T if max_new is None else max_new) * (n_head // cache.n_head_kv) > 16:
             _ws.asked = ws_at, ws                                     # (the calls with bounded waits; kept until the next operator, for last_op_status)
@@ -601,9 +632,9 @@ def attention_tree(cache: KvCachePaged, q: torch.Tensor, q_start: torch.Tensor, 
 def kv_keep_paged(cache: KvCachePaged, path: torch.Tensor, n_path: torch.Tensor, pos0: torch.Tensor, seq: torch.Tensor | None = None) -> None:
     """The path that stays, in all layers: rows of slots pos0[i] + path[i, r] move to slots pos0[i] + r of sequence seq[i] (None: i), r < n_path[i]; path int32 [n, max_path] ascending, as tree_accept
     gives it.  The sequence then has pos0[i] + n_path[i] slots in use."""
-    n = n_path.numel()
-    if path.dim() != 2 or path.shape[0] != n:
+    n, shape, device = n_path.numel(), path.shape, _on(cache)
+    if len(shape) != 2 or shape[0] != n:
         raise ValueError(f"path must be [{n}, max_path]")
-    _here(cache.k, path, n_path, pos0, seq)
-    check(lib.pi_kv_keep_paged(cache.c, _ints(path, path.numel(), "path"), path.shape[1], _ints(n_path, n, "n_path"), _ints(pos0, n, "pos0"),
-                               None if seq is None else _ints(seq, n, "seq"), n, _stream()))
+    most = shape[1]
+    check(lib.pi_kv_keep_paged(cache.c, _whole(path, n * most, device, "path"), most, _whole(n_path, n, device, "n_path"), _whole(pos0, n, device, "pos0"),
+                               None if seq is None else _whole(seq, n, device, "seq"), n, _stream()))
