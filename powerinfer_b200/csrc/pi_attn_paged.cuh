@@ -61,17 +61,17 @@ __device__ __forceinline__ uint32_t ap_sees(const AttnPagedP & p, const SeqB & s
     return there & (u0 < 0 ? (uint32_t)x << -u0 | ap_ones(-u0) : (uint32_t)x);
 }
 
-// The same for 128 slots: the words of the mask that hold them are on their way at once
-__device__ __forceinline__ void ap_sees128(const AttnPagedP & p, const SeqB & s, int tok, int u0, uint32_t (&sees)[4]) {
+// The same for 128 slots; `word`: the first two words of the token's mask
+__device__ __forceinline__ void ap_sees128(const AttnPagedP & p, const SeqB & s, int tok, int u0, const uint64_t (&word)[2], uint32_t (&sees)[4]) {
     const int n_new = min(s.n_new, p.c.n_ctx - s.pos);
     const bool none = s.sq < 0 || tok >= n_new;
     const int end = none ? -0x40000000 : (p.mask ? n_new : tok + 1) - u0;
-    uint64_t x[3] = {0, 0, 0};
     const int lo = max(u0, 0), w = lo >> 6, sh = lo & 63;
-    if (p.mask && !none) {
+    uint64_t x[3] = {w == 0 ? word[0] : w == 1 ? word[1] : 0, w == 0 ? word[1] : 0, 0};
+    if (p.words > 2 && p.mask && !none) {
         const uint64_t * row = p.mask + (size_t)(s.first + tok) * p.words;
 #pragma unroll
-        for (int i = 0; i < 3; i++) if (w + i < p.words) x[i] = __ldg(row + w + i);
+        for (int i = 0; i < 3; i++) x[i] = w + i < p.words ? __ldg(row + w + i) : 0;
     }
     // bits from lo on, then ones in front of them for the slots before the new ones
     uint64_t a = x[0] >> sh | (sh ? x[1] << (64 - sh) : 0), b = x[1] >> sh | (sh ? x[2] << (64 - sh) : 0);

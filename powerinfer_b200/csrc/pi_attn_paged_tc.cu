@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     for (int i = 0, left = span; i < tiles && ok; i++, g++, left -= PT_KEYS) {
                         const uint32_t idesc = tc_idesc(left >= PT_KEYS ? PT_KEYS : (left + 15) / 16 * 16, false), d = tmem + T_S + buf.at * PT_KEYS;
                         const uint64_t k = tc_desc_k(keys + slot_k.at * TILE);
-                        if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1);       // the buffer's probabilities have been used
-                        ok = wait_at(slot_k.here(), slot_k.parity) && ok;
+                        ok = wait_at(slot_k.here(), slot_k.parity);
+                        if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1) && ok;       // the buffer's probabilities have been used
                         if (!ok) break;
                         tc_fence_after();
                         // (lower halves of the queries first)
@@ -333,6 +333,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             if (tiles < 0) break;
             // (-infinity times 0 would be no number)
             const float f = fmaxf(TWO ? (r < w->n_rows ? __ldg(p.factor + (size_t)(w->hk * p.b.T + w->s.first) * p.group + w->first + r) : 0.f) : fabsf(p.scale_log2), 0x1p-126f);
+            // the words of its mask (of trees of more than 128 tokens only when they are needed)
+            const int tok = r < w->n_rows ? p.by_group.of(w->first + r) : 0x7fffffff;
+            uint64_t word[2] = {0, 0};
+            if (p.mask && r < w->n_rows) {
+                const uint64_t * m = p.mask + (size_t)(w->s.first + tok) * p.words;
+                word[0] = __ldg(m);
+                if (p.words > 1) word[1] = __ldg(m + 1);
+            }
             const bool idle = (warp & 3) * 32 >= w->n_rows;           // no rows: their probabilities may be anything
             for (; at < g + tiles; at += PT_GROUPS, parity ^= 1) {
                 const int i = at - g;
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 const bool masked = info & 256u;
                 uint32_t sees[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
                 if (masked && !idle) {
-                    ap_sees128(p, w->s, r < w->n_rows ? p.by_group.of(w->first + r) : 0x7fffffff, w->k0 + i * PT_KEYS - w->s.pos, sees);
+                    ap_sees128(p, w->s, tok, w->k0 + i * PT_KEYS - w->s.pos, word, sees);
 #pragma unroll
                     for (int c = 0; c < 4; c++) sees[c] &= ((info >> (2 * c) & 1 ? 0x0000ffffu : 0u) | (info >> (2 * c + 1) & 1 ? 0xffff0000u : 0u));
                 }
