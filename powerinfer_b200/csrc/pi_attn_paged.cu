@@ -342,45 +342,49 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) k_attn_paged_join(const AttnPag
     pdl_launch();
     pdl_wait();
     if (item >= p.items) return;
+    const size_t first = (size_t)k * p.n_splits * R + r;
+    // (before it is known how many parts there are: what lies behind the last one is read, and counts nothing)
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < p.n_splits) ml = __ldcg(&p.part_ml[first + (size_t)lane * R]);
+    float u[PJ_AT][N * W];
+    auto load = [&](int i0, int last) {
+#pragma unroll
+        for (int c = 0; c < PJ_AT; c++) {
+            const float * from = p.part + (first + (size_t)min(i0 + c, last) * R) * HD + lane * W;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                if constexpr (W == 4)      { const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + j * 128)); u[c][4 * j] = x.x; u[c][4 * j + 1] = x.y; u[c][4 * j + 2] = x.z; u[c][4 * j + 3] = x.w; }
+                else if constexpr (W == 2) { const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + j * 64)); u[c][2 * j] = x.x; u[c][2 * j + 1] = x.y; }
+                else                       u[c][j] = __ldcg(from + j * 32);
+            }
+        }
+    };
+    load(0, p.n_splits - 1);
     const int of_head = p.by_tiles.of(item), nt = item - of_head * p.row_tiles, rt = R == PT_ROWS ? p.row_tiles - 1 - nt : nt, entry = p.by_heads.of(of_head), hk = of_head - entry * p.c.H;
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, entry);
     const TileP t = ap_tile(p, s, rt, R);
     if (r >= t.n_rows) return;
     const int n = max(1, min(p.n_splits, (t.seen + p.split - 1) / p.split));       // parts that were written
-    const size_t first = (size_t)k * p.n_splits * R + r;
-    float top = -INFINITY, sum = 0.f, v[N * W];
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(&p.part_ml[first + (size_t)i * R]).x);
+    float top = lane < n ? ml.x : -INFINITY, sum = 0.f, v[N * W];
+    for (int i = lane + 32; i < n; i += 32) top = fmaxf(top, __ldcg(&p.part_ml[first + (size_t)i * R]).x);
     top = warp_max(top);
     const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int j = 0; j < N * W; j++) v[j] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        float is = 0.f;
-        if (i0 + lane < n) {
-            const float2 ml = __ldcg(&p.part_ml[first + (size_t)(i0 + lane) * R]);
-            is = exp2_approx(ml.x - ref);
-            sum = fmaf(is, ml.y, sum);
+    float is = 0.f;
+    for (int i = 0; i < n; i += PJ_AT) {
+        if ((i & 31) == 0) {                                          // weights of 32 parts
+            if (i > 0 && i + lane < n) ml = __ldcg(&p.part_ml[first + (size_t)(i + lane) * R]);
+            is = i + lane < n ? exp2_approx(ml.x - ref) : 0.f;
+            if (i + lane < n) sum = fmaf(is, ml.y, sum);
         }
-        const int here = min(32, n - i0);
-        for (int i = 0; i < here; i += PJ_AT) {
-            float u[PJ_AT][N * W];
+        if (i > 0) load(i, n - 1);
 #pragma unroll
-            for (int c = 0; c < PJ_AT; c++) {
-                const float * from = p.part + (first + (size_t)(i0 + min(i + c, here - 1)) * R) * HD + lane * W;
+        for (int c = 0; c < PJ_AT; c++) {
+            const float w = __shfl_sync(0xffffffffu, is, (i + c) & 31);
+            if (i + c >= n) break;
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    if constexpr (W == 4)      { const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + j * 128)); u[c][4 * j] = x.x; u[c][4 * j + 1] = x.y; u[c][4 * j + 2] = x.z; u[c][4 * j + 3] = x.w; }
-                    else if constexpr (W == 2) { const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + j * 64)); u[c][2 * j] = x.x; u[c][2 * j + 1] = x.y; }
-                    else                       u[c][j] = __ldcg(from + j * 32);
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < PJ_AT; c++) {
-                const float w = __shfl_sync(0xffffffffu, is, min(i + c, 31));
-                if (i + c >= here) break;
-#pragma unroll
-                for (int j = 0; j < N * W; j++) v[j] = fmaf(w, u[c][j], v[j]);
-            }
+            for (int j = 0; j < N * W; j++) v[j] = fmaf(w, u[c][j], v[j]);
         }
     }
     sum = warp_sum(sum);
@@ -406,10 +410,12 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) k_attn_paged_join(const AttnPag
 // ---- how the work is cut
 struct PaPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t words, q, factor, ml, part; };
 
-// CTAs run in rounds of as many as the SMs hold.  Items that fill rounds are a CTA each; those of the last round, or all where there are fewer, are split into ranges of at least PA_LEAST
-// slots: into the number of parts for which its CTAs, in rounds of their own, take the least.  A CTA costs as much as its slots and PA_TURN times 64 more (on tcgen05 PA_TURN_TC), the kernel that joins as
-// PA_TURN times 64.
-static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 10, PA_ROUNDS = 4;
+// Items are a CTA (a piece of work) each, or split into ranges of at least PA_LEAST slots: none of them, those beyond as many as fill rounds of all CTAs that the SMs hold, or
+// all; into the number of parts that is estimated to take the least.  A piece costs as much as its slots and PA_TURN times 64 more (on tcgen05, where parts are larger too, PA_TURN_TC
+// whole and PA_TURN_PART as a part), the kernel that joins as PA_TURN times 64.
+// With mma.sync: pieces are as long as max_kv says and run in rounds.  On tcgen05 CTAs take one after the other: the same for one sequence; of several half of that and half of the time of sequences of half
+// to all of max_kv's length (work over SMs, and half of a piece at the end).
+static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 3, PA_TURN_PART = 8, PA_ROUNDS = 4;        // (more rounds of parts than that: room for the parts, and nothing gained)
 static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_head, int max_kv) {
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
@@ -418,13 +424,23 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_hea
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? PT_KEYS : PA_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), rest = items % slots, units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
-    const int64_t turn = r.tc ? PA_TURN_TC : PA_TURN;
-    int64_t n = 1, least = -1;
-    for (int64_t k = 1; rest && k <= 128 && (k == 1 || k * PA_LEAST < keys + PA_LEAST); k++) {
-        const int64_t rounds = (rest * k + slots - 1) / slots, cost = rounds * ((units + k - 1) / k + turn) + (k > 1 ? PA_TURN : 0);
-        if (rounds > PA_ROUNDS) break;
-        if (least < 0 || cost < least) { least = cost; n = k; }
+    const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
+    const int turn = r.tc ? PA_TURN_TC : PA_TURN, turn_part = r.tc ? PA_TURN_PART : PA_TURN;
+    int64_t n = 1, rest = 0;
+    double least = -1;
+    for (int all = 0; all <= (r.tc ? 1 : 0); all++) {
+        const int64_t of = all ? items : items % slots, whole = items - of;           // items that are split, and not
+        for (int64_t k = 1; of && k <= 128 && (k == 1 || k * PA_LEAST < keys + PA_LEAST); k++) {
+            const int64_t rounds = (of * k + slots - 1) / slots, part = (units + k - 1) / k + (k > 1 ? turn_part : turn);
+            if (k > 1 && rounds > PA_ROUNDS * (all ? 2 : 1)) break;
+            double cost = (double)(whole / slots * (units + turn) + rounds * part);
+            if (r.tc && b.n > 1) {
+                const double work = (0.75 * items * units + whole * turn + of * k * (part - (units + k - 1) / k)) / slots + 0.5 * part, longest = (double)(whole ? units + turn : part);
+                cost = 0.5 * (cost + (whole + of * k > slots && work > longest ? work : longest));
+            }
+            if (k > 1) cost += PA_TURN;
+            if (least < 0 || cost < least) { least = cost; n = k; rest = of; }
+        }
     }
     const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;
     r.split = (int)per; r.n_splits = (int)((keys + per - 1) / per);
