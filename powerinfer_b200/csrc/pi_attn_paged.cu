@@ -252,8 +252,16 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                 ldsm4_t(b, vt + S::at(v_row, n + v_piece));
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    if constexpr (TWO) mma16816(o[n + h], pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
-                    mma16816(o[n + h], pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
+                    if constexpr (TWO) {                              // (the tensor cores cut FP32 sums: FP32 rows' are added with rounding)
+                        float w[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma16816(w, pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
+                        mma16816(w, pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n + h][e] += w[e];
+                    } else {
+                        mma16816(o[n + h], pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
+                        mma16816(o[n + h], pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
+                    }
                 }
             }
         } else {
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                         const uint32_t b0 = b[2 * h] & lo8, b1 = b[2 * h + 1] & hi8;
                         float w[4] = {0.f, 0.f, 0.f, 0.f}, wl[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816(w, pa[0], pa[1], pa[2], pa[3], b0, b1);
-                        if constexpr (TWO) mma16816(wl, pl[0], pl[1], pl[2], pl[3], b0, b1);
+                        mma16816(wl, pl[0], pl[1], pl[2], pl[3], b0, b1);
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             if (e < 2 ? see0 : see1) o[n + h][e] += fabsf(w[e]) <= FLT_MAX ? w[e] + wl[e] : w[e];
