@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             PtRing qs(s_qfull);
             const uint32_t qempty = smem_u32(s_qempty);
             bool ok = true;
-            for (int n = 0, u = 0; ok; n++) {
+            int u = 0;                                                // pieces with tiles
+            for (int n = 0; ok; n++) {
                 if (n >= PT_WORK && !(ok = wait(s_wempty + n % PT_WORK, n / PT_WORK & 1 ^ 1))) break;
                 PtWork w;
                 w.tiles = -1;
@@ -312,8 +313,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 done_with(n);
             }
-            // (copies of queries in flight when a wait ran out: those of the last piece at most)
-            if (!ok && lane == 0) for (int i = 0; i < QB; i++) for (int spins = 0; spins < 1024 && !mbar_try_wait(s_qfull + i, 0u) && !mbar_try_wait(s_qfull + i, 1u); spins++) {}
+            if (!ok && lane == 0) ring_land(s_qfull, u, QB);          // (else they have been waited for)
             __syncwarp();
         }
     } else if (warp < 8 + 4 * PT_GROUPS) {
