@@ -356,31 +356,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 const int chunks = idle ? 0 : min(4, (span - i * PT_KEYS + 31) >> 5);         // of 32 slots
                 float m = -INFINITY;
-                // (the scores of slots that a row does not see are put back as -infinity: their probabilities are 0)
-                auto largest = [&](auto with_mask) {
 #pragma unroll 1
-                    for (int c = 0; c < chunks; c++) {
-                        float x[32];
-                        tc_ld32(x, mine + 32 * c);
-                        if (decltype(with_mask)::value) {
-                            const uint32_t see = c == 0 ? sees[0] : c == 1 ? sees[1] : c == 2 ? sees[2] : sees[3];
+                for (int c = 0; c < chunks; c++) {
+                    float x[32];
+                    tc_ld32(x, mine + 32 * c);
+                    if (masked) {                                     // the scores of slots that a row does not see are put back as -infinity: their probabilities are 0
+                        const uint32_t see = c == 0 ? sees[0] : c == 1 ? sees[1] : c == 2 ? sees[2] : sees[3];
+                        if (__any_sync(0xffffffffu, see != 0xffffffffu)) {
 #pragma unroll
                             for (int j = 0; j < 32; j++) if (!(see >> j & 1)) x[j] = -INFINITY;
                             tc_st32(mine + 32 * c, x);
                         }
-                        float a[4];
-#pragma unroll
-                        for (int j = 0; j < 4; j++) a[j] = max3(x[j], x[4 + j], x[8 + j]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[12 + j], x[16 + j]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[20 + j], x[24 + j]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) a[j] = fmaxf(a[j], x[28 + j]);
-                        m = fmaxf(m, max3(a[0], a[1], fmaxf(a[2], a[3])));
                     }
-                };
-                if (masked) { largest(std::true_type()); tc_wait_st(); } else largest(std::false_type());
+                    float a[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) a[j] = max3(x[j], x[4 + j], x[8 + j]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[12 + j], x[16 + j]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) a[j] = max3(a[j], x[20 + j], x[24 + j]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) a[j] = fmaxf(a[j], x[28 + j]);
+                    m = fmaxf(m, max3(a[0], a[1], fmaxf(a[2], a[3])));
+                }
+                if (masked) tc_wait_st();
                 const bool none = m == -INFINITY;
                 m *= f;
                 const float2 ref = f2(none ? 14.f : 14.f - m), fc = f2(f);
@@ -407,12 +406,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     // the tile's values: a row a thread.  Rows of slots that are not there become zeros; so do those with a value that is not finite, and who sees them has no numbers
                     const int slot = at % NW;
                     if (!(ok = wait(s_vfull + slot, at / NW & 1))) break;
-                    const bool is = info >> (r >> 4) & 1 && w->k0 + i * PT_KEYS + r < w->there;
+                    const int at_slot = w->k0 + i * PT_KEYS + r;
+                    const bool is = info >> (r >> 4) & 1 && at_slot < w->there;
                     const uint32_t row = values + (uint32_t)slot * TILE + (uint32_t)r * 128u;
                     const __half2 null = __floats2half2_rn(0.f, 0.f);
                     __half2 zero[4] = {null, null, null, null};       // no more 0 where a value is not finite
-                    if (is) {
-#pragma unroll 2
+                    if (is && at_slot >= w->clear) {                  // (what every row sees may be anything)
+#pragma unroll 4
                         for (int u = 0; u < SUBS * 8; u++) {
                             uint4 x;
                             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(row + (uint32_t)(u >> 3) * PT_SUB + (uint32_t)((u + lane) & 7) * 16u));
