@@ -165,7 +165,8 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
         const int j0 = first + it * PA_STEP;
         const bool masked = j0 + 16 > s.pos;                          // not wholly of the context, which every row sees
         // ---- scores of 16 slots
-        float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        // (the tensor cores cut sums at every step: lower parts have sums of their own, whose steps are small)
+        float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, low[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int k = 0; k < S::KS; k++) {
             uint32_t b[4];
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
             if constexpr (Q_REGS) {
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    if constexpr (TWO) mma16816(x[n], a_low[k][0], a_low[k][1], a_low[k][2], a_low[k][3], b[2 * n], b[2 * n + 1]);
+                    if constexpr (TWO) mma16816(low[n], a_low[k][0], a_low[k][1], a_low[k][2], a_low[k][3], b[2 * n], b[2 * n + 1]);
                     mma16816(x[n], a[k][0], a[k][1], a[k][2], a[k][3], b[2 * n], b[2 * n + 1]);
                 }
             } else {
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                 if constexpr (TWO) {
                     ldsm4(w, q_at + PA_R * Q::PITCH + k * 32);
 #pragma unroll
-                    for (int n = 0; n < 2; n++) mma16816(x[n], w[0], w[1], w[2], w[3], b[2 * n], b[2 * n + 1]);
+                    for (int n = 0; n < 2; n++) mma16816(low[n], w[0], w[1], w[2], w[3], b[2 * n], b[2 * n + 1]);
                 }
                 ldsm4(w, q_at + k * 32);
 #pragma unroll
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    y[n][j] = x[n][2 * h + j] * f[h];
+                    y[n][j] = (TWO ? x[n][2 * h + j] + low[n][2 * h + j] : x[n][2 * h + j]) * f[h];
                     if (masked && !(sees[h] >> (n * 8 + 2 * q + j) & 1)) y[n][j] = -INFINITY;
                 }
             float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));

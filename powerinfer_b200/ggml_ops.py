@@ -547,7 +547,7 @@ def tree_mask(parents: torch.Tensor, q_start: torch.Tensor, pos0: torch.Tensor, 
     if words is None:
         words = -(-(T if max_new is None else max_new) // 64) or 1
     at, b = _whole(parents, T, device, "parents"), _entries(q_start, pos0, None, T, max_new, device)
-    mask, pos = parents.new_empty((T, max(0, words)), dtype=_I64), parents.new_empty(T)
+    mask, pos = torch.empty(T, max(0, words), dtype=_I64, device=parents.device), parents.new_empty(T)
     check(lib.pi_tree_mask(b, at, mask.data_ptr(), words, pos.data_ptr(), _stream()))
     return mask, pos
 
@@ -559,7 +559,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, choice: torch.Tenso
     most = T if max_new is None else max_new
     a, b, c = _whole(tokens, T, device, "tokens"), _whole(parents, T, device, "parents"), _whole(choice, T, device, "choice")
     of = _KV_BATCH.pack(_whole(q_start, n + 1, device, "q_start"), 0, 0, n, T, most)
-    path, n_path, then = tokens.new_empty((n, max(0, most))), tokens.new_empty(n), tokens.new_empty(n)
+    path, n_path, then = tokens.new_empty(n, max(0, most)), tokens.new_empty(n), tokens.new_empty(n)
     check(lib.pi_tree_accept(of, a, b, c, path.data_ptr(), n_path.data_ptr(), then.data_ptr(), _stream()))
     return path, n_path, then
 
