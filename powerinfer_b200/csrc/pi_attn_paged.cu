@@ -22,7 +22,7 @@
 
 namespace pi {
 
-static constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, PA_STEP = PA_WARPS * 16, PA_R = 16;
+static constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, PA_STEP = PA_WARPS * 16;
 static constexpr float PA_RISE = 7.f, PA_P = 256.f;                   // bits a maximum may lag; probabilities are held times this (2^7 * 256 < 65504)
 
 template <int HD> struct PaShape {
@@ -32,13 +32,13 @@ template <int HD> struct PaShape {
     }
     static constexpr int STAGES = HD <= 96 ? 4 : 3, STAGE = 2 * 16 * HD * 2;
     static constexpr int CTAS = HD == 64 ? 3 : HD <= 128 ? 2 : 1;     // that an SM holds
-    static constexpr size_t RING = (size_t)PA_WARPS * STAGES * STAGE, JOIN = (size_t)PA_WARPS * PA_R * (HD + 4) * 4, QUERIES = 2 * PA_R * (2 * HD + 16);
+    static constexpr size_t RING = (size_t)PA_WARPS * STAGES * STAGE, JOIN = (size_t)PA_WARPS * 16 * (HD + 4) * 4, QUERIES = 2 * 16 * (2 * HD + 16);
     static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + QUERIES;
 };
 
-// 16 rows in shared memory as halves [upper, lower][row][HD + 8], and the factors of their scores
-template <int HD, bool TWO> struct PaQueries {
-    static constexpr int TPR = PA_THREADS / PA_R, W = HD / 4, N = W / TPR, PITCH = 2 * HD + 16;
+// R rows in shared memory as halves [upper, lower][row][HD + 8], and the factors of their scores
+template <int HD, bool TWO, int R> struct PaQueries {
+    static constexpr int TPR = PA_THREADS / R, W = HD / 4, N = (W + TPR - 1) / TPR, PITCH = 2 * HD + 16;
     float4 x[N];
     __device__ __forceinline__ void load(const AttnPagedP & p, const SeqB & s, const TileP & t, int hk) {
         const int r = threadIdx.x / TPR, j = threadIdx.x % TPR, row = t.first + r, tok = p.by_group.of(row);
@@ -46,7 +46,7 @@ template <int HD, bool TWO> struct PaQueries {
 #pragma unroll
         for (int u = 0; u < N; u++) {
             x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < t.n_rows) x[u] = aq_query(p.xtype, p.q, at + (j + u * TPR) * 4);
+            if (r < t.n_rows && j + u * TPR < W) x[u] = aq_query(p.xtype, p.q, at + (j + u * TPR) * 4);
         }
     }
     __device__ __forceinline__ void put(const AttnPagedP & p, unsigned char * to, float * factor) {
@@ -69,21 +69,23 @@ template <int HD, bool TWO> struct PaQueries {
             uint2 hi, lo;
             aq_split(x[u].x * up, x[u].y * up, hi.x, lo.x);
             aq_split(x[u].z * up, x[u].w * up, hi.y, lo.y);
+            if (j + u * TPR >= W) break;
             *reinterpret_cast<uint2 *>(to + r * PITCH + (j + u * TPR) * 8) = hi;
-            if (TWO) *reinterpret_cast<uint2 *>(to + (PA_R + r) * PITCH + (j + u * TPR) * 8) = lo;
+            if (TWO || R == 8) *reinterpret_cast<uint2 *>(to + (R + r) * PITCH + (j + u * TPR) * 8) = lo;      // (of FP16 rows 0)
         }
     }
 };
 
-// TWO: two halves for queries and probabilities (FP32 rows)
-template <int HD, bool TWO>
+// TWO: two halves for queries (FP32 rows).  R: 16 rows, or 8: then rows 0 .. 7 of the products' operands are the upper and rows 8 .. 15 the lower halves of queries and of probabilities, one product in the
+// place of two (FP32, 64 heads over 8 of 128: 8 sequences of 8000 slots 44 us with two products, 37 so; one of 32768 35 and 32).
+template <int HD, bool TWO, int R>
 __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(const AttnPagedP p) {
     using S = PaShape<HD>;
-    using Q = PaQueries<HD, TWO>;
-    constexpr int ST = S::STAGES;
-    constexpr bool Q_REGS = HD <= 128;                                // queries stay in registers
+    using Q = PaQueries<HD, TWO, R>;
+    constexpr int ST = S::STAGES, NH = R / 8, NO = 2 * NH;            // rows and sums of a lane
+    constexpr bool PACK = R == 8, Q_REGS = PACK || HD <= 128;         // queries stay in registers
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float s_m[PA_WARPS][PA_R], s_l[PA_WARPS][PA_R], s_f[PA_R];
+    __shared__ float s_m[PA_WARPS][R], s_l[PA_WARPS][R], s_f[R];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const AqItem wk = ap_item(p, blockIdx.x);
     const int split = wk.split, hk = wk.hk;
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
     pdl_wait();
     if (blockIdx.x == 0 && threadIdx.x == 0 && p.status) *p.status = 0u;          // (no wait of this kernel runs out)
     const SeqB s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, wk.entry);
-    const TileP t = ap_tile(p, s, wk.rt, PA_R);
+    const TileP t = ap_tile(p, s, wk.rt, R);
     if (t.n_rows <= 0) return;
     const int k0 = split * p.split, k1 = split == wk.n_splits - 1 ? t.seen : min(t.seen, k0 + p.split);
     if (k0 >= k1 && split > 0) return;                                // (split 0 answers for rows that see nothing)
@@ -131,28 +133,28 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
 
     qs.put(p, queries, s_f);
     __syncthreads();
-    float f[2], m[2], l[2]; int tok[2]; bool any[2];                  // of rows g and g + 8
+    float f[NH], m[NH], l[NH]; int tok[NH]; bool any[NH];             // of rows g and g + 8
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < NH; h++) {
         const int r = g + 8 * h;
         tok[h] = r < t.n_rows ? p.by_group.of(t.first + r) : 0x7fffffff;
         f[h] = s_f[r]; m[h] = -INFINITY; l[h] = 0.f; any[h] = false;
     }
     // ldmatrix: a lane names a row of one of four 8 x 8 pieces
     const uint32_t q_at = smem_u32(queries) + (uint32_t)((lane & 15) * Q::PITCH + (lane >> 4) * 16);
-    uint32_t a[Q_REGS ? S::KS : 1][4], a_low[Q_REGS && TWO ? S::KS : 1][4];
+    uint32_t a[Q_REGS ? S::KS : 1][4], a_low[Q_REGS && TWO && !PACK ? S::KS : 1][4];
     if constexpr (Q_REGS) {
 #pragma unroll
         for (int k = 0; k < S::KS; k++) {
             ldsm4(a[k], q_at + k * 32);
-            if constexpr (TWO) ldsm4(a_low[k], q_at + PA_R * Q::PITCH + k * 32);
+            if constexpr (TWO && !PACK) ldsm4(a_low[k], q_at + R * Q::PITCH + k * 32);
         }
     }
-    float o[S::NT][4];
+    float o[S::NT][NO];
 #pragma unroll
     for (int n = 0; n < S::NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[n][j] = 0.f;
+        for (int j = 0; j < NO; j++) o[n][j] = 0.f;
     const int k_row = (lane & 7) + (lane >> 4) * 8, k_piece = lane >> 3 & 1, v_row = lane & 15, v_piece = lane >> 4;
 
     for (int it = 0; it < steps; it++) {
@@ -174,13 +176,13 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
             if constexpr (Q_REGS) {
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    if constexpr (TWO) mma16816(low[n], a_low[k][0], a_low[k][1], a_low[k][2], a_low[k][3], b[2 * n], b[2 * n + 1]);
+                    if constexpr (TWO && !PACK) mma16816(low[n], a_low[k][0], a_low[k][1], a_low[k][2], a_low[k][3], b[2 * n], b[2 * n + 1]);
                     mma16816(x[n], a[k][0], a[k][1], a[k][2], a[k][3], b[2 * n], b[2 * n + 1]);
                 }
             } else {
                 uint32_t w[4];
                 if constexpr (TWO) {
-                    ldsm4(w, q_at + PA_R * Q::PITCH + k * 32);
+                    ldsm4(w, q_at + R * Q::PITCH + k * 32);
 #pragma unroll
                     for (int n = 0; n < 2; n++) mma16816(low[n], w[0], w[1], w[2], w[3], b[2 * n], b[2 * n + 1]);
                 }
@@ -190,23 +192,26 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
             }
         }
         // ---- probabilities, as A operands of the value products
-        uint32_t sees[2] = {0xffffu, 0xffffu};
+        uint32_t sees[NH];
+#pragma unroll
+        for (int h = 0; h < NH; h++) sees[h] = 0xffffu;
         if (masked) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) sees[h] = ap_sees(p, s, tok[h], j0 - s.pos) & 0xffffu;
+            for (int h = 0; h < NH; h++) sees[h] = ap_sees(p, s, tok[h], j0 - s.pos) & 0xffffu;
         }
         uint32_t pa[4], pl[4];
-        float alpha[2] = {1.f, 1.f};
+        float alpha[NH];
         bool moved = false;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < NH; h++) {
+            alpha[h] = 1.f;
             any[h] |= sees[h] != 0;
             float y[2][2];
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    y[n][j] = (TWO ? x[n][2 * h + j] + low[n][2 * h + j] : x[n][2 * h + j]) * f[h];
+                    y[n][j] = (PACK ? x[n][j] + x[n][2 + j] : TWO ? x[n][2 * h + j] + low[n][2 * h + j] : x[n][2 * h + j]) * f[h];
                     if (masked && !(sees[h] >> (n * 8 + 2 * q + j) & 1)) y[n][j] = -INFINITY;
                 }
             float top = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[1][0], y[1][1]));
@@ -224,12 +229,15 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
             for (int n = 0; n < 2; n++) {
                 const float p0 = exp2_approx(y[n][0] - ref), p1 = exp2_approx(y[n][1] - ref);
                 l[h] += p0 + p1;
-                aq_split(p0 * PA_P, p1 * PA_P, pa[2 * n + h], pl[2 * n + h]);
+                if constexpr (PACK) aq_split(p0 * PA_P, p1 * PA_P, pa[2 * n], pa[2 * n + 1]);
+                else                aq_split(p0 * PA_P, p1 * PA_P, pa[2 * n + h], pl[2 * n + h]);
             }
         }
         if (moved && it > 0) {
 #pragma unroll
-            for (int n = 0; n < S::NT; n++) { o[n][0] *= alpha[0]; o[n][1] *= alpha[0]; o[n][2] *= alpha[1]; o[n][3] *= alpha[1]; }
+            for (int n = 0; n < S::NT; n++)
+#pragma unroll
+                for (int j = 0; j < NO; j++) o[n][j] *= alpha[j >> 1];
         }
         // ---- values
         bool odd = false;                                             // a value that is not finite, where not every row sees every slot
@@ -253,7 +261,11 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                 ldsm4_t(b, vt + S::at(v_row, n + v_piece));
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    if constexpr (TWO) {                              // (the tensor cores cut FP32 sums: FP32 rows' are added with rounding)
+                    if constexpr (PACK) {
+                        float w[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma16816(w, pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
+                        o[n + h][0] += w[0] + w[2]; o[n + h][1] += w[1] + w[3];
+                    } else if constexpr (TWO) {                       // (the tensor cores cut FP32 sums: FP32 rows' are added with rounding)
                         float w[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816(w, pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
                         mma16816(w, pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
@@ -273,7 +285,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                 const bool mine = (j >> 1 & 3) == q;                  // this lane's slots are 2q, 2q + 1, 8 + 2q, 9 + 2q
                 const uint32_t keep = mine ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
                 const uint32_t lo8 = j < 8 ? keep : 0u, hi8 = j < 8 ? 0u : keep;
-                const bool see0 = sees[0] >> j & 1, see1 = sees[1] >> j & 1;
+                const bool see0 = sees[0] >> j & 1, see1 = sees[NH - 1] >> j & 1;
 #pragma unroll
                 for (int n = 0; n < S::NT; n += 2) {
                     uint32_t b[4];
@@ -283,9 +295,10 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                         const uint32_t b0 = b[2 * h] & lo8, b1 = b[2 * h + 1] & hi8;
                         float w[4] = {0.f, 0.f, 0.f, 0.f}, wl[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816(w, pa[0], pa[1], pa[2], pa[3], b0, b1);
-                        mma16816(wl, pl[0], pl[1], pl[2], pl[3], b0, b1);
+                        if constexpr (!PACK) mma16816(wl, pl[0], pl[1], pl[2], pl[3], b0, b1);
+                        else                 { wl[0] = w[2]; wl[1] = w[3]; }
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
+                        for (int e = 0; e < NO; e++)
                             if (e < 2 ? see0 : see1) o[n + h][e] += fabsf(w[e]) <= FLT_MAX ? w[e] + wl[e] : w[e];
                     }
                 }
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
     constexpr int PITCH = HD + 4;
     float * so = reinterpret_cast<float *>(smem);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < NH; h++) {
         float sum = l[h];
         if (any[h] && m[h] == -INFINITY) sum = __int_as_float(0x7fc00000);         // (every score that it sees is -infinity: no number)
         const bool none = tok[h] >= p.c.n_ctx - s.pos;                // a token without a slot of its own
@@ -308,12 +321,12 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const int r = g + 8 * h;
         if (q == 0) { s_m[warp][r] = m[h]; s_l[warp][r] = sum; }
-        float * row = so + (size_t)(warp * PA_R + r) * PITCH + 2 * q;
+        float * row = so + (size_t)(warp * R + r) * PITCH + 2 * q;
 #pragma unroll
         for (int n = 0; n < S::NT; n++) *reinterpret_cast<float2 *>(row + n * 8) = none ? make_float2(0.f, 0.f) : make_float2(o[n][2 * h], o[n][2 * h + 1]);
     }
     __syncthreads();
-    const size_t part0 = ((size_t)(wk.item - p.whole) * p.n_splits + split) * PA_R;
+    const size_t part0 = ((size_t)(wk.item - p.whole) * p.n_splits + split) * R;
     for (int e = threadIdx.x; e < t.n_rows * (HD / 4); e += PA_THREADS) {
         const int r = e / (HD / 4), d = (e - r * (HD / 4)) * 4;
         float top = s_m[0][r];
@@ -324,7 +337,7 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
 #pragma unroll
         for (int w = 0; w < PA_WARPS; w++) {
             const float is = exp2_approx(s_m[w][r] - ref), k = is * (1.f / PA_P);
-            const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * PA_R + r) * PITCH + d);
+            const float4 u = *reinterpret_cast<const float4 *>(so + (size_t)(w * R + r) * PITCH + d);
             sum = fmaf(is, s_l[w][r], sum);
             v.x = fmaf(k, u.x, v.x); v.y = fmaf(k, u.y, v.y); v.z = fmaf(k, u.z, v.z); v.w = fmaf(k, u.w, v.w);
         }
@@ -429,7 +442,7 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_hea
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
     r.tc = attn_paged_tc_takes(c.hd, rows);
-    r.R = r.tc ? PT_ROWS : PA_R;
+    r.R = r.tc ? PT_ROWS : rows <= 8 ? 8 : 16;
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? PT_KEYS : PA_STEP;
     const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
@@ -469,23 +482,23 @@ size_t attn_paged_scratch(const KvPaged & c, const RaggedB & b, int xtype, int n
     return r.words + r.q + r.factor + r.ml + r.part;
 }
 
-template <int HD, bool TWO>
+template <int HD, bool TWO, int R>
 static int pa_go(const AttnPagedP & p, cudaStream_t st) {
     static bool done[16] = {false};
     int dev = 0;
     PI_CUDA(cudaGetDevice(&dev));
     constexpr size_t smem = PaShape<HD>::SMEM;
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        PI_CUDA(cudaFuncSetAttribute(k_attn_paged<HD, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        PI_CUDA(cudaFuncSetAttribute(k_attn_paged<HD, TWO, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    PI_CUDA(launch_k(k_attn_paged<HD, TWO>, dim3(ap_grid(p)), dim3(PA_THREADS), smem, st, true, p));
+    PI_CUDA(launch_k(k_attn_paged<HD, TWO, R>, dim3(ap_grid(p)), dim3(PA_THREADS), smem, st, true, p));
     return PI_OK;
 }
 
 template <int HD>
 static int pa_run(const AttnPagedP & p, const PaPlan & r, cudaStream_t st) {
-    const int rc = r.tc ? launch_attn_paged_tc(p, st) : p.xtype == PI_TYPE_F16 ? pa_go<HD, false>(p, st) : pa_go<HD, true>(p, st);
+    const int rc = r.tc ? launch_attn_paged_tc(p, st) : r.R == 8 ? (p.xtype == PI_TYPE_F16 ? pa_go<HD, false, 8>(p, st) : pa_go<HD, true, 8>(p, st)) : p.xtype == PI_TYPE_F16 ? pa_go<HD, false, 16>(p, st) : pa_go<HD, true, 16>(p, st);
     if (rc) return rc;
     if (p.items > p.whole) PI_CUDA(launch_k(k_attn_paged_join<HD>, dim3((unsigned)(((int64_t)(p.items - p.whole) * r.R + PJ_WARPS - 1) / PJ_WARPS)), dim3(PJ_WARPS * 32), 0, st, true, p, r.R));
     return PI_OK;
