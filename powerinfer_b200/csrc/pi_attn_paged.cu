@@ -441,11 +441,12 @@ static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 3, PA_TURN_PART =
 static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_head, int max_kv) {
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
-    r.tc = attn_paged_tc_takes(c.hd, rows);
+    const int64_t keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
+    r.tc = attn_paged_tc_takes(c.hd, rows, (int64_t)b.n * c.H * keys * c.hd);
     r.R = r.tc ? PT_ROWS : rows <= 8 ? 8 : 16;
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? PT_KEYS : PA_STEP;
-    const int64_t items = (int64_t)b.n * c.H * r.row_tiles, keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
+    const int64_t items = (int64_t)b.n * c.H * r.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
     const int turn = r.tc ? PA_TURN_TC : PA_TURN, turn_part = r.tc ? PA_TURN_PART : PA_TURN;
     int64_t n = 1, rest = 0;
