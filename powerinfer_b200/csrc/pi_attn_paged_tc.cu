@@ -20,8 +20,7 @@
 #include "pi_tc.cuh"
 #include "pi_tc_math.cuh"
 
-#include <cfloat>
-#include <type_traits>
+#include <cstdlib>
 
 namespace pi {
 
@@ -607,7 +606,13 @@ __global__ void __launch_bounds__(256) k_attn_paged_queries(const AttnPagedP p, 
 // With mma.sync every 16 rows of a KV head read its keys and values again, 16 us for 2^25 values of keys (after the first ones); here 128 rows take 5 us more whatever there is, and 7 us more for as many values.
 // Both sides measured (us, here and with mma.sync; FP32, 4 query heads a KV head, head_dim 128): 8 sequences of 4096 slots and 8 KV heads 16 rows 39 and 28, 24 rows 39 and 43, 64 rows 41 and 74; one such
 // sequence 24 rows 17 and 14, 48 rows 18 and 16, 64 rows 18 and 17; one of 500 slots and 32 KV heads 64 rows 15 and 14.
-bool attn_paged_tc_takes(int hd, int64_t rows, int64_t values) { return hd <= 128 && rows > 16 && ((rows + 15) / 16 - 1) * 16 * (double)values > 5.0 * (1 << 25) + 7.0 * values; }
+// (PI_ATTN_TREE_TC=1 takes 17 rows and more whatever there is, 0 none: a diagnostic switch, read once.)
+bool attn_paged_tc_takes(int hd, int64_t rows, int64_t values) {
+    static int forced = -2;
+    if (forced == -2) { const char * v = getenv("PI_ATTN_TREE_TC"); forced = v ? v[0] != '0' : -1; }
+    if (hd > 128 || rows <= 16 || forced == 0) return false;
+    return forced == 1 || ((rows + 15) / 16 - 1) * 16 * (double)values > 5.0 * (1 << 25) + 7.0 * values;
+}
 
 template <int HD, bool TWO>
 static int pt_go(const AttnPagedP & a, cudaStream_t st) {

@@ -84,7 +84,7 @@ int pi_kv_append_paged(const pi_kv_paged * cache, const pi_kv_batch * batch, int
                    "kv_append_paged: keys or values overlap q_out");
     }
     const int64_t heads = (q ? n_head : 0) + 2 * (int64_t)a.c.H;
-    PI_REQUIRE((int64_t)a.b.max_new * (heads * a.c.hd / 2048 + 1) < (int64_t(1) << 31) && heads * a.c.hd <= KV_BIG, "kv_append_paged: too many tokens for one call");
+    PI_REQUIRE((int64_t)a.b.max_new * (heads * a.c.hd / 512 + 2) < (int64_t(1) << 31) && heads * a.c.hd <= KV_BIG, "kv_append_paged: too many tokens for one call");
     a.xtype = xtype; a.x[0] = q; a.x[1] = k; a.x[2] = v; a.x_stride[0] = q_stride; a.x_stride[1] = k_stride; a.x_stride[2] = v_stride;
     a.q_out = q_out; a.q_out_stride = q_out_stride; a.n_head = n_head; a.pos = pos; a.freqs = freqs; a.n_rot = freqs ? n_rot : 0; a.halves = neox != 0; a.mscale = mscale;
     return launch_kv_append_paged(a, (cudaStream_t)stream);

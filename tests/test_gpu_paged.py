@@ -119,6 +119,19 @@ def test_tree_accept(ops, news, vocab):
     assert all(x == -1 for r, n in zip(path.cpu().tolist(), n_path.cpu().tolist()) for x in r[n:])
 
 
+def test_no_trees(ops):
+    """No entries, entries without tokens, no rows at all, no room for a path."""
+    none, z = ints([]), ints([0])
+    mask, pos = ops.tree_mask(none, z, none)
+    assert mask.shape == (0, 1) and pos.shape == (0,)
+    mask, pos = ops.tree_mask(none, ints([0, 0, 0]), ints([5, 6]), max_new=70)
+    assert mask.shape == (0, 2)
+    for T, most in ((0, 0), (0, 3), (4, 0), (4, 3)):
+        t = ints([1] * T)
+        path, n_path, then = ops.tree_accept(t, t, t, ints([0, 0, 0, 0]), max_new=most)
+        assert path.shape == (3, most) and n_path.tolist() == [0] * 3 and then.tolist() == [-1] * 3 and path.eq(-1).all()
+
+
 # ------------------------------------------------------------------------------------------------ append
 
 def pair_sums(x, hd, n_rot, halves):
@@ -554,6 +567,16 @@ def test_other_streams_and_captured_graphs(ops):
         want = step(four)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, captured)) and torch.equal(three.k, four.k) and torch.equal(three.v, four.v)
+
+
+def test_the_same_on_tcgen05_whatever_the_size():
+    """Small calls of many rows run with mma.sync: all of the attention's tests again with those on tcgen05."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-m", "pytest", __file__, "-x", "-q", "-p", "no:cacheprovider", "-k", "attention or mask or row or sizes or parts or pool or speculative or streams"],
+                       env={**os.environ, "PI_ATTN_TREE_TC": "1"}, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-4000:]
 
 
 def test_refusals(ops):
