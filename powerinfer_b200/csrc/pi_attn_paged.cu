@@ -446,23 +446,23 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_hea
     r.R = r.tc ? PT_ROWS : rows <= 8 ? 8 : 16;
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? PT_KEYS : PA_STEP;
-    const int64_t items = (int64_t)b.n * c.H * r.row_tiles;
+    const int64_t items = (int64_t)b.n * c.H * r.row_tiles, pieces = r.tc && c.hd > 128 ? 2 : 1;       // (pieces of work that an item is)
     const int64_t slots = (int64_t)sm_count() * (r.tc ? 1 : c.hd == 64 ? 3 : c.hd <= 128 ? 2 : 1), units = (keys + PA_LEAST / 4 - 1) / (PA_LEAST / 4);
     const int turn = r.tc ? PA_TURN_TC : PA_TURN, turn_part = r.tc ? PA_TURN_PART : PA_TURN;
     int64_t n = 1, rest = 0;
     double least = -1;
     for (int all = 0; all <= (r.tc ? 1 : 0); all++) {
-        const int64_t of = all ? items : items % slots, whole = items - of;           // items that are split, and not
+        const int64_t of = all ? items * pieces : items * pieces % slots / pieces * pieces, whole = items * pieces - of;        // pieces that are split, and not
         for (int64_t k = 1; of && k <= 128 && (k == 1 || k * PA_LEAST < keys + PA_LEAST); k++) {
             const int64_t rounds = (of * k + slots - 1) / slots, part = (units + k - 1) / k + (k > 1 ? turn_part : turn);
             if (k > 1 && rounds > PA_ROUNDS * (all ? 2 : 1)) break;
             double cost = (double)(whole / slots * (units + turn) + rounds * part);
             if (r.tc && b.n > 1) {
-                const double work = (0.75 * items * units + whole * turn + of * k * (part - (units + k - 1) / k)) / slots + 0.5 * part, longest = (double)(whole ? units + turn : part);
+                const double work = (0.75 * items * pieces * units + whole * turn + of * k * (part - (units + k - 1) / k)) / slots + 0.5 * part, longest = (double)(whole ? units + turn : part);
                 cost = 0.5 * (cost + (whole + of * k > slots && work > longest ? work : longest));
             }
             if (k > 1) cost += PA_TURN;
-            if (least < 0 || cost < least) { least = cost; n = k; rest = of; }
+            if (least < 0 || cost < least) { least = cost; n = k; rest = of / pieces; }
         }
     }
     const int64_t per = ((keys + n - 1) / n + step - 1) / step * step;

@@ -34,15 +34,19 @@ static constexpr int PT_INFO = 16;                                    // tiles w
 struct PtP { AttnPagedP a; int box, units, wide; unsigned int * next; CUtensorMap m_q, m_k, m_v; };
 
 // what is in shared memory besides the ring: queries' buffers (upper and, of FP32 rows, lower halves), tiles in the ring
+// Of more than 128 columns a piece of work has all scores and half of the values' columns (the sums of all would leave tensor memory for one buffer of scores, FP32 rows' queries no room for a tile's
+// keys: the scores are made twice); keys then come 64 columns at a time.
 template <int HD, bool TWO> struct PtShape {
-    static constexpr int SUBS = (HD + 63) / 64;
-    static constexpr uint32_t TILE = SUBS * PT_SUB, QUERIES = TILE * (TWO ? 2 : 1);
-    static constexpr int QB = HD <= 64 ? 2 : 1, NS = (int)((196608u - QB * QUERIES) / TILE), NK = NS / 2, NW = NS - NK;       // of keys, of values
-    static constexpr size_t SMEM = QB * QUERIES + NS * TILE + 1024;
+    static constexpr bool WIDE = HD > 128;
+    static constexpr int HV = WIDE ? HD / 2 : HD, QSUBS = (HD + 63) / 64, SUBS = (HV + 63) / 64;     // columns of the values; pieces of 64 columns of queries and keys, of values
+    static constexpr uint32_t TILE = SUBS * PT_SUB, HALF = QSUBS * PT_SUB, QUERIES = HALF * (TWO ? 2 : 1), FILL = WIDE ? PT_SUB : TILE;      // FILL: what a place for keys holds
+    static constexpr int QB = HD <= 64 ? 2 : 1, NS = WIDE ? 13 - (int)(QUERIES / PT_SUB) : (int)((196608u - QB * QUERIES) / TILE);
+    static constexpr int NW = !WIDE ? NS - NS / 2 : NS >= 7 ? 2 : 1, NK = WIDE ? NS - SUBS * NW : NS - NW;      // places of values, of keys
+    static constexpr size_t SMEM = QB * QUERIES + NK * FILL + NW * TILE + 1024;
 };
 
 // A piece of work: 128 rows of one KV head and a range of slots
-struct PtWork { int tiles, k0, k1, first, n_rows, hk, there, clear, dst; SeqB s; };      // tiles -1: there is no more; dst: number of the part that it makes, -1: results
+struct PtWork { int tiles, k0, k1, first, n_rows, hk, there, clear, dst, v0; SeqB s; };      // tiles -1: there is no more; dst: number of the part that it makes, -1: results; v0: first column of the values
 
 // Barriers by their addresses in shared memory.  Code is kept short: seven roles run at once, and warps that waited for instructions were a third of the time.
 // A wait of up to some 20 us at a time (warps that ask again and again take issue slots), some 65536 times, or until another one of the CTA ran out.
@@ -93,11 +97,12 @@ struct PtRing {
 template <int HD, bool TWO>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_constant__ PtP pp) {
     using Z = PtShape<HD, TWO>;
-    constexpr int KS = HD / 16, SUBS = Z::SUBS, NV = SUBS * 64;       // steps of 16 columns; pieces of 64 columns; columns of the sums (behind HD: zeros)
-    constexpr uint32_t TILE = Z::TILE;
+    constexpr int KS = HD / 16, SUBS = Z::SUBS, NV = SUBS * 64;       // steps of 16 columns; pieces of 64 columns of the values; columns of the sums (behind HV: unused)
+    constexpr bool WIDE = Z::WIDE;
+    constexpr uint32_t TILE = Z::TILE, FILL = Z::FILL;
     constexpr int NK = Z::NK, NW = Z::NW, QB = Z::QB;
     constexpr int OB = (512 - PT_GROUPS * PT_KEYS) / NV;              // buffers of sums.  (Two halves of 64 columns, of which one is drained while the other is made: products of 64 columns take as long as those of 128)
-    constexpr int DH = HD / 2, DC = HD == 96 ? 16 : 32;               // columns of a thread that drains, and at a time
+    constexpr int DH = Z::HV / 2, DC = DH == 48 ? 16 : 32;               // columns of a thread that drains, and at a time
     constexpr uint32_t T_S = 0, T_O = PT_GROUPS * PT_KEYS;            // tensor memory: three buffers of scores, one or two of sums
     static_assert(NK + PT_GROUPS < PT_INFO && OB >= 1 && PT_REGS_M + PT_REGS_Q + PT_GROUPS * PT_REGS_S + 2 * PT_REGS_D <= 7 * 72, "");
     const AttnPagedP & p = pp.a;
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     __shared__ uint32_t s_odd[PT_GROUPS][4];                           // slots of a special tile with a value that is not finite
     __shared__ float s_top[PT_GROUPS][PT_ROWS], s_sum[PT_GROUPS][PT_ROWS];         // of a tile: maximum, sum of the probabilities
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, keys = queries + QB * Z::QUERIES, values = keys + NK * TILE;
+    const uint32_t queries = (smem_u32(smem_raw) + 1023u) & ~1023u, keys = queries + QB * Z::QUERIES, values = keys + NK * FILL;
 
     if (tid < NK) { mbar_init(s_kfull + tid, 1); mbar_init(s_kempty + tid, 1); }
     if (tid < NW) { mbar_init(s_vfull + tid, 1); mbar_init(s_vempty + tid, 1); }
@@ -154,28 +159,41 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     const uint64_t q = tc_desc_k(queries + qs.at * Z::QUERIES);
                     for (int i = 0, left = span; i < tiles && ok; i++, g++, left -= PT_KEYS) {
                         const uint32_t idesc = tc_idesc(left >= PT_KEYS ? PT_KEYS : (left + 15) / 16 * 16, false), d = tmem + T_S + buf.at * PT_KEYS;
-                        const uint64_t k = tc_desc_k(keys + slot_k.at * TILE);
-                        ok = wait_at(slot_k.here(), slot_k.parity);
+                        if constexpr (!WIDE) ok = wait_at(slot_k.here(), slot_k.parity);
                         if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1) && ok;       // the buffer's probabilities have been used
                         if (!ok) break;
                         tc_fence_after();
                         // (lower halves of the queries first)
+                        if constexpr (WIDE) {
 #pragma unroll 1
-                        for (int low = TWO ? 1 : 0; low >= 0; low--) {
+                            for (int c = 0; c < Z::QSUBS && (ok = wait_at(slot_k.here(), slot_k.parity)); c++) {
+                                const uint64_t k = tc_desc_k(keys + slot_k.at * FILL);
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int low = TWO ? 1 : 0; low >= 0; low--) pt_scores<4>(d, q + (uint64_t)low * (Z::HALF >> 4) + c * (PT_SUB >> 4), k, idesc, (TWO && low == 0) || c > 0);
+                                pt_commit(empty + slot_k.at * 8);
+                                slot_k.template step<NK>();
+                            }
+                            if (!ok) break;
+                        } else {
+                            const uint64_t k = tc_desc_k(keys + slot_k.at * FILL);
+#pragma unroll 1
+                            for (int low = TWO ? 1 : 0; low >= 0; low--) {
 #pragma unroll
-                            for (int c = 0; c < SUBS; c++) {
-                                const uint64_t at = q + (uint64_t)low * (TILE >> 4) + c * (PT_SUB >> 4);
-                                if (KS - 4 * c >= 4) pt_scores<4>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
-                                else                 pt_scores<2>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
+                                for (int c = 0; c < SUBS; c++) {
+                                    const uint64_t at = q + (uint64_t)low * (TILE >> 4) + c * (PT_SUB >> 4);
+                                    if (KS - 4 * c >= 4) pt_scores<4>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
+                                    else                 pt_scores<2>(d, at, k + c * (PT_SUB >> 4), idesc, (TWO && low == 0) || c > 0);
+                                }
                             }
                         }
                         pt_commit(buf.here());
                         if (lane == 0) pt_arrive(buf.here());         // (what this warp has seen others write is seen by whoever waits)
                         __syncwarp();
-                        pt_commit(empty + slot_k.at * 8);
+                        if constexpr (!WIDE) pt_commit(empty + slot_k.at * 8);
                         if (i + 1 == tiles) pt_commit(qempty + qs.at * 8);
                         buf.template step<PT_GROUPS>();
-                        slot_k.template step<NK>();
+                        if constexpr (!WIDE) slot_k.template step<NK>();
                     }
                     qs.template step<QB>();
                 }
@@ -227,11 +245,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             const CUtensorMap * map = is_k ? &pp.m_k : &pp.m_v;
             const uint32_t full = smem_u32(is_k ? s_kfull : s_vfull), empty = smem_u32(is_k ? s_kempty : s_vempty), lot = is_k ? keys : values;
             const unsigned slots = is_k ? NK : NW;
-            const int box = SUBS == 2 ? lane >> 1 : lane, x = SUBS == 2 ? (lane & 1) * 64 : 0;
+            const uint32_t fill = is_k ? FILL : TILE;
+            const int side = SUBS == 1 || (WIDE && is_k) ? 1 : 2, fills = WIDE && is_k ? Z::QSUBS : 1;       // copies side by side; places that a tile takes
+            const int box = side == 2 ? lane >> 1 : lane, x = side == 2 ? (lane & 1) * 64 : 0;
             const bool mine = box * pp.box < PT_KEYS;
             const uint32_t place = (uint32_t)(x >> 6) * PT_SUB + (uint32_t)(box * pp.box) * 128u;
             unsigned slot = 0, parity = 0;
-            int at = 0;                                               // tiles in all
+            int at = 0, asked = 0;                                    // tiles in all, places
             bool ok = true;
             for (int n = 0; ok; n++) {
                 ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
@@ -250,21 +270,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     const int row = y;
                     const unsigned copies = __ballot_sync(0xffffffffu, row >= 0);
                     if (is_k) {                                       // which groups of 16 slots are there; whether the tile is special
-                        const int j0 = w->k0 + i * PT_KEYS, of = (lane & 7) * 16 / pp.box * SUBS;
+                        const int j0 = w->k0 + i * PT_KEYS, of = (lane & 7) * 16 / pp.box * side;
                         const uint32_t groups = __ballot_sync(0xffffffffu, lane < 8 && j0 + lane * 16 < w->there && (copies >> of & 1));
                         if (lane == 0) s_info[at % PT_INFO] = groups | (groups != 0xffu || j0 + PT_KEYS > w->clear ? 256u : 0u);
                     }
-                    if (at >= (int)slots && !(ok = wait_at(empty + slot * 8, parity ^ 1))) break;
-                    if (lane == 0) mbar_expect_tx((is_k ? s_kfull : s_vfull) + slot, (unsigned)__popc(copies) * pp.box * 128u);
-                    __syncwarp();
-                    if (row >= 0) tma_tile(lot + slot * TILE + place, map, x, row, (is_k ? s_kfull : s_vfull) + slot);
-                    if (i + 1 < tiles) y = look(i + 1);
-                    __syncwarp();
-                    if (++slot == slots) { slot = 0; parity ^= 1; }
+                    for (int c = 0; c < fills; c++, asked++) {
+                        if (asked >= (int)slots && !(ok = wait_at(empty + slot * 8, parity ^ 1))) break;
+                        if (lane == 0) mbar_expect_tx((is_k ? s_kfull : s_vfull) + slot, (unsigned)__popc(copies) * pp.box * 128u);
+                        __syncwarp();
+                        if (row >= 0) tma_tile(lot + slot * fill + place, map, x + (!WIDE ? 0 : is_k ? c * 64 : w->v0), row, (is_k ? s_kfull : s_vfull) + slot);
+                        if (c == 0 && i + 1 < tiles) y = look(i + 1);
+                        __syncwarp();
+                        if (++slot == slots) { slot = 0; parity ^= 1; }
+                    }
+                    if (!ok) break;
                 }
                 if (ok) done_with(n);
             }
-            if (!ok && lane == 0) ring_land(is_k ? s_kfull : s_vfull, at, (int)slots);          // (else all have been waited for)
+            if (!ok && lane == 0) ring_land(is_k ? s_kfull : s_vfull, asked, (int)slots);          // (else all have been waited for)
             __syncwarp();
         }
     } else if (warp < 8) {
@@ -281,7 +304,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 PtWork w;
                 w.tiles = -1;
                 while (unit < pp.units) {                             // the next piece that has something to do
-                    const AqItem it = ap_item(p, unit);
+                    const AqItem it = ap_item(p, WIDE ? unit >> 1 : unit);
+                    w.v0 = WIDE && unit & 1 ? Z::HV : 0;
                     w.s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, it.entry);
                     const TileP t = ap_tile(p, w.s, p.row_tiles - 1 - it.rt, PT_ROWS);      // (the longest rows first)
                     w.k0 = it.split * p.split; w.k1 = it.split == it.n_splits - 1 ? t.seen : min(t.seen, w.k0 + p.split);
@@ -304,8 +328,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                         mbar_expect_tx(s_qfull + qs.at, Z::QUERIES);
                         const int row = (w.hk * p.b.T + w.s.first) * p.group + w.first;
                         for (int low = 0; low <= (TWO ? 1 : 0); low++)
-                            for (int c = 0; c < SUBS; c++)
-                                tma_tile(queries + qs.at * Z::QUERIES + low * TILE + c * PT_SUB, &pp.m_q, c * 64, row + low * p.c.H * p.b.T * p.group, s_qfull + qs.at);
+                            for (int c = 0; c < Z::QSUBS; c++)
+                                tma_tile(queries + qs.at * Z::QUERIES + low * Z::HALF + c * PT_SUB, &pp.m_q, c * 64, row + low * p.c.H * p.b.T * p.group, s_qfull + qs.at);
                     }
                     __syncwarp();
                     qs.template step<QB>();
@@ -510,12 +534,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 // (32 bytes a store where rows lie so: a row a thread meets a line of its own at every store)
                 if (w->dst >= 0) {
                     const size_t at = (size_t)w->dst * PT_ROWS + r;
+                    if (WIDE && sum != sum) {                         // (the part's sum stands for both halves of the columns, no numbers for the one that has them)
 #pragma unroll
-                    for (int j = 0; j < DH; j += 8) pt_store8(p.part + at * HD + d0 + j, acc + j);
-                    if (d0 == 0) p.part_ml[at] = make_float2(top, sum);
+                        for (int j = 0; j < DH; j++) acc[j] = sum;
+                    }
+#pragma unroll
+                    for (int j = 0; j < DH; j += 8) pt_store8(p.part + at * HD + w->v0 + d0 + j, acc + j);
+                    if (d0 + w->v0 == 0) p.part_ml[at] = make_float2(top, sum);
                 } else {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    const size_t at = (size_t)(w->s.first + of) * p.out_stride + (size_t)h * HD + d0;
+                    const size_t at = (size_t)(w->s.first + of) * p.out_stride + (size_t)h * HD + w->v0 + d0;
 #pragma unroll
                     for (int j = 0; j < DH; j++) acc[j] *= inv;
                     if constexpr (!TWO) {
@@ -606,11 +634,12 @@ __global__ void __launch_bounds__(256) k_attn_paged_queries(const AttnPagedP p, 
 // With mma.sync every 16 rows of a KV head read its keys and values again, 16 us for 2^25 values of keys (after the first ones); here 128 rows take 5 us more whatever there is, and 7 us more for as many values.
 // Both sides measured (us, here and with mma.sync; FP32, 4 query heads a KV head, head_dim 128): 8 sequences of 4096 slots and 8 KV heads 16 rows 39 and 28, 24 rows 39 and 43, 64 rows 41 and 74; one such
 // sequence 24 rows 17 and 14, 48 rows 18 and 16, 64 rows 18 and 17; one of 500 slots and 32 KV heads 64 rows 15 and 14.
+// The same of head_dim 256 and 192: 8 sequences of 4096 24 rows 88 and 99, 72 and 82; one 24 rows 23 and 21, 21 and 18; 64 rows 24 and 32, 22 and 28; one of 500 and 32 KV heads of 256 64 rows 20 and 19, 128 rows 22 and 36.
 // (PI_ATTN_TREE_TC=1 takes 17 rows and more whatever there is, 0 none: a diagnostic switch, read once.)
 bool attn_paged_tc_takes(int hd, int64_t rows, int64_t values) {
     static int forced = -2;
     if (forced == -2) { const char * v = getenv("PI_ATTN_TREE_TC"); forced = v ? v[0] != '0' : -1; }
-    if (hd > 128 || rows <= 16 || forced == 0) return false;
+    if (rows <= 16 || forced == 0) return false;
     return forced == 1 || ((rows + 15) / 16 - 1) * 16 * (double)values > 5.0 * (1 << 25) + 7.0 * values;
 }
 
@@ -631,7 +660,7 @@ static int pt_go(const AttnPagedP & a, cudaStream_t st) {
     if ((rc = tensor_map(&p.m_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.k, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B)) ||
         (rc = tensor_map(&p.m_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.v, HD, rows, HD * 2, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * 4 % 32 == 0;
-    p.units = (int)ap_grid(a);
+    p.units = (int)ap_grid(a) * (PtShape<HD, TWO>::WIDE ? 2 : 1);
     p.next = a.status + 8;
     const int64_t q_rows = (int64_t)a.b.T * a.n_head;
     if ((rc = tensor_map(&p.m_q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.queries, HD, q_rows * (TWO ? 2 : 1), HD * 2, 64, PT_ROWS, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
@@ -645,7 +674,9 @@ int launch_attn_paged_tc(const AttnPagedP & p, cudaStream_t st) {
     switch (p.c.hd) {
         case 64: return half ? pt_go<64, false>(p, st) : pt_go<64, true>(p, st);
         case 96: return half ? pt_go<96, false>(p, st) : pt_go<96, true>(p, st);
-        default: return half ? pt_go<128, false>(p, st) : pt_go<128, true>(p, st);
+        case 128: return half ? pt_go<128, false>(p, st) : pt_go<128, true>(p, st);
+        case 192: return half ? pt_go<192, false>(p, st) : pt_go<192, true>(p, st);
+        default: return half ? pt_go<256, false>(p, st) : pt_go<256, true>(p, st);
     }
 }
 

@@ -623,7 +623,7 @@ def attention_tree(cache: KvCachePaged, q: torch.Tensor, q_start: torch.Tensor, 
     if need:
         ws = q_start.new_empty(need // 4)
         ws_at = ws.data_ptr()
-        if hd <= 128 and min(T, T if max_new is None else max_new) * (n_head // cache.n_head_kv) > 16:
+        if min(T, T if max_new is None else max_new) * (n_head // cache.n_head_kv) > 16:
             _ws.asked = ws_at, ws                                     # (the calls with bounded waits; kept until the next operator, for last_op_status)
     check(lib.pi_attention_tree(cache.c, b, layer, xtype, q_at, q_step, n_head, mask_at, words, most, hd ** -0.5 if scale is None else scale, out.data_ptr(), n, ws_at, need, _stream()))
     return out

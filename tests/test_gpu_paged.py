@@ -316,6 +316,30 @@ def test_what_a_row_does_not_see_has_no_part_in_it(ops, x, hd, group, m):
 
 
 @pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("hd,group,m,context", [(128, 2, 40, 4000), (192, 4, 40, 4000), (256, 2, 40, 4000), (256, 8, 20, 40), (192, 1, 5, 900)])
+def test_a_row_with_one_column_that_is_no_number(ops, x, hd, group, m, context):
+    """A value of a drafted token that is not finite, in the first or the last column alone: whoever sees it is not finite there, the others are as before."""
+    rng = np.random.default_rng(hd + context)
+    lens = [context + m, m]
+    c = pool(rng, 1, 2, hd, 64, lens)
+    news, q_start, pos0 = [m, m], [0, m, 2 * m], [context, 0]
+    masks, _ = po.tree_mask(trees(rng, news), q_start, pos0, m, 1)
+    mask = words_of(masks, 1)
+    q = rows(rng, 2 * m, 2 * group * hd, x)
+    want, tol = po.attention(c, 0, q, 2 * group, q_start, pos0, None, m, mask, hd ** -0.5, U[x], U["f16"] if x == "f16" else 0.0)
+    seeing = np.array([bool(masks[t] >> 2 & 1) for t in range(2 * m)])
+    want, tol = want.reshape(2 * m, 2, group, hd), tol.reshape(2 * m, 2, group, hd)
+    for column, value in ((0, np.nan), (hd - 1, np.inf), (hd // 2, -np.inf), (hd // 2 - 1, np.nan)):
+        odd = po.Cache(c.k.copy(), c.v.copy(), c.table)
+        for i in range(2):
+            p, r = odd.place(i, pos0[i] + 2)
+            odd.v[0, p, 1, r, column] = value
+        got = attend(ops, odd, x, q, 2 * group, q_start, pos0, None, m, mask).float().cpu().numpy().astype(np.float64).reshape(want.shape)
+        near = np.abs(got - want) <= tol
+        assert near[~seeing].all() and near[:, 0].all() and seeing.any() and not np.isfinite(got[seeing][:, 1, :, column]).any()
+
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
 def test_attention_of_what_the_cache_lacks(ops, x):
     """Entries of no sequence, first slots behind the table, tokens without a slot, rows of no entry, one sequence twice, an end below the start."""
     rng = np.random.default_rng(9)
