@@ -11,10 +11,15 @@
 // become zeros, rows with a value that is not finite too, and whoever sees such a slot has a row of no numbers; scores of slots that a row does not see are replaced by what its
 // mask says.
 //
+// What bounds it, by shape (FP32 128, a chunk of 1024 tokens over 4096 slots, 64 heads over 8: 203 us, of which the products, two for one, would take 146): at head_dim 128 FP32 a tile takes 2650 clocks, the
+// products 2048, and the sums of a tile, one buffer, wait for the ones before to be drained; FP16 2400, the copies of keys and values 2150 (43 bytes a clock and SM); at head_dim 64 FP16 1660, the exponents 1024 and
+// the chain from a score to its probability the rest.  One sequence of 32768 slots, 25 FP32 tokens, 64 heads over 8: 63 us; 8 of 1000 to 2000,
+// 48 FP16 tokens, 32 heads over 32: 51; 16 of 750 to 1500, 32 FP16 tokens, 128 heads over 8 of 64: 46.  Head_dim 256: 2 x 300 tokens of 3000 slots, 32 heads over 8: FP32 143, FP16 130 (copies: 96 KB a tile and half).
+//
 // Precision.  FP32 rows: queries and probabilities are the sum of two halves each, 22 bits, i.e. two products in the place of one.  FP16 rows: queries as they are, probabilities
 // one half, 11 bits like the result's own rounding.  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
 //
-// Warps: 0 issues the products of scores and 2 those of values; 1 asks for keys and 3 for values; 4..7 take work and lay out its queries; 8..19 have the
+// Warps: 0 issues the products of scores and 2 those of values; 1 asks for keys and 3 for values; 4 takes work and asks for its queries (5..7 make a warpgroup of it, for the registers); 8..19 have the
 // probabilities, three groups a tile each in turn, a row a thread; 20..27 drain the sums, a row and half of the columns a thread.
 #include "pi_attn_paged.cuh"
 #include "pi_tc.cuh"

@@ -3,7 +3,8 @@
 //     k_cache[slot] = fp16(R(pos) k)     v_cache[slot] = fp16(v)     q_out = R(pos) q     R as in pi_rope.cu
 //
 // A CTA takes one token and a share of its heads (queries, keys, values): every thread requests its values first, the angles of the token are made while they
-// travel (n_rot / 2 of them, once for all heads, in 64 bits).  Bound by the bytes for many tokens, by the launch for few.
+// travel (n_rot / 2 of them, once for all heads, in 64 bits).  Bound by the bytes for many tokens (3329 of 128 FP16 heads over 8 of 64: 28 us, 4.4 TB/s; 256 threads of a token, with its angles in 64 bits
+// in front of the products), by the launch and the angles for few (150 tokens of 64 FP32 heads over 8 of 128: 6.5 us).
 #include "pi_kv_paged.cuh"
 #include "pi_rope.cuh"
 
@@ -201,6 +202,7 @@ int launch_kv_append_paged(const AppendArgs & a, cudaStream_t st) {
 // ------------------------------------------------------------------------------------------------
 // A warp takes the path's rows of one layer, of keys or values, of one KV head: KEEP_AT passes of 32 / (row's 16-byte pieces) rows are read before any of them is written.  The
 // path rises, so a row is written to a place that is not behind the one it came from, and no later row comes from there.  The rows' places are found once for a CTA's warps.
+// Bound by the way from the lengths over the path and the table to the rows (32 layers of 32 heads of 128, a path of 4: 3.8 us), or by rows of 256 bytes apart (80 layers of 8, 8 sequences, 6 rows each: 8 us).
 static constexpr int KEEP_WARPS = 8, KEEP_ROWS = 128, KEEP_AT = 4;
 
 __global__ void __launch_bounds__(KEEP_WARPS * 32) k_kv_keep(const KeepArgs p) {
