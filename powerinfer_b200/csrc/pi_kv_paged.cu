@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(KEEP_WARPS * 32) k_kv_keep(const KeepArgs p) {
     const bool mine = layer < p.c.n_layer && sub < rows_at;
     __half * pool = (lw & 1 ? p.c.v : p.c.k) + (size_t)min(layer, p.c.n_layer - 1) * p.c.n_pages * p.c.H * p.c.page * hd + (size_t)h * p.c.page * hd + col * 8;
     for (int r0 = 0; r0 < n; r0 += KEEP_ROWS) {
-        // rows of this round that do not rise end the path
+        // rows of this pass that do not rise end the path
         const int r = r0 + tid;
         int end = n;
         if (tid < KEEP_ROWS && r < n) {
