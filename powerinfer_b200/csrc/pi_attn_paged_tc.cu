@@ -62,6 +62,14 @@ __device__ __forceinline__ bool pt_wait(uint32_t bar, unsigned parity, uint32_t 
                  : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u), "r"(dead) : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
+// The same without being suspended, for the two warps that issue products: they are told some 100 clocks earlier (chunk 203 -> 198 us); of more warps the asking costs what it gains
+__device__ __forceinline__ bool pt_poll(uint32_t bar, unsigned parity, uint32_t dead) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p, q;\n .reg .u32 n, d;\n mov.u32 n, 0;\nWAIT:\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+                 " ld.volatile.shared.u32 d, [%3];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, 16777216, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%3], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(dead) : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
+}
 __device__ __forceinline__ void pt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
 __device__ __forceinline__ void pt_commit(uint32_t bar) {
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" :: "r"(bar) : "memory");
@@ -114,7 +122,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint64_t s_kfull[NK], s_kempty[NK], s_vfull[NW], s_vempty[NW];
     __shared__ uint64_t s_wfull[PT_WORK], s_wempty[PT_WORK], s_qfull[QB], s_qempty[QB];
-    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_scan[PT_GROUPS], s_fin[2];
+    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_scan[PT_GROUPS], s_fin[2], s_asked;
     __shared__ PtWork s_work[PT_WORK];
     __shared__ uint32_t s_tmem, s_info[PT_INFO];                      // of a tile: which groups of 16 slots are there; bit 8: special
     __shared__ volatile unsigned s_dead;
@@ -129,6 +137,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     if (tid < QB) { mbar_init(s_qfull + tid, 1); mbar_init(s_qempty + tid, 1); }
     if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 12); mbar_init(s_stat + tid, 8); mbar_init(s_scan + tid, 4); }
     if (tid < 2) mbar_init(s_fin + tid, 1);
+    if (tid == 2) mbar_init(&s_asked, 1);
     if (tid == 0) s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
@@ -142,6 +151,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     asm volatile("fence.proxy.async;" ::: "memory");                // (what kernels before wrote is read by tensor copies)
     const uint32_t dead = smem_u32((const void *)&s_dead);
     auto wait_at = [&](uint32_t bar, unsigned parity) { return pt_wait(bar, parity, dead); };      // warp-uniform; false: the wait ran out, here or elsewhere in the CTA
+    auto poll_at = [&](uint32_t bar, unsigned parity) { return pt_poll(bar, parity, dead); };
     auto wait = [&](uint64_t * bar, unsigned parity) { return wait_at(smem_u32(bar), parity); };
     auto work_of = [&](int n) { return s_work + n % PT_WORK; };
     auto done_with = [&](int n) { __syncwarp(); if (lane == 0) mbar_arrive(s_wempty + n % PT_WORK); };
@@ -155,23 +165,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_kempty), qempty = smem_u32(s_qempty);
             int g = 0;                                                // tiles in all
             for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
-                ok = wait_at(work.here(), work.parity);
+                ok = poll_at(work.here(), work.parity);
                 if (!ok) break;
                 const int tiles = __shfl_sync(0xffffffffu, s_work[work.at].tiles, 0), span = __shfl_sync(0xffffffffu, s_work[work.at].k1 - s_work[work.at].k0, 0);      // (uniform for the compiler)
                 if (tiles < 0) break;
                 if (tiles > 0) {
-                    ok = wait_at(qs.here(), qs.parity);
+                    ok = poll_at(qs.here(), qs.parity);
                     const uint64_t q = tc_desc_k(queries + qs.at * Z::QUERIES);
                     for (int i = 0, left = span; i < tiles && ok; i++, g++, left -= PT_KEYS) {
                         const uint32_t idesc = tc_idesc(left >= PT_KEYS ? PT_KEYS : (left + 15) / 16 * 16, false), d = tmem + T_S + buf.at * PT_KEYS;
-                        if constexpr (!WIDE) ok = wait_at(slot_k.here(), slot_k.parity);
-                        if (g >= PT_GROUPS) ok = wait_at(pv + buf.at * 8, buf.parity ^ 1) && ok;       // the buffer's probabilities have been used
+                        if constexpr (!WIDE) ok = poll_at(slot_k.here(), slot_k.parity);
+                        if (g >= PT_GROUPS) ok = poll_at(pv + buf.at * 8, buf.parity ^ 1) && ok;       // the buffer's probabilities have been used
                         if (!ok) break;
                         tc_fence_after();
                         // (lower halves of the queries first)
                         if constexpr (WIDE) {
 #pragma unroll 1
-                            for (int c = 0; c < Z::QSUBS && (ok = wait_at(slot_k.here(), slot_k.parity)); c++) {
+                            for (int c = 0; c < Z::QSUBS && (ok = poll_at(slot_k.here(), slot_k.parity)); c++) {
                                 const uint64_t k = tc_desc_k(keys + slot_k.at * FILL);
                                 tc_fence_after();
 #pragma unroll 1
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             const uint32_t pv = smem_u32(s_pv), empty = smem_u32(s_vempty);
             unsigned ob = 0;                                          // buffer of sums
             for (int n = 0; ok; n++, work.template step<PT_WORK>()) {
-                ok = wait_at(work.here(), work.parity);
+                ok = poll_at(work.here(), work.parity);
                 if (!ok) break;
                 const int tiles = __shfl_sync(0xffffffffu, s_work[work.at].tiles, 0), span = __shfl_sync(0xffffffffu, s_work[work.at].k1 - s_work[work.at].k0, 0);
                 if (tiles < 0) break;
@@ -222,8 +232,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     const uint32_t a = tmem + T_S + buf.at * PT_KEYS, d = tmem + T_O + ob * NV;
                     const uint64_t v = tc_desc_mn(values + slot_v.at * TILE, PT_SUB);
                     const int steps = left >= PT_KEYS ? PT_KEYS / 16 : (left + 15) / 16;
-                    ok = wait_at(slot_v.here(), slot_v.parity);
-                    ok = wait_at(buf.here(), buf.parity) && ok;       // (the buffer of sums has been drained too)
+                    ok = poll_at(slot_v.here(), slot_v.parity);
+                    ok = poll_at(buf.here(), buf.parity) && ok;       // (the buffer of sums has been drained too)
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -290,6 +300,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     }
                     if (!ok) break;
                 }
+                if (is_k && lane == 0) mbar_arrive(&s_asked);         // (the next piece may be taken)
                 if (ok) done_with(n);
             }
             if (!ok && lane == 0) ring_land(is_k ? s_kfull : s_vfull, asked, (int)slots);          // (else all have been waited for)
@@ -300,12 +311,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(PT_REGS_Q));
         if (warp == 4) {
             int unit = blockIdx.x;
+            auto take = [&]() {
+                int then = 0;
+                if (lane == 0) then = (int)gridDim.x + (int)atomicAdd(pp.next, 1u);
+                unit = __shfl_sync(0xffffffffu, then, 0);
+            };
             PtRing qs(s_qfull);
             const uint32_t qempty = smem_u32(s_qempty);
             bool ok = true;
             int u = 0;                                                // pieces with tiles
             for (int n = 0; ok; n++) {
                 if (n >= PT_WORK && !(ok = wait(s_wempty + n % PT_WORK, n / PT_WORK & 1 ^ 1))) break;
+                // the next piece when the keys of the last one have all been asked for, two or three tiles before it ends: taken as soon as there is room, all pieces of a call of 400
+                // were dealt out at its start, and one CTA had 38 tiles where 29 is the mean (trees of many users)
+                if (n > 0) {
+                    if (!(ok = wait(&s_asked, n & 1 ^ 1))) break;
+                    take();
+                }
                 PtWork w;
                 w.tiles = -1;
                 while (unit < pp.units) {                             // the next piece that has something to do
@@ -318,10 +340,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     w.dst = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1;
                     w.clear = p.mask ? w.s.pos : w.s.pos + p.by_group.of(t.first) + 1;      // every row sees the slots before it
                     if (t.n_rows > 0 && (w.k0 < w.k1 || it.split == 0)) w.tiles = w.k0 < w.k1 ? (w.k1 - w.k0 + PT_KEYS - 1) / PT_KEYS : 0;      // (split 0 answers for rows that see nothing)
-                    int then = 0;
-                    if (lane == 0) then = (int)gridDim.x + (int)atomicAdd(pp.next, 1u);
-                    unit = __shfl_sync(0xffffffffu, then, 0);
                     if (w.tiles >= 0) break;
+                    take();
                 }
                 if (lane == 0) { *work_of(n) = w; mbar_arrive(s_wfull + n % PT_WORK); }
                 __syncwarp();
