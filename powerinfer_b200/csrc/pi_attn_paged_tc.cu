@@ -12,7 +12,7 @@
 // mask says.
 //
 // What bounds it, by shape (FP32 128, a chunk of 1024 tokens over 4096 slots, 64 heads over 8: 194 us, of which the products, two for one, would take 146): at head_dim 128 FP32 a tile takes 2650 clocks, the
-// products 2048, and the sums of a tile, one buffer, wait for the ones before to be drained; FP16 2400, the copies of keys and values 2150 (43 bytes a clock and SM); at head_dim 64 FP16 1660, the exponents 1024 and
+// products 2048, and the sums of a tile, one buffer, wait for the ones before to be drained; FP16 2400, the copies of keys and values 2150 (30 bytes a clock and SM, the rate of the memory); at head_dim 64 FP16 1660, the exponents 1024 and
 // the chain from a score to its probability the rest.  One sequence of 32768 slots, 25 FP32 tokens, 64 heads over 8: 62 us; 8 of 1000 to 2000,
 // 48 FP16 tokens, 32 heads over 32: 47; 16 of 750 to 1500, 32 FP16 tokens, 128 heads over 8 of 64: 44.  Head_dim 256: 2 x 300 tokens of 3000 slots, 32 heads over 8: FP32 129, FP16 113 (copies: 96 KB a tile and half).
 //

@@ -2,20 +2,22 @@
 //
 //     k_cache[slot] = fp16(R(pos) k)     v_cache[slot] = fp16(v)     q_out = R(pos) q     R as in pi_rope.cu
 //
-// A CTA takes one token and a share of its heads (queries, keys, values): every thread requests its values first, the angles of the token are made while they
-// travel (n_rot / 2 of them, once for all heads, in 64 bits).  Bound by the bytes for many tokens (3329 of 128 FP16 heads over 8 of 64: 28 us, 4.4 TB/s; 256 threads of a token, with its angles in 64 bits
-// in front of the products), by the launch and the angles for few (150 tokens of 64 FP32 heads over 8 of 128: 6.5 us).
+// A CTA takes up to 8 tokens, one after the other, and a share of their heads (queries, keys, values).  A thread has 16 values of one head, which it finds once; it requests those of the first token,
+// and the angles of all tokens (n_rot / 2 each, once for all heads, in 64 bits) are made while they travel; then every token's are asked for before the last one's are turned and stored.  Bound by the bytes
+// for many tokens (3329 of 128 FP16 heads over 8 of 64: 24 us, 5.1 TB/s; FP32 40 us), by the launch and the angles for few (150 tokens of 64 FP32 heads over 8 of 128: 6.2 us).
+#include "pi_attn_q8.cuh"
 #include "pi_kv_paged.cuh"
 #include "pi_rope.cuh"
 
 namespace pi {
 
-static constexpr int AP_THREADS = 256;
+static constexpr int AP_THREADS = 256, AP_TOKENS = 8, AP_LEAST = 896;
 
 struct AppendP {
     AppendArgs a;
     int heads[3];                                                     // queries (0: none), keys, values
-    int parts, per_head;                                              // CTAs of a token; units of a head (of queries and keys)
+    int parts, per_head, tokens;                                      // CTAs that share a token; units of a head (of queries and keys); tokens of a CTA
+    AqDiv by_unit, by_value, by_half;                                 // units of a head of queries and keys, of values; n_rot / 2
 };
 
 // 8 values of a row, as they are stored
@@ -45,137 +47,102 @@ __device__ __forceinline__ void store8(__half * p, const float (&v)[8]) {
 
 // A unit is 16 values of a head: 8 at d0 and 8 at d1.  KIND 0: pairs (2i, 2i + 1), 16 in a row; 1: pairs (i, i + half), 8 of each half, or 16 in a row of the dimensions
 // that pass; 2: the same where a half is no multiple of 8, pair by pair (values still 16 in a row).  In place is fine: a unit is read and written by one thread.
-template <typename T, int KIND, int U>
+template <typename T, int KIND>
 __global__ void __launch_bounds__(AP_THREADS) k_kv_append(const AppendP p) {
-    __shared__ float2 cs[128];
+    __shared__ float2 cs[AP_TOKENS * 128];
+    __shared__ int64_t s_at[AP_TOKENS];                               // a token's row in the pools, without the head; -1: not stored
+    __shared__ int s_later;
     const AppendArgs & a = p.a;
-    const int t = blockIdx.x / p.parts, part = blockIdx.x - t * p.parts, i = blockIdx.y, half = a.n_rot >> 1, hd = a.c.hd, lane = threadIdx.x & 31;
+    const int group = blockIdx.x / p.parts, part = blockIdx.x - group * p.parts, i = blockIdx.y, half = a.n_rot >> 1, hd = a.c.hd, tid = threadIdx.x, t0 = group * p.tokens;
     pdl_launch();
     pdl_wait();
     const SeqB s = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, i);
-    if (t >= s.n_new) return;
-    const int slot = s.pos + t;
-    const size_t row_in = (size_t)(s.first + t);
-    // ---- values on their way
-    const int turning = (p.heads[0] + p.heads[1]) * p.per_head, units = turning + p.heads[2] * (hd >> 4);
-    Eight<T> v[U][KIND == 2 ? 1 : 2]; T pair[KIND == 2 ? U : 1][2]; int which[U], at[U], head[U];
-    (void)pair;
-    // first and second 8 of unit `at`: of queries and keys, of values
-    auto places = [&](int which, int at, bool & turns, int & d0, int & d1) {
-        turns = KIND == 1 && which < 2 && at * 8 < half;
-        d0 = KIND != 1 || which == 2 ? at * 16 : turns ? at * 8 : a.n_rot + (at * 8 - half) * 2;
-        d1 = turns ? d0 + half : d0 + 8;
+    const int nt = min(p.tokens, s.n_new - t0);
+    if (nt <= 0) return;
+    // ---- this thread's unit, and its values of the first token on their way
+    const size_t row = (size_t)(s.first + t0);
+    const int turning = (p.heads[0] + p.heads[1]) * p.per_head, units = turning + p.heads[2] * (hd >> 4), n = part * (int)blockDim.x + tid;
+    const bool mine = n < units;
+    const int m = n < turning ? n : n - turning, h = n < turning ? p.by_unit.of(m) : p.by_value.of(m), at = m - h * (n < turning ? p.per_head : hd >> 4);
+    const int which = n >= turning ? 2 : h < p.heads[0] ? 0 : 1, head = which == 1 ? h - p.heads[0] : h;
+    const bool pairs = KIND == 2 && which < 2, turns = KIND != 0 && which < 2 && at * (KIND == 2 ? 1 : 8) < half;
+    const int step = pairs ? 1 : 8;                                   // values at d0 and at d1
+    const int d0 = KIND == 0 || which == 2 ? at * 16 : turns ? at * step : a.n_rot + (at * step - half) * 2, d1 = turns ? d0 + half : d0 + step;
+    const int64_t x_stride = mine ? a.x_stride[which] : 0;
+    const T * x = mine ? (const T *)a.x[which] + row * x_stride + (size_t)head * hd : nullptr;
+    Eight<T> v[2], next[2];
+    T pair[2], pair_next[2];
+    auto load = [&](Eight<T> (&e)[2], T (&w)[2]) {
+        if (pairs) { w[0] = x[d0]; w[1] = x[d1]; }
+        else       { load8(x + d0, e[0]); load8(x + d1, e[1]); }
+        x += x_stride;
     };
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int n = (part * U + u) * (int)blockDim.x + (int)threadIdx.x;
-        which[u] = -1;
-        if (n >= units) continue;
-        const int per = n < turning ? p.per_head : hd >> 4, m = n < turning ? n : n - turning;
-        int h = m / per;
-        at[u] = m - h * per;
-        which[u] = n >= turning ? 2 : h < p.heads[0] ? 0 : 1;
-        if (which[u] == 1) h -= p.heads[0];
-        head[u] = h;
-        const T * x = (const T *)a.x[which[u]] + row_in * a.x_stride[which[u]] + (size_t)h * hd;
-        if constexpr (KIND == 2) {
-            if (which[u] < 2) {
-                const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
-                pair[u][0] = x[d0]; pair[u][1] = x[d1];
+    if (mine) load(v, pair);
+    // ---- meanwhile where the tokens go, and their angles
+    if (tid < 32) {
+        bool later = false;
+        if (a.b.seq) {                                                // of entries that name one sequence the last one counts
+            for (int j = i + 1 + tid; j < a.b.n; j += 32) {
+                const SeqB o = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, j);
+                later |= o.sq == s.sq && o.n_new > 0;
             }
-        } else {
-            bool turns; int d0, d1;
-            places(which[u], at[u], turns, d0, d1);
-            load8(x + d0, v[u][0]);
-            load8(x + d1, v[u][KIND == 2 ? 0 : 1]);
+            later = __any_sync(0xffffffffu, later);
+        }
+        if (tid < nt) {
+            const int slot = s.pos + t0 + tid, page = s.sq >= 0 && slot < a.c.n_ctx && !later ? page_of(a.c, s.sq, slot >> a.c.shift) : -1;
+            s_at[tid] = page < 0 ? -1 : (int64_t)page_at(a.c, page, 0) + (slot & (a.c.page - 1)) * hd;
         }
     }
-    // ---- meanwhile where they go, and the angles
-    int page = -1;
-    if (s.sq >= 0 && slot < a.c.n_ctx) page = page_of(a.c, s.sq, slot >> a.c.shift);
-    const int pos = a.pos ? a.pos[row_in] : slot;
-    for (int j = threadIdx.x; j < half; j += blockDim.x) cs[j] = rope_angle(pos, a.freqs[j], a.mscale);
-    if (a.b.seq && page >= 0) {                                       // of entries that name one sequence the last one counts
-        bool later = false;
-        for (int j = i + 1 + lane; j < a.b.n; j += 32) {
-            const SeqB o = seq_entry(a.b, a.c.n_seq, a.c.n_ctx, j);
-            later |= o.sq == s.sq && o.n_new > 0;
-        }
-        if (__any_sync(0xffffffffu, later)) page = -1;                // (the same in every warp)
+    for (int j = tid; j < nt * half; j += blockDim.x) {
+        const int g = p.by_half.of(j), k = j - g * half;
+        cs[g * 128 + k] = rope_angle(a.pos ? a.pos[row + g] : s.pos + t0 + g, a.freqs[k], a.mscale);
     }
     __syncthreads();
-    auto put = [&](int which, int head, int d, const float (&y)[8]) {
-        if (which == 0)     store8((T *)a.q_out + row_in * a.q_out_stride + (size_t)head * hd + d, y);
-        else if (page >= 0) store8((which == 1 ? a.c.k : a.c.v) + page_at(a.c, page, head) + (size_t)(slot & (a.c.page - 1)) * hd + d, y);
-    };
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (which[u] < 0) continue;
-        if constexpr (KIND == 2) {
-            if (which[u] < 2) {
-                const int d0 = at[u] < half ? at[u] : a.n_rot + (at[u] - half) * 2, d1 = at[u] < half ? d0 + half : d0 + 1;
-                float y0 = rope_get(&pair[u][0]), y1 = rope_get(&pair[u][1]);
-                if (at[u] < half) {
-                    const float2 c = cs[at[u]];
-                    const float x0 = y0, x1 = y1;
-                    y0 = x0 * c.x - x1 * c.y; y1 = x0 * c.y + x1 * c.x;
-                }
-                if (which[u] == 0) {
-                    T * to = (T *)a.q_out + row_in * a.q_out_stride + (size_t)head[u] * hd;
-                    rope_put(to + d0, y0); rope_put(to + d1, y1);
-                } else if (page >= 0) {
-                    __half * to = a.c.k + page_at(a.c, page, head[u]) + (size_t)(slot & (a.c.page - 1)) * hd;
-                    rope_put(to + d0, y0); rope_put(to + d1, y1);
-                }
-            } else {
-                const T * x = (const T *)a.x[2] + row_in * a.x_stride[2] + (size_t)head[u] * hd + at[u] * 16;
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    float y[8];
-                    load8(x + 8 * w, v[u][0]);
-                    open8(v[u][0], y);
-                    put(2, head[u], at[u] * 16 + 8 * w, y);
-                }
+    if (!mine) return;
+    T * q_out = which == 0 ? (T *)a.q_out + row * a.q_out_stride + (size_t)head * hd : nullptr;
+    __half * pool = (which == 1 ? a.c.k : a.c.v) + ((size_t)head << a.c.shift) * hd;
+    for (int g = 0; g < nt; g++) {
+        if (g + 1 < nt) load(next, pair_next);
+        const float2 * c = cs + g * 128;
+        const int64_t to = s_at[g];
+        if (KIND == 2 && pairs) {
+            float y0 = rope_get(&pair[0]), y1 = rope_get(&pair[1]);
+            if (turns) {
+                const float2 w = c[at];
+                const float x0 = y0, x1 = y1;
+                y0 = x0 * w.x - x1 * w.y; y1 = x0 * w.y + x1 * w.x;
             }
+            if (which == 0)   { rope_put(q_out + d0, y0); rope_put(q_out + d1, y1); }
+            else if (to >= 0) { rope_put(pool + to + d0, y0); rope_put(pool + to + d1, y1); }
         } else {
-            bool turns; int d0, d1;
-            places(which[u], at[u], turns, d0, d1);
             float x0[8], x1[8];
-            open8(v[u][0], x0);
-            open8(v[u][1], x1);
-            if (KIND == 0 && which[u] < 2) {
+            open8(v[0], x0);
+            open8(v[1], x1);
+            if (KIND == 0 && which < 2) {
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const int k = (d0 + j) >> 1;
-                    if (k < half) { const float2 c = cs[k]; const float a0 = x0[j], a1 = x0[j + 1]; x0[j] = a0 * c.x - a1 * c.y; x0[j + 1] = a0 * c.y + a1 * c.x; }
-                    if (k + 4 < half) { const float2 c = cs[k + 4]; const float a0 = x1[j], a1 = x1[j + 1]; x1[j] = a0 * c.x - a1 * c.y; x1[j + 1] = a0 * c.y + a1 * c.x; }
+                    if (k < half) { const float2 w = c[k]; const float a0 = x0[j], a1 = x0[j + 1]; x0[j] = a0 * w.x - a1 * w.y; x0[j + 1] = a0 * w.y + a1 * w.x; }
+                    if (k + 4 < half) { const float2 w = c[k + 4]; const float a0 = x1[j], a1 = x1[j + 1]; x1[j] = a0 * w.x - a1 * w.y; x1[j + 1] = a0 * w.y + a1 * w.x; }
                 }
             } else if (turns) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float2 c = cs[d0 + j];
+                    const float2 w = c[d0 + j];
                     const float a0 = x0[j], a1 = x1[j];
-                    x0[j] = a0 * c.x - a1 * c.y; x1[j] = a0 * c.y + a1 * c.x;
+                    x0[j] = a0 * w.x - a1 * w.y; x1[j] = a0 * w.y + a1 * w.x;
                 }
             }
-            put(which[u], head[u], d0, x0);
-            put(which[u], head[u], d1, x1);
+            if (which == 0)   { store8(q_out + d0, x0); store8(q_out + d1, x1); }
+            else if (to >= 0) { store8(pool + to + d0, x0); store8(pool + to + d1, x1); }
         }
+        if (which == 0) q_out += a.q_out_stride;
+        v[0] = next[0]; v[1] = next[1]; pair[0] = pair_next[0]; pair[1] = pair_next[1];
     }
 }
 
-template <typename T, int KIND>
-static int append_run(const AppendP & p, int U, int threads, cudaStream_t st) {
-    const dim3 grid((unsigned)((int64_t)p.parts * p.a.b.max_new), p.a.b.n), block(threads);
-    if (U == 1)      PI_CUDA(launch_k(k_kv_append<T, KIND, 1>, grid, block, 0, st, true, p));
-    else if (U == 2 || sizeof(T) == 4) PI_CUDA(launch_k(k_kv_append<T, KIND, 2>, grid, block, 0, st, true, p));
-    else if (U == 3) PI_CUDA(launch_k(k_kv_append<T, KIND, 3>, grid, block, 0, st, true, p));
-    else             PI_CUDA(launch_k(k_kv_append<T, KIND, 4>, grid, block, 0, st, true, p));
-    return PI_OK;
-}
-
-// Few tokens: a unit a thread, so that there are threads for all SMs.  Many: two to four units a thread (FP32: one or two, 64 bytes each), the number of units and threads that leaves the fewest without one (of 576 units of the
-// falcon shape 2 x 256 and a second CTA of 64 took 40 us for 3329 tokens).
+// Tokens of a CTA: as many as leave AP_LEAST threads an SM, 4 at most, or 8 where the unit is a pair.  Measured with 1, 2, 4 and 8 (us): 3329 FP16 tokens of 128 heads over 8 of 64 38, 27, 24, 24, FP32 52, 41, 40, 45;
+// 32 heads over 32 of 128 48, 37, 35, 36; pairs 91, 50, 33, 25; 384 tokens of the first 6.3, 5.0, 6.1, 7.2; 150 of 64 FP32 heads over 8 of 128 6.1, 8.1, 10, 11.
 template <typename T>
 static int append_go(const AppendArgs & a, cudaStream_t st) {
     AppendP p;
@@ -183,16 +150,18 @@ static int append_go(const AppendArgs & a, cudaStream_t st) {
     p.heads[0] = a.x[0] ? a.n_head : 0; p.heads[1] = p.heads[2] = a.c.H;
     const int half = a.n_rot / 2, kind = !a.halves || half == 0 ? 0 : half % 8 == 0 ? 1 : 2;
     p.per_head = kind == 2 ? a.c.hd / 2 : a.c.hd / 16;
+    p.by_unit = AqDiv::by(p.per_head); p.by_value = AqDiv::by(a.c.hd / 16); p.by_half = AqDiv::by(half > 0 ? half : 1);
     const int64_t units = (int64_t)(p.heads[0] + p.heads[1]) * p.per_head + (int64_t)p.heads[2] * (a.c.hd / 16);
-    int U = 1; int64_t least = -1;
-    for (int u = 1; u <= 4; u++) {
-        const bool many = (int64_t)a.b.n * a.b.max_new * units >= (int64_t)sm_count() * 8 * AP_THREADS;
-        if (many ? (sizeof(T) == 2 ? u == 1 : u > 2) : u > 1) continue;
-        const int64_t parts = (units + (int64_t)u * AP_THREADS - 1) / ((int64_t)u * AP_THREADS), threads = ((units + parts * u - 1) / (parts * u) + 31) / 32 * 32;
-        if (least < 0 || parts * threads * u <= least) { least = parts * threads * u; U = u; p.parts = (int)parts; }
-    }
-    const int threads = (int)(((units + (int64_t)p.parts * U - 1) / ((int64_t)p.parts * U) + 31) / 32 * 32);
-    return kind == 0 ? append_run<T, 0>(p, U, threads, st) : kind == 1 ? append_run<T, 1>(p, U, threads, st) : append_run<T, 2>(p, U, threads, st);
+    p.parts = (int)((units + AP_THREADS - 1) / AP_THREADS);
+    const int threads = (int)((units + p.parts * 32 - 1) / (p.parts * 32) * 32);
+    const int64_t all = (int64_t)a.b.n * a.b.max_new * p.parts * threads;
+    p.tokens = 1;
+    while (p.tokens < (kind == 2 ? AP_TOKENS : AP_TOKENS / 2) && all / (2 * p.tokens) >= (int64_t)sm_count() * AP_LEAST) p.tokens *= 2;
+    const dim3 grid((unsigned)((int64_t)p.parts * ((a.b.max_new + p.tokens - 1) / p.tokens)), a.b.n), block(threads);
+    if (kind == 0)      PI_CUDA(launch_k(k_kv_append<T, 0>, grid, block, 0, st, true, p));
+    else if (kind == 1) PI_CUDA(launch_k(k_kv_append<T, 1>, grid, block, 0, st, true, p));
+    else                PI_CUDA(launch_k(k_kv_append<T, 2>, grid, block, 0, st, true, p));
+    return PI_OK;
 }
 
 int launch_kv_append_paged(const AppendArgs & a, cudaStream_t st) {

@@ -146,7 +146,8 @@ def pair_sums(x, hd, n_rot, halves):
 @pytest.mark.parametrize("halves", [False, True])
 @pytest.mark.parametrize("news,lens,H,group,hd,n_rot,page,far", [
     ([1], [1], 2, 2, 64, 64, 16, 0), ([1] * 5, [40, 1, 17, 16, 64], 8, 8, 128, 128, 64, 0), ([25, 7, 0, 1], [300, 40, 16, 33], 1, 7, 96, 96, 32, 100000),
-    ([130], [200], 5, 1, 192, 42, 128, 1000000), ([3, 64], [90, 64], 2, 3, 256, 256, 16, 5), ([17, 2], [17, 100], 4, 2, 64, 2, 16, 70), ([9], [9], 3, 1, 128, 96, 64, 2000000)])
+    ([130], [200], 5, 1, 192, 42, 128, 1000000), ([3, 64], [90, 64], 2, 3, 256, 256, 16, 5), ([17, 2], [17, 100], 4, 2, 64, 2, 16, 70), ([9], [9], 3, 1, 128, 96, 64, 2000000),
+    ([700, 77, 1, 133], [900, 80, 100, 133], 8, 8, 64, 64, 16, 0), ([701, 9], [701, 64], 4, 4, 96, 40, 32, 3000), ([211, 214], [300, 214], 8, 7, 128, 128, 64, 5000)])        # (several tokens a CTA)
 def test_append(ops, x, halves, news, lens, H, group, hd, n_rot, page, far):
     rng = np.random.default_rng(hd + sum(news) + n_rot)
     n, T, layer = len(news), sum(news), 1
@@ -203,6 +204,23 @@ def test_append_without_rotation_and_what_the_cache_lacks(ops):
     with np.errstate(over="ignore"):
         assert np.array_equal(one.k.cpu().numpy(), kw.astype(np.float16)) and np.array_equal(one.v.cpu().numpy(), vw.astype(np.float16), equal_nan=True)
     assert 0 < wrote.sum() < T * 2
+
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("news,mode,n_rot", [([3, 2], 0, 64), ([3, 2], 2, 64), ([900, 31], 0, 64), ([900, 31], 2, 64), ([900, 31], 2, 36)])
+def test_queries_turned_in_place(ops, x, news, mode, n_rot):
+    """q_out may be q where address and stride are the same: the same bits as into another array."""
+    from powerinfer_b200._lib import lib
+    rng = np.random.default_rng(n_rot + news[0])
+    c, T, f = pool(rng, 1, 4, 64, 16, news), sum(news), ops.rope_freqs(n_rot)
+    there, one, two = dev(rows(rng, T, (32 + 8) * 64, x)), on(ops, c), on(ops, c)
+    q, k, v = there[:, :2048], there[:, 2048:2304], there[:, 2304:]
+    q_start, pos0 = ints(starts(news)), ints([0, 0])
+    want = ops.kv_append_paged(one, k, v, q_start, pos0, max_new=max(news), q=q, freqs=f, mode=mode)
+    b, size, stride = ops._entries(q_start, pos0, None, T, max(news), 0), there.element_size(), there.stride(0)
+    assert lib.pi_kv_append_paged(two.c, b, 0, 0 if x == "f32" else 1, k.data_ptr(), stride, v.data_ptr(), stride, q.data_ptr(), stride, 32, q.data_ptr(), stride,
+                                  None, f.freqs.data_ptr(), n_rot, 1 if mode else 0, f.mscale, ops._stream()) == 0
+    assert size in (2, 4) and torch.equal(q, want) and torch.equal(one.k, two.k) and torch.equal(one.v, two.v)
 
 
 def test_queries_of_entries_that_are_not_stored_turn_all_the_same(ops):
