@@ -51,7 +51,6 @@ template <typename T, int KIND>
 __global__ void __launch_bounds__(AP_THREADS) k_kv_append(const AppendP p) {
     __shared__ float2 cs[AP_TOKENS * 128];
     __shared__ int64_t s_at[AP_TOKENS];                               // a token's row in the pools, without the head; -1: not stored
-    __shared__ int s_later;
     const AppendArgs & a = p.a;
     const int group = blockIdx.x / p.parts, part = blockIdx.x - group * p.parts, i = blockIdx.y, half = a.n_rot >> 1, hd = a.c.hd, tid = threadIdx.x, t0 = group * p.tokens;
     pdl_launch();
