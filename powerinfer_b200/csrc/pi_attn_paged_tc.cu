@@ -16,8 +16,8 @@
 // the chain from a score to its probability the rest.  One sequence of 32768 slots, 25 FP32 tokens, 64 heads over 8: 62 us; 8 of 1000 to 2000,
 // 48 FP16 tokens, 32 heads over 32: 47; 16 of 750 to 1500, 32 FP16 tokens, 128 heads over 8 of 64: 44.  Head_dim 256: 2 x 300 tokens of 3000 slots, 32 heads over 8: FP32 129, FP16 113 (copies: 96 KB a tile and half).
 //
-// Precision.  FP32 rows: queries and probabilities are the sum of two halves each, 22 bits, i.e. two products in the place of one.  FP16 rows: queries as they are, probabilities
-// one half, 11 bits like the result's own rounding.  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
+// Precision.  Probabilities, and queries of FP32 rows, are the sum of two halves each, 22 bits, i.e. two products in the place of one; queries of FP16 rows are halves as they are.  (One half for
+// FP16 rows' probabilities left 1.3 times the error of the result's own rounding, and 9 to 16 rows, which go to the other kernel, had other bits.)  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
 //
 // Warps: 0 issues the products of scores and 2 those of values; 1 asks for keys and 3 for values; 4 takes work and asks for its queries (5..7 make a warpgroup of it, for the registers); 8..19 have the
 // probabilities, three groups a tile each in turn, a row a thread; 20..27 drain the sums, a row and half of the columns a thread.
@@ -106,7 +106,7 @@ struct PtRing {
     __device__ __forceinline__ uint32_t here() const { return bar + at * 8u; }
 };
 
-// TWO: two halves for queries and probabilities
+// TWO: two halves for queries (FP32 rows)
 template <int HD, bool TWO>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_constant__ PtP pp) {
     using Z = PtShape<HD, TWO>;
@@ -237,12 +237,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int low = TWO ? 1 : 0; low >= 0; low--) {    // (lower halves of the probabilities first)
+                    for (int low = 1; low >= 0; low--) {              // (lower halves of the probabilities first)
                         int j = 0;
 #pragma unroll 1
-                        for (; j + 4 <= steps; j += 4) pt_values(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, (TWO && low == 0) || j > 0);
+                        for (; j + 4 <= steps; j += 4) pt_values(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, low == 0 || j > 0);
 #pragma unroll 1
-                        for (; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, (TWO && low == 0) || j > 0);
+                        for (; j < steps; j++) tc_mma_f16_ta(d, a + (uint32_t)(j * 16 + low * 8), v + 128 * j, idesc_v, low == 0 || j > 0);
                     }
                     pt_commit(pv + buf.at * 8);
                     pt_commit(empty + slot_v.at * 8);
@@ -443,10 +443,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                         for (int j = 0; j < 16; j += 2) {
                             const float2 y = f2_fma(make_float2(x[h * 16 + j], x[h * 16 + j + 1]), fc, ref), pr = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                             l[j >> 1 & 1] = f2_add(l[j >> 1 & 1], pr);
-                            if constexpr (TWO) f2_split(pr, hl[j / 2], hl[8 + j / 2]);
-                            else               hl[j / 2] = h2u(__floats2half2_rn(pr.x, pr.y));
+                            f2_split(pr, hl[j / 2], hl[8 + j / 2]);
                         }
-                        if constexpr (TWO) tc_st16(mine + 32 * c + 16 * h, hl); else tc_put<8>(mine + 32 * c + 16 * h, hl);
+                        tc_st16(mine + 32 * c + 16 * h, hl);
                     }
                 }
                 float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);

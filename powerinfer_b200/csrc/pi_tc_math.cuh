@@ -42,14 +42,5 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const float (&v)[32]) {
                  :: "r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]),
                     "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]) : "memory");
 }
-// N columns (8, 12 or 16) back
-template <int N> __device__ __forceinline__ void tc_put(uint32_t addr, const uint32_t (&v)[16]) {
-    static_assert(N == 8 || N == 12 || N == 16, "");
-    if constexpr (N == 16) tc_st16(addr, v);
-    else {
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-        if constexpr (N == 12) asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr + 8), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]) : "memory");
-    }
-}
 
 }  // namespace pi

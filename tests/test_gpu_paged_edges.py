@@ -1,0 +1,33 @@
+"""Calls of the operators of drafted tokens over a paged cache where they went wrong once or that the tests beside them do not reach, against paged_oracle.  Half a step is
+u = 2^-24 in FP32, 2^-11 in FP16."""
+import numpy as np
+import pytest
+
+import paged_oracle as po
+from test_gpu_paged import TY, U, attend, check, dev, ints, on, ops, pool, rows, starts, trees, words_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ------------------------------------------------------------------------------------------------ bits of the probabilities
+
+def norms(got, want):
+    """Norms of the error and of what rounding the exact result would leave, over the exact result's."""
+    got = got.double().cpu().numpy().reshape(want.shape)
+    n = np.linalg.norm(want)
+    return np.linalg.norm(got - want) / n, np.linalg.norm(want.astype(np.float16).astype(np.float64) - want) / n
+
+
+@pytest.mark.parametrize("hd,m,group,slots", [(64, 16, 8, 4096), (96, 16, 8, 4096), (128, 16, 8, 4096), (128, 40, 4, 1500), (64, 1, 8, 4096), (128, 2, 8, 1000), (256, 1, 16, 600), (192, 1, 5, 900)])
+def test_f16_rows_have_the_error_of_their_own_rounding(ops, hd, m, group, slots):
+    """Results are the roundings of sums with 22 bits of each probability.  Values of both signs: a probability's rounding to 11 bits would leave errors as large as the result's own
+    rounding, 1.3 times in all.  Scores are off by less than 2^-17 of a probability here (|s| < 16, hd u of the terms' sizes), as is all else: the rounding itself and 2^-16 beside it."""
+    rng = np.random.default_rng(hd + m)
+    H = 8
+    c = pool(rng, 1, H, hd, 64, [slots])
+    q = rows(rng, m, H * group * hd, "f16")
+    want, _ = po.attention(c, 0, q, H * group, [0, m], [slots - m], None, m, None, hd ** -0.5, U["f16"], 0.0)
+    got = attend(ops, c, "f16", q, H * group, [0, m], [slots - m], None, m, None, max_kv=slots)
+    error, rounding = norms(got, want)
+    assert error <= 1.02 * rounding + 2.0 ** -16, (error, rounding)
