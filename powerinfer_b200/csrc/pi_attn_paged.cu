@@ -10,7 +10,7 @@
 //
 // Precision.  Queries of FP32 rows, over a power of two of their row's largest value, and probabilities are the sum of two halves each, 22 bits, i.e. two products in the place
 // of one (the bytes bound it all the same); queries of FP16 rows are halves as they are.  Probabilities are held times 2^8: their steps end 2^-32 below the largest one.  Maxima, sums and
-// the exponents' arguments are FP32; FP32 rows' sums of values are added with rounding, as the tensor cores cut theirs.
+// the exponents' arguments are FP32; sums of values are added with rounding, as the tensor cores cut theirs (FP16 rows' over 2048 steps were 2^-12 too small).
 //
 // What a row does not see: scores are set to -infinity by the mask's bits, whatever the keys are; slots behind the entry's last and pages that are not there come as zeros; and where a step that not
 // every row sees whole holds a value that is not finite, its slots are added one by one to the rows that see them.
@@ -266,15 +266,12 @@ __global__ void __launch_bounds__(PA_THREADS, PaShape<HD>::CTAS) k_attn_paged(co
                         float w[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816(w, pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
                         o[n + h][0] += w[0] + w[2]; o[n + h][1] += w[1] + w[3];
-                    } else if constexpr (TWO) {                       // (the tensor cores cut FP32 sums: FP32 rows' are added with rounding)
+                    } else {                                          // (the tensor cores cut FP32 sums: they are added with rounding)
                         float w[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816(w, pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
                         mma16816(w, pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[n + h][e] += w[e];
-                    } else {
-                        mma16816(o[n + h], pl[0], pl[1], pl[2], pl[3], b[2 * h], b[2 * h + 1]);
-                        mma16816(o[n + h], pa[0], pa[1], pa[2], pa[3], b[2 * h], b[2 * h + 1]);
                     }
                 }
             }
