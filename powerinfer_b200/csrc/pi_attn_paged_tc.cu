@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 float total = (l[0].x + l[0].y) + (l[1].x + l[1].y);
                 if (masked) {
                     // the tile's values: a row a thread.  Rows of slots that are not there become zeros; so do those with a value that is not finite, and who sees them has no numbers
-                    const int slot = at % NW;
+                    // (A wait tells phases apart by their parity alone: first the place's former tile has to be used up.  With three places and more it is, as this tile's scores took its buffer.)
+                    const int slot = at % NW, former = at - NW;
+                    if (NW < PT_GROUPS && former >= 0 && !(ok = wait(s_pv + former % PT_GROUPS, former / PT_GROUPS & 1))) break;
                     if (!(ok = wait(s_vfull + slot, at / NW & 1))) break;
                     const int at_slot = w->k0 + i * PT_KEYS + r;
                     const bool is = info >> (r >> 4) & 1 && at_slot < w->there;

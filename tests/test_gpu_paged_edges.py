@@ -44,3 +44,32 @@ def test_f16_sums_of_many_steps_are_added_with_rounding(ops):
     want, _ = po.attention(c, 0, q, 8, [0, 2], [slots - 2], None, 2, None, hd ** -0.5, U["f16"], 0.0)
     got = attend(ops, c, "f16", q, 8, [0, 2], [slots - 2], None, 2, None, max_kv=1).double().cpu().numpy().reshape(want.shape)
     assert abs(((got - want.astype(np.float16)) / want).mean()) <= 2.0 ** -16
+
+
+# ------------------------------------------------------------------------------------------------ pieces after pieces
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+def test_values_of_special_tiles_are_waited_for(ops, x, hd):
+    """Contexts of a few tiles, many of them a CTA: the last tile's values are gone over before they are used, and the tile before it may still be on its way.  What lies behind the ends is no
+    number, so values that were gone over too early (or another tile's in their place) show."""
+    rng = np.random.default_rng(hd)
+    n, H, group, m = 24, 8, 8, 5
+    lens = [int(v) for v in rng.integers(m + 100, 700, n)]
+    c = pool(rng, 1, H, hd, 64, lens, holes=[(3, 1), (5, 0)])
+    news, q_start, pos0 = [m] * n, starts([m] * n), [v - m for v in lens]
+    masks, _ = po.tree_mask(trees(rng, news), q_start, pos0, m, 1)
+    mask = words_of(masks, 1)
+    q = rows(rng, n * m, H * group * hd, x)
+    odd = po.Cache(np.full_like(c.k, np.nan), np.full_like(c.v, np.nan), c.table)
+    for i in range(n):
+        for j in range(lens[i]):
+            if (at := c.place(i, j)) is not None:
+                odd.k[0, at[0], :, at[1]], odd.v[0, at[0], :, at[1]] = c.k[0, at[0], :, at[1]], c.v[0, at[0], :, at[1]]
+    for causal in (False, True):
+        args = (c, x, q, H * group, q_start, pos0, None, m, None if causal else mask)
+        plain = attend(ops, *args, max_kv=max(lens))
+        check(plain, *args)
+        for _ in range(10):
+            assert torch.equal(plain, attend(ops, odd, *args[1:], max_kv=max(lens)))
+        assert ops.last_op_status() == 0
