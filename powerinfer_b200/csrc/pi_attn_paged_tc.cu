@@ -36,7 +36,7 @@ static constexpr int PT_BOX = 64;                                     // rows of
 static constexpr int PT_WORK = 4;                                     // pieces of work that a CTA has in hand
 static constexpr int PT_INFO = 16;                                    // tiles whose description is kept: more than keys may be ahead of probabilities
 
-struct PtP { AttnPagedP a; int box, units, wide; unsigned int * next; CUtensorMap m_q, m_k, m_v; };
+struct PtP { AttnPagedP a; int box, units, wide; unsigned int tries; unsigned int * next; CUtensorMap m_q, m_k, m_v; };
 
 // what is in shared memory besides the ring: queries' buffers (upper and, of FP32 rows, lower halves), tiles in the ring
 // Of more than 128 columns a piece of work has all scores and half of the values' columns (the sums of all would leave tensor memory for one buffer of scores, FP32 rows' queries no room for a tile's
@@ -54,25 +54,32 @@ template <int HD, bool TWO> struct PtShape {
 struct PtWork { int tiles, k0, k1, first, n_rows, hk, there, clear, dst, v0; SeqB s; };      // tiles -1: there is no more; dst: number of the part that it makes, -1: results; v0: first column of the values
 
 // Barriers by their addresses in shared memory.  Code is kept short: seven roles run at once, and warps that waited for instructions were a third of the time.
-// A wait of up to some 20 us at a time (warps that ask again and again take issue slots), some 65536 times, or until another one of the CTA ran out.
-__device__ __forceinline__ bool pt_wait(uint32_t bar, unsigned parity, uint32_t dead) {
+// A wait of up to some 20 us at a time (warps that ask again and again take issue slots), `tries` times (PT_TRIES), or until another one of the CTA ran out.
+static constexpr unsigned PT_TRIES = 65536;
+__device__ __forceinline__ bool pt_wait(uint32_t bar, unsigned parity, uint32_t dead, unsigned tries) {
     unsigned ok;
     asm volatile("{\n .reg .pred p, q;\n .reg .u32 n, d;\n mov.u32 n, 0;\nWAIT:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n @p bra DONE;\n"
-                 " ld.volatile.shared.u32 d, [%4];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, 65536, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%4], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u), "r"(dead) : "memory");
+                 " ld.volatile.shared.u32 d, [%4];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, %5, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%4], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u), "r"(dead), "r"(tries) : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
 // The same without being suspended, for the two warps that issue products: they are told some 100 clocks earlier (chunk 203 -> 198 us); of more warps the asking costs what it gains
-__device__ __forceinline__ bool pt_poll(uint32_t bar, unsigned parity, uint32_t dead) {
+__device__ __forceinline__ bool pt_poll(uint32_t bar, unsigned parity, uint32_t dead, unsigned tries) {
     unsigned ok;
     asm volatile("{\n .reg .pred p, q;\n .reg .u32 n, d;\n mov.u32 n, 0;\nWAIT:\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
-                 " ld.volatile.shared.u32 d, [%3];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, 16777216, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%3], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(dead) : "memory");
+                 " ld.volatile.shared.u32 d, [%3];\n add.u32 n, n, 1;\n setp.eq.u32 q, d, 0;\n setp.lt.and.u32 q, n, %4, q;\n @q bra WAIT;\n st.volatile.shared.u32 [%3], 1;\nDONE:\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(dead), "r"(tries << 8) : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
 __device__ __forceinline__ void pt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
 __device__ __forceinline__ void pt_commit(uint32_t bar) {
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" :: "r"(bar) : "memory");
+}
+// The end of a warp that issues products: none is in flight when tensor memory is given back, whatever ran out before (the wait does not look at that)
+__device__ __forceinline__ void pt_end(uint64_t * bar) {
+    tc_commit(bar);
+    for (unsigned n = 0; n < PT_TRIES && !mbar_try_wait(bar, 0u); n++) {}
+    __syncwarp();
 }
 // N products of 16 steps of K each, both operands in shared memory, 32 bytes on from one to the next (64 columns of a piece are four); the first one adds to D if `add`
 template <int N> __device__ __forceinline__ void pt_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -150,8 +157,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     pdl_wait();
     asm volatile("fence.proxy.async;" ::: "memory");                // (what kernels before wrote is read by tensor copies)
     const uint32_t dead = smem_u32((const void *)&s_dead);
-    auto wait_at = [&](uint32_t bar, unsigned parity) { return pt_wait(bar, parity, dead); };      // warp-uniform; false: the wait ran out, here or elsewhere in the CTA
-    auto poll_at = [&](uint32_t bar, unsigned parity) { return pt_poll(bar, parity, dead); };
+    auto wait_at = [&](uint32_t bar, unsigned parity) { return pt_wait(bar, parity, dead, pp.tries); };      // warp-uniform; false: the wait ran out, here or elsewhere in the CTA
+    auto poll_at = [&](uint32_t bar, unsigned parity) { return pt_poll(bar, parity, dead, pp.tries); };
     auto wait = [&](uint64_t * bar, unsigned parity) { return wait_at(smem_u32(bar), parity); };
     auto work_of = [&](int n) { return s_work + n % PT_WORK; };
     auto done_with = [&](int n) { __syncwarp(); if (lane == 0) mbar_arrive(s_wempty + n % PT_WORK); };
@@ -214,8 +221,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 if (ok) done_with(n);
             }
-            tc_commit(s_fin);                                         // nothing is in flight when tensor memory is given back
-            wait(s_fin, 0u);
+            pt_end(s_fin);
         } else if (warp == 2) {
             // ============================================================= sums of values
             constexpr uint32_t idesc_v = tc_idesc(NV, true);
@@ -252,8 +258,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 if (ok) done_with(n);
             }
-            tc_commit(s_fin + 1);
-            wait(s_fin + 1, 0u);
+            pt_end(s_fin + 1);
         } else {
             // ============================================================= tiles of keys (warp 1) and of values (warp 3): a lane takes a copy of 64 columns of a box's rows
             const bool is_k = warp == 1;
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 if (is_k && lane == 0) mbar_arrive(&s_asked);         // (the next piece may be taken)
                 if (ok) done_with(n);
             }
-            if (!ok && lane == 0) ring_land(is_k ? s_kfull : s_vfull, asked, (int)slots);          // (else all have been waited for)
+            if (lane == 0) ring_land(is_k ? s_kfull : s_vfull, asked, (int)slots);      // (whoever was to wait for them may have given up)
             __syncwarp();
         }
     } else if (warp < 8) {
@@ -361,7 +366,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 done_with(n);
             }
-            if (!ok && lane == 0) ring_land(s_qfull, u, QB);          // (else they have been waited for)
+            if (lane == 0) ring_land(s_qfull, u, QB);
             __syncwarp();
         }
     } else if (warp < 8 + 4 * PT_GROUPS) {
@@ -498,6 +503,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             g += tiles;
             if (ok) done_with(n);
         }
+        tc_wait_st();                                                 // (of a tile that was given up)
     } else {
         // ================================================================= sums out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(PT_REGS_D));
@@ -688,6 +694,8 @@ static int pt_go(const AttnPagedP & a, cudaStream_t st) {
     p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * 4 % 32 == 0;
     p.units = (int)ap_grid(a) * (PtShape<HD, TWO>::WIDE ? 2 : 1);
     p.next = a.status + 8;
+    static const char * tries = getenv("PI_ATTN_TREE_TRIES");         // (a diagnostic switch, read once: how often the kernel's waits ask)
+    p.tries = tries ? (unsigned)strtoul(tries, nullptr, 10) & 0xffffu : PT_TRIES;
     const int64_t q_rows = (int64_t)a.b.T * a.n_head;
     if ((rc = tensor_map(&p.m_q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.queries, HD, q_rows * (TWO ? 2 : 1), HD * 2, 64, PT_ROWS, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     PI_CUDA(launch_k(k_attn_paged_queries<HD, TWO>, dim3((unsigned)((q_rows + 31) / 32)), dim3(256), 0, st, true, a, a.queries, a.factor, p.next));

@@ -73,3 +73,54 @@ def test_values_of_special_tiles_are_waited_for(ops, x, hd):
         for _ in range(10):
             assert torch.equal(plain, attend(ops, odd, *args[1:], max_kv=max(lens)))
         assert ops.last_op_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ waits that run out
+
+def test_last_op_status_is_that_of_the_attention(ops):
+    """The status word that last_op_status reads is the last operator's: set as if a wait had run out, cleared by the next call."""
+    rng = np.random.default_rng(6)
+    c = pool(rng, 1, 8, 64, 64, [4096])
+    q = rows(rng, 40, 32 * 64)
+    attend(ops, c, "f32", q, 32, [0, 40], [4056], None, 40, None)
+    assert ops.last_op_status() == 0
+    ops._ws.asked[1].view(torch.int32)[2] = 16
+    assert ops.last_op_status() == 5
+    attend(ops, c, "f32", q, 32, [0, 40], [4056], None, 40, None)
+    assert ops.last_op_status() == 0
+    attend(ops, c, "f32", q[:1], 32, [0, 1], [50], None, 1, None, max_kv=64)
+    assert ops.last_op_status() == 0
+
+
+def run_out(hd, x):
+    """In a process whose waits ask a few times only: statuses, what comes of rows, and calls behind them."""
+    from powerinfer_b200 import ggml_ops as g
+    rng = np.random.default_rng(hd)
+    n, H, group, m = 24, 8, 8, 5
+    lens = [int(v) for v in rng.integers(m + 100, 1500, n)]
+    c = pool(rng, 1, H, hd, 64, lens)
+    q_start, pos0, T = [1 + i * m for i in range(n + 1)], [v - m for v in lens], n * m + 3
+    q = dev(rows(rng, T, H * group * hd, x))
+    seen = []
+    for max_kv in (max(lens), 6000, max(lens)):
+        out = torch.full((T, H * group * hd), 7.0, dtype=TY[x], device="cuda")
+        attend(g, c, x, q, H * group, q_start, pos0, None, m, None, max_kv=max_kv, out=out)
+        seen.append(g.last_op_status())
+        few = attend(g, c, x, q[1:2], H * group, [0, 1], [300], None, 1, None)         # (no bounded waits)
+        check(few, c, x, q[1:2].cpu().numpy(), H * group, [0, 1], [300], None, 1, None)
+        assert (out[0] == 7).all() and (out[n * m + 1:] == 7).all()   # rows of no entry
+    return seen
+
+
+@pytest.mark.parametrize("tries", [0, 1, 20])
+def test_waits_that_run_out_end_with_a_status(ops, tries):
+    """PI_ATTN_TREE_TRIES shortens the waits (the first one, for the work in hand, asks once with 0): the kernel ends, reports, and the calls behind it are right."""
+    import os
+    import subprocess
+    import sys
+    code = f"import sys; sys.path[:0] = [{os.path.dirname(__file__)!r}, {os.path.dirname(os.path.dirname(__file__))!r}]\nimport test_gpu_paged_edges as t\n" + \
+        "print('status', *[s for hd in (64, 96, 128, 192, 256) for x in ('f32', 'f16') for s in t.run_out(hd, x)])"
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PI_ATTN_TREE_TRIES": str(tries)}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "status" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+    seen = [int(v) for v in r.stdout.split("status")[1].split()]
+    assert len(seen) == 30 and set(seen) <= {0, 5} and (tries > 0 or set(seen) == {5})
