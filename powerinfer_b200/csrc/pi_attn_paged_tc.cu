@@ -53,6 +53,22 @@ template <int HD, bool TWO> struct PtShape {
 // A piece of work: 128 rows of one KV head and a range of slots
 struct PtWork { int tiles, k0, k1, first, n_rows, hk, there, clear, dst, v0; SeqB s; };      // tiles -1: there is no more; dst: number of the part that it makes, -1: results; v0: first column of the values
 
+template <bool WIDE, int HV> __device__ __forceinline__ PtWork pt_piece(const PtP & pp, int unit) {      // (tiles -1: there are no rows, or another part answers for them)
+    const AttnPagedP & p = pp.a;
+    const AqItem it = ap_item(p, WIDE ? unit >> 1 : unit);
+    PtWork w;
+    w.tiles = -1;
+    w.v0 = WIDE && unit & 1 ? HV : 0;
+    w.s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, it.entry);
+    const TileP t = ap_tile(p, w.s, p.row_tiles - 1 - it.rt, PT_ROWS);          // (the longest rows first)
+    w.k0 = it.split * p.split; w.k1 = it.split == it.n_splits - 1 ? t.seen : min(t.seen, w.k0 + p.split);
+    w.first = t.first; w.n_rows = t.n_rows; w.hk = it.hk; w.there = t.there;
+    w.dst = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1;
+    w.clear = p.mask ? w.s.pos : w.s.pos + p.by_group.of(t.first) + 1;          // every row sees the slots before it
+    if (t.n_rows > 0 && (w.k0 < w.k1 || it.split == 0)) w.tiles = w.k0 < w.k1 ? (w.k1 - w.k0 + PT_KEYS - 1) / PT_KEYS : 0;      // (split 0 answers for rows that see nothing)
+    return w;
+}
+
 // Barriers by their addresses in shared memory.  Code is kept short: seven roles run at once, and warps that waited for instructions were a third of the time.
 // A wait of up to some 20 us at a time (warps that ask again and again take issue slots), `tries` times (PT_TRIES), or until another one of the CTA ran out.
 static constexpr unsigned PT_TRIES = 65536;
@@ -129,10 +145,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ uint64_t s_kfull[NK], s_kempty[NK], s_vfull[NW], s_vempty[NW];
     __shared__ uint64_t s_wfull[PT_WORK], s_wempty[PT_WORK], s_qfull[QB], s_qempty[QB];
-    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_scan[PT_GROUPS], s_fin[2], s_asked;
+    __shared__ uint64_t s_qk[PT_GROUPS], s_pv[PT_GROUPS], s_pfull[PT_GROUPS], s_stat[PT_GROUPS], s_scan[PT_GROUPS], s_fin[2], s_asked, s_over;
     __shared__ PtWork s_work[PT_WORK];
     __shared__ uint32_t s_tmem, s_info[PT_INFO];                      // of a tile: which groups of 16 slots are there; bit 8: special
     __shared__ volatile unsigned s_dead;
+    __shared__ int s_given;                                           // pieces that this CTA had, there with s_over
     __shared__ uint32_t s_odd[PT_GROUPS][4];                           // slots of a special tile with a value that is not finite
     __shared__ float s_top[PT_GROUPS][PT_ROWS], s_sum[PT_GROUPS][PT_ROWS];         // of a tile: maximum, sum of the probabilities
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -145,6 +162,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     if (tid < PT_GROUPS) { mbar_init(s_qk + tid, 2); mbar_init(s_pv + tid, 1); mbar_init(s_pfull + tid, 12); mbar_init(s_stat + tid, 8); mbar_init(s_scan + tid, 4); }
     if (tid < 2) mbar_init(s_fin + tid, 1);
     if (tid == 2) mbar_init(&s_asked, 1);
+    if (tid == 3) mbar_init(&s_over, 1);
     if (tid == 0) s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
@@ -305,7 +323,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                     }
                     if (!ok) break;
                 }
-                if (is_k && lane == 0) mbar_arrive(&s_asked);         // (the next piece may be taken)
+                if (is_k && ok && lane == 0) mbar_arrive(&s_asked);   // (the next piece may be taken)
                 if (ok) done_with(n);
             }
             if (lane == 0) ring_land(is_k ? s_kfull : s_vfull, asked, (int)slots);      // (whoever was to wait for them may have given up)
@@ -324,33 +342,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
             PtRing qs(s_qfull);
             const uint32_t qempty = smem_u32(s_qempty);
             bool ok = true;
-            int u = 0;                                                // pieces with tiles
+            int u = 0, given = 0;                                     // pieces with tiles, pieces
             for (int n = 0; ok; n++) {
                 if (n >= PT_WORK && !(ok = wait(s_wempty + n % PT_WORK, n / PT_WORK & 1 ^ 1))) break;
                 // the next piece when the keys of the last one have all been asked for, two or three tiles before it ends: taken as soon as there is room, all pieces of a call of 400
                 // were dealt out at its start, and one CTA had 38 tiles where 29 is the mean (trees of many users)
                 if (n > 0) {
-                    if (!(ok = wait(&s_asked, n & 1 ^ 1))) break;
+                    if (!(ok = wait(&s_asked, n & 1 ^ 1) && __all_sync(0xffffffffu, s_dead == 0))) break;       // (nothing is taken behind a wait that ran out)
                     take();
                 }
                 PtWork w;
                 w.tiles = -1;
                 while (unit < pp.units) {                             // the next piece that has something to do
-                    const AqItem it = ap_item(p, WIDE ? unit >> 1 : unit);
-                    w.v0 = WIDE && unit & 1 ? Z::HV : 0;
-                    w.s = seq_entry(p.b, p.c.n_seq, p.c.n_ctx, it.entry);
-                    const TileP t = ap_tile(p, w.s, p.row_tiles - 1 - it.rt, PT_ROWS);      // (the longest rows first)
-                    w.k0 = it.split * p.split; w.k1 = it.split == it.n_splits - 1 ? t.seen : min(t.seen, w.k0 + p.split);
-                    w.first = t.first; w.n_rows = t.n_rows; w.hk = it.hk; w.there = t.there;
-                    w.dst = it.n_splits > 1 ? (it.item - p.whole) * p.n_splits + it.split : -1;
-                    w.clear = p.mask ? w.s.pos : w.s.pos + p.by_group.of(t.first) + 1;      // every row sees the slots before it
-                    if (t.n_rows > 0 && (w.k0 < w.k1 || it.split == 0)) w.tiles = w.k0 < w.k1 ? (w.k1 - w.k0 + PT_KEYS - 1) / PT_KEYS : 0;      // (split 0 answers for rows that see nothing)
+                    w = pt_piece<WIDE, Z::HV>(pp, unit);
                     if (w.tiles >= 0) break;
                     take();
                 }
                 if (lane == 0) { *work_of(n) = w; mbar_arrive(s_wfull + n % PT_WORK); }
                 __syncwarp();
                 if (w.tiles < 0) break;
+                given = n + 1;
                 if (w.tiles > 0) {
                     if (u >= QB && !(ok = wait_at(qempty + qs.at * 8, qs.parity ^ 1))) break;
                     u++;
@@ -366,7 +377,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
                 done_with(n);
             }
-            if (lane == 0) ring_land(s_qfull, u, QB);
+            if (lane == 0) { s_given = given; mbar_arrive(&s_over); ring_land(s_qfull, u, QB); }
             __syncwarp();
         }
     } else if (warp < 8 + 4 * PT_GROUPS) {
@@ -515,10 +526,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
         bool ok = true;
         if (lane == 0) for (int i = 0; i < OB; i++) pt_arrive(pfull + i * 8);       // (nothing to drain before the first tiles)
         for (int n = 0; ; n++) {
-            // (after a wait that ran out: the rows of the work in hand are no numbers)
             if (ok) ok = wait(s_wfull + n % PT_WORK, n / PT_WORK & 1);
-            else if (!__all_sync(0xffffffffu, mbar_try_wait(s_wfull + n % PT_WORK, n / PT_WORK & 1))) break;
-            if (!ok && !__all_sync(0xffffffffu, mbar_try_wait(s_wfull + n % PT_WORK, n / PT_WORK & 1))) break;
+            if (!ok) {                                                // after a wait that ran out: the rows of the pieces in hand are no numbers
+                for (unsigned k = 0; k < PT_TRIES && !mbar_try_wait(&s_over, 0u); k++) {}
+                __syncwarp();
+                if (n >= __shfl_sync(0xffffffffu, s_given, 0)) break;
+            }
             const PtWork * w = work_of(n);
             const int tiles = w->tiles;
             if (tiles < 0) break;
@@ -596,6 +609,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
                 }
             }
             if (ok) done_with(n);
+        }
+        if (!ok) {                                                    // nor are those of pieces that nobody may take any more: a warp of these takes one at a time
+            for (;;) {
+                int unit = 0;
+                if (lane == 0) unit = (int)gridDim.x + (int)atomicAdd(pp.next, 1u);
+                unit = __shfl_sync(0xffffffffu, unit, 0);
+                if (unit >= pp.units) break;
+                const PtWork w = pt_piece<WIDE, Z::HV>(pp, unit);
+                const float none = __int_as_float(0x7fc00000);
+                for (int row = lane; w.tiles >= 0 && row < w.n_rows; row += 32) {
+                    const int of = p.by_group.of(w.first + row), h = w.hk * p.group + w.first + row - of * p.group;
+                    const size_t at = (size_t)(w.s.first + of) * p.out_stride + (size_t)h * HD + w.v0, part = (size_t)w.dst * PT_ROWS + row;
+                    if (w.dst >= 0 && w.v0 == 0) p.part_ml[part] = make_float2(-INFINITY, none);
+#pragma unroll 1
+                    for (int j = 0; j < Z::HV; j++) {
+                        if (w.dst >= 0)   p.part[part * HD + w.v0 + j] = none;
+                        else if (TWO)     ((float *)p.out)[at + j] = none;
+                        else              ((__half *)p.out)[at + j] = __float2half_rn(none);
+                    }
+                }
+            }
         }
     }
     tc_fence_before();
