@@ -46,6 +46,26 @@ def test_f16_sums_of_many_steps_are_added_with_rounding(ops):
     assert abs(((got - want.astype(np.float16)) / want).mean()) <= 2.0 ** -16
 
 
+@pytest.mark.parametrize("hd,m,group,slots", [(64, 16, 8, 4096), (96, 16, 8, 4096), (128, 16, 8, 4096), (192, 16, 8, 2000), (256, 16, 8, 2000), (64, 3, 8, 20000), (128, 1, 4, 20000),
+                                              (64, 1, 8, 900), (96, 2, 8, 900), (192, 2, 5, 900), (256, 1, 16, 900)])
+def test_f32_rows_keep_the_bits_of_both_halves(ops, hd, m, group, slots):
+    """The norm of the error, over the result's.  Queries or probabilities of one half alone would leave 2^-12.8 (a score is some units); with both, errors of a query and of a probability are 2^-22
+    of it or less, a score of up to 8 is a sum of hd / 16 steps off by 2^-22 at most, 4 of which in the root of their squares are 2^-20, and a probability is off by as much of itself: twice that, and
+    as much again for the sums."""
+    rng = np.random.default_rng(hd + m)
+    H = 8
+    c = pool(rng, 1, H, hd, 32, [slots])
+    q = rows(rng, m, H * group * hd)
+    want, _ = po.attention(c, 0, q, H * group, [0, m], [slots - m], None, m, None, hd ** -0.5, U["f32"], 0.0)
+    got = attend(ops, c, "f32", q, H * group, [0, m], [slots - m], None, m, None, max_kv=slots)
+    assert norms(got, want)[0] <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("hd,m", [(192, 16), (256, 16)])
+def test_wide_f16_rows_have_the_error_of_their_own_rounding(ops, hd, m):
+    test_f16_rows_have_the_error_of_their_own_rounding(ops, hd, m, 8, 2000)
+
+
 # ------------------------------------------------------------------------------------------------ pieces after pieces
 
 @pytest.mark.parametrize("x", ["f32", "f16"])
@@ -73,6 +93,36 @@ def test_values_of_special_tiles_are_waited_for(ops, x, hd):
         for _ in range(10):
             assert torch.equal(plain, attend(ops, odd, *args[1:], max_kv=max(lens)))
         assert ops.last_op_status() == 0
+
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("n,H,m,group,hd,kv,cut", [
+    (20, 16, 5, 8, 128, 700, "whole"), (20, 16, 5, 8, 64, 500, "whole"), (7, 22, 5, 8, 64, 2000, "both"), (5, 30, 5, 8, 96, 2000, "both"), (5, 30, 5, 8, 128, 2000, "both"),
+    (5, 16, 5, 8, 192, 2000, "both"), (5, 16, 5, 8, 256, 1500, "whole"), (5, 16, 5, 8, 256, 2000, "both"), (1, 22, 60, 8, 64, 700, "few"), (1, 22, 120, 8, 64, 700, "whole"),
+    (40, 8, 1, 8, 128, 1000, "both"), (60, 8, 1, 8, 64, 1500, "both"), (40, 8, 2, 8, 96, 1500, "both"), (20, 8, 2, 8, 192, 1500, "both"), (20, 8, 1, 4, 256, 1000, "both")])
+def test_more_items_than_processors(ops, x, n, H, m, group, hd, kv, cut):
+    """More pieces of work than CTAs run at once, of unequal lengths; items that are a piece each beside others in parts ("both"); entries without tokens and without a context."""
+    from powerinfer_b200 import _lib
+    rng = np.random.default_rng(n + hd)
+    news = [m if i in (0, 3) else int(v) for i, v in enumerate(rng.integers(0, m + 1, n))]
+    lens = [kv if i == 0 else news[i] if i % 5 == 4 else int(v) for i, v in enumerate(rng.integers(m, kv + 1, n))]
+    c = pool(rng, 1, H, hd, 32, lens)
+    q_start, pos0, T = starts(news), [a - b for a, b in zip(lens, news)], sum(news)
+    masks, _ = po.tree_mask(trees(rng, news), q_start, pos0, m, 1)
+    q = rows(rng, T, H * group * hd, x)
+    # the parts that the workspace has room for, in tiles of rows
+    many = m * group > 16
+    R, size = 128 if many else 8 if m * group <= 8 else 16, 2 if x == "f16" else 4
+    need = _lib.lib.pi_attention_tree_workspace_bytes(on(ops, c).c, ops._entries(ints(q_start), ints(pos0), None, T, m, 0), ops._ROW_TYPES[TY[x]], H * group, kv)
+    parts = (need - (256 + T * H * group * (hd * size + (4 if x == "f32" else 0)) if many else min(need, 256))) // ((8 + 4 * hd) * R)
+    items = n * H * -(-m * group // R) * (2 if many and hd > 128 else 1)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert (items > 148) == (cut != "few") and (0 < parts < items // 2 if cut == "both" else parts == 0), (parts, items)
+    for mask in (None, words_of(masks, 1)):
+        args = (c, x, q, H * group, q_start, pos0, None, m, mask)
+        got = attend(ops, *args, max_kv=kv)
+        check(got, *args)
+        assert ops.last_op_status() == 0 and torch.equal(got, attend(ops, *args, max_kv=kv))
 
 
 # ------------------------------------------------------------------------------------------------ waits that run out
