@@ -441,7 +441,7 @@ static PaPlan pa_plan(const KvPaged & c, const RaggedB & b, int xtype, int n_hea
     PaPlan r;
     const int64_t rows = (int64_t)b.max_new * (n_head / c.H);
     const int64_t keys = max_kv < 1 ? 1 : max_kv > c.n_ctx ? c.n_ctx : max_kv;
-    r.tc = attn_paged_tc_takes(c.hd, rows, (int64_t)b.n * c.H * keys * c.hd);
+    r.tc = attn_paged_tc_takes(rows, (double)b.n * c.H * keys * c.hd);
     r.R = r.tc ? PT_ROWS : rows <= 8 ? 8 : 16;
     r.row_tiles = (int)((rows + r.R - 1) / r.R);
     const int step = r.tc ? PT_KEYS : PA_STEP;

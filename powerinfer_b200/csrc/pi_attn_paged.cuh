@@ -92,7 +92,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 
 // Many rows of a KV head on tcgen05 (pi_attn_paged_tc.cu): tiles of PT_ROWS rows, splits a multiple of PT_KEYS slots
 static constexpr int PT_ROWS = 128, PT_KEYS = 128;
-bool attn_paged_tc_takes(int hd, int64_t rows, int64_t values);     // rows of a KV head, values of all keys
+bool attn_paged_tc_takes(int64_t rows, double values);             // rows of a KV head, values of all keys
 
 int launch_attn_paged_tc(const AttnPagedP & p, cudaStream_t st);
 

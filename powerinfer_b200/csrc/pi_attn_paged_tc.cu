@@ -702,11 +702,11 @@ __global__ void __launch_bounds__(256) k_attn_paged_queries(const AttnPagedP p, 
 // sequence 24 rows 17 and 14, 48 rows 18 and 16, 64 rows 18 and 17; one of 500 slots and 32 KV heads 64 rows 15 and 14.
 // The same of head_dim 256 and 192: 8 sequences of 4096 24 rows 85 and 99, 72 and 82; one 24 rows 23 and 21, 21 and 18; 64 rows 23 and 32, 22 and 28; one of 500 and 32 KV heads of 256 64 rows 20 and 19, 128 rows 22 and 36.
 // (PI_ATTN_TREE_TC=1 takes 17 rows and more whatever there is, 0 none: a diagnostic switch, read once.)
-bool attn_paged_tc_takes(int hd, int64_t rows, int64_t values) {
+bool attn_paged_tc_takes(int64_t rows, double values) {
     static int forced = -2;
     if (forced == -2) { const char * v = getenv("PI_ATTN_TREE_TC"); forced = v ? v[0] != '0' : -1; }
     if (rows <= 16 || forced == 0) return false;
-    return forced == 1 || ((rows + 15) / 16 - 1) * 16 * (double)values > 5.0 * (1 << 25) + 7.0 * values;
+    return forced == 1 || ((rows + 15) / 16 - 1) * 16 * values > 5.0 * (1 << 25) + 7.0 * values;
 }
 
 template <int HD, bool TWO>

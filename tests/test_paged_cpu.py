@@ -121,6 +121,13 @@ def test_workspace_is_sized_by_the_same_arguments():
     assert lib.pi_attention_tree_workspace_bytes(C.byref(cache(page=5)), C.byref(b), F32, 8, 32768) == 0 and "page" in err()
 
 
+@pytest.mark.parametrize("n", [500, 520, 600, 900, 1200])
+def test_more_values_than_64_bits_count_are_many(n):
+    """n caches of 65535 KV heads of 256, 2^30 slots each: the queries are laid out (F16) as for all large calls."""
+    c, b = cache(max_pages=1 << 26, page=16, n_head_kv=65535, head_dim=256, n_pages=1), batch(n=n, T=500, max_new=1)
+    assert lib.pi_attention_tree_workspace_bytes(C.byref(c), C.byref(b), F16, 65535 * 32, 1 << 30) >= 500 * 65535 * 32 * 256 * 2
+
+
 def test_structures_are_packed_as_c_lays_them_out():
     pytest.importorskip("torch")
     from powerinfer_b200 import ggml_ops as g
