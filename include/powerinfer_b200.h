@@ -282,7 +282,7 @@ int pi_kv_append_paged(const pi_kv_paged * cache, const pi_kv_batch * batch, int
 /* llm_build_kqv (llama.cpp:4764-4850) over the pages of layer `layer`, the new tokens' keys and values in them already: token t of entry i sees the slots 0 .. pos0[i] - 1 and
  * pos0[i] + u for those new tokens u of its entry that its row of mask [T, mask_words] names (pi_tree_mask's, or any other; mask NULL: u <= t), where the cache has
  * them; out = softmax(scale * q . k) v for every query head, heads h of group h / (n_head / n_head_kv).  q, out [T, n_head * head_dim] (F32 or F16).  A token that sees nothing has
- * zeros, so has one whose own slot lies behind n_ctx; what it does not see has no part in its row, whatever is there.  (What it sees has to be finite numbers: a row that sees others is not.)
+ * zeros, so has one whose own slot lies behind n_ctx; what it does not see has no part in its row, whatever is there.  (Keys and values that a row sees have to be finite numbers: what it holds otherwise is not said, and is not the same for few rows and for many.)
  * F32 rows: queries to 2^-22 of their row's largest value; F16 rows: queries as they are.  A probability has 22 bits down to 2^-10 of its row's largest one and an error of 2^-32 of that below.
  * Sums are FP32.
  * max_kv: the slots that the longest sequence is expected to have (it sets how the work is cut; more slots are read too, more slowly).

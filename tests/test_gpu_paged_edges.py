@@ -125,6 +125,34 @@ def test_more_items_than_processors(ops, x, n, H, m, group, hd, kv, cut):
         assert ops.last_op_status() == 0 and torch.equal(got, attend(ops, *args, max_kv=kv))
 
 
+# ------------------------------------------------------------------------------------------------ strides
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("n,m,kv", [(3, 1, 700), (3, 2, 3000), (12, 9, 700), (1, 9, 6000)])
+def test_rows_16_bytes_off(ops, x, hd, n, m, kv):
+    """Queries and results as columns of wider matrices that begin 16 bytes behind a boundary of 32, rows an odd number of 16 bytes apart: the bits of contiguous ones, and nothing beside them."""
+    from powerinfer_b200 import _lib
+    rng = np.random.default_rng(hd + m)
+    H, group = 4, 8
+    lens = [kv] + [int(v) for v in rng.integers(m, kv, n - 1)]
+    c, T, width, pad = on(ops, pool(rng, 1, H, hd, 16, lens)), n * m, H * group * hd, 16 // (4 if x == "f32" else 2)
+    wide = dev(rows(rng, T, width + 3 * pad, x))
+    q = wide[:, pad:pad + width]
+    q_start, pos0 = ints(starts([m] * n)), ints([v - m for v in lens])
+    want = ops.attention_tree(c, q.contiguous(), q_start, pos0, max_new=m, max_kv=kv)
+    assert q.data_ptr() % 32 == 16 and q.stride(0) * q.element_size() % 32 == 16
+    assert torch.equal(want, ops.attention_tree(c, q, q_start, pos0, max_new=m, max_kv=kv))
+    to = torch.full((T, width + 5 * pad), 7.0, dtype=TY[x], device="cuda")
+    b = ops._entries(q_start, pos0, None, T, m, 0)
+    need = _lib.lib.pi_attention_tree_workspace_bytes(c.c, b, ops._ROW_TYPES[TY[x]], H * group, kv)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device="cuda")
+    assert _lib.lib.pi_attention_tree(c.c, b, 0, ops._ROW_TYPES[TY[x]], q.data_ptr(), q.stride(0), H * group, None, 0, kv, hd ** -0.5, to[:, pad:].data_ptr(), to.stride(0), ws.data_ptr(), ws.numel(),
+                                      ops._stream()) == 0
+    assert torch.equal(to[:, pad:pad + width], want) and (to[:, :pad] == 7).all() and (to[:, pad + width:] == 7).all()
+    assert torch.isfinite(want).all() and _lib.lib.pi_op_status(ws.data_ptr(), ops._stream()) == 0
+
+
 # ------------------------------------------------------------------------------------------------ waits that run out
 
 def test_last_op_status_is_that_of_the_attention(ops):
