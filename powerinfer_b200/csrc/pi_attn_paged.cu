@@ -433,7 +433,8 @@ struct PaPlan { bool tc; int R, row_tiles, split, n_splits, items, whole; size_t
 // Items are a CTA (a piece of work) each, or split into ranges of at least PA_LEAST slots: none of them, those beyond as many as fill rounds of all CTAs that the SMs hold, or
 // all; into the number of parts that is estimated to take the least.  A piece costs as much as its slots and PA_TURN times 64 more (on tcgen05, where parts are larger too, PA_TURN_TC
 // whole and PA_TURN_PART as a part), the kernel that joins as PA_TURN times 64 (PA_JOIN_TC on tcgen05, whose CTAs even out whole pieces by themselves).  Measured on tcgen05 (us): 2 x 1024 FP16 tokens over 3000
-// slots, 32 heads over 8 of 128, 512 pieces whole 99, 68 of them in two parts 108; 1024 FP32 tokens over 4096, 64 heads over 8 of 128 196 and 195; 3 x 64 FP32 tokens over 6000, 32 heads of 64, 96 pieces whole 61, all in three 51.
+// slots in pages of 16, 32 heads over 8 of 128, 512 pieces whole 109, 68 of them in two parts 118; 6 x 300 over 2000 65 and 68; 1024 FP32 tokens over 4096, 64 heads over 8 of 128 196 and 195; 3 x 64 FP32 tokens over 6000, 32 heads of 64,
+// 96 pieces whole 61, all in three 51.
 // With mma.sync: pieces are as long as max_kv says and run in rounds.  On tcgen05 CTAs take one after the other: the same for one sequence; of several half of that and half of the time of sequences of half
 // to all of max_kv's length (work over SMs, and half of a piece at the end).
 static constexpr int PA_LEAST = 256, PA_TURN = 4, PA_TURN_TC = 3, PA_TURN_PART = 8, PA_JOIN_TC = 12, PA_ROUNDS = 4;        // (more rounds of parts than that: room for the parts, and nothing gained)

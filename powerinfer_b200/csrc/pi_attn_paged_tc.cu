@@ -11,10 +11,10 @@
 // become zeros, rows with a value that is not finite too, and whoever sees such a slot has a row of no numbers; scores of slots that a row does not see are replaced by what its
 // mask says.
 //
-// What bounds it, by shape (FP32 128, a chunk of 1024 tokens over 4096 slots, 64 heads over 8: 194 us, of which the products, two for one, would take 146): at head_dim 128 FP32 a tile takes 2650 clocks, the
-// products 2048, and the sums of a tile, one buffer, wait for the ones before to be drained; FP16 2400, the copies of keys and values 2150 (30 bytes a clock and SM, the rate of the memory); at head_dim 64 FP16 1660, the exponents 1024 and
-// the chain from a score to its probability the rest.  One sequence of 32768 slots, 25 FP32 tokens, 64 heads over 8: 62 us; 8 of 1000 to 2000,
-// 48 FP16 tokens, 32 heads over 32: 47; 16 of 750 to 1500, 32 FP16 tokens, 128 heads over 8 of 64: 44.  Head_dim 256: 2 x 300 tokens of 3000 slots, 32 heads over 8: FP32 129, FP16 113 (copies: 96 KB a tile and half).
+// What bounds it, by shape, warm and in a graph (FP32 128, a chunk of 1024 tokens over 4096 slots, 64 heads over 8: 198 us, of which the products, two for one, would take 146; FP16 162): at head_dim 128 FP32 a
+// tile takes 2670 clocks, the products 2048, and the sums of a tile, one buffer, wait for the ones before to be drained; FP16 2580, the copies of keys and values 2150 (30 bytes a clock and SM, the rate of the
+// memory) and the products 1536; at head_dim 64 FP16 1900, the exponents 1024, the products 768 and the chain from a score to its probability.  One sequence of 32768 slots, 25 FP32 tokens, 64 heads over 8: 63 us; 8 of
+// 1000 to 2000, 48 FP16 tokens, 32 heads over 32: 50; 16 of 750 to 1500, 32 FP16 tokens, 128 heads over 8 of 64: 51.  Head_dim 256: 2 x 300 tokens of 3000 slots, 32 heads over 8: FP32 132, FP16 123 (copies: 96 KB a tile and half).
 //
 // Precision.  Probabilities, and queries of FP32 rows, are the sum of two halves each, 22 bits, i.e. two products in the place of one; queries of FP16 rows are halves as they are.  (One half for
 // FP16 rows' probabilities left 1.3 times the error of the result's own rounding, and 9 to 16 rows, which go to the other kernel, had other bits.)  Probabilities are held times 2^14, so their steps end 2^-38 below a tile's largest one.
@@ -700,7 +700,8 @@ __global__ void __launch_bounds__(256) k_attn_paged_queries(const AttnPagedP p, 
 // With mma.sync every 16 rows of a KV head read its keys and values again, 16 us for 2^25 values of keys (after the first ones); here 128 rows take 5 us more whatever there is, and 7 us more for as many values.
 // Both sides measured (us, here and with mma.sync; FP32, 4 query heads a KV head, head_dim 128): 8 sequences of 4096 slots and 8 KV heads 16 rows 39 and 28, 24 rows 38 and 43, 64 rows 39 and 74; one such
 // sequence 24 rows 17 and 14, 48 rows 18 and 16, 64 rows 18 and 17; one of 500 slots and 32 KV heads 64 rows 15 and 14.
-// The same of head_dim 256 and 192: 8 sequences of 4096 24 rows 85 and 99, 72 and 82; one 24 rows 23 and 21, 21 and 18; 64 rows 23 and 32, 22 and 28; one of 500 and 32 KV heads of 256 64 rows 20 and 19, 128 rows 22 and 36.
+// The same of head_dim 256 and 192: 8 sequences of 4096 24 rows 86 and 99, 69 and 82; one 24 rows 23 and 21, 21 and 18; 64 rows 23 and 32, 22 and 28; one of 500 and 32 KV heads of 256 64 rows 19 and 19, 128 rows 21 and 36.
+// FP16 rows of 128: 8 sequences of 4096 24 rows 35 and 37, 64 rows 36 and 63; one 24 rows 16 and 13, 48 rows 17 and 14, 64 rows 17 and 16.
 // (PI_ATTN_TREE_TC=1 takes 17 rows and more whatever there is, 0 none: a diagnostic switch, read once.)
 bool attn_paged_tc_takes(int64_t rows, double values) {
     static int forced = -2;
