@@ -25,6 +25,7 @@
 #include "pi_tc.cuh"
 #include "pi_tc_math.cuh"
 
+#include <algorithm>
 #include <cstdlib>
 
 namespace pi {
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attn_paged_tc(const __grid_co
     if (tid < 2) mbar_init(s_fin + tid, 1);
     if (tid == 2) mbar_init(&s_asked, 1);
     if (tid == 3) mbar_init(&s_over, 1);
-    if (tid == 0) s_dead = 0;
+    if (tid == 0) { s_dead = 0; s_given = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 0) tc_alloc(&s_tmem, 512);
     tc_fence_before();
@@ -730,7 +731,7 @@ static int pt_go(const AttnPagedP & a, cudaStream_t st) {
     p.units = (int)ap_grid(a) * (PtShape<HD, TWO>::WIDE ? 2 : 1);
     p.next = a.status + 8;
     static const char * tries = getenv("PI_ATTN_TREE_TRIES");         // (a diagnostic switch, read once: how often the kernel's waits ask)
-    p.tries = tries ? (unsigned)strtoul(tries, nullptr, 10) & 0xffffu : PT_TRIES;
+    p.tries = tries ? (unsigned)std::min(strtoul(tries, nullptr, 10), (unsigned long)PT_TRIES) : PT_TRIES;
     const int64_t q_rows = (int64_t)a.b.T * a.n_head;
     if ((rc = tensor_map(&p.m_q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.queries, HD, q_rows * (TWO ? 2 : 1), HD * 2, 64, PT_ROWS, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     PI_CUDA(launch_k(k_attn_paged_queries<HD, TWO>, dim3((unsigned)((q_rows + 31) / 32)), dim3(256), 0, st, true, a, a.queries, a.factor, p.next));
