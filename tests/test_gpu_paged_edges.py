@@ -118,11 +118,10 @@ def test_more_items_than_processors(ops, x, n, H, m, group, hd, kv, cut):
     items = n * H * -(-m * group // R) * (2 if many and hd > 128 else 1)
     if torch.cuda.get_device_properties(0).multi_processor_count == 148:
         assert (items > 148) == (cut != "few") and (0 < parts < items // 2 if cut == "both" else parts == 0), (parts, items)
-    for mask in (None, words_of(masks, 1)):
-        args = (c, x, q, H * group, q_start, pos0, None, m, mask)
-        got = attend(ops, *args, max_kv=kv)
-        check(got, *args)
-        assert ops.last_op_status() == 0 and torch.equal(got, attend(ops, *args, max_kv=kv))
+    args = (c, x, q, H * group, q_start, pos0, None, m, None if x == "f32" else words_of(masks, 1))
+    got = attend(ops, *args, max_kv=kv)
+    check(got, *args)
+    assert ops.last_op_status() == 0 and torch.equal(got, attend(ops, *args, max_kv=kv))
 
 
 # ------------------------------------------------------------------------------------------------ strides
@@ -153,6 +152,49 @@ def test_rows_16_bytes_off(ops, x, hd, n, m, kv):
     assert torch.isfinite(want).all() and _lib.lib.pi_op_status(ws.data_ptr(), ops._stream()) == 0
 
 
+# ------------------------------------------------------------------------------------------------ calls at once
+
+@pytest.mark.parametrize("x", ["f32", "f16"])
+def test_two_calls_at_once(ops, x):
+    """Steps on two streams at the same time, and two captured graphs of them replayed at the same time: the bits of each alone."""
+    steps, want, streams, graphs, captured = [], [], [torch.cuda.Stream() for _ in range(2)], [], []
+    for hd, m, kv in ((128, 20, 1500), (256, 9, 900)):
+        rng = np.random.default_rng(hd)
+        c, H, group = pool(rng, 1, 8, hd, 32, [kv, kv // 2, m]), 8, 8
+        pos0, q_start, T = ints([kv - m, kv // 2 - m, 0]), ints(starts([m] * 3)), 3 * m
+        masks, _ = po.tree_mask(trees(rng, [m] * 3), starts([m] * 3), [0] * 3, m, 1)
+        cache, q, kv_rows, mask, f = on(ops, c), dev(rows(rng, T, H * group * hd, x)), dev(rows(rng, T, H * hd, x)), dev(words_of(masks, 1)), ops.rope_freqs(hd)
+
+        def step(cache=cache, q=q, kv_rows=kv_rows, mask=mask, f=f, pos0=pos0, q_start=q_start, m=m, kv=kv):
+            turned = ops.kv_append_paged(cache, kv_rows, kv_rows, q_start, pos0, max_new=m, q=q, freqs=f)
+            return [ops.attention_tree(cache, turned, q_start, pos0, max_new=m, max_kv=kv, mask=mask) for _ in range(8)]
+
+        steps.append(step)
+        want.append(step()[0])
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, step in zip(streams, steps):
+            with torch.cuda.stream(s):
+                got.append(step())
+        torch.cuda.synchronize()
+        assert all(torch.equal(w, o) for w, g in zip(want, got) for o in g)
+    for s, step in zip(streams, steps):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            captured.append(step())
+    for _ in range(3):
+        for outs in captured:
+            for o in outs:
+                o.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(w, o) for w, g in zip(want, captured) for o in g)
+
+
 # ------------------------------------------------------------------------------------------------ waits that run out
 
 def test_last_op_status_is_that_of_the_attention(ops):
@@ -179,8 +221,8 @@ def run_out(hd, x):
     c = pool(rng, 1, H, hd, 64, lens)
     q_start, pos0, T = [1 + i * m for i in range(n + 1)], [v - m for v in lens], n * m + 3
     q = dev(rows(rng, T, H * group * hd, x))
-    want, tol = po.attention(c, 0, q.cpu().numpy(), H * group, q_start, pos0, None, m, None, hd ** -0.5, U[x], U["f16"] if x == "f16" else 0.0)
-    want, tol = want[1:n * m + 1].reshape(n * m, -1), tol[1:n * m + 1].reshape(n * m, -1)
+    some = range(0, n, 5)                                             # entries whose rows are compared
+    exact = [po.attention(c, 0, q[1 + i * m:1 + i * m + m].cpu().numpy(), H * group, [0, m], [pos0[i]], [i], m, None, hd ** -0.5, U[x], U["f16"] if x == "f16" else 0.0) for i in some]
     seen = []
     for max_kv in (max(lens), 6000, max(lens)):
         out = torch.full((T, H * group * hd), 7.0, dtype=TY[x], device="cuda")
@@ -190,12 +232,15 @@ def run_out(hd, x):
         check(few, c, x, q[1:2].cpu().numpy(), H * group, [0, 1], [300], None, 1, None)
         assert (out[0] == 7).all() and (out[n * m + 1:] == 7).all()   # rows of no entry
         got = out[1:n * m + 1].double().cpu().numpy()
-        none = np.isnan(got)                                          # right, or no numbers
-        assert np.all((np.abs(got - want) <= tol) | none) and none.any() == (seen[-1] != 0)
+        none = np.isnan(got)                                          # right, or no numbers; none as it was
+        assert none.any() == (seen[-1] != 0) and not (got == 7).any()
+        for i, (want, tol) in zip(some, exact):
+            rows_ = slice(i * m, i * m + m)
+            assert np.all((np.abs(got[rows_] - want.reshape(m, -1)) <= tol.reshape(m, -1)) | none[rows_])
     return seen
 
 
-@pytest.mark.parametrize("tries", [0, 1, 20])
+@pytest.mark.parametrize("tries", [0, 1])
 def test_waits_that_run_out_end_with_a_status(ops, tries):
     """PI_ATTN_TREE_TRIES shortens the waits (the first one, for the work in hand, asks once with 0): the kernel ends, reports, rows are right or no numbers, and the
     calls behind it are right."""
